@@ -669,6 +669,103 @@ int zkv_peer_wait(const uint32_t* flags, uint32_t* epoch, int world,
  * exchanges nothing between GPUs on this path.                            */
 int zkv_peer_set_wait_ms(int ms);
 
+/* ------------------------------------------------------------ pooled KV cache */
+
+/* One layer's K and V of many requests of their own lengths, in a pool of
+ * fixed-size blocks that the requests own through a block table (no
+ * reference counterpart: the reference keeps one dense buffer per row and
+ * one length for the whole batch).  Token t of request b lives in block
+ * block_table[b][t / block_size] at t % block_size.  Four operators, as a
+ * serving step runs them: zkv_pool_plan (once per step), zkv_pool_write and
+ * zkv_pool_decode (per layer), zkv_pool_release (when requests finish).   */
+#define ZKV_DT_BF16 0
+#define ZKV_DT_F16 1
+#define ZKV_DT_F8E4M3 2 /* pool blocks only: value = stored * scale of its kv head */
+
+typedef struct zkv_pool {
+    void* k;                            /* element (block i, token t, head h, dim d) at      */
+    void* v;                            /*   base + i*block + t*token + h*head + d           */
+    int64_t k_block, k_token, k_head;   /* strides in elements, > 0, multiples of 16 bytes   */
+    int64_t v_block, v_token, v_head;
+    int64_t n_blocks;
+    int32_t block_size;                 /* tokens per block: a power of two, 16..1024        */
+    int32_t kv_heads;
+    int32_t head_dim;                   /* 64, 128 or 256                                    */
+    int32_t dtype;                      /* ZKV_DT_*                                          */
+    const float* k_scale;               /* [kv_heads] device fp32, e4m3 pools only (NULL: 1) */
+    const float* v_scale;
+    uint64_t maps[32];                  /* tensor maps of k and v, filled by zkv_pool_init   */
+} zkv_pool;
+
+/* Checks the fields of `pool` and fills `maps` (host only, no launch).  To be
+ * called once per pool, and again when a field above `maps` changes.      */
+int zkv_pool_init(zkv_pool* pool);
+
+/* Block table, slot map and lengths of the next step, from the requests'
+ * lengths.  Request b holds lens[b] tokens and appends new_lens[b] (NULL: 1
+ * each).  The free blocks are a stack, its top at free_blocks[*n_free - 1].
+ *   have = ceil(len / S), need = ceil((len + new) / S), cu = running sum of new
+ *   a request fits if len, new >= 0, need <= width and its tokens end
+ *   within n_slots; it takes need - have blocks, in request order; it is
+ *   served if it takes none or the blocks taken up to it are within *n_free.
+ *   block_table[b][have + j] = free_blocks[*n_free - 1 - (taken before b) - j]
+ *   slots[cu[b] + j] = block * S + (len + j) % S;  positions[..] = len + j
+ *   lens_out[b] = len + new;  *n_free_out = *n_free - blocks taken.
+ * Slots and positions of a request that is not served, and past the last
+ * token, are -1; its length and blocks stay, and ZKV_ERR_CAPACITY goes to
+ * `status`.  A block id outside [0, n_blocks) gives the slot -1 and
+ * ZKV_ERR_RANGE.  `status` keeps the largest code.
+ *   block_table [batch][table_ld], width <= table_ld entries of a row used
+ *   free_blocks [n_blocks]; n_free, n_free_out, status: one word each
+ *   slots [n_slots] int64; positions [n_slots], cu_new [batch + 1] (may be NULL)
+ *   lens_out / n_free_out may be lens / n_free.  batch <= 8192.             */
+int zkv_pool_plan(const int32_t* lens, const int32_t* new_lens, int batch, int block_size, int32_t* block_table,
+                  int64_t table_ld, int width, const int32_t* free_blocks, const int32_t* n_free, int64_t n_blocks,
+                  int64_t* slots, int32_t* positions, int64_t n_slots, int32_t* cu_new, int32_t* lens_out,
+                  int32_t* n_free_out, int32_t* status, void* stream);
+
+/* Pushes the blocks of the requests with done[b] != 0 on the free stack, in
+ * request and then block order, and sets their lengths to 0 (their table rows
+ * stay as they are).  A push past n_blocks (a block released twice) is left
+ * out and reported as ZKV_ERR_CAPACITY.  lens_out / n_free_out may be lens /
+ * n_free.  batch <= 8192.                                                  */
+int zkv_pool_release(const uint8_t* done, const int32_t* lens, int batch, int block_size, const int32_t* block_table,
+                     int64_t table_ld, int width, int32_t* free_blocks, const int32_t* n_free, int64_t n_blocks,
+                     int32_t* lens_out, int32_t* n_free_out, int32_t* status, void* stream);
+
+/* K and V rows of n_tokens new tokens into their slots: pool row slots[i]
+ * (block slots[i] / S, token slots[i] % S) of every head = the source row, or
+ * for e4m3 blocks e4m3(row / scale[head]), rounded to nearest even and
+ * saturated at +-448.  Slot -1 is skipped; any other slot outside the pool
+ * too, with ZKV_ERR_RANGE.  Two tokens with one slot: either row may stay.
+ *   k, v  element (i, h, d) at i*token + h*head + d, 16-byte rows; `dtype`
+ *   bf16 or fp16, the pool's own type unless the pool is e4m3             */
+int zkv_pool_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                   int dtype, const int64_t* slots, int64_t n_tokens, const zkv_pool* pool, int32_t* status,
+                   void* stream);
+
+/* Attention of one new token per request over its blocks (grouped heads: q
+ * head j reads kv head j / (q_heads / kv_heads)):
+ *   out = sum_t p_t v_t,  p = softmax over t in [max(0, len - window), len)
+ *   of cap(scale q . k_t),  cap(x) = softcap tanh(x / softcap) (0: x);
+ *   window 0: every token.  lse = log of the sum of exponentials (natural).
+ * A request without tokens gives out 0 and lse -inf.  Rows past `len` may
+ * hold anything.  fp32 inside; the split over a long cache is decided on the
+ * GPU from the lengths, and the parts are joined in a fixed order.
+ *   q [batch][q_heads][head_dim] at b*q_row + j*q_head (16-byte rows), `dtype`
+ *   bf16 or fp16, the pool's own type unless the pool is e4m3; out dense in
+ *   `dtype`; lse [batch][q_heads] fp32 or NULL
+ *   max_len: a bound of lens known to the host (0: width * block_size); a
+ *   longer or negative length is cut to the bound or 0, and a block id
+ *   outside the pool leaves its tokens out, both with ZKV_ERR_RANGE
+ *   workspace: device, 256-byte aligned, >= zkv_pool_decode_ws_bytes
+ *   (scratch only, no state between calls).                               */
+size_t zkv_pool_decode_ws_bytes(int batch, int q_heads, int kv_heads, int head_dim, int64_t max_len);
+int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int dtype, const zkv_pool* pool,
+                    const int32_t* lens, const int32_t* block_table, int64_t table_ld, int width, int batch,
+                    int q_heads, float scale, int window, float softcap, int64_t max_len, void* out, float* lse,
+                    int32_t* status, void* workspace, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

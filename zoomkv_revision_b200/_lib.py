@@ -74,6 +74,14 @@ class ZkvPeerSeg(ctypes.Structure):
                 ("row_bytes", _i64), ("rows", _i32), ("pad", _i32)]
 
 
+class ZkvPool(ctypes.Structure):
+    """Mirror of `zkv_pool` (include/zkv.h)."""
+    _fields_ = [("k", _c_void_p), ("v", _c_void_p), ("k_block", _i64), ("k_token", _i64), ("k_head", _i64),
+                ("v_block", _i64), ("v_token", _i64), ("v_head", _i64), ("n_blocks", _i64), ("block_size", _i32),
+                ("kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32), ("k_scale", _c_void_p),
+                ("v_scale", _c_void_p), ("maps", ctypes.c_uint64 * 32)]
+
+
 _RQ = ctypes.POINTER(ZkvRqLayout)
 
 # name -> argtypes (restype is int status unless noted)
@@ -152,6 +160,16 @@ _SIGNATURES = {
     "zkv_gqa_mean": [_c_void_p, _i32, _i32, _c_void_p, _c_void_p],
     "zkv_page_attend": [_c_void_p, ctypes.POINTER(ZkvPageLayer), _i32, _i32, _i32, _c_void_p, _i32, _i64, _i64, _i32,
                         _i32, _i32, _f32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p],
+    "zkv_pool_init": [_c_void_p],
+    "zkv_pool_plan": [_c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i64, _c_void_p,
+                      _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    "zkv_pool_release": [_c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i64,
+                         _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    "zkv_pool_write": [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i32, _c_void_p, _i64, _c_void_p, _c_void_p,
+                       _c_void_p],
+    "zkv_pool_decode_ws_bytes": [_i32, _i32, _i32, _i32, _i64],
+    "zkv_pool_decode": [_c_void_p, _i64, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _i32, _f32,
+                        _i32, _f32, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p],
     "zkv_version": [],
     "zkv_status_string": [_i32],
 }
@@ -159,7 +177,7 @@ _SIGNATURES = {
 _RESTYPES = {"zkv_status_string": ctypes.c_char_p, "zkv_reference_select_ws_bytes": ctypes.c_size_t,
              "zkv_page_decode_split_ws_bytes": ctypes.c_size_t, "zkv_page_decode_raw_ws_bytes": ctypes.c_size_t,
              "zkv_page_decode_raw_hier_ws_bytes": ctypes.c_size_t, "zkv_raw_split_buffer_bytes": ctypes.c_size_t,
-             "zkv_page_decode_raw_split_ws_bytes": ctypes.c_size_t}
+             "zkv_page_decode_raw_split_ws_bytes": ctypes.c_size_t, "zkv_pool_decode_ws_bytes": ctypes.c_size_t}
 
 _lock = threading.Lock()
 _lib = None

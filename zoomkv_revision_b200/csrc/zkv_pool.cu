@@ -1,0 +1,407 @@
+// zkv_pool.cu -- the pooled KV cache around its attention: the plan of a step
+// (block table, slot map, lengths), the write of new K/V rows into their
+// slots, and the release of finished requests' blocks.
+//
+// Plan and release are a running sum over the requests followed by work per
+// token (per block).  Both run as ONE cluster: every CTA makes the sums for
+// itself (a few values per thread), the cluster meets once, and then its CTAs
+// share the tokens, so the outputs may be the inputs' own buffers without a
+// second launch or a counter in memory.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "zkv_pool.cuh"
+
+namespace zkv {
+namespace pool {
+
+constexpr int kMaxBatch = 8192;
+constexpr int kMaxThreads = 1024;
+
+// Exclusive sum over the block's threads (blockDim.x a multiple of 32); *total gets the sum.
+__device__ int64_t block_sum_before(int64_t x, int64_t* sh, int64_t* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    int64_t incl = x;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += y;
+    }
+    __syncthreads();  // the previous use of sh
+    if (lane == 31) sh[warp] = incl;
+    __syncthreads();
+    int64_t w = lane < nw ? sh[lane] : 0;
+    int64_t wi = w;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, wi, off);
+        if (lane >= off) wi += y;
+    }
+    *total = __shfl_sync(0xffffffffu, wi, 31);
+    return incl - x + __shfl_sync(0xffffffffu, wi - w, warp);
+}
+
+// The last b in [0, n) with start[b] <= i (start ascending, start[0] <= i).
+__device__ __forceinline__ int owner_of(const int32_t* start, int n, int i) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= i) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+struct PlanArgs {
+    const int32_t* lens;
+    const int32_t* new_lens;
+    int32_t* table;
+    const int32_t* free_blocks;
+    const int32_t* n_free;
+    int64_t* slots;
+    int32_t* positions;
+    int32_t* cu_new;
+    int32_t* lens_out;
+    int32_t* n_free_out;
+    int32_t* status;
+    int64_t table_ld, n_blocks;
+    int batch, shift, width, n_slots;
+};
+
+__global__ void __launch_bounds__(kMaxThreads) pool_plan_kernel(const __grid_constant__ PlanArgs a) {
+    extern __shared__ int32_t sm[];
+    __shared__ int64_t sh[32];
+    __shared__ int s_used;
+    int32_t* s_cu = sm;                    // [batch + 1] first token of a request
+    int32_t* s_base = s_cu + a.batch + 1;  // [batch] blocks taken before it; -1: not served
+    int32_t* s_len = s_base + a.batch;     // [batch]
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
+    const int tid = threadIdx.x, nt = blockDim.x;
+    const int S = 1 << a.shift;
+    int code = 0;
+    int64_t n_free = *a.n_free;
+    if (n_free < 0 || n_free > a.n_blocks) {
+        code = ZKV_ERR_RANGE;
+        n_free = n_free < 0 ? 0 : a.n_blocks;
+    }
+    if (tid == 0) s_used = 0;
+    int64_t cu0 = 0, take0 = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += nt) {
+        const int b = b0 + tid;
+        const bool in = b < a.batch;
+        const int len = in ? a.lens[b] : 0;
+        const int add = in ? (a.new_lens ? a.new_lens[b] : 1) : 0;
+        const int64_t n = add > 0 ? add : 0;
+        int64_t total;
+        const int64_t cu = cu0 + block_sum_before(n, sh, &total);
+        cu0 += total;
+        const int64_t have = ((int64_t)len + S - 1) >> a.shift, need = ((int64_t)len + n + S - 1) >> a.shift;
+        const bool fits = in && len >= 0 && add >= 0 && need <= a.width && cu + n <= a.n_slots && len + n <= INT32_MAX;
+        const int64_t take = fits ? need - have : 0;
+        const int64_t base = take0 + block_sum_before(take, sh, &total);
+        take0 += total;
+        const bool served = fits && (take == 0 || base + take <= n_free);
+        if (in) {
+            s_cu[b] = (int)(cu < INT32_MAX ? cu : INT32_MAX);
+            s_base[b] = served ? (int)base : -1;
+            s_len[b] = len;
+            // takers are served in order until one is not, so the blocks taken end with the last one served
+            if (served && take > 0) atomicMax(&s_used, (int)(base + take));
+            if (!served && code == 0) code = ZKV_ERR_CAPACITY;
+        }
+    }
+    if (tid == 0) s_cu[a.batch] = (int)(cu0 < INT32_MAX ? cu0 : INT32_MAX);
+    cluster.sync();  // every CTA has read lens and n_free: rank 0 may write over them
+    if (rank == 0) {
+        for (int b = tid; b < a.batch; b += nt) {
+            const int len = s_len[b];
+            a.lens_out[b] = s_base[b] >= 0 ? len + (s_cu[b + 1] - s_cu[b]) : len;
+        }
+        if (a.cu_new)
+            for (int b = tid; b <= a.batch; b += nt) a.cu_new[b] = s_cu[b];
+        if (tid == 0) *a.n_free_out = (int)n_free - s_used;
+    }
+    const int total = s_cu[a.batch];
+    for (int64_t i = (int64_t)rank * nt + tid; i < a.n_slots; i += (int64_t)ranks * nt) {
+        int64_t slot = -1;
+        int pos = -1;
+        if (i < total) {
+            const int b = owner_of(s_cu, a.batch, (int)i);
+            const int base = s_base[b];
+            if (base >= 0) {
+                const int p = s_len[b] + ((int)i - s_cu[b]);
+                const int have = (s_len[b] + S - 1) >> a.shift, j = p >> a.shift;
+                int32_t* entry = a.table + b * a.table_ld + j;
+                int id;
+                if (j < have) {
+                    id = *entry;
+                } else {  // a new block: its first token is new, and that token's thread enters it
+                    id = a.free_blocks[n_free - 1 - base - (j - have)];
+                    if ((p & (S - 1)) == 0) *entry = id;
+                }
+                if (id >= 0 && id < a.n_blocks) {
+                    slot = ((int64_t)id << a.shift) + (p & (S - 1));
+                    pos = p;
+                } else {
+                    code = ZKV_ERR_RANGE;
+                }
+            }
+        }
+        a.slots[i] = slot;
+        if (a.positions) a.positions[i] = pos;
+    }
+    if (code) raise_status(a.status, code);
+}
+
+struct ReleaseArgs {
+    const uint8_t* done;
+    const int32_t* lens;
+    const int32_t* table;
+    int32_t* free_blocks;
+    const int32_t* n_free;
+    int32_t* lens_out;
+    int32_t* n_free_out;
+    int32_t* status;
+    int64_t table_ld, n_blocks;
+    int batch, shift, width;
+};
+
+__global__ void __launch_bounds__(kMaxThreads) pool_release_kernel(const __grid_constant__ ReleaseArgs a) {
+    extern __shared__ int32_t sm[];
+    __shared__ int64_t sh[32];
+    int32_t* s_start = sm;             // [batch] blocks pushed before a request
+    int32_t* s_len = s_start + a.batch;  // [batch] its new length
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
+    const int tid = threadIdx.x, nt = blockDim.x;
+    const int S = 1 << a.shift;
+    int code = 0;
+    int64_t n_free = *a.n_free;
+    if (n_free < 0 || n_free > a.n_blocks) {
+        code = ZKV_ERR_RANGE;
+        n_free = n_free < 0 ? 0 : a.n_blocks;
+    }
+    int64_t start0 = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += nt) {
+        const int b = b0 + tid;
+        const bool in = b < a.batch;
+        const int len = in ? a.lens[b] : 0;
+        const bool done = in && a.done[b];
+        int64_t count = done && len > 0 ? ((int64_t)len + S - 1) >> a.shift : 0;
+        if (count > a.width || (done && len < 0)) {
+            code = ZKV_ERR_RANGE;
+            count = count > a.width ? a.width : count;
+        }
+        int64_t total;
+        const int64_t start = start0 + block_sum_before(count, sh, &total);
+        start0 += total;
+        if (in) {
+            s_start[b] = (int)(start < INT32_MAX ? start : INT32_MAX);
+            s_len[b] = done ? 0 : len;
+        }
+    }
+    const int64_t room = a.n_blocks - n_free;
+    if (start0 > room) {
+        code = code ? code : ZKV_ERR_CAPACITY;
+        start0 = room;
+    }
+    cluster.sync();  // every CTA has read lens and n_free
+    if (rank == 0) {
+        for (int b = tid; b < a.batch; b += nt) a.lens_out[b] = s_len[b];
+        if (tid == 0) *a.n_free_out = (int)(n_free + start0);
+    }
+    for (int64_t i = (int64_t)rank * nt + tid; i < start0; i += (int64_t)ranks * nt) {
+        const int b = owner_of(s_start, a.batch, (int)i);
+        const int id = a.table[b * a.table_ld + ((int)i - s_start[b])];
+        if (id < 0 || id >= a.n_blocks) code = ZKV_ERR_RANGE;
+        a.free_blocks[n_free + i] = id;
+    }
+    if (code) raise_status(a.status, code);
+}
+
+// ---------------------------------------------------------------- write
+struct WriteArgs {
+    const uint8_t* src[2];
+    uint8_t* dst[2];
+    const float* scale[2];
+    int64_t src_token[2], src_head[2];               // bytes
+    int64_t dst_block[2], dst_token[2], dst_head[2];  // bytes
+    const int64_t* slots;
+    int32_t* status;
+    int64_t pool_tokens, items;
+    int heads, lg_parts, shift;
+};
+
+template <bool kBf16>
+__device__ __forceinline__ void to_floats(uint32_t w, float& lo, float& hi) {
+    if (kBf16) {
+        lo = __uint_as_float(w << 16);
+        hi = __uint_as_float(w & 0xffff0000u);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        lo = f.x;
+        hi = f.y;
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t to_e4m3x4(uint32_t w0, uint32_t w1, float scale) {
+    float a, b, c, d;
+    to_floats<kBf16>(w0, a, b);
+    to_floats<kBf16>(w1, c, d);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(a, scale), __fdiv_rn(b, scale)), __NV_SATFINITE,
+                                                 __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(c, scale), __fdiv_rn(d, scale)), __NV_SATFINITE,
+                                                 __NV_E4M3);
+    return lo | (hi << 16);
+}
+
+constexpr int kWriteThreads = 256;
+constexpr int kWriteUnroll = 4;
+
+// One 16-byte store per item (token, head, part of the row); K at blockIdx.y
+// 0, V at 1.  A thread's kWriteUnroll source loads are in flight together.
+// kMode 0: 16-bit copy; 1: bf16 -> e4m3; 2: fp16 -> e4m3 (two loads an item).
+template <int kMode>
+__global__ void __launch_bounds__(kWriteThreads) pool_write_kernel(const __grid_constant__ WriteArgs a) {
+    const int y = blockIdx.y;
+    constexpr int kLoads = kMode ? 2 : 1;
+    const int64_t first = (int64_t)blockIdx.x * (kWriteThreads * kWriteUnroll) + threadIdx.x;
+    const float* sc = a.scale[y];
+    uint4 x[kWriteUnroll][kLoads];
+    int64_t slot[kWriteUnroll];
+    uint32_t head[kWriteUnroll];
+#pragma unroll
+    for (int u = 0; u < kWriteUnroll; ++u) {
+        const int64_t it = first + u * kWriteThreads;
+        slot[u] = -1;
+        if (it >= a.items) continue;
+        const uint32_t row = (uint32_t)(it >> a.lg_parts), part = (uint32_t)it & ((1u << a.lg_parts) - 1);
+        const uint32_t tok = row / (uint32_t)a.heads;
+        head[u] = row - tok * (uint32_t)a.heads;
+        slot[u] = a.slots[tok];
+        const uint4* p = reinterpret_cast<const uint4*>(a.src[y] + tok * a.src_token[y] + head[u] * a.src_head[y]) +
+                         part * kLoads;
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l) x[u][l] = __ldg(p + l);
+    }
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < kWriteUnroll; ++u) {
+        const int64_t it = first + u * kWriteThreads;
+        const int64_t s = slot[u];
+        if (it >= a.items || s == -1) continue;
+        if (s < 0 || s >= a.pool_tokens) {
+            bad = true;
+            continue;
+        }
+        const uint32_t part = (uint32_t)it & ((1u << a.lg_parts) - 1);
+        uint8_t* d = a.dst[y] + (s >> a.shift) * a.dst_block[y] + (s & ((1 << a.shift) - 1)) * a.dst_token[y] +
+                     head[u] * a.dst_head[y] + part * 16;
+        uint4 out;
+        if constexpr (kMode == 0) {
+            out = x[u][0];
+        } else {
+            const float f = sc ? __ldg(sc + head[u]) : 1.f;
+            out.x = to_e4m3x4<kMode == 1>(x[u][0].x, x[u][0].y, f);
+            out.y = to_e4m3x4<kMode == 1>(x[u][0].z, x[u][0].w, f);
+            out.z = to_e4m3x4<kMode == 1>(x[u][1].x, x[u][1].y, f);
+            out.w = to_e4m3x4<kMode == 1>(x[u][1].z, x[u][1].w, f);
+        }
+        *reinterpret_cast<uint4*>(d) = out;
+    }
+    if (bad) raise_status(a.status, ZKV_ERR_RANGE);
+}
+
+// CTAs of the cluster and threads of a CTA for `work` items and `batch` requests.
+static void plan_shape(int batch, int64_t work, int* ctas, int* threads) {
+    const int64_t want = std::max<int64_t>(batch, work);
+    *ctas = want > 2 * kMaxThreads ? 8 : 1;
+    *threads = (int)std::min<int64_t>(kMaxThreads, (want + 31) / 32 * 32);
+}
+
+}  // namespace pool
+}  // namespace zkv
+
+using namespace zkv;
+
+extern "C" int zkv_pool_plan(const int32_t* lens, const int32_t* new_lens, int batch, int block_size,
+                             int32_t* block_table, int64_t table_ld, int width, const int32_t* free_blocks,
+                             const int32_t* n_free, int64_t n_blocks, int64_t* slots, int32_t* positions,
+                             int64_t n_slots, int32_t* cu_new, int32_t* lens_out, int32_t* n_free_out,
+                             int32_t* status, void* stream) {
+    if (batch < 0 || n_slots < 0 || width < 0 || table_ld < width || n_blocks < 0) return ZKV_ERR_ARG;
+    if (!pool::block_size_ok(block_size)) return ZKV_ERR_UNSUPPORTED;
+    if (batch > pool::kMaxBatch || n_slots > INT32_MAX - 1 || n_blocks > INT32_MAX) return ZKV_ERR_CAPACITY;
+    if ((batch > 0 && (!lens || !lens_out || (!block_table && width > 0))) || (!free_blocks && n_blocks > 0) ||
+        !n_free || !n_free_out || (!slots && n_slots > 0))
+        return ZKV_ERR_ARG;
+    pool::PlanArgs a{lens, new_lens, block_table, free_blocks, n_free, slots, positions, cu_new, lens_out, n_free_out,
+                     status, table_ld, n_blocks, batch, pool::log2_of(block_size), width, (int)n_slots};
+    int ctas, threads;
+    pool::plan_shape(std::max(batch, 1), n_slots, &ctas, &threads);
+    void* args[] = {&a};
+    return launch_clustered((const void*)pool::pool_plan_kernel, ctas, threads, ctas,
+                            (size_t)(3 * batch + 1) * sizeof(int32_t), (cudaStream_t)stream, args);
+}
+
+extern "C" int zkv_pool_release(const uint8_t* done, const int32_t* lens, int batch, int block_size,
+                                const int32_t* block_table, int64_t table_ld, int width, int32_t* free_blocks,
+                                const int32_t* n_free, int64_t n_blocks, int32_t* lens_out, int32_t* n_free_out,
+                                int32_t* status, void* stream) {
+    if (batch < 0 || width < 0 || table_ld < width || n_blocks < 0) return ZKV_ERR_ARG;
+    if (!pool::block_size_ok(block_size)) return ZKV_ERR_UNSUPPORTED;
+    if (batch > pool::kMaxBatch || n_blocks > INT32_MAX) return ZKV_ERR_CAPACITY;
+    if ((batch > 0 && (!done || !lens || !lens_out || (!block_table && width > 0))) ||
+        (!free_blocks && n_blocks > 0) || !n_free || !n_free_out)
+        return ZKV_ERR_ARG;
+    pool::ReleaseArgs a{done, lens, block_table, free_blocks, n_free, lens_out, n_free_out, status, table_ld, n_blocks,
+                        batch, pool::log2_of(block_size), width};
+    int ctas, threads;
+    pool::plan_shape(std::max(batch, 1), std::min<int64_t>((int64_t)batch * width, n_blocks), &ctas, &threads);
+    void* args[] = {&a};
+    return launch_clustered((const void*)pool::pool_release_kernel, ctas, threads, ctas,
+                            (size_t)(2 * batch) * sizeof(int32_t), (cudaStream_t)stream, args);
+}
+
+extern "C" int zkv_pool_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                              int64_t v_head, int dtype, const int64_t* slots, int64_t n_tokens, const zkv_pool* p,
+                              int32_t* status, void* stream) {
+    const int rc = pool::check_pool(p);
+    if (rc != ZKV_OK) return rc;
+    if (n_tokens < 0 || (dtype != ZKV_DT_BF16 && dtype != ZKV_DT_F16)) return ZKV_ERR_ARG;
+    if (p->dtype != ZKV_DT_F8E4M3 && p->dtype != dtype) return ZKV_ERR_ARG;
+    if (n_tokens == 0) return ZKV_OK;
+    if (!k || !v || !slots) return ZKV_ERR_ARG;
+    if (!pool::aligned16(k) || !pool::aligned16(v) || k_token % 8 || k_head % 8 || v_token % 8 || v_head % 8)
+        return ZKV_ERR_ALIGN;
+    if (n_tokens > INT32_MAX / p->kv_heads) return ZKV_ERR_CAPACITY;
+    const int el = pool::element_bytes(p->dtype);
+    const int lg = pool::log2_of(p->head_dim * el / 16);
+    pool::WriteArgs a;
+    a.src[0] = (const uint8_t*)k, a.src[1] = (const uint8_t*)v;
+    a.dst[0] = (uint8_t*)p->k, a.dst[1] = (uint8_t*)p->v;
+    a.scale[0] = p->k_scale, a.scale[1] = p->v_scale;
+    a.src_token[0] = k_token * 2, a.src_token[1] = v_token * 2;
+    a.src_head[0] = k_head * 2, a.src_head[1] = v_head * 2;
+    a.dst_block[0] = p->k_block * el, a.dst_block[1] = p->v_block * el;
+    a.dst_token[0] = p->k_token * el, a.dst_token[1] = p->v_token * el;
+    a.dst_head[0] = p->k_head * el, a.dst_head[1] = p->v_head * el;
+    a.slots = slots, a.status = status;
+    a.pool_tokens = p->n_blocks * p->block_size;
+    a.items = (n_tokens * p->kv_heads) << lg;
+    a.heads = p->kv_heads, a.lg_parts = lg, a.shift = pool::log2_of(p->block_size);
+    const int64_t per = pool::kWriteThreads * pool::kWriteUnroll;
+    const dim3 grid((unsigned)((a.items + per - 1) / per), 2);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (el == 2)
+        pool::pool_write_kernel<0><<<grid, pool::kWriteThreads, 0, st>>>(a);
+    else if (dtype == ZKV_DT_BF16)
+        pool::pool_write_kernel<1><<<grid, pool::kWriteThreads, 0, st>>>(a);
+    else
+        pool::pool_write_kernel<2><<<grid, pool::kWriteThreads, 0, st>>>(a);
+    return launch_status();
+}

@@ -31,6 +31,8 @@ collision_topk                         get_cache_cnt_fused + _coarse_filter_trun
 partial_rerank_cuda                    cache_hub/rerank/rerank.py:352-400 (+ topk/gather :1750-1832)
 coarse_2bit_score_cuda                 cache_hub/rerank/rerank.py:636-690
 rq_popcount_topk                       (1-bit x 4-bit popcount rerank + exact IP; no counterpart)
+KVPool / pool_plan / pool_write /      (pooled KV cache with block tables, requests of their own lengths;
+pool_decode / pool_release             no counterpart)
 =====================================  ==============================================
 
 Errors follow the reference: wrong dtype -> TypeError, wrong shape / range ->
@@ -53,6 +55,7 @@ __all__ = [
     "h2d_gather_kv", "h2d_gather_kv_packed", "h2d_gather_rows", "page_decode_scored",
     "PageLayer", "page_attend", "RawLayer", "page_decode_raw", "page_decode_raw_ws_bytes", "gqa_mean", "reference_select", "reference_select_ws_bytes", "RqLayout", "rq_encode", "batch_encode", "rq_query", "get_cache_cnt_fused", "collision_topk",
     "partial_rerank_cuda", "coarse_2bit_score_cuda", "rq_popcount_topk", "MAG_CENTERS", "MAG_THRESHOLDS",
+    "KVPool", "pool_plan", "pool_release", "pool_write", "pool_decode", "pool_decode_ws_bytes",
 ]
 
 
@@ -1108,3 +1111,231 @@ def rq_popcount_topk(cand, lay: RqLayout, planes, qparams, K: int, *, C: int | N
     check(lib().zkv_rq_popcount_topk(_p(cand), C, lay.struct, _p(planes), _p(qparams), rows, K, _p(sel), _p(est_out),
                                      _p(keys), ld, _p(q_mean), _p(ip), _stream(planes)), "zkv_rq_popcount_topk")
     return sel, est_out, ip
+
+
+# ----------------------------------------------------------------- pooled KV cache
+_POOL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
+_INT32 = torch.int32
+
+
+class KVPool:
+    """One layer's pooled KV cache: k, v [n_blocks, block_size, kv_heads, head_dim]
+    bf16, fp16 or float8_e4m3fn CUDA tensors, any strides with whole 16-byte
+    rows (a head-before-token pool is passed as `t.transpose(1, 2)`).
+    k_scale, v_scale [kv_heads] fp32: an e4m3 element stands for
+    stored * scale of its head (None: 1).  Made once when the pool is
+    allocated: it holds the tensors, their addresses and strides."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "struct", "ref", "dtype", "device", "kv_heads", "head_dim",
+                 "block_size", "n_blocks")
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        _cuda(("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale))
+        if k.dim() != 4 or k.shape != v.shape:
+            raise ValueError(f"k and v must be [n_blocks, block_size, kv_heads, head_dim]; got {tuple(k.shape)} and "
+                             f"{tuple(v.shape)}")
+        if k.dtype not in _POOL_DTYPES or v.dtype != k.dtype:
+            raise TypeError(f"k and v must both be bfloat16, float16 or float8_e4m3fn; got {k.dtype} and {v.dtype}")
+        for t in (v, k_scale, v_scale):
+            if t is not None and t.device != k.device:
+                raise ValueError("the pool's tensors must be on one device")
+        n, S, H, D = k.shape
+        if k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError("the last dim of k and v must be contiguous")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is None:
+                continue
+            if k.dtype != torch.float8_e4m3fn:
+                raise ValueError(f"{name} belongs to a float8_e4m3fn pool")
+            _dtype(name, t, torch.float32)
+            if tuple(t.shape) != (H,):
+                raise ValueError(f"{name} must be [kv_heads]")
+            _contig(name, t)
+
+        def strides(t):  # a dimension of one element has no stride of its own
+            row = D
+            s = [t.stride(0) if n > 1 else row, t.stride(1), t.stride(2) if H > 1 else row]
+            return s
+
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.dtype, self.device = k.dtype, k.device
+        self.n_blocks, self.block_size, self.kv_heads, self.head_dim = n, S, H, D
+        self.struct = _lib.ZkvPool(_p(k), _p(v), *strides(k), *strides(v), n, S, H, D, _POOL_DTYPES[k.dtype],
+                                   _p(k_scale), _p(v_scale))
+        self.ref = ctypes.addressof(self.struct)
+        check(lib().zkv_pool_init(self.ref), "zkv_pool_init")
+
+
+def _ints32(**tensors):
+    """int32, contiguous CUDA tensors of one device (None is left out)."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.dtype is not _INT32:
+            raise TypeError(f"{name} must be torch.int32; got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError("tensors must be on one device")
+
+
+def _block_table(block_table, batch, dev):
+    if block_table.dtype is not _INT32:
+        raise TypeError(f"block_table must be torch.int32; got {block_table.dtype}")
+    if block_table.dim() != 2 or block_table.shape[0] != batch or block_table.device != dev:
+        raise ValueError("block_table must be [batch, width] on the device of lens")
+    width = block_table.shape[1]
+    ld = block_table.stride(0) if batch > 1 else width
+    if (width > 1 and block_table.stride(1) != 1) or ld < width:
+        raise ValueError("block_table rows must be contiguous and not overlap")
+    return ld, width
+
+
+def pool_plan(lens, new_lens, block_table, free_blocks, n_free, block_size: int, slots, *, positions=None,
+              cu_new=None, lens_out=None, n_free_out=None, status=None):
+    """The next step's blocks, slots and lengths, in one launch and without
+    asking the GPU: request b holds lens[b] tokens and appends new_lens[b]
+    (None: one each).  Blocks come off the stack free_blocks[:n_free].
+
+    lens, new_lens [B] int32; block_table [B, width] int32 (updated);
+    free_blocks [n_blocks] int32 (as many as the pool has blocks); n_free [1]
+    int32; slots [n_slots] int64 and positions [n_slots] int32 (written: one
+    per new token in request order, -1 past the last and for a request that
+    is not served); cu_new [B + 1] int32 (written: first token of a request).
+    lens_out / n_free_out default to lens / n_free in place.  A request that
+    finds no room keeps its length and blocks; status [1] int32 then gets
+    ZKV_ERR_CAPACITY (3).  Returns slots."""
+    _ints32(lens=lens, new_lens=new_lens, free_blocks=free_blocks, n_free=n_free, positions=positions, cu_new=cu_new,
+            lens_out=lens_out, n_free_out=n_free_out, status=status)
+    B = lens.numel()
+    ld, width = _block_table(block_table, B, lens.device)
+    if slots.dtype != torch.int64:
+        raise TypeError(f"slots must be torch.int64; got {slots.dtype}")
+    if not slots.is_contiguous() or slots.device != lens.device:
+        raise ValueError("slots must be contiguous, on the device of lens")
+    if (new_lens is not None and new_lens.numel() != B) or (lens_out is not None and lens_out.numel() != B):
+        raise ValueError("new_lens and lens_out must have one value per request")
+    if (positions is not None and positions.numel() < slots.numel()) or (cu_new is not None and cu_new.numel() < B + 1):
+        raise ValueError("positions needs one value per slot and cu_new [B + 1]")
+    if lens_out is None:
+        lens_out = lens
+    if n_free_out is None:
+        n_free_out = n_free
+    check(lib().zkv_pool_plan(_p(lens), _p(new_lens), B, block_size, _p(block_table), ld, width, _p(free_blocks),
+                              _p(n_free), free_blocks.numel(), _p(slots), _p(positions), slots.numel(), _p(cu_new),
+                              _p(lens_out), _p(n_free_out), _p(status), _stream(lens)), "zkv_pool_plan")
+    return slots
+
+
+def pool_release(done, lens, block_table, free_blocks, n_free, block_size: int, *, lens_out=None, n_free_out=None,
+                 status=None):
+    """Pushes the blocks of the requests with done[b] on the free stack
+    (free_blocks, n_free) and sets their lengths to 0.  done [B] bool;
+    the others as in pool_plan; lens_out / n_free_out default to in place."""
+    _ints32(lens=lens, free_blocks=free_blocks, n_free=n_free, lens_out=lens_out, n_free_out=n_free_out, status=status)
+    B = lens.numel()
+    ld, width = _block_table(block_table, B, lens.device)
+    if done.dtype != torch.bool:
+        raise TypeError(f"done must be torch.bool; got {done.dtype}")
+    if done.numel() != B or not done.is_contiguous() or done.device != lens.device:
+        raise ValueError("done must be contiguous [B], on the device of lens")
+    if lens_out is not None and lens_out.numel() != B:
+        raise ValueError("lens_out must have one value per request")
+    if lens_out is None:
+        lens_out = lens
+    if n_free_out is None:
+        n_free_out = n_free
+    check(lib().zkv_pool_release(_p(done), _p(lens), B, block_size, _p(block_table), ld, width, _p(free_blocks),
+                                 _p(n_free), free_blocks.numel(), _p(lens_out), _p(n_free_out), _p(status),
+                                 _stream(lens)), "zkv_pool_release")
+
+
+def _whole_rows(t):
+    """t with its last dim contiguous and 16-byte rows (a copy where it has not)."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def pool_write(k, v, slots, pool: KVPool, *, status=None):
+    """K and V rows of new tokens into their slots of the pool: k, v
+    [n_tokens, kv_heads, head_dim] bf16 or fp16 (the pool's type; any of the
+    two for an e4m3 pool, which stores e4m3(row / scale), saturated at 448);
+    slots [n_tokens] int64 of pool_plan, -1 = none."""
+    if k.shape != v.shape or k.dim() != 3 or k.shape[1] != pool.kv_heads or k.shape[2] != pool.head_dim:
+        raise ValueError(f"k and v must be [n_tokens, {pool.kv_heads}, {pool.head_dim}]; got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    dt = k.dtype
+    if v.dtype != dt or dt not in (torch.bfloat16, torch.float16) or (pool.dtype != dt and
+                                                                      pool.dtype != torch.float8_e4m3fn):
+        raise TypeError(f"k {dt} and v {v.dtype} do not go into a {pool.dtype} pool")
+    if slots.dtype != torch.int64:
+        raise TypeError(f"slots must be torch.int64; got {slots.dtype}")
+    n = k.shape[0]
+    if slots.numel() < n or not slots.is_contiguous():
+        raise ValueError("slots must be contiguous, one per token")
+    dev = pool.device
+    if k.device != dev or v.device != dev or slots.device != dev:
+        raise ValueError("tensors must be on the pool's device")
+    k, v = _whole_rows(k), _whole_rows(v)
+    check(lib().zkv_pool_write(_p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _POOL_DTYPES[dt],
+                               _p(slots), n, pool.ref, _p(status), _stream(k)), "zkv_pool_write")
+
+
+def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int = 0, softcap: float = 0.0,
+                max_len: int = 0, out=None, lse=None, return_lse: bool = False, status=None, workspace=None):
+    """Attention of one new token per request over its blocks of the pool.
+
+    q [B, q_heads, head_dim] (or [B, 1, q_heads, head_dim]) bf16 or fp16, the
+    pool's type unless the pool is e4m3; lens [B] int32, the tokens of each
+    request (the new one among them, written by pool_write); block_table
+    [B, width] int32.  Softmax over the last `window` tokens (0: all) of
+    scale * q.k (default 1 / sqrt(head_dim)), soft-capped if softcap > 0.
+    max_len: a bound of lens that the host knows (0: width * block_size).
+    Returns out like q, with return_lse (out, lse [B, q_heads] fp32, natural
+    log, -inf for a request without tokens, whose out is 0).  workspace:
+    uint8 CUDA tensor of pool_decode_ws_bytes(...) bytes, scratch only
+    (default: allocated per call from torch's caching allocator)."""
+    B, Hq, D = q.shape[0], q.shape[-2], q.shape[-1]
+    if D != pool.head_dim or Hq % pool.kv_heads or q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[1] != 1):
+        raise ValueError(f"q must be [B, (1,) q_heads, {pool.head_dim}] with q_heads a multiple of {pool.kv_heads}; got "
+                         f"{tuple(q.shape)}")
+    dt = q.dtype
+    if dt not in (torch.bfloat16, torch.float16) or (pool.dtype != dt and pool.dtype != torch.float8_e4m3fn):
+        raise TypeError(f"q {dt} does not fit a {pool.dtype} pool")
+    dev = pool.device
+    if q.device != dev or lens.device != dev:
+        raise ValueError("tensors must be on the pool's device")
+    _ints32(lens=lens, status=status)
+    if lens.numel() != B:
+        raise ValueError("lens must have one value per request")
+    ld, width = _block_table(block_table, B, dev)
+    q3 = _whole_rows(q if q.dim() == 3 else q[:, 0])
+    if out is None:
+        out = torch.empty(q.shape, dtype=dt, device=dev)
+    elif out.shape != q.shape or out.dtype != dt or not out.is_contiguous() or out.device != dev:
+        raise ValueError("out must be contiguous, shaped and typed like q")
+    if lse is None:
+        if return_lse:
+            lse = torch.empty(B, Hq, dtype=torch.float32, device=dev)
+    elif lse.dtype != torch.float32 or lse.numel() != B * Hq or not lse.is_contiguous() or lse.device != dev:
+        raise ValueError("lse must be contiguous fp32 [B, q_heads]")
+    if workspace is None:
+        workspace = torch.empty(pool_decode_ws_bytes(B, Hq, pool, width, max_len), dtype=torch.uint8, device=dev)
+    check(lib().zkv_pool_decode(_p(q3), q3.stride(0), q3.stride(1), _POOL_DTYPES[dt], pool.ref, _p(lens),
+                                _p(block_table), ld, width, B, Hq, D ** -0.5 if scale is None else float(scale),
+                                int(window), float(softcap), int(max_len), _p(out), _p(lse), _p(status),
+                                _p(workspace), workspace.numel(), _stream(q)), "zkv_pool_decode")
+    return (out, lse) if return_lse else out
+
+
+def pool_decode_ws_bytes(batch: int, q_heads: int, pool: KVPool, width: int, max_len: int = 0) -> int:
+    """Bytes of workspace that pool_decode needs for a block table of `width` columns."""
+    room = width * pool.block_size
+    return int(lib().zkv_pool_decode_ws_bytes(batch, q_heads, pool.kv_heads, pool.head_dim,
+                                              min(max_len, room) if max_len > 0 else room))
