@@ -20,29 +20,6 @@ namespace pool {
 constexpr int kMaxBatch = 8192;
 constexpr int kMaxThreads = 1024;
 
-// Exclusive sum over the block's threads (blockDim.x a multiple of 32); *total gets the sum.
-__device__ int64_t block_sum_before(int64_t x, int64_t* sh, int64_t* total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    int64_t incl = x;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += y;
-    }
-    __syncthreads();  // the previous use of sh
-    if (lane == 31) sh[warp] = incl;
-    __syncthreads();
-    int64_t w = lane < nw ? sh[lane] : 0;
-    int64_t wi = w;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, wi, off);
-        if (lane >= off) wi += y;
-    }
-    *total = __shfl_sync(0xffffffffu, wi, 31);
-    return incl - x + __shfl_sync(0xffffffffu, wi - w, warp);
-}
-
 // The last b in [0, n) with start[b] <= i (start ascending, start[0] <= i).
 __device__ __forceinline__ int owner_of(const int32_t* start, int n, int i) {
     int lo = 0, hi = n;

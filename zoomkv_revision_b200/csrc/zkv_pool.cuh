@@ -13,6 +13,29 @@ __device__ __forceinline__ void raise_status(int32_t* status, int code) {
     if (status) atomicMax(status, code);
 }
 
+// Exclusive sum over the block's threads (blockDim.x a multiple of 32); *total gets the sum.
+static __device__ __forceinline__ int64_t block_sum_before(int64_t x, int64_t* sh, int64_t* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    int64_t incl = x;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += y;
+    }
+    __syncthreads();  // the previous use of sh
+    if (lane == 31) sh[warp] = incl;
+    __syncthreads();
+    int64_t w = lane < nw ? sh[lane] : 0;
+    int64_t wi = w;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, wi, off);
+        if (lane >= off) wi += y;
+    }
+    *total = __shfl_sync(0xffffffffu, wi, 31);
+    return incl - x + __shfl_sync(0xffffffffu, wi - w, warp);
+}
+
 static inline int log2_of(int x) {
     int s = 0;
     while ((1 << s) < x) ++s;

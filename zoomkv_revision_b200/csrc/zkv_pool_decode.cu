@@ -3,29 +3,69 @@
 //
 //   o = sum_t p_t v_t / sum_t p_t,  p_t = exp(cap(scale q . k_t) - max)
 //
-// First form: one CTA per (request, kv head, 8 query heads) and 512 tokens;
-// each warp runs the softmax over every fourth token with the row's dims over
-// its lanes, the warps' and then the splits' partials (m, l, o) are joined.
+// Every K and V byte is used for 2 G products of one grouped head (G = 4: 4
+// operations a byte), so the bytes bound it.  The kernel is built to keep
+// reads in flight on every SM until the last tile:
+//
+//  * The work is the list of all (request, kv head, 64-token tile) units, in
+//    that order, cut into equal ranges, one per CTA of a one-wave grid.  Each
+//    CTA finds its range from the lengths by itself (a sum over the requests),
+//    so uneven requests, one long request and many short ones are spread the
+//    same way and the host needs no length.  A row (request, kv head) that
+//    ends in another CTA than it began in leaves partials (m, l, o), which
+//    pool_join_kernel joins in CTA order.
+//  * One producer warp per CTA walks the range: block ids from the table, one
+//    5-D TMA copy per block and tensor (dims | tokens | 128-byte pieces | head
+//    | block; any strides, so both memory orders), a ring of stages.  An id
+//    outside the pool is not copied.
+//  * Four consumer warps take 16 tokens of a tile each: S^T = K Q^T (tokens x
+//    heads) and O^T += V^T P^T (dims x heads) by mma.sync m16n8k16, so a
+//    group of up to 8 heads fills the 8 columns of one product.  tcgen05
+//    needs 64 or 128 rows of M per product and TMEM round trips for the
+//    softmax of a 16-token tile; at 4-16 heads and an HBM-bound tile it has
+//    nothing to win here.
+//  * A warp keeps its own running max, sum and O^T in registers through the
+//    row; the four are joined in the last tile's stage.
+//
+// Roundings: scores, statistics and accumulators are fp32.  The probability
+// enters the second product as two 16-bit parts (p = hi + lo, 16 bits of
+// mantissa for bf16), so that it adds nothing visible to the output's own
+// rounding; over e4m3 blocks with bf16 output one fp16 part (11 bits) does.
+// e4m3 blocks are widened to fp16, exactly; a bf16 query is scaled by the
+// power of two that puts its largest element into [1, 2) first, which leaves
+// it exact in fp16 but for elements below 2^-14 of the largest.
 #include <cuda.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include <algorithm>
 #include <cstring>
+#include <mutex>
 
 #include "zkv_pool.cuh"
 
 namespace zkv {
 namespace pool {
 
-constexpr int kHeads = 8;      // query heads of a row
-constexpr int kSplit = 512;    // tokens of a CTA
-constexpr int kDecodeWarps = 4;
+constexpr int kTile = 64;                       // tokens of a unit
+constexpr int kConsumers = 4;                   // warps, 16 tokens of a tile each
+constexpr int kThreads = 32 * (kConsumers + 1);
+constexpr int kMaxGrid = 320;                   // CTAs that a workspace is sized for
+constexpr uint64_t kWaitNs = 2000000000ull;     // limit of each wait inside a CTA
+
+// What a unit is, written by the producer beside its stage.
+struct Unit {
+    int b, hg;        // request; kv head * chunks + chunk of query heads
+    int tile0;        // first token
+    int lo, len;      // tokens [lo, len) of the request are attended
+    int flags;        // kFirst, kLast of the row in this CTA
+    int part;         // -1: the row is this CTA's alone; else its partial slot
+    int bad;          // boxes of the tile that are not in the pool
+};
+constexpr int kFirst = 1, kLast = 2;
 
 struct DecodeArgs {
+    CUtensorMap tk, tv;  // [block][head][128-byte piece][token][bytes]
     const uint8_t* q;
-    const uint8_t* k;
-    const uint8_t* v;
     const float* k_scale;
     const float* v_scale;
     const int32_t* lens;
@@ -33,149 +73,827 @@ struct DecodeArgs {
     void* out;
     float* lse;
     int32_t* status;
-    float* parts;  // [rows][splits][kHeads][D + 2]
-    int64_t q_row, q_head, k_block, k_token, k_head, v_block, v_token, v_head;  // bytes
+    int4* joins;    // [grid] {b, hg, CTAs of the row, 0}: the row whose first part is this CTA's last one
+    float* parts;   // [grid][2][heads][D] o, then [grid][2][heads][2] m, l
+    float* stats;
+    int64_t q_row, q_head;  // bytes
     int64_t table_ld, n_blocks;
-    int64_t cap;  // longest length
-    int kv_heads, G, chunks, splits, shift, window;
+    int cap;        // longest length
+    int batch, kv_heads, G, chunks, heads;  // heads: query heads of a chunk (the last one may have fewer)
+    int shift, lg_box, width, window;
     float scale, softcap;
 };
 
-template <int kType>
-__device__ __forceinline__ float load_el(const uint8_t* p, int i) {
-    if constexpr (kType == ZKV_DT_BF16) return bfbits2f(reinterpret_cast<const uint16_t*>(p)[i]);
-    else if constexpr (kType == ZKV_DT_F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
-    else return __half2float(__half(__nv_cvt_fp8_to_halfraw(p[i], __NV_E4M3)));
+template <int kQ, bool kF8, int D, int NT>
+struct Cfg {
+    static constexpr int kEl = kF8 ? 1 : 2;
+    static constexpr int kRow = D * kEl;                         // bytes of a token's row
+    static constexpr int kInner = kRow < 128 ? kRow : 128;       // swizzled span
+    static constexpr int kPieces = kRow / kInner;
+    static constexpr int kKv = kTile * kRow;                     // K (or V) of a stage
+    static constexpr int kHeadsMax = 8 * NT;
+    static constexpr int kQPitch = D * 2 + 16;
+    static constexpr int kQSlot = kHeadsMax * kQPitch;
+    static constexpr int kFixed = 1024 + 1024;                   // alignment; barriers, units, statistics
+    static constexpr int kStage = 2 * kKv + kQSlot + (int)sizeof(Unit);
+    static constexpr int kMl = 2 * kConsumers * kHeadsMax * 8;
+    static constexpr int kHalf = 232448 / 2 - 1024;              // shared memory of one of two CTAs on an SM
+    static constexpr int kWhole = 232448 - 1024;
+    static constexpr int kPerSm = (kHalf - kFixed - kMl) / kStage >= 3 ? 2 : 1;
+    static constexpr int kFit = ((kPerSm == 2 ? kHalf : kWhole) - kFixed - kMl) / kStage;
+    static constexpr int kStages = kFit < 8 ? kFit : 8;
+    static constexpr int kSmem = kStages * kStage + kFixed + kMl;
+    static constexpr bool kTwoParts = !(kF8 && kQ == ZKV_DT_BF16);  // the probability as hi + lo
+    static constexpr int kMTiles = D / 16;
+    // n-tiles of O that fit into a stage's K and V when the warps are joined
+    static constexpr int kJoinTiles = (2 * kKv) / (kConsumers * 8 * D * 4) < NT ? (2 * kKv) / (kConsumers * 8 * D * 4) : NT;
+    static_assert(kJoinTiles >= 1 && NT % kJoinTiles == 0, "join buffer");
+};
+
+// ------------------------------------------------------------ device helpers
+__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 
-template <int kType>
-__device__ __forceinline__ void store_el(void* p, int64_t i, float x) {
-    if constexpr (kType == ZKV_DT_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
-    else reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
-}
-
-__device__ __forceinline__ int request_len(const DecodeArgs& a, int b, bool report) {
-    const int n = a.lens[b];
-    if (n >= 0 && n <= a.cap) return n;
-    if (report) raise_status(a.status, ZKV_ERR_RANGE);
-    return n < 0 ? 0 : (int)a.cap;
-}
-
-template <int kQ, int kPool, int D>
-__global__ void __launch_bounds__(kDecodeWarps * 32) pool_decode_kernel(const __grid_constant__ DecodeArgs a) {
-    constexpr int E = D / 32;
-    __shared__ float s_o[kDecodeWarps][kHeads][D];
-    __shared__ float s_ml[kDecodeWarps][kHeads][2];
-    const int row = blockIdx.x, split = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c = row % a.chunks, h = row / a.chunks % a.kv_heads, b = row / (a.chunks * a.kv_heads);
-    const int len = request_len(a, b, split == 0 && threadIdx.x == 0);
-    const int lo = a.window > 0 && len > a.window ? len - a.window : 0;
-    const int t0 = max(lo, split * kSplit), t1 = min((int64_t)len, (int64_t)(split + 1) * kSplit);
-    float* part = a.parts + ((int64_t)row * a.splits + split) * kHeads * (D + 2);
-    const int n_heads = min(kHeads, a.G - c * kHeads);
-    float q[kHeads][E], o[kHeads][E], m[kHeads], l[kHeads];
-    for (int g = 0; g < kHeads; ++g) {
-        m[g] = -INFINITY;
-        l[g] = 0.f;
-        for (int e = 0; e < E; ++e) {
-            o[g][e] = 0.f;
-            q[g][e] = g < n_heads ? load_el<kQ>(a.q + b * a.q_row + (int64_t)(h * a.G + c * kHeads + g) * a.q_head,
-                                                lane + 32 * e)
-                                  : 0.f;
+// Wait for a phase, at most kWaitNs; false and ZKV_ERR_TIMEOUT on expiry.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int32_t* status) {
+    if (mbar_try(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try(bar, parity)) {
+        if (globaltimer_ns() - t0 > kWaitNs) {
+            raise_status(status, ZKV_ERR_TIMEOUT);
+            return false;
         }
     }
-    const float ks = a.k_scale ? a.k_scale[h] : 1.f, vs = a.v_scale ? a.v_scale[h] : 1.f;
-    for (int t = t0 + warp; t < t1; t += kDecodeWarps) {
-        const int id = a.table[b * a.table_ld + (t >> a.shift)];
-        if (id < 0 || id >= a.n_blocks) {
-            if (lane == 0) raise_status(a.status, ZKV_ERR_RANGE);
-            continue;
+    return true;
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int token, int head, int block,
+                                            uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(token), "r"(0), "r"(head), "r"(block), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t x) {
+    uint32_t y;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"(x));
+    return y;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// D(16x8 f32) += A(16x16, row) * B(16x8, col), both bf16 or both fp16
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (kBf16) {
+        mma_bf16_16816(d, a[0], a[1], a[2], a[3], b0, b1);
+    } else {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+            "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (kBf16) return pack_bf162(lo, hi);
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <bool kBf16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if constexpr (kBf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+__device__ __forceinline__ int request_len(const DecodeArgs& a, int n) {
+    return n < 0 ? 0 : (n > a.cap ? a.cap : n);
+}
+__device__ __forceinline__ int first_token(const DecodeArgs& a, int len) {
+    return a.window > 0 && len > a.window ? len - a.window : 0;
+}
+// 64-token tiles of a row; a row without tokens has one, which writes its zeros.
+__device__ __forceinline__ int row_tiles(const DecodeArgs& a, int len) {
+    const int t = (len + kTile - 1) / kTile - first_token(a, len) / kTile;
+    return t > 0 ? t : 1;
+}
+
+// ------------------------------------------------------------ consumers
+template <int kQ, bool kF8, int D, int NT>
+struct Row {
+    using C = Cfg<kQ, kF8, D, NT>;
+    static constexpr bool kMmaBf16 = kQ == ZKV_DT_BF16 && !kF8;
+    float m[NT][2], l[NT][2];   // log2 units; heads 2t, 2t+1 of n-tile (t = lane % 4); l: this lane's tokens
+    float f[NT][2];             // score factor of those heads, log2 units (natural under a soft cap)
+    float o[C::kMTiles][NT][4];
+    uint32_t q[D / 16][NT][2];  // B fragments of Q^T
+
+    __device__ __forceinline__ void init(const DecodeArgs& a, const uint8_t* qs, int n_heads, float k_scale) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const float base = a.scale * k_scale * (a.softcap > 0.f ? 1.f : 1.4426950408889634f);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int head = 8 * n + g;
+            const uint8_t* row = qs + head * C::kQPitch;
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) {
+                if constexpr (kF8) {  // k index 2t, 2t+1, 2t+8, 2t+9 <- dims 4t .. 4t+3, as the e4m3 rows are read
+                    const uint2 w = *reinterpret_cast<const uint2*>(row + 32 * s + 8 * t);
+                    q[s][n][0] = head < n_heads ? w.x : 0u;
+                    q[s][n][1] = head < n_heads ? w.y : 0u;
+                } else {
+                    q[s][n][0] = head < n_heads ? *reinterpret_cast<const uint32_t*>(row + 32 * s + 4 * t) : 0u;
+                    q[s][n][1] = head < n_heads ? *reinterpret_cast<const uint32_t*>(row + 32 * s + 16 + 4 * t) : 0u;
+                }
+            }
+            f[n][0] = f[n][1] = base;
+            if constexpr (kF8 && kQ == ZKV_DT_BF16) {
+                float mx = 0.f;
+#pragma unroll
+                for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 x = unpack2<true>(q[s][n][i]);
+                        mx = fmaxf(mx, fmaxf(fabsf(x.x), fabsf(x.y)));
+                    }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                int e = (int)(__float_as_uint(mx) >> 23) - 127;  // mx in [2^e, 2^(e+1))
+                e = mx > 0.f ? (e < -126 ? -126 : (e > 126 ? 126 : e)) : 0;
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 x = unpack2<true>(q[s][n][i]);
+                        q[s][n][i] = pack2<false>(x.x * down, x.y * down);
+                    }
+                f[n][0] *= __shfl_sync(0xffffffffu, up, 8 * t);
+                f[n][1] *= __shfl_sync(0xffffffffu, up, 8 * t + 4);
+            }
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
         }
-        const int at = t & ((1 << a.shift) - 1);
-        const uint8_t* kp = a.k + id * a.k_block + at * a.k_token + h * a.k_head;
-        const uint8_t* vp = a.v + id * a.v_block + at * a.v_token + h * a.v_head;
-        float k[E], v[E];
-        for (int e = 0; e < E; ++e) {
-            k[e] = load_el<kPool>(kp, lane + 32 * e);
-            v[e] = load_el<kPool>(vp, lane + 32 * e);
+#pragma unroll
+        for (int j = 0; j < C::kMTiles; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
+    }
+
+    // 16 tokens: K rows at ks, V rows at vs (this warp's first row of the
+    // swizzled box; `piece` bytes from one 128-byte piece to the next), of
+    // which tokens [v0, v1) count.
+    __device__ __forceinline__ void step(const DecodeArgs& a, uint32_t ks, uint32_t vs, uint32_t piece, int v0, int v1) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        constexpr int kPerPiece = C::kInner / 16;  // 16-byte chunks of a row in a piece
+        // address of chunk c of this lane's row: the swizzle permutes the chunks of a row by the row's number
+        const int tok_k = lane & 15, off_k = lane >> 4;
+        const int sw_k = C::kInner == 128 ? tok_k & 7 : (tok_k >> 1) & 3;
+        auto chunk = [&](uint32_t base, int tok, int sw, int c) {
+            return base + (uint32_t)(c / kPerPiece) * piece + tok * C::kInner + (((c % kPerPiece) ^ sw) << 4);
+        };
+        float x[NT][4];
+        {
+            float x2[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[n][e] = x2[n][e] = 0.f;
+            // two chains of products, so that one does not wait for the other
+            if constexpr (kF8) {
+#pragma unroll
+                for (int s = 0; s < D / 16; s += 2) {
+                    uint32_t r[4];
+                    ldsm4(chunk(ks, tok_k, sw_k, s + off_k), r);
+                    const uint32_t a0[4] = {e4m3x2_to_f16x2((uint16_t)r[0]), e4m3x2_to_f16x2((uint16_t)r[1]),
+                                            e4m3x2_to_f16x2((uint16_t)(r[0] >> 16)), e4m3x2_to_f16x2((uint16_t)(r[1] >> 16))};
+                    const uint32_t a1[4] = {e4m3x2_to_f16x2((uint16_t)r[2]), e4m3x2_to_f16x2((uint16_t)r[3]),
+                                            e4m3x2_to_f16x2((uint16_t)(r[2] >> 16)), e4m3x2_to_f16x2((uint16_t)(r[3] >> 16))};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16816<false>(x[n], a0, q[s][n][0], q[s][n][1]);
+                        mma16816<false>(x2[n], a1, q[s + 1][n][0], q[s + 1][n][1]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < D / 16; s += 2) {
+                    uint32_t a0[4], a1[4];
+                    ldsm4(chunk(ks, tok_k, sw_k, 2 * s + off_k), a0);
+                    ldsm4(chunk(ks, tok_k, sw_k, 2 * s + 2 + off_k), a1);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16816<kMmaBf16>(x[n], a0, q[s][n][0], q[s][n][1]);
+                        mma16816<kMmaBf16>(x2[n], a1, q[s + 1][n][0], q[s + 1][n][1]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[n][e] += x2[n][e];
         }
-        for (int g = 0; g < kHeads; ++g) {
-            float x = 0.f;
-            for (int e = 0; e < E; ++e) x += q[g][e] * k[e];
-            for (int off = 16; off >= 1; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-            x *= a.scale * ks;
-            if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
-            if (x == -INFINITY) continue;
-            const float mn = fmaxf(m[g], x), f = m[g] == -INFINITY ? 0.f : expf(m[g] - mn), p = expf(x - mn);
-            l[g] = l[g] * f + p;
-            m[g] = mn;
-            for (int e = 0; e < E; ++e) o[g][e] = o[g][e] * f + p * v[e];
+        // x[n][0..3]: (token g, head 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
+        const bool in0 = g >= v0 && g < v1, in1 = g + 8 >= v0 && g + 8 < v1;
+        uint32_t hi[NT][2], lo[NT][2];
+        float alpha[NT][2];
+        bool moved = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float y[4], p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                y[e] = x[n][e] * f[n][e & 1];
+                if (a.softcap > 0.f) y[e] = a.softcap * 1.4426950408889634f * tanhf(y[e] / a.softcap);
+                if (!(e < 2 ? in0 : in1)) y[e] = -INFINITY;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float mx = fmaxf(y[c], y[c + 2]);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                mx = fmaxf(mx, m[n][c]);
+                const float ref = mx == -INFINITY ? 0.f : mx;  // nothing seen yet: no inf - inf
+                alpha[n][c] = exp2_fast(m[n][c] - ref);
+                moved |= mx != m[n][c];
+                m[n][c] = mx;
+                p[c] = exp2_fast(y[c] - ref);
+                p[c + 2] = exp2_fast(y[c + 2] - ref);
+                l[n][c] = l[n][c] * alpha[n][c] + (p[c] + p[c + 2]);
+            }
+            const uint32_t h0 = pack2<kMmaBf16>(p[0], p[1]), h1 = pack2<kMmaBf16>(p[2], p[3]);
+            hi[n][0] = transposed(h0);
+            hi[n][1] = transposed(h1);
+            if constexpr (C::kTwoParts) {
+                const float2 r0 = unpack2<kMmaBf16>(h0), r1 = unpack2<kMmaBf16>(h1);
+                lo[n][0] = transposed(pack2<kMmaBf16>(p[0] - r0.x, p[1] - r0.y));
+                lo[n][1] = transposed(pack2<kMmaBf16>(p[2] - r1.x, p[3] - r1.y));
+            }
+        }
+        if (__any_sync(0xffffffffu, moved)) {  // most tiles of a long row leave the maxima as they are
+#pragma unroll
+            for (int j = 0; j < C::kMTiles; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][n][e] *= alpha[n][e & 1];
+        }
+        if constexpr (kF8) {
+#pragma unroll
+            for (int j = 0; j < C::kMTiles; j += 2) {
+                uint32_t r[4];
+                ldsm4_t(chunk(vs, tok_k, sw_k, j + off_k), r);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = __byte_perm(r[i], 0, 0x3120);  // (dim 2g: tokens 2t, 2t+1), (dim 2g+1)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t v[4] = {e4m3x2_to_f16x2((uint16_t)r[2 * i]), e4m3x2_to_f16x2((uint16_t)(r[2 * i] >> 16)),
+                                           e4m3x2_to_f16x2((uint16_t)r[2 * i + 1]),
+                                           e4m3x2_to_f16x2((uint16_t)(r[2 * i + 1] >> 16))};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16816<false>(o[j + i][n], v, hi[n][0], hi[n][1]);
+                        if constexpr (C::kTwoParts) mma16816<false>(o[j + i][n], v, lo[n][0], lo[n][1]);
+                    }
+                }
+            }
+        } else {
+            const int tok_v = (lane & 7) + ((lane >> 4) << 3), off_v = (lane >> 3) & 1;
+            const int sw_v = tok_v & 7;
+#pragma unroll
+            for (int j = 0; j < C::kMTiles; ++j) {
+                uint32_t v[4];
+                ldsm4_t(chunk(vs, tok_v, sw_v, 2 * j + off_v), v);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma16816<kMmaBf16>(o[j][n], v, hi[n][0], hi[n][1]);
+                    if constexpr (C::kTwoParts) mma16816<kMmaBf16>(o[j][n], v, lo[n][0], lo[n][1]);
+                }
+            }
         }
     }
-    for (int g = 0; g < kHeads; ++g) {
-        for (int e = 0; e < E; ++e) s_o[warp][g][lane + 32 * e] = o[g][e] * vs;
-        if (lane == 0) {
-            s_ml[warp][g][0] = m[g];
-            s_ml[warp][g][1] = l[g];
+
+    // V rows of tokens outside [v0, v1) to zero: their probability is 0, but 0 times what an unwritten row may hold
+    // (NaN, infinities) is not.
+    __device__ __forceinline__ void clear_rows(uint8_t* vs, uint32_t piece, int v0, int v1) {
+        constexpr int kPer = C::kRow / 16;
+        for (int i = threadIdx.x & 31; i < 16 * kPer; i += 32) {
+            const int tok = i / kPer, c = i % kPer;
+            if (tok < v0 || tok >= v1)
+                *reinterpret_cast<uint4*>(vs + (c / (C::kInner / 16)) * piece + tok * C::kInner +
+                                          (c % (C::kInner / 16)) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+    }
+};
+
+template <int kQ>
+__device__ __forceinline__ void store4(void* out, int64_t i, float4 x) {
+    constexpr bool kBf16 = kQ == ZKV_DT_BF16;
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + i) =
+        make_uint2(pack2<kBf16>(x.x, x.y), pack2<kBf16>(x.z, x.w));
+}
+
+template <int kQ, bool kF8, int D, int NT>
+__global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
+    pool_decode_kernel(const __grid_constant__ DecodeArgs a) {
+    using C = Cfg<kQ, kF8, D, NT>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+    uint8_t* kv = smem;                                                  // [stages] K, V
+    uint8_t* qs = kv + C::kStages * 2 * C::kKv;                          // [stages] query heads, by row
+    Unit* units = reinterpret_cast<Unit*>(qs + C::kStages * C::kQSlot);  // [stages]
+    float2* ml = reinterpret_cast<float2*>(units + C::kStages);          // [2][warps][heads]
+    __shared__ uint64_t full[C::kStages], empty[C::kStages], epi;
+    __shared__ int64_t sh[32];
+    __shared__ int64_t s_at[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, kConsumers);
+        }
+        mbar_init(&epi, kConsumers);
+        mbar_fence_init();
+    }
+    grid_dep_wait();
+    grid_dep_launch_next();  // the join kernel may become resident; it waits for this grid
+    // ---- this CTA's range of units
+    const int rows = a.kv_heads * a.chunks;  // rows of a request
+    const int per = (a.batch + kThreads - 1) / kThreads;
+    const int b_lo = min(a.batch, tid * per), b_hi = min(a.batch, b_lo + per);
+    int64_t mine = 0;
+    for (int b = b_lo; b < b_hi; ++b) {
+        const int n = __ldcg(a.lens + b);
+        if (blockIdx.x == 0 && (n < 0 || n > a.cap)) raise_status(a.status, ZKV_ERR_RANGE);
+        mine += (int64_t)row_tiles(a, request_len(a, n)) * rows;
+    }
+    int64_t total;
+    const int64_t before = block_sum_before(mine, sh, &total);
+    const int64_t ctas = min((int64_t)gridDim.x, total);
+    const int64_t c = blockIdx.x;
+    const int64_t u0 = c < ctas ? total * c / ctas : total, u1 = c < ctas ? total * (c + 1) / ctas : total;
+    if (u0 >= before && u0 < before + mine) {
+        int64_t at = before;
+        for (int b = b_lo; b < b_hi; ++b) {
+            const int64_t n = (int64_t)row_tiles(a, request_len(a, __ldcg(a.lens + b))) * rows;
+            if (u0 < at + n) {
+                s_at[0] = b;
+                s_at[1] = u0 - at;
+                break;
+            }
+            at += n;
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < kHeads * D; i += blockDim.x) {
-        const int g = i / D, d = i % D;
-        float mm = -INFINITY, ll = 0.f, oo = 0.f;
-        for (int w = 0; w < kDecodeWarps; ++w) mm = fmaxf(mm, s_ml[w][g][0]);
-        for (int w = 0; w < kDecodeWarps; ++w) {
-            const float f = s_ml[w][g][0] == -INFINITY ? 0.f : expf(s_ml[w][g][0] - mm);
-            ll += f * s_ml[w][g][1];
-            oo += f == 0.f ? 0.f : f * s_o[w][g][d];
+    const int n_units = (int)(u1 - u0);
+    if (n_units == 0) {
+        if (tid == 0) a.joins[c] = make_int4(0, 0, 0, 0);
+        return;
+    }
+
+    if (warp == kConsumers) {
+        // ---------------------------------------------------- producer
+        int b = (int)s_at[0];
+        int len = request_len(a, __ldcg(a.lens + b));
+        int lo = first_token(a, len), tile_first = lo / kTile, tiles = row_tiles(a, len);
+        int hg = (int)(s_at[1] / tiles), tile = (int)(s_at[1] % tiles);
+        int64_t row_begin = u0 - tile;  // unit at which the row begins
+        int ids = -1, ids_next = -1, ids_b = -1, ids_at = 0;
+        int n_row = 0;                  // rows begun in this CTA
+        int4 join = make_int4(0, 0, 0, 0);
+        const int boxes = kTile >> a.lg_box, box_bytes = C::kRow << a.lg_box;
+        bool ok = true;
+        int done = 0;
+        for (; done < n_units; ++done) {
+            const int stage = done % C::kStages;
+            const bool first = done == 0 || tile == 0;
+            const bool last = tile == tiles - 1 || done == n_units - 1;
+            int part = -1;
+            if (row_begin < u0) part = 0;
+            else if (row_begin + tiles > u1) part = 1;
+            if (part == 1 && first) {
+                const int64_t end = row_begin + tiles;  // the CTA of unit end - 1 is the row's last
+                join = make_int4(b, hg, (int)((end * ctas - 1) / total - c) + 1, 0);
+            }
+            // ---- block ids of the tile: 32 entries of the table at a time, the next 32 on their way
+            const int tile0 = (tile_first + tile) * kTile;
+            const int entry = tile0 >> a.shift;
+            const int n_entries = (len + (1 << a.shift) - 1) >> a.shift;
+            if (ids_b != b || ids_at != (entry & ~31)) {
+                const int32_t* row = a.table + b * a.table_ld;
+                const int at = entry & ~31;
+                if (ids_b == b && at == ids_at + 32) ids = ids_next;
+                else ids = at + lane < n_entries ? __ldcg(row + at + lane) : -1;
+                ids_next = at + 32 + lane < n_entries ? __ldcg(row + at + 32 + lane) : -1;
+                ids_b = b;
+                ids_at = at;
+            }
+            const int id = __shfl_sync(0xffffffffu, ids, (entry - ids_at + lane) & 31);  // lane j: box j
+            const int tok = tile0 + (lane << a.lg_box);
+            const bool wanted = lane < boxes && tok < len && tok + (1 << a.lg_box) > lo;
+            const bool there = wanted && id >= 0 && id < a.n_blocks;
+            if (wanted && !there) raise_status(a.status, ZKV_ERR_RANGE);
+            const unsigned copy = __ballot_sync(0xffffffffu, there), bad = __ballot_sync(0xffffffffu, wanted && !there);
+            const int h = hg / a.chunks, chunk = hg - h * a.chunks;
+            const int n_heads = min(a.heads, a.G - chunk * a.heads);
+            if (first) ++n_row;
+            const int q_slot = (n_row - 1) % C::kStages;
+            if (done >= C::kStages) ok = wait_for(empty + stage, (uint32_t)((done / C::kStages - 1) & 1), a.status);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            if (lane == 0) {
+                Unit& x = units[stage];
+                x.b = b;
+                x.hg = hg;
+                x.tile0 = tile0;
+                x.lo = lo;
+                x.len = len;
+                x.flags = (first ? kFirst : 0) | (last ? kLast : 0);
+                x.part = part;
+                x.bad = (int)bad;
+                mbar_arrive_expect_tx(full + stage, (uint32_t)(__popc(copy) * 2 * box_bytes + (first ? n_heads * D * 2 : 0)));
+            }
+            __syncwarp();
+            if (there) {
+                const uint32_t dst = smem_u32(kv + stage * 2 * C::kKv) + lane * box_bytes;
+                const int at = tile0 & ((1 << a.shift) - 1);
+                const int in_block = a.shift > a.lg_box ? at : 0;  // a box is a whole block, or 64 tokens of one
+                tma_load_5d(dst, &a.tk, in_block, h, id, full + stage);
+                tma_load_5d(dst + C::kKv, &a.tv, in_block, h, id, full + stage);
+            }
+            if (first && lane >= 32 - C::kHeadsMax && lane - (32 - C::kHeadsMax) < n_heads) {
+                const int j = lane - (32 - C::kHeadsMax);
+                bulk_g2s(qs + q_slot * C::kQSlot + j * C::kQPitch,
+                         a.q + b * a.q_row + (int64_t)(h * a.G + chunk * a.heads + j) * a.q_head, D * 2, full + stage);
+            }
+            // ---- next unit
+            if (++tile == tiles) {
+                tile = 0;
+                row_begin += tiles;
+                if (++hg == rows) {
+                    hg = 0;
+                    if (++b < a.batch) {
+                        len = request_len(a, __ldcg(a.lens + b));
+                        lo = first_token(a, len);
+                        tile_first = lo / kTile;
+                        tiles = row_tiles(a, len);
+                    }
+                }
+            }
         }
-        part[g * (D + 2) + d] = oo;
-        if (d == 0) {
-            part[g * (D + 2) + D] = mm;
-            part[g * (D + 2) + D + 1] = ll;
+        if (lane == 0) a.joins[c] = join;
+        if (!ok)  // a consumer gave up: the copies on their way land in this CTA's memory, so wait for them
+            for (int i = max(0, done - C::kStages); i < done; ++i)
+                wait_for(full + i % C::kStages, (uint32_t)((i / C::kStages) & 1), a.status);
+        return;
+    }
+
+    // -------------------------------------------------------- consumers
+    Row<kQ, kF8, D, NT> row;
+    uint32_t epi_phase = 0;
+    int n_row = 0, n_heads = 0;
+    const int g = lane >> 2, t = lane & 3;
+    for (int i = 0; i < n_units; ++i) {
+        const int stage = i % C::kStages;
+        if (!__all_sync(0xffffffffu, wait_for(full + stage, (uint32_t)((i / C::kStages) & 1), a.status))) return;
+        const Unit x = units[stage];
+        uint8_t* const base = kv + stage * 2 * C::kKv;
+        const int h = x.hg / a.chunks, chunk = x.hg - h * a.chunks;
+        if (x.flags & kFirst) {
+            n_heads = min(a.heads, a.G - chunk * a.heads);
+            row.init(a, qs + (n_row % C::kStages) * C::kQSlot, n_heads, kF8 && a.k_scale ? __ldcg(a.k_scale + h) : 1.f);
+            ++n_row;
         }
+        // this warp's 16 tokens lie in one box (a box has 16, 32 or 64)
+        const int t0 = x.tile0 + 16 * warp;
+        const int v0 = max(x.lo - t0, 0), v1 = min(x.len - t0, 16);
+        const int box = (16 * warp) >> a.lg_box, in_box = 16 * warp - (box << a.lg_box);
+        if (v0 < v1 && !((x.bad >> box) & 1)) {
+            const uint32_t piece = (uint32_t)C::kInner << a.lg_box;
+            const uint32_t at = (uint32_t)((box << a.lg_box) * C::kRow + in_box * C::kInner);
+            if (v0 > 0 || v1 < 16) row.clear_rows(base + C::kKv + at, piece, v0, v1);
+            row.step(a, smem_u32(base) + at, smem_u32(base) + C::kKv + at, piece, v0, v1);
+            if (v0 > 0 || v1 < 16) proxy_fence();
+        }
+        if (!(x.flags & kLast)) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + stage);
+            continue;
+        }
+        // ---- the row's end: join the warps in the stage's K and V
+        float2* mine_ml = ml + (n_row & 1) * kConsumers * C::kHeadsMax;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float s = row.l[n][e];
+                s += __shfl_xor_sync(0xffffffffu, s, 4);
+                s += __shfl_xor_sync(0xffffffffu, s, 8);
+                s += __shfl_xor_sync(0xffffffffu, s, 16);
+                if (g == 0) mine_ml[warp * C::kHeadsMax + 8 * n + 2 * t + e] = make_float2(row.m[n][e], s);
+            }
+        auto meet = [&]() -> bool {  // the four warps, at most kWaitNs
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&epi);
+            const bool got = __all_sync(0xffffffffu, wait_for(&epi, epi_phase, a.status));
+            epi_phase ^= 1;
+            return got;
+        };
+        if (!meet()) return;  // statistics written, stage read by all
+        float* buf = reinterpret_cast<float*>(base);
+        const float v_scale = kF8 && a.v_scale ? __ldcg(a.v_scale + h) : 1.f;
+        const int64_t head0 = ((int64_t)x.b * a.kv_heads + h) * a.G + chunk * a.heads;
+        const int64_t slot = c * 2 + x.part;
+#pragma unroll
+        for (int r = 0; r < NT; r += C::kJoinTiles) {
+            if (r > 0 && !meet()) return;
+#pragma unroll
+            for (int n = 0; n < C::kJoinTiles; ++n) {
+                float fac[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < kConsumers; ++w)
+                        mx = fmaxf(mx, mine_ml[w * C::kHeadsMax + 8 * (r + n) + 2 * t + e].x);
+                    fac[e] = exp2_fast(row.m[r + n][e] - (mx == -INFINITY ? 0.f : mx));
+                }
+                // dims of a head are permuted by its pair's number, so that the 32 lanes meet 32 banks
+                float* p = buf + (warp * 8 * C::kJoinTiles + 8 * n + 2 * t) * D;
+#pragma unroll
+                for (int j = 0; j < C::kMTiles; ++j) {
+                    const float* o = row.o[j][r + n];
+                    if constexpr (kF8) {
+                        const int d = (16 * j + 2 * g) ^ (t << 3);
+                        *reinterpret_cast<float2*>(p + d) = make_float2(o[0] * fac[0], o[2] * fac[0]);
+                        *reinterpret_cast<float2*>(p + D + d) = make_float2(o[1] * fac[1], o[3] * fac[1]);
+                    } else {
+                        const int d = (16 * j + g) ^ (t << 3), d8 = (16 * j + g + 8) ^ (t << 3);
+                        p[d] = o[0] * fac[0];
+                        p[D + d] = o[1] * fac[1];
+                        p[d8] = o[2] * fac[0];
+                        p[D + d8] = o[3] * fac[1];
+                    }
+                }
+            }
+            if (!meet()) return;
+            for (int idx = tid; idx < 8 * C::kJoinTiles * (D / 4); idx += 32 * kConsumers) {
+                const int hl = idx / (D / 4), d = 4 * (idx % (D / 4)), head = 8 * r + hl;
+                if (head >= n_heads) continue;
+                float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < kConsumers; ++w) mx = fmaxf(mx, mine_ml[w * C::kHeadsMax + head].x);
+                const float ref = mx == -INFINITY ? 0.f : mx;
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kConsumers; ++w) {
+                    const float2 s = mine_ml[w * C::kHeadsMax + head];
+                    sum += s.y * exp2_fast(s.x - ref);
+                    const float4 y = *reinterpret_cast<const float4*>(buf + (w * 8 * C::kJoinTiles + hl) * D +
+                                                                      (d ^ (((hl >> 1) & 3) << 3)));
+                    o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+                }
+                if (x.part < 0) {
+                    const float inv = sum == 0.f ? 0.f : v_scale / sum;
+                    store4<kQ>(a.out, (head0 + head) * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+                    if (a.lse && d == 0) a.lse[head0 + head] = (mx + log2f(sum)) * 0.6931471805599453f;
+                } else {
+                    *reinterpret_cast<float4*>(a.parts + (slot * C::kHeadsMax + head) * D + d) = o;
+                    if (d == 0) *reinterpret_cast<float2*>(a.stats + (slot * C::kHeadsMax + head) * 2) = make_float2(mx, sum);
+                }
+            }
+        }
+        proxy_fence();  // the stage was written by these threads; the next copy into it is the async proxy's
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + stage);
     }
 }
 
+// ------------------------------------------------------------ joining split rows
+constexpr int kJoinThreads = 256;
+
+// One CTA per (CTA of the decode grid whose last row goes on in others, query
+// head): the row's parts, in CTA order: slot 1 of the first CTA, slot 0 of the
+// others.  A warp takes every eighth part with the dims over its lanes.
 template <int kQ, int D>
-__global__ void pool_join_kernel(const __grid_constant__ DecodeArgs a) {
-    const int row = blockIdx.x, g = blockIdx.y, d = threadIdx.x;
-    const int c = row % a.chunks, h = row / a.chunks % a.kv_heads, b = row / (a.chunks * a.kv_heads);
-    if (g >= a.G - c * kHeads) return;
-    const float* part = a.parts + (int64_t)row * a.splits * kHeads * (D + 2) + g * (D + 2);
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, part[(int64_t)s * kHeads * (D + 2) + D]);
-    for (int s = 0; s < a.splits; ++s) {
-        const float* p = part + (int64_t)s * kHeads * (D + 2);
-        const float f = p[D] == -INFINITY ? 0.f : expf(p[D] - m);
-        l += f * p[D + 1];
-        if (f != 0.f) o += f * p[d];
+__global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_constant__ DecodeArgs a, int heads_max) {
+    constexpr int kWarps = kJoinThreads / 32, E = D / 32;
+    __shared__ float s_w[kMaxGrid];
+    __shared__ float s_o[kWarps][D];
+    __shared__ float s_red[2][kWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int c = blockIdx.x, head = blockIdx.y;
+    grid_dep_wait();
+    const int4 join = __ldcg(a.joins + c);
+    const int n = join.z;
+    const int h = join.y / a.chunks, chunk = join.y - h * a.chunks;
+    if (n == 0 || head >= min(a.heads, a.G - chunk * a.heads)) return;
+    auto slot_of = [&](int i) { return ((int64_t)(c + i) * 2 + (i == 0 ? 1 : 0)) * heads_max + head; };
+    float mx = -INFINITY;
+    for (int i = tid; i < n; i += kJoinThreads) mx = fmaxf(mx, __ldcg(a.stats + slot_of(i) * 2));
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    if (lane == 0) s_red[0][warp] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_red[0][w]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f;
+    for (int i = tid; i < n; i += kJoinThreads) {
+        const float2 s = __ldcg(reinterpret_cast<const float2*>(a.stats + slot_of(i) * 2));
+        const float w = exp2_fast(s.x - ref);
+        s_w[i] = w;
+        sum += w * s.y;
     }
-    const int64_t head = (int64_t)b * a.kv_heads * a.G + h * a.G + c * kHeads + g;
-    store_el<kQ>(a.out, head * D + d, l > 0.f ? o / l : 0.f);
-    if (a.lse && d == 0) a.lse[head] = m + logf(l);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) s_red[1][warp] = sum;
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) sum += s_red[1][w];
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+    for (int i = warp; i < n; i += kWarps) {
+        const float* p = a.parts + slot_of(i) * D;
+        const float w = s_w[i];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            const float2 y = __ldcg(reinterpret_cast<const float2*>(p + 64 * (e / 2) + 2 * lane));
+            o[e] += w * y.x;
+            o[e + 1] += w * y.y;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+        *reinterpret_cast<float2*>(&s_o[warp][64 * (e / 2) + 2 * lane]) = make_float2(o[e], o[e + 1]);
+    __syncthreads();
+    const int64_t at = ((int64_t)join.x * a.kv_heads + h) * a.G + chunk * a.heads + head;
+    const float inv = sum == 0.f ? 0.f : (a.v_scale ? __ldcg(a.v_scale + h) : 1.f) / sum;
+    if (tid < D / 4) {
+        float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(&s_o[w][4 * tid]);
+            r.x += y.x, r.y += y.y, r.z += y.z, r.w += y.w;
+        }
+        store4<kQ>(a.out, at * D + 4 * tid, make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv));
+    }
+    if (tid == 0 && a.lse) a.lse[at] = (mx + log2f(sum)) * 0.6931471805599453f;
 }
 
-static int decode_splits(int64_t max_len) { return (int)std::max<int64_t>(1, (max_len + kSplit - 1) / kSplit); }
+// ------------------------------------------------------------ host side
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-template <int kQ, int kPool>
-static void launch_decode(const DecodeArgs& a, int rows, int D, cudaStream_t st) {
-    const dim3 g1(rows, a.splits), g2(rows, std::min(kHeads, a.G));
-    switch (D) {
-        case 64:
-            pool_decode_kernel<kQ, kPool, 64><<<g1, kDecodeWarps * 32, 0, st>>>(a);
-            pool_join_kernel<kQ, 64><<<g2, 64, 0, st>>>(a);
-            break;
-        case 128:
-            pool_decode_kernel<kQ, kPool, 128><<<g1, kDecodeWarps * 32, 0, st>>>(a);
-            pool_join_kernel<kQ, 128><<<g2, 128, 0, st>>>(a);
-            break;
-        default:
-            pool_decode_kernel<kQ, kPool, 256><<<g1, kDecodeWarps * 32, 0, st>>>(a);
-            pool_join_kernel<kQ, 256><<<g2, 256, 0, st>>>(a);
-            break;
-    }
+static EncodeTiled encode_fn() {
+    static EncodeTiled fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult qr;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &qr) ==
+                cudaSuccess &&
+            qr == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiled>(p);
+    });
+    return fn;
 }
+
+// [block][head][piece][token][bytes of a piece]; a box is one head's tokens of a block, at most 64
+static bool encode_pool(uint64_t* to, const zkv_pool* p, void* base, int64_t block, int64_t token, int64_t head) {
+    EncodeTiled fn = encode_fn();
+    if (!fn) return false;
+    const int el = element_bytes(p->dtype), row = p->head_dim * el, inner = std::min(row, 128);
+    const cuuint64_t dims[5] = {(cuuint64_t)(inner / el), (cuuint64_t)p->block_size, (cuuint64_t)(row / inner),
+                                (cuuint64_t)p->kv_heads, (cuuint64_t)p->n_blocks};
+    const cuuint64_t strides[4] = {(cuuint64_t)(token * el), (cuuint64_t)inner, (cuuint64_t)(head * el),
+                                   (cuuint64_t)(block * el)};
+    const cuuint32_t box[5] = {(cuuint32_t)(inner / el), (cuuint32_t)std::min(p->block_size, kTile),
+                               (cuuint32_t)(row / inner), 1, 1};
+    const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+    const CUtensorMapDataType type = p->dtype == ZKV_DT_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                     : p->dtype == ZKV_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                              : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    CUtensorMap map;
+    if (fn(&map, type, 5, base, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return false;
+    static_assert(sizeof(map) == 128, "tensor map");
+    std::memcpy(to, &map, sizeof(map));
+    return true;
+}
+
+static int sm_count() {
+    static int cached[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!cached[dev]) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+        cached[dev] = n;
+    }
+    return cached[dev];
+}
+
+// Query heads of a row: the G heads of a kv head in equal chunks of at most 16.
+struct Heads {
+    int chunks, heads, tiles;  // tiles: n-tiles of 8 heads
+};
+static Heads split_heads(int G) {
+    Heads h;
+    h.chunks = (G + 15) / 16;
+    h.heads = (G + h.chunks - 1) / h.chunks;
+    h.chunks = (G + h.heads - 1) / h.heads;  // no chunk without a head
+    h.tiles = h.heads <= 8 ? 1 : 2;
+    return h;
+}
+
+// Units of a call at most, cut at the largest grid.
+static int64_t grid_bound(int batch, int kv_heads, int chunks, int64_t max_len) {
+    const int64_t tiles = std::max<int64_t>(1, (max_len + kTile - 1) / kTile);
+    const int64_t rows = (int64_t)batch * kv_heads * chunks;
+    return rows >= kMaxGrid ? kMaxGrid : std::min<int64_t>(kMaxGrid, rows * tiles);
+}
+
+template <int kQ, bool kF8, int D, int NT>
+static int launch_decode(DecodeArgs& a, int64_t bound, cudaStream_t st) {
+    using C = Cfg<kQ, kF8, D, NT>;
+    const int grid = (int)std::min<int64_t>(bound, (int64_t)C::kPerSm * sm_count());
+    static int raised[64] = {};  // devices whose shared-memory limit of this kernel was raised
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ZKV_ERR_LAUNCH;
+    if (!raised[dev]) {
+        if (cudaFuncSetAttribute((const void*)pool_decode_kernel<kQ, kF8, D, NT>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+            return ZKV_ERR_LAUNCH;
+        raised[dev] = 1;
+    }
+    int rc = launch_pdl_kernel(pool_decode_kernel<kQ, kF8, D, NT>, dim3(grid), dim3(kThreads), C::kSmem, st, a);
+    if (rc == ZKV_OK)
+        rc = launch_pdl_kernel(pool_join_kernel<kQ, D>, dim3(grid, a.heads), dim3(kJoinThreads), 0, st, a, C::kHeadsMax);
+    return rc;
+}
+
+template <int kQ, bool kF8>
+static int launch_shape(DecodeArgs& a, int D, int tiles, int64_t bound, cudaStream_t st) {
+    if (tiles == 1) {
+        if (D == 64) return launch_decode<kQ, kF8, 64, 1>(a, bound, st);
+        if (D == 128) return launch_decode<kQ, kF8, 128, 1>(a, bound, st);
+        return launch_decode<kQ, kF8, 256, 1>(a, bound, st);
+    }
+    if (D == 64) return launch_decode<kQ, kF8, 64, 2>(a, bound, st);
+    if (D == 128) return launch_decode<kQ, kF8, 128, 2>(a, bound, st);
+    return launch_decode<kQ, kF8, 256, 2>(a, bound, st);
+}
+
+static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 }  // namespace pool
 }  // namespace zkv
@@ -184,14 +902,19 @@ using namespace zkv;
 
 extern "C" int zkv_pool_init(zkv_pool* p) {
     const int rc = pool::check_pool(p);
-    if (rc == ZKV_OK) std::memset(p->maps, 0, sizeof(p->maps));
-    return rc;
+    if (rc != ZKV_OK) return rc;
+    if (!pool::encode_pool(p->maps, p, p->k, p->k_block, p->k_token, p->k_head) ||
+        !pool::encode_pool(p->maps + 16, p, p->v, p->v_block, p->v_token, p->v_head))
+        return ZKV_ERR_LAUNCH;
+    return ZKV_OK;
 }
 
 extern "C" size_t zkv_pool_decode_ws_bytes(int batch, int q_heads, int kv_heads, int head_dim, int64_t max_len) {
     if (batch < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || head_dim < 1 || max_len < 0) return 0;
-    const int chunks = (q_heads / kv_heads + pool::kHeads - 1) / pool::kHeads;
-    return (size_t)batch * kv_heads * chunks * pool::decode_splits(max_len) * pool::kHeads * (head_dim + 2) * 4 + 256;
+    const pool::Heads h = pool::split_heads(q_heads / kv_heads);
+    const size_t grid = (size_t)pool::grid_bound(batch, kv_heads, h.chunks, max_len);
+    const size_t rows = grid * 2 * 8 * h.tiles;
+    return pool::up256(grid * sizeof(int4)) + pool::up256(rows * 8) + pool::up256(rows * head_dim * 4) + 256;
 }
 
 extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int dtype, const zkv_pool* p,
@@ -210,27 +933,30 @@ extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int
     if (!pool::aligned16(q) || q_row % 8 || q_head % 8 || !pool::aligned16(out)) return ZKV_ERR_ALIGN;
     if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return ZKV_ERR_ALIGN;
     const int64_t room = (int64_t)width * p->block_size;
-    const int64_t cap = std::min<int64_t>(max_len > 0 ? std::min(max_len, room) : room, INT32_MAX);
+    const int64_t cap = std::min<int64_t>(max_len > 0 ? std::min(max_len, room) : room, INT32_MAX - 2 * pool::kTile);
     if (ws_bytes < zkv_pool_decode_ws_bytes(batch, q_heads, p->kv_heads, p->head_dim, cap)) return ZKV_ERR_CAPACITY;
-    const int el = pool::element_bytes(p->dtype);
+    uint64_t any = 0;
+    for (uint64_t w : p->maps) any |= w;
+    if (!any) return ZKV_ERR_ARG;  // zkv_pool_init was not called
+    const pool::Heads hs = pool::split_heads(q_heads / p->kv_heads);
+    const int64_t bound = pool::grid_bound(batch, p->kv_heads, hs.chunks, cap);
     pool::DecodeArgs a;
-    a.q = (const uint8_t*)q, a.k = (const uint8_t*)p->k, a.v = (const uint8_t*)p->v;
+    std::memcpy(&a.tk, p->maps, sizeof(a.tk));
+    std::memcpy(&a.tv, p->maps + 16, sizeof(a.tv));
+    a.q = (const uint8_t*)q;
     a.k_scale = p->k_scale, a.v_scale = p->v_scale;
     a.lens = lens, a.table = block_table, a.out = out, a.lse = lse, a.status = status;
-    a.parts = (float*)workspace;
+    a.joins = (int4*)workspace;
+    a.stats = (float*)((uint8_t*)workspace + pool::up256(bound * sizeof(int4)));
+    a.parts = a.stats + pool::up256((size_t)bound * 16 * hs.tiles * 8) / 4;
     a.q_row = q_row * 2, a.q_head = q_head * 2;
-    a.k_block = p->k_block * el, a.k_token = p->k_token * el, a.k_head = p->k_head * el;
-    a.v_block = p->v_block * el, a.v_token = p->v_token * el, a.v_head = p->v_head * el;
-    a.table_ld = table_ld, a.n_blocks = p->n_blocks, a.cap = cap;
-    a.kv_heads = p->kv_heads, a.G = q_heads / p->kv_heads, a.chunks = (a.G + pool::kHeads - 1) / pool::kHeads;
-    a.splits = pool::decode_splits(cap), a.shift = pool::log2_of(p->block_size), a.window = window;
+    a.table_ld = table_ld, a.n_blocks = p->n_blocks, a.cap = (int)cap;
+    a.batch = batch, a.kv_heads = p->kv_heads, a.G = q_heads / p->kv_heads, a.chunks = hs.chunks, a.heads = hs.heads;
+    a.shift = pool::log2_of(p->block_size), a.lg_box = std::min(a.shift, 6), a.width = width, a.window = window;
     a.scale = scale, a.softcap = softcap;
-    if (a.splits > 65535) return ZKV_ERR_CAPACITY;
-    const int rows = batch * p->kv_heads * a.chunks;
     cudaStream_t st = (cudaStream_t)stream;
-    if (p->dtype == ZKV_DT_BF16) pool::launch_decode<ZKV_DT_BF16, ZKV_DT_BF16>(a, rows, p->head_dim, st);
-    else if (p->dtype == ZKV_DT_F16) pool::launch_decode<ZKV_DT_F16, ZKV_DT_F16>(a, rows, p->head_dim, st);
-    else if (dtype == ZKV_DT_BF16) pool::launch_decode<ZKV_DT_BF16, ZKV_DT_F8E4M3>(a, rows, p->head_dim, st);
-    else pool::launch_decode<ZKV_DT_F16, ZKV_DT_F8E4M3>(a, rows, p->head_dim, st);
-    return launch_status();
+    if (p->dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, false>(a, p->head_dim, hs.tiles, bound, st);
+    if (p->dtype == ZKV_DT_F16) return pool::launch_shape<ZKV_DT_F16, false>(a, p->head_dim, hs.tiles, bound, st);
+    if (dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, true>(a, p->head_dim, hs.tiles, bound, st);
+    return pool::launch_shape<ZKV_DT_F16, true>(a, p->head_dim, hs.tiles, bound, st);
 }
