@@ -22,13 +22,12 @@ constexpr int kMaxThreads = 1024;
 
 // The last b in [0, n) with start[b] <= i (start ascending, start[0] <= i).
 __device__ __forceinline__ int owner_of(const int32_t* start, int n, int i) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (start[mid] <= i) lo = mid;
-        else hi = mid;
+    int b = 0;
+    for (int step = n > 1 ? 1 << (31 - __clz(n - 1)) : 0; step > 0; step >>= 1) {
+        const int at = b + step;
+        if (at < n && start[at] <= i) b = at;
     }
-    return lo;
+    return b;
 }
 
 struct PlanArgs {
@@ -45,6 +44,7 @@ struct PlanArgs {
     int32_t* status;
     int64_t table_ld, n_blocks;
     int batch, shift, width, n_slots;
+    bool vectors;  // slots and positions are 16-byte aligned
 };
 
 __global__ void __launch_bounds__(kMaxThreads) pool_plan_kernel(const __grid_constant__ PlanArgs a) {
@@ -101,34 +101,73 @@ __global__ void __launch_bounds__(kMaxThreads) pool_plan_kernel(const __grid_con
             for (int b = tid; b <= a.batch; b += nt) a.cu_new[b] = s_cu[b];
         if (tid == 0) *a.n_free_out = (int)n_free - s_used;
     }
-    const int total = s_cu[a.batch];
-    for (int64_t i = (int64_t)rank * nt + tid; i < a.n_slots; i += (int64_t)ranks * nt) {
-        int64_t slot = -1;
-        int pos = -1;
-        if (i < total) {
-            const int b = owner_of(s_cu, a.batch, (int)i);
-            const int base = s_base[b];
-            if (base >= 0) {
-                const int p = s_len[b] + ((int)i - s_cu[b]);
-                const int have = (s_len[b] + S - 1) >> a.shift, j = p >> a.shift;
-                int32_t* entry = a.table + b * a.table_ld + j;
-                int id;
-                if (j < have) {
-                    id = *entry;
-                } else {  // a new block: its first token is new, and that token's thread enters it
-                    id = a.free_blocks[n_free - 1 - base - (j - have)];
-                    if ((p & (S - 1)) == 0) *entry = id;
+    // Four tokens a turn: one search, the block ids' loads in flight together, 16-byte stores.
+    const uint32_t total = (uint32_t)s_cu[a.batch], n_slots = (uint32_t)a.n_slots;
+    for (uint32_t i0 = (uint32_t)(rank * nt + tid) * 4; i0 < n_slots; i0 += (uint32_t)(ranks * nt) * 4) {
+        int id[4] = {-1, -1, -1, -1}, pos[4] = {-1, -1, -1, -1};
+        if (i0 < total) {
+            int b = owner_of(s_cu, a.batch, (int)i0);
+            // a new block's id comes off the stack: the table's new entries are written, never read, here
+            auto id_at = [&](int r, int base, int have, int j) {
+                return j < have ? a.table[r * a.table_ld + j] : a.free_blocks[(int)n_free - 1 - base - (j - have)];
+            };
+            if (i0 + 3 < (uint32_t)s_cu[b + 1]) {  // one request, and so at most two blocks
+                const int base = s_base[b];
+                if (base >= 0) {
+                    const int have = (int)(((uint32_t)s_len[b] + S - 1) >> a.shift);
+                    const int p = s_len[b] + ((int)i0 - s_cu[b]), j0 = p >> a.shift, j1 = (p + 3) >> a.shift;
+                    const int first = id_at(b, base, have, j0), second = id_at(b, base, have, j1);
+                    // the thread of a block's first token enters it (that token is new, so the block is)
+                    const int edge = -p & (S - 1);
+                    if (edge < 4) a.table[b * a.table_ld + (edge ? j1 : j0)] = edge ? second : first;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        id[e] = (p + e) >> a.shift == j0 ? first : second;
+                        pos[e] = p + e;
+                    }
                 }
-                if (id >= 0 && id < a.n_blocks) {
-                    slot = ((int64_t)id << a.shift) + (p & (S - 1));
-                    pos = p;
-                } else {
-                    code = ZKV_ERR_RANGE;
+            } else {
+                int row[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    row[e] = -1;
+                    if (i0 + e >= total) continue;
+                    while ((int)i0 + e >= s_cu[b + 1]) ++b;
+                    if (s_base[b] < 0) continue;
+                    row[e] = b;
+                    pos[e] = s_len[b] + ((int)i0 + e - s_cu[b]);
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (row[e] >= 0)
+                        id[e] = id_at(row[e], s_base[row[e]], (int)(((uint32_t)s_len[row[e]] + S - 1) >> a.shift),
+                                      pos[e] >> a.shift);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (row[e] >= 0 && (pos[e] & (S - 1)) == 0) a.table[row[e] * a.table_ld + (pos[e] >> a.shift)] = id[e];
             }
         }
-        a.slots[i] = slot;
-        if (a.positions) a.positions[i] = pos;
+        int64_t slot[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool ok = pos[e] >= 0 && (uint32_t)id[e] < (uint32_t)a.n_blocks;
+            if (pos[e] >= 0 && !ok) code = ZKV_ERR_RANGE;
+            slot[e] = ok ? ((int64_t)id[e] << a.shift) + (pos[e] & (S - 1)) : -1;
+            pos[e] = ok ? pos[e] : -1;
+        }
+        if (a.vectors && i0 + 4 <= n_slots) {
+            longlong2* d = reinterpret_cast<longlong2*>(a.slots + i0);
+            d[0] = make_longlong2(slot[0], slot[1]);
+            d[1] = make_longlong2(slot[2], slot[3]);
+            if (a.positions) *reinterpret_cast<int4*>(a.positions + i0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i0 + e < n_slots) {
+                    a.slots[i0 + e] = slot[e];
+                    if (a.positions) a.positions[i0 + e] = pos[e];
+                }
+        }
     }
     if (code) raise_status(a.status, code);
 }
@@ -144,6 +183,7 @@ struct ReleaseArgs {
     int32_t* status;
     int64_t table_ld, n_blocks;
     int batch, shift, width;
+    bool vectors;  // free_blocks is 16-byte aligned
 };
 
 __global__ void __launch_bounds__(kMaxThreads) pool_release_kernel(const __grid_constant__ ReleaseArgs a) {
@@ -190,11 +230,31 @@ __global__ void __launch_bounds__(kMaxThreads) pool_release_kernel(const __grid_
         for (int b = tid; b < a.batch; b += nt) a.lens_out[b] = s_len[b];
         if (tid == 0) *a.n_free_out = (int)(n_free + start0);
     }
-    for (int64_t i = (int64_t)rank * nt + tid; i < start0; i += (int64_t)ranks * nt) {
-        const int b = owner_of(s_start, a.batch, (int)i);
-        const int id = a.table[b * a.table_ld + ((int)i - s_start[b])];
-        if (id < 0 || id >= a.n_blocks) code = ZKV_ERR_RANGE;
-        a.free_blocks[n_free + i] = id;
+    // Four places of the stack a turn, from a multiple of four on: one search, 16-byte stores.
+    const int64_t end = n_free + start0;
+    for (int64_t w0 = (n_free & ~3) + ((int64_t)rank * nt + tid) * 4; w0 < end; w0 += (int64_t)ranks * nt * 4) {
+        const int i0 = (int)(w0 - n_free);  // -3 .. : below 0 only in the first group
+        int b = owner_of(s_start, a.batch, i0 > 0 ? i0 : 0);
+        const int32_t* from[4];
+        int id[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = i0 + e >= 0 && w0 + e < end;
+            while (in && b + 1 < a.batch && i0 + e >= s_start[b + 1]) ++b;
+            from[e] = in ? a.table + b * a.table_ld + (i0 + e - s_start[b]) : nullptr;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) id[e] = from[e] ? *from[e] : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (from[e] && (uint32_t)id[e] >= (uint32_t)a.n_blocks) code = ZKV_ERR_RANGE;
+        if (a.vectors && from[0] && from[3]) {
+            *reinterpret_cast<int4*>(a.free_blocks + w0) = make_int4(id[0], id[1], id[2], id[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (from[e]) a.free_blocks[w0 + e] = id[e];
+        }
     }
     if (code) raise_status(a.status, code);
 }
@@ -224,17 +284,41 @@ __device__ __forceinline__ void to_floats(uint32_t w, float& lo, float& hi) {
     }
 }
 
-template <bool kBf16>
-__device__ __forceinline__ uint32_t to_e4m3x4(uint32_t w0, uint32_t w1, float scale) {
-    float a, b, c, d;
-    to_floats<kBf16>(w0, a, b);
-    to_floats<kBf16>(w1, c, d);
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(a, scale), __fdiv_rn(b, scale)), __NV_SATFINITE,
-                                                 __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(c, scale), __fdiv_rn(d, scale)), __NV_SATFINITE,
-                                                 __NV_E4M3);
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
 }
+
+// x / scale to e4m3 without a division in the common case: x times the
+// reciprocal shrunk and grown by 2^-21 encloses the quotient and its fp32
+// rounding (the products are off by 3 * 2^-24 at most), rounding is monotone,
+// so where both ends give one code the quotient has that code; else (a
+// quotient that close to the middle of two codes) it is divided.  The
+// division in every element made 8191 tokens of 8 x 128 take 13.2 us.
+struct Divisor {
+    float scale, low, high;
+    bool plain;  // the reciprocal is not a normal number: divide
+
+    __device__ __forceinline__ explicit Divisor(float s) {
+        const float r = 1.f / s;
+        scale = s;
+        low = r * (1.f - 4.76837158203125e-7f);
+        high = r * (1.f + 4.76837158203125e-7f);
+        plain = !(fabsf(s) > 1e-30f && fabsf(s) < 1e30f);
+    }
+
+    template <bool kBf16>
+    __device__ __forceinline__ uint32_t e4m3(uint32_t w0, uint32_t w1) const {
+        float a, b, c, d;
+        to_floats<kBf16>(w0, a, b);
+        to_floats<kBf16>(w1, c, d);
+        const uint32_t x = e4m3x4(a * low, b * low, c * low, d * low);
+        const uint32_t y = e4m3x4(a * high, b * high, c * high, d * high);
+        if (x == y && !plain) return x;
+        return e4m3x4(__fdiv_rn(a, scale), __fdiv_rn(b, scale), __fdiv_rn(c, scale), __fdiv_rn(d, scale));
+    }
+};
 
 constexpr int kWriteThreads = 256;
 constexpr int kWriteUnroll = 4;
@@ -282,22 +366,27 @@ __global__ void __launch_bounds__(kWriteThreads) pool_write_kernel(const __grid_
         if constexpr (kMode == 0) {
             out = x[u][0];
         } else {
-            const float f = sc ? __ldg(sc + head[u]) : 1.f;
-            out.x = to_e4m3x4<kMode == 1>(x[u][0].x, x[u][0].y, f);
-            out.y = to_e4m3x4<kMode == 1>(x[u][0].z, x[u][0].w, f);
-            out.z = to_e4m3x4<kMode == 1>(x[u][1].x, x[u][1].y, f);
-            out.w = to_e4m3x4<kMode == 1>(x[u][1].z, x[u][1].w, f);
+            const Divisor by(sc ? __ldg(sc + head[u]) : 1.f);
+            out.x = by.e4m3<kMode == 1>(x[u][0].x, x[u][0].y);
+            out.y = by.e4m3<kMode == 1>(x[u][0].z, x[u][0].w);
+            out.z = by.e4m3<kMode == 1>(x[u][1].x, x[u][1].y);
+            out.w = by.e4m3<kMode == 1>(x[u][1].z, x[u][1].w);
         }
         *reinterpret_cast<uint4*>(d) = out;
     }
     if (bad) raise_status(a.status, ZKV_ERR_RANGE);
 }
 
-// CTAs of the cluster and threads of a CTA for `work` items and `batch` requests.
-static void plan_shape(int batch, int64_t work, int* ctas, int* threads) {
-    const int64_t want = std::max<int64_t>(batch, work);
-    *ctas = want > 2 * kMaxThreads ? 8 : 1;
-    *threads = (int)std::min<int64_t>(kMaxThreads, (want + 31) / 32 * 32);
+// One cluster of CTAs for `work` tokens (or blocks) and `batch` requests.  A
+// CTA alone up to 2048 of both (no cluster to gather: 256 x 1 tokens 6.0 us, in
+// 8 CTAs 6.9), else 8 or, beyond 32768, the 16 that a GPC of this GPU holds.
+static int launch_cluster(const void* fn, int batch, int64_t work, size_t smem, cudaStream_t st, void** args) {
+    const int64_t want = std::max<int64_t>({batch, work, 1});
+    const int ctas = want <= 2 * kMaxThreads ? 1 : want <= 32768 ? 8 : 16;
+    const int threads = (int)std::min<int64_t>(kMaxThreads, (want + 31) / 32 * 32);
+    if (ctas == 16 && cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return ZKV_ERR_LAUNCH;
+    return launch_clustered(fn, ctas, threads, ctas, smem, st, args);
 }
 
 }  // namespace pool
@@ -312,17 +401,16 @@ extern "C" int zkv_pool_plan(const int32_t* lens, const int32_t* new_lens, int b
                              int32_t* status, void* stream) {
     if (batch < 0 || n_slots < 0 || width < 0 || table_ld < width || n_blocks < 0) return ZKV_ERR_ARG;
     if (!pool::block_size_ok(block_size)) return ZKV_ERR_UNSUPPORTED;
-    if (batch > pool::kMaxBatch || n_slots > INT32_MAX - 1 || n_blocks > INT32_MAX) return ZKV_ERR_CAPACITY;
+    if (batch > pool::kMaxBatch || n_slots > INT32_MAX / 2 || n_blocks > INT32_MAX) return ZKV_ERR_CAPACITY;
     if ((batch > 0 && (!lens || !lens_out || (!block_table && width > 0))) || (!free_blocks && n_blocks > 0) ||
         !n_free || !n_free_out || (!slots && n_slots > 0))
         return ZKV_ERR_ARG;
     pool::PlanArgs a{lens, new_lens, block_table, free_blocks, n_free, slots, positions, cu_new, lens_out, n_free_out,
-                     status, table_ld, n_blocks, batch, pool::log2_of(block_size), width, (int)n_slots};
-    int ctas, threads;
-    pool::plan_shape(std::max(batch, 1), n_slots, &ctas, &threads);
+                     status, table_ld, n_blocks, batch, pool::log2_of(block_size), width, (int)n_slots,
+                     pool::aligned16(slots) && pool::aligned16(positions)};
     void* args[] = {&a};
-    return launch_clustered((const void*)pool::pool_plan_kernel, ctas, threads, ctas,
-                            (size_t)(3 * batch + 1) * sizeof(int32_t), (cudaStream_t)stream, args);
+    return pool::launch_cluster((const void*)pool::pool_plan_kernel, batch, n_slots,
+                                (size_t)(3 * batch + 1) * sizeof(int32_t), (cudaStream_t)stream, args);
 }
 
 extern "C" int zkv_pool_release(const uint8_t* done, const int32_t* lens, int batch, int block_size,
@@ -336,12 +424,11 @@ extern "C" int zkv_pool_release(const uint8_t* done, const int32_t* lens, int ba
         (!free_blocks && n_blocks > 0) || !n_free || !n_free_out)
         return ZKV_ERR_ARG;
     pool::ReleaseArgs a{done, lens, block_table, free_blocks, n_free, lens_out, n_free_out, status, table_ld, n_blocks,
-                        batch, pool::log2_of(block_size), width};
-    int ctas, threads;
-    pool::plan_shape(std::max(batch, 1), std::min<int64_t>((int64_t)batch * width, n_blocks), &ctas, &threads);
+                        batch, pool::log2_of(block_size), width, pool::aligned16(free_blocks)};
     void* args[] = {&a};
-    return launch_clustered((const void*)pool::pool_release_kernel, ctas, threads, ctas,
-                            (size_t)(2 * batch) * sizeof(int32_t), (cudaStream_t)stream, args);
+    return pool::launch_cluster((const void*)pool::pool_release_kernel, batch,
+                                std::min<int64_t>((int64_t)batch * width, n_blocks),
+                                (size_t)(2 * batch) * sizeof(int32_t), (cudaStream_t)stream, args);
 }
 
 extern "C" int zkv_pool_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,

@@ -820,9 +820,15 @@ static bool encode_pool(uint64_t* to, const zkv_pool* p, void* base, int64_t blo
     const CUtensorMapDataType type = p->dtype == ZKV_DT_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                      : p->dtype == ZKV_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                               : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    // L2 fills no more than the bytes a box wants in a row: a 256-byte fill for a token-major pool's 128-byte rows reads
+    // the next head's row too, long before its CTA comes to it
+    const int64_t run = token * el == row ? 256 : row;
+    const CUtensorMapL2promotion fill = run >= 256   ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                                        : run >= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                                     : CU_TENSOR_MAP_L2_PROMOTION_L2_64B;
     CUtensorMap map;
     if (fn(&map, type, 5, base, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, fill,
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return false;
     static_assert(sizeof(map) == 128, "tensor map");
