@@ -7,23 +7,29 @@
 // operations a byte), so the bytes bound it.  The kernel is built to keep
 // reads in flight on every SM until the last tile:
 //
-//  * The work is the list of all (request, kv head, 64-token tile) units, in
+//  * The work is the list of all (request, kv head, tile of tokens) units, in
 //    that order, cut into equal ranges, one per CTA of a one-wave grid.  Each
 //    CTA finds its range from the lengths by itself (a sum over the requests),
 //    so uneven requests, one long request and many short ones are spread the
 //    same way and the host needs no length.  A row (request, kv head) that
 //    ends in another CTA than it began in leaves partials (m, l, o), which
-//    pool_join_kernel joins in CTA order.
+//    pool_join_kernel joins in CTA order.  Where no request can have more than
+//    kWholeTokens tokens the rows are cut whole and one launch does.
 //  * One producer warp per CTA walks the range: block ids from the table, one
 //    5-D TMA copy per block and tensor (dims | tokens | 128-byte pieces | head
 //    | block; any strides, so both memory orders), a ring of stages.  An id
 //    outside the pool is not copied.
-//  * Four consumer warps take 16 tokens of a tile each: S^T = K Q^T (tokens x
-//    heads) and O^T += V^T P^T (dims x heads) by mma.sync m16n8k16, so a
-//    group of up to 8 heads fills the 8 columns of one product.  tcgen05
-//    needs 64 or 128 rows of M per product and TMEM round trips for the
-//    softmax of a 16-token tile; at 4-16 heads and an HBM-bound tile it has
-//    nothing to win here.
+//  * Four consumer warps share a tile's tokens: S^T = K Q^T (tokens x heads)
+//    and O^T += V^T P^T (dims x heads) by mma.sync m16n8k16, so a group of up
+//    to 8 heads fills the 8 columns of one product, 16 heads two.  More heads
+//    are cut into chunks, whose CTAs walk the same range side by side, so that
+//    K and V come from HBM once and from L2 again.  tcgen05 needs 64 or 128
+//    rows of M per product and TMEM round trips for the softmax of a 16-token
+//    tile; at 4-16 heads and an HBM-bound tile it has nothing to win here.
+//  * A tile is 16 KiB of K (32 for 512-byte rows): what bounds a warp is the
+//    latency of its chain product - maximum - exponential - product, so rows of
+//    128 bytes get 32 tokens a warp and chain instead of 16, rows of 64 get 64
+//    (e4m3, 128 dims, 32 requests of 8192: 131 us with 16 tokens a chain).
 //  * A warp keeps its own running max, sum and O^T in registers through the
 //    row; the four are joined in the last tile's stage.
 //
@@ -46,22 +52,25 @@
 namespace zkv {
 namespace pool {
 
-constexpr int kTile = 64;                       // tokens of a unit
-constexpr int kConsumers = 4;                   // warps, 16 tokens of a tile each
+constexpr int kConsumers = 4;                   // warps that share a tile's tokens
 constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxGrid = 320;                   // CTAs that a workspace is sized for
+constexpr int kWholeTokens = ZKV_POOL_WHOLE_TOKENS;  // longest request of a call whose rows are not split
 constexpr uint64_t kWaitNs = 2000000000ull;     // limit of each wait inside a CTA
 
 // What a unit is, written by the producer beside its stage.
 struct Unit {
-    int b, hg;        // request; kv head * chunks + chunk of query heads
+    int b, h;         // request, kv head
     int tile0;        // first token
     int lo, len;      // tokens [lo, len) of the request are attended
-    int flags;        // kFirst, kLast of the row in this CTA
+    int flags;        // kFirst, kLast of the row in this CTA; kEnd: the CTA's last unit
     int part;         // -1: the row is this CTA's alone; else its partial slot
     int bad;          // boxes of the tile that are not in the pool
 };
-constexpr int kFirst = 1, kLast = 2;
+constexpr int kFirst = 1, kLast = 2, kEnd = 4;
+
+// Tokens of a tile, for a row of `bytes` bytes.
+__host__ __device__ constexpr int tile_tokens(int bytes) { return bytes >= 256 ? 64 : 64 * 256 / bytes; }
 
 struct DecodeArgs {
     CUtensorMap tk, tv;  // [block][head][128-byte piece][token][bytes]
@@ -73,14 +82,15 @@ struct DecodeArgs {
     void* out;
     float* lse;
     int32_t* status;
-    int4* joins;    // [grid] {b, hg, CTAs of the row, 0}: the row whose first part is this CTA's last one
-    float* parts;   // [grid][2][heads][D] o, then [grid][2][heads][2] m, l
-    float* stats;
+    float* parts;   // [grid][2][heads][D] o of a row's part: slot 0 began in an earlier CTA, slot 1 goes on in later ones
+    float* stats;   // [grid][2][heads][2] its m, l
     int64_t q_row, q_head;  // bytes
     int64_t table_ld, n_blocks;
     int cap;        // longest length
     int batch, kv_heads, G, chunks, heads;  // heads: query heads of a chunk (the last one may have fewer)
-    int shift, lg_box, width, window;
+    int groups;     // CTAs of a chunk; CTA x: chunk x % chunks of range x / chunks
+    int whole;      // rows are not split
+    int shift, lg_box, window;
     float scale, softcap;
 };
 
@@ -90,6 +100,8 @@ struct Cfg {
     static constexpr int kRow = D * kEl;                         // bytes of a token's row
     static constexpr int kInner = kRow < 128 ? kRow : 128;       // swizzled span
     static constexpr int kPieces = kRow / kInner;
+    static constexpr int kTile = tile_tokens(kRow);              // tokens of a unit
+    static constexpr int kSub = kTile / (16 * kConsumers);       // 16-token products of a warp in a tile
     static constexpr int kKv = kTile * kRow;                     // K (or V) of a stage
     static constexpr int kHeadsMax = 8 * NT;
     static constexpr int kQPitch = D * 2 + 16;
@@ -211,10 +223,46 @@ __device__ __forceinline__ int request_len(const DecodeArgs& a, int n) {
 __device__ __forceinline__ int first_token(const DecodeArgs& a, int len) {
     return a.window > 0 && len > a.window ? len - a.window : 0;
 }
-// 64-token tiles of a row; a row without tokens has one, which writes its zeros.
+// Tiles of a row; a row without tokens has one, which writes its zeros.
+template <int kTile>
 __device__ __forceinline__ int row_tiles(const DecodeArgs& a, int len) {
     const int t = (len + kTile - 1) / kTile - first_token(a, len) / kTile;
     return t > 0 ? t : 1;
+}
+
+// The list of units, seen by a block of kN threads: each thread holds the
+// requests [b_lo, b_hi), whose units are [before, before + mine).
+struct Units {
+    int b_lo, b_hi;
+    int64_t before, mine, total;
+};
+template <int kTile, int kN>
+__device__ __forceinline__ Units count_units(const DecodeArgs& a, int64_t* sh) {
+    Units u;
+    const int per = (a.batch + kN - 1) / kN;
+    u.b_lo = min(a.batch, (int)threadIdx.x * per);
+    u.b_hi = min(a.batch, u.b_lo + per);
+    u.mine = 0;
+    for (int b = u.b_lo; b < u.b_hi; ++b)
+        u.mine += (int64_t)row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + b))) * a.kv_heads;
+    u.before = block_sum_before(u.mine, sh, &u.total);
+    return u;
+}
+// The request of unit `u` and the unit's number in it, by the one thread that holds it.
+template <int kTile>
+__device__ __forceinline__ bool locate(const DecodeArgs& a, const Units& x, int64_t u, int& b, int64_t& off, int& tiles) {
+    if (u < x.before || u >= x.before + x.mine) return false;
+    off = u - x.before;
+    for (b = x.b_lo;; ++b) {
+        tiles = row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + b)));
+        const int64_t n = (int64_t)tiles * a.kv_heads;
+        if (off < n || b + 1 >= x.b_hi) return true;
+        off -= n;
+    }
+}
+// CTA (of `ctas`) that has unit u of `total`: ranges are [total c / ctas, total (c + 1) / ctas).
+__device__ __forceinline__ int64_t owner_cta(int64_t u, int64_t total, int64_t ctas) {
+    return ((u + 1) * ctas - 1) / total;
 }
 
 // ------------------------------------------------------------ consumers
@@ -281,95 +329,97 @@ struct Row {
                 for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
     }
 
-    // 16 tokens: K rows at ks, V rows at vs (this warp's first row of the
-    // swizzled box; `piece` bytes from one 128-byte piece to the next), of
-    // which tokens [v0, v1) count.
-    __device__ __forceinline__ void step(const DecodeArgs& a, uint32_t ks, uint32_t vs, uint32_t piece, int v0, int v1) {
-        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // The warp's tokens of a tile, 16 a product: product i's K and V rows begin
+    // at base + at[i] and base + kKv + at[i] (in a swizzled box, `piece` bytes
+    // from one 128-byte piece to the next); its tokens [v0[i], v1[i]) count.
+    __device__ __forceinline__ void step(const DecodeArgs& a, uint32_t base, const uint32_t (&at)[C::kSub], uint32_t piece,
+                                         const int (&v0)[C::kSub], const int (&v1)[C::kSub]) {
+        const int lane = threadIdx.x & 31, g = lane >> 2;
         constexpr int kPerPiece = C::kInner / 16;  // 16-byte chunks of a row in a piece
+        constexpr int kSub = C::kSub;
         // address of chunk c of this lane's row: the swizzle permutes the chunks of a row by the row's number
         const int tok_k = lane & 15, off_k = lane >> 4;
         const int sw_k = C::kInner == 128 ? tok_k & 7 : (tok_k >> 1) & 3;
-        auto chunk = [&](uint32_t base, int tok, int sw, int c) {
-            return base + (uint32_t)(c / kPerPiece) * piece + tok * C::kInner + (((c % kPerPiece) ^ sw) << 4);
+        auto chunk = [&](uint32_t from, int tok, int sw, int c) {
+            return from + (uint32_t)(c / kPerPiece) * piece + tok * C::kInner + (((c % kPerPiece) ^ sw) << 4);
         };
-        float x[NT][4];
-        {
-            float x2[NT][4];
+        float x[kSub][NT][4];
+        // two chains of products at least, so that one does not wait for the other
+        constexpr int kChains = kSub == 1 ? 2 : 1;
+        float x2[kChains == 2 ? NT : 1][4];
+#pragma unroll
+        for (int i = 0; i < kSub; ++i)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[n][e] = x2[n][e] = 0.f;
-            // two chains of products, so that one does not wait for the other
-            if constexpr (kF8) {
-#pragma unroll
-                for (int s = 0; s < D / 16; s += 2) {
-                    uint32_t r[4];
-                    ldsm4(chunk(ks, tok_k, sw_k, s + off_k), r);
-                    const uint32_t a0[4] = {e4m3x2_to_f16x2((uint16_t)r[0]), e4m3x2_to_f16x2((uint16_t)r[1]),
-                                            e4m3x2_to_f16x2((uint16_t)(r[0] >> 16)), e4m3x2_to_f16x2((uint16_t)(r[1] >> 16))};
-                    const uint32_t a1[4] = {e4m3x2_to_f16x2((uint16_t)r[2]), e4m3x2_to_f16x2((uint16_t)r[3]),
-                                            e4m3x2_to_f16x2((uint16_t)(r[2] >> 16)), e4m3x2_to_f16x2((uint16_t)(r[3] >> 16))};
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma16816<false>(x[n], a0, q[s][n][0], q[s][n][1]);
-                        mma16816<false>(x2[n], a1, q[s + 1][n][0], q[s + 1][n][1]);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    x[i][n][e] = 0.f;
+                    if (kChains == 2) x2[n][e] = 0.f;
                 }
-            } else {
 #pragma unroll
-                for (int s = 0; s < D / 16; s += 2) {
-                    uint32_t a0[4], a1[4];
-                    ldsm4(chunk(ks, tok_k, sw_k, 2 * s + off_k), a0);
-                    ldsm4(chunk(ks, tok_k, sw_k, 2 * s + 2 + off_k), a1);
+        for (int s = 0; s < D / 16; s += 2)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma16816<kMmaBf16>(x[n], a0, q[s][n][0], q[s][n][1]);
-                        mma16816<kMmaBf16>(x2[n], a1, q[s + 1][n][0], q[s + 1][n][1]);
-                    }
+            for (int i = 0; i < kSub; ++i) {
+                uint32_t a0[4], a1[4];
+                if constexpr (kF8) {
+                    uint32_t r[4];
+                    ldsm4(chunk(base + at[i], tok_k, sw_k, s + off_k), r);
+                    a0[0] = e4m3x2_to_f16x2((uint16_t)r[0]), a0[1] = e4m3x2_to_f16x2((uint16_t)r[1]);
+                    a0[2] = e4m3x2_to_f16x2((uint16_t)(r[0] >> 16)), a0[3] = e4m3x2_to_f16x2((uint16_t)(r[1] >> 16));
+                    a1[0] = e4m3x2_to_f16x2((uint16_t)r[2]), a1[1] = e4m3x2_to_f16x2((uint16_t)r[3]);
+                    a1[2] = e4m3x2_to_f16x2((uint16_t)(r[2] >> 16)), a1[3] = e4m3x2_to_f16x2((uint16_t)(r[3] >> 16));
+                } else {
+                    ldsm4(chunk(base + at[i], tok_k, sw_k, 2 * s + off_k), a0);
+                    ldsm4(chunk(base + at[i], tok_k, sw_k, 2 * s + 2 + off_k), a1);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma16816<kMmaBf16>(x[i][n], a0, q[s][n][0], q[s][n][1]);
+                    if constexpr (kChains == 2) mma16816<kMmaBf16>(x2[n], a1, q[s + 1][n][0], q[s + 1][n][1]);
+                    else mma16816<kMmaBf16>(x[i][n], a1, q[s + 1][n][0], q[s + 1][n][1]);
                 }
             }
+        if constexpr (kChains == 2) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[n][e] += x2[n][e];
+                for (int e = 0; e < 4; ++e) x[0][n][e] += x2[n][e];
         }
-        // x[n][0..3]: (token g, head 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
-        const bool in0 = g >= v0 && g < v1, in1 = g + 8 >= v0 && g + 8 < v1;
-        uint32_t hi[NT][2], lo[NT][2];
+        // x[i][n][0..3]: (token g, head 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
         float alpha[NT][2];
         bool moved = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float y[4], p[4];
+            float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                y[e] = x[n][e] * f[n][e & 1];
-                if (a.softcap > 0.f) y[e] = a.softcap * 1.4426950408889634f * tanhf(y[e] / a.softcap);
-                if (!(e < 2 ? in0 : in1)) y[e] = -INFINITY;
-            }
+            for (int i = 0; i < kSub; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float y = x[i][n][e] * f[n][e & 1];
+                    if (a.softcap > 0.f) y = a.softcap * 1.4426950408889634f * tanhf(y / a.softcap);
+                    const int tok = e < 2 ? g : g + 8;
+                    if (tok < v0[i] || tok >= v1[i]) y = -INFINITY;
+                    x[i][n][e] = y;
+                    mx[e & 1] = fmaxf(mx[e & 1], y);
+                }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float mx = fmaxf(y[c], y[c + 2]);
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                mx = fmaxf(mx, m[n][c]);
-                const float ref = mx == -INFINITY ? 0.f : mx;  // nothing seen yet: no inf - inf
+                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
+                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
+                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
+                mx[c] = fmaxf(mx[c], m[n][c]);
+                const float ref = mx[c] == -INFINITY ? 0.f : mx[c];  // nothing seen yet: no inf - inf
                 alpha[n][c] = exp2_fast(m[n][c] - ref);
-                moved |= mx != m[n][c];
-                m[n][c] = mx;
-                p[c] = exp2_fast(y[c] - ref);
-                p[c + 2] = exp2_fast(y[c + 2] - ref);
-                l[n][c] = l[n][c] * alpha[n][c] + (p[c] + p[c + 2]);
-            }
-            const uint32_t h0 = pack2<kMmaBf16>(p[0], p[1]), h1 = pack2<kMmaBf16>(p[2], p[3]);
-            hi[n][0] = transposed(h0);
-            hi[n][1] = transposed(h1);
-            if constexpr (C::kTwoParts) {
-                const float2 r0 = unpack2<kMmaBf16>(h0), r1 = unpack2<kMmaBf16>(h1);
-                lo[n][0] = transposed(pack2<kMmaBf16>(p[0] - r0.x, p[1] - r0.y));
-                lo[n][1] = transposed(pack2<kMmaBf16>(p[2] - r1.x, p[3] - r1.y));
+                moved |= mx[c] != m[n][c];
+                m[n][c] = mx[c];
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < kSub; ++i) {
+                    x[i][n][c] = exp2_fast(x[i][n][c] - ref);
+                    x[i][n][c + 2] = exp2_fast(x[i][n][c + 2] - ref);
+                    sum += x[i][n][c] + x[i][n][c + 2];
+                }
+                l[n][c] = l[n][c] * alpha[n][c] + sum;
             }
         }
         if (__any_sync(0xffffffffu, moved)) {  // most tiles of a long row leave the maxima as they are
@@ -380,36 +430,51 @@ struct Row {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[j][n][e] *= alpha[n][e & 1];
         }
-        if constexpr (kF8) {
 #pragma unroll
-            for (int j = 0; j < C::kMTiles; j += 2) {
-                uint32_t r[4];
-                ldsm4_t(chunk(vs, tok_k, sw_k, j + off_k), r);
+        for (int i = 0; i < kSub; ++i) {
+            uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = __byte_perm(r[i], 0, 0x3120);  // (dim 2g: tokens 2t, 2t+1), (dim 2g+1)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t v[4] = {e4m3x2_to_f16x2((uint16_t)r[2 * i]), e4m3x2_to_f16x2((uint16_t)(r[2 * i] >> 16)),
-                                           e4m3x2_to_f16x2((uint16_t)r[2 * i + 1]),
-                                           e4m3x2_to_f16x2((uint16_t)(r[2 * i + 1] >> 16))};
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma16816<false>(o[j + i][n], v, hi[n][0], hi[n][1]);
-                        if constexpr (C::kTwoParts) mma16816<false>(o[j + i][n], v, lo[n][0], lo[n][1]);
+                for (int r = 0; r < 2; ++r) {
+                    const float p0 = x[i][n][2 * r], p1 = x[i][n][2 * r + 1];
+                    const uint32_t w = pack2<kMmaBf16>(p0, p1);
+                    hi[n][r] = transposed(w);
+                    if constexpr (C::kTwoParts) {
+                        const float2 back = unpack2<kMmaBf16>(w);
+                        lo[n][r] = transposed(pack2<kMmaBf16>(p0 - back.x, p1 - back.y));
                     }
                 }
-            }
-        } else {
-            const int tok_v = (lane & 7) + ((lane >> 4) << 3), off_v = (lane >> 3) & 1;
-            const int sw_v = tok_v & 7;
+            const uint32_t vs = base + C::kKv + at[i];
+            if constexpr (kF8) {
 #pragma unroll
-            for (int j = 0; j < C::kMTiles; ++j) {
-                uint32_t v[4];
-                ldsm4_t(chunk(vs, tok_v, sw_v, 2 * j + off_v), v);
+                for (int j = 0; j < C::kMTiles; j += 2) {
+                    uint32_t r[4];
+                    ldsm4_t(chunk(vs, tok_k, sw_k, j + off_k), r);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    mma16816<kMmaBf16>(o[j][n], v, hi[n][0], hi[n][1]);
-                    if constexpr (C::kTwoParts) mma16816<kMmaBf16>(o[j][n], v, lo[n][0], lo[n][1]);
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t w0 = __byte_perm(r[2 * k], 0, 0x3120);  // (dim 2g: tokens 2t, 2t+1), (dim 2g+1)
+                        const uint32_t w1 = __byte_perm(r[2 * k + 1], 0, 0x3120);
+                        const uint32_t v[4] = {e4m3x2_to_f16x2((uint16_t)w0), e4m3x2_to_f16x2((uint16_t)(w0 >> 16)),
+                                               e4m3x2_to_f16x2((uint16_t)w1), e4m3x2_to_f16x2((uint16_t)(w1 >> 16))};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma16816<false>(o[j + k][n], v, hi[n][0], hi[n][1]);
+                            if constexpr (C::kTwoParts) mma16816<false>(o[j + k][n], v, lo[n][0], lo[n][1]);
+                        }
+                    }
+                }
+            } else {
+                const int tok_v = (lane & 7) + ((lane >> 4) << 3), off_v = (lane >> 3) & 1, sw_v = tok_v & 7;
+#pragma unroll
+                for (int j = 0; j < C::kMTiles; ++j) {
+                    uint32_t v[4];
+                    ldsm4_t(chunk(vs, tok_v, sw_v, 2 * j + off_v), v);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16816<kMmaBf16>(o[j][n], v, hi[n][0], hi[n][1]);
+                        if constexpr (C::kTwoParts) mma16816<kMmaBf16>(o[j][n], v, lo[n][0], lo[n][1]);
+                    }
                 }
             }
         }
@@ -448,7 +513,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     float2* ml = reinterpret_cast<float2*>(units + C::kStages);          // [2][warps][heads]
     __shared__ uint64_t full[C::kStages], empty[C::kStages], epi;
     __shared__ int64_t sh[32];
-    __shared__ int64_t s_at[2];
+    __shared__ int64_t s_off;
+    __shared__ int s_b;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < C::kStages; ++i) {
@@ -458,72 +524,69 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         mbar_init(&epi, kConsumers);
         mbar_fence_init();
     }
+    const int chunk = blockIdx.x % a.chunks;
+    const int64_t c = blockIdx.x / a.chunks;
+    const int n_heads = min(a.heads, a.G - chunk * a.heads);
     grid_dep_wait();
     grid_dep_launch_next();  // the join kernel may become resident; it waits for this grid
-    // ---- this CTA's range of units
-    const int rows = a.kv_heads * a.chunks;  // rows of a request
-    const int per = (a.batch + kThreads - 1) / kThreads;
-    const int b_lo = min(a.batch, tid * per), b_hi = min(a.batch, b_lo + per);
-    int64_t mine = 0;
-    for (int b = b_lo; b < b_hi; ++b) {
-        const int n = __ldcg(a.lens + b);
-        if (blockIdx.x == 0 && (n < 0 || n > a.cap)) raise_status(a.status, ZKV_ERR_RANGE);
-        mine += (int64_t)row_tiles(a, request_len(a, n)) * rows;
-    }
-    int64_t total;
-    const int64_t before = block_sum_before(mine, sh, &total);
-    const int64_t ctas = min((int64_t)gridDim.x, total);
-    const int64_t c = blockIdx.x;
-    const int64_t u0 = c < ctas ? total * c / ctas : total, u1 = c < ctas ? total * (c + 1) / ctas : total;
-    if (u0 >= before && u0 < before + mine) {
-        int64_t at = before;
-        for (int b = b_lo; b < b_hi; ++b) {
-            const int64_t n = (int64_t)row_tiles(a, request_len(a, __ldcg(a.lens + b))) * rows;
-            if (u0 < at + n) {
-                s_at[0] = b;
-                s_at[1] = u0 - at;
-                break;
-            }
-            at += n;
+    // ---- this CTA's range [u0, u1): of units, or of rows where those are not split
+    int64_t u0, u1;
+    if (a.whole) {
+        const int64_t rows = (int64_t)a.batch * a.kv_heads;
+        u0 = rows * c / a.groups;
+        u1 = rows * (c + 1) / a.groups;
+        __syncthreads();
+        if (u0 == u1) return;
+    } else {
+        const Units x = count_units<C::kTile, kThreads>(a, sh);
+        const int64_t ctas = min((int64_t)a.groups, x.total);
+        if (c >= ctas) return;
+        u0 = x.total * c / ctas;
+        u1 = x.total * (c + 1) / ctas;
+        int b, tiles;
+        int64_t off;
+        if (locate<C::kTile>(a, x, u0, b, off, tiles)) {
+            s_b = b;
+            s_off = off;
         }
-    }
-    __syncthreads();
-    const int n_units = (int)(u1 - u0);
-    if (n_units == 0) {
-        if (tid == 0) a.joins[c] = make_int4(0, 0, 0, 0);
-        return;
+        __syncthreads();
     }
 
     if (warp == kConsumers) {
         // ---------------------------------------------------- producer
-        int b = (int)s_at[0];
-        int len = request_len(a, __ldcg(a.lens + b));
-        int lo = first_token(a, len), tile_first = lo / kTile, tiles = row_tiles(a, len);
-        int hg = (int)(s_at[1] / tiles), tile = (int)(s_at[1] % tiles);
-        int64_t row_begin = u0 - tile;  // unit at which the row begins
+        int b = a.whole ? (int)(u0 / a.kv_heads) : s_b;
+        int next = __ldcg(a.lens + b);  // the length of the next request to begin, asked for one request ahead
+        int len, lo, tile_first, tiles;
+        auto begin_request = [&]() {
+            if (next < 0 || next > a.cap) raise_status(a.status, ZKV_ERR_RANGE);
+            len = request_len(a, next);
+            lo = first_token(a, len);
+            tile_first = lo / C::kTile;
+            tiles = row_tiles<C::kTile>(a, len);
+            if (b + 1 < a.batch) next = __ldcg(a.lens + b + 1);
+        };
+        begin_request();
+        int h = a.whole ? (int)(u0 % a.kv_heads) : (int)(s_off / tiles);
+        int tile = a.whole ? 0 : (int)(s_off % tiles);
+        int64_t row_begin = u0 - tile;  // unit at which the row begins (its number, where rows are whole)
         int ids = -1, ids_next = -1, ids_b = -1, ids_at = 0;
         int n_row = 0;                  // rows begun in this CTA
-        int4 join = make_int4(0, 0, 0, 0);
-        const int boxes = kTile >> a.lg_box, box_bytes = C::kRow << a.lg_box;
-        bool ok = true;
+        const int boxes = C::kTile >> a.lg_box, box_bytes = C::kRow << a.lg_box;
+        bool ok = true, end = false;
         int done = 0;
-        for (; done < n_units; ++done) {
+        for (; !end; ++done) {
             const int stage = done % C::kStages;
             const bool first = done == 0 || tile == 0;
-            const bool last = tile == tiles - 1 || done == n_units - 1;
+            end = a.whole ? tile == tiles - 1 && row_begin + 1 == u1 : u0 + done + 1 == u1;
+            const bool last = end || tile == tiles - 1;
             int part = -1;
-            if (row_begin < u0) part = 0;
-            else if (row_begin + tiles > u1) part = 1;
-            if (part == 1 && first) {
-                const int64_t end = row_begin + tiles;  // the CTA of unit end - 1 is the row's last
-                join = make_int4(b, hg, (int)((end * ctas - 1) / total - c) + 1, 0);
-            }
+            if (!a.whole) part = row_begin < u0 ? 0 : row_begin + tiles > u1 ? 1 : -1;
             // ---- block ids of the tile: 32 entries of the table at a time, the next 32 on their way
-            const int tile0 = (tile_first + tile) * kTile;
+            const int tile0 = (tile_first + tile) * C::kTile;
             const int entry = tile0 >> a.shift;
-            const int n_entries = (len + (1 << a.shift) - 1) >> a.shift;
             if (ids_b != b || ids_at != (entry & ~31)) {
                 const int32_t* row = a.table + b * a.table_ld;
+                const int n_entries = (len + (1 << a.shift) - 1) >> a.shift;
                 const int at = entry & ~31;
                 if (ids_b == b && at == ids_at + 32) ids = ids_next;
                 else ids = at + lane < n_entries ? __ldcg(row + at + lane) : -1;
@@ -537,8 +600,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             const bool there = wanted && id >= 0 && id < a.n_blocks;
             if (wanted && !there) raise_status(a.status, ZKV_ERR_RANGE);
             const unsigned copy = __ballot_sync(0xffffffffu, there), bad = __ballot_sync(0xffffffffu, wanted && !there);
-            const int h = hg / a.chunks, chunk = hg - h * a.chunks;
-            const int n_heads = min(a.heads, a.G - chunk * a.heads);
             if (first) ++n_row;
             const int q_slot = (n_row - 1) % C::kStages;
             if (done >= C::kStages) ok = wait_for(empty + stage, (uint32_t)((done / C::kStages - 1) & 1), a.status);
@@ -546,11 +607,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             if (lane == 0) {
                 Unit& x = units[stage];
                 x.b = b;
-                x.hg = hg;
+                x.h = h;
                 x.tile0 = tile0;
                 x.lo = lo;
                 x.len = len;
-                x.flags = (first ? kFirst : 0) | (last ? kLast : 0);
+                x.flags = (first ? kFirst : 0) | (last ? kLast : 0) | (end ? kEnd : 0);
                 x.part = part;
                 x.bad = (int)bad;
                 mbar_arrive_expect_tx(full + stage, (uint32_t)(__popc(copy) * 2 * box_bytes + (first ? n_heads * D * 2 : 0)));
@@ -558,8 +619,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             __syncwarp();
             if (there) {
                 const uint32_t dst = smem_u32(kv + stage * 2 * C::kKv) + lane * box_bytes;
-                const int at = tile0 & ((1 << a.shift) - 1);
-                const int in_block = a.shift > a.lg_box ? at : 0;  // a box is a whole block, or 64 tokens of one
+                // a box is a whole block, or a tile's tokens of one
+                const int in_block = a.shift > a.lg_box ? tile0 & ((1 << a.shift) - 1) : 0;
                 tma_load_5d(dst, &a.tk, in_block, h, id, full + stage);
                 tma_load_5d(dst + C::kKv, &a.tv, in_block, h, id, full + stage);
             }
@@ -571,19 +632,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             // ---- next unit
             if (++tile == tiles) {
                 tile = 0;
-                row_begin += tiles;
-                if (++hg == rows) {
-                    hg = 0;
-                    if (++b < a.batch) {
-                        len = request_len(a, __ldcg(a.lens + b));
-                        lo = first_token(a, len);
-                        tile_first = lo / kTile;
-                        tiles = row_tiles(a, len);
-                    }
+                row_begin += a.whole ? 1 : tiles;
+                if (++h == a.kv_heads) {
+                    h = 0;
+                    if (++b < a.batch) begin_request();
                 }
             }
         }
-        if (lane == 0) a.joins[c] = join;
         if (!ok)  // a consumer gave up: the copies on their way land in this CTA's memory, so wait for them
             for (int i = max(0, done - C::kStages); i < done; ++i)
                 wait_for(full + i % C::kStages, (uint32_t)((i / C::kStages) & 1), a.status);
@@ -593,29 +648,40 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     // -------------------------------------------------------- consumers
     Row<kQ, kF8, D, NT> row;
     uint32_t epi_phase = 0;
-    int n_row = 0, n_heads = 0;
+    int n_row = 0;
     const int g = lane >> 2, t = lane & 3;
-    for (int i = 0; i < n_units; ++i) {
+    bool end = false;
+    for (int i = 0; !end; ++i) {
         const int stage = i % C::kStages;
         if (!__all_sync(0xffffffffu, wait_for(full + stage, (uint32_t)((i / C::kStages) & 1), a.status))) return;
         const Unit x = units[stage];
+        end = x.flags & kEnd;
         uint8_t* const base = kv + stage * 2 * C::kKv;
-        const int h = x.hg / a.chunks, chunk = x.hg - h * a.chunks;
         if (x.flags & kFirst) {
-            n_heads = min(a.heads, a.G - chunk * a.heads);
-            row.init(a, qs + (n_row % C::kStages) * C::kQSlot, n_heads, kF8 && a.k_scale ? __ldcg(a.k_scale + h) : 1.f);
+            row.init(a, qs + (n_row % C::kStages) * C::kQSlot, n_heads, kF8 && a.k_scale ? __ldcg(a.k_scale + x.h) : 1.f);
             ++n_row;
         }
-        // this warp's 16 tokens lie in one box (a box has 16, 32 or 64)
-        const int t0 = x.tile0 + 16 * warp;
-        const int v0 = max(x.lo - t0, 0), v1 = min(x.len - t0, 16);
-        const int box = (16 * warp) >> a.lg_box, in_box = 16 * warp - (box << a.lg_box);
-        if (v0 < v1 && !((x.bad >> box) & 1)) {
+        // 16 tokens lie in one box (a box has 16 or more)
+        uint32_t at[C::kSub];
+        int v0[C::kSub], v1[C::kSub];
+        bool any = false, partial = false;
+#pragma unroll
+        for (int k = 0; k < C::kSub; ++k) {
+            const int in_tile = 16 * (C::kSub * warp + k), box = in_tile >> a.lg_box;
+            at[k] = (uint32_t)((box << a.lg_box) * C::kRow + (in_tile - (box << a.lg_box)) * C::kInner);
+            v0[k] = max(x.lo - x.tile0 - in_tile, 0);
+            v1[k] = (x.bad >> box) & 1 ? 0 : min(x.len - x.tile0 - in_tile, 16);
+            any |= v0[k] < v1[k];
+            partial |= v0[k] > 0 || v1[k] < 16;
+        }
+        if (any) {
             const uint32_t piece = (uint32_t)C::kInner << a.lg_box;
-            const uint32_t at = (uint32_t)((box << a.lg_box) * C::kRow + in_box * C::kInner);
-            if (v0 > 0 || v1 < 16) row.clear_rows(base + C::kKv + at, piece, v0, v1);
-            row.step(a, smem_u32(base) + at, smem_u32(base) + C::kKv + at, piece, v0, v1);
-            if (v0 > 0 || v1 < 16) proxy_fence();
+            if (partial) {
+#pragma unroll
+                for (int k = 0; k < C::kSub; ++k) row.clear_rows(base + C::kKv + at[k], piece, v0[k], v1[k]);
+            }
+            row.step(a, smem_u32(base), at, piece, v0, v1);
+            if (partial) proxy_fence();
         }
         if (!(x.flags & kLast)) {
             __syncwarp();
@@ -643,9 +709,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         };
         if (!meet()) return;  // statistics written, stage read by all
         float* buf = reinterpret_cast<float*>(base);
-        const float v_scale = kF8 && a.v_scale ? __ldcg(a.v_scale + h) : 1.f;
-        const int64_t head0 = ((int64_t)x.b * a.kv_heads + h) * a.G + chunk * a.heads;
-        const int64_t slot = c * 2 + x.part;
+        const float v_scale = kF8 && a.v_scale ? __ldcg(a.v_scale + x.h) : 1.f;
+        const int64_t head0 = ((int64_t)x.b * a.kv_heads + x.h) * a.G + chunk * a.heads;
+        const int64_t slot = (int64_t)blockIdx.x * 2 + x.part;
 #pragma unroll
         for (int r = 0; r < NT; r += C::kJoinTiles) {
             if (r > 0 && !meet()) return;
@@ -714,72 +780,124 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
 // ------------------------------------------------------------ joining split rows
 constexpr int kJoinThreads = 256;
 
-// One CTA per (CTA of the decode grid whose last row goes on in others, query
-// head): the row's parts, in CTA order: slot 1 of the first CTA, slot 0 of the
-// others.  A warp takes every eighth part with the dims over its lanes.
-template <int kQ, int D>
-__global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_constant__ DecodeArgs a, int heads_max) {
-    constexpr int kWarps = kJoinThreads / 32, E = D / 32;
-    __shared__ float s_w[kMaxGrid];
+// The parts of a split row, in CTA order: slot 1 of its first CTA, slot 0 of
+// the others.  One block per (candidate row, chunk; query head of the chunk):
+// the candidates are the rows if there are no more of them than CTAs, else the
+// rows in which a CTA's range ends.  Which parts there are follows from the
+// lengths, so it is known before the decode grid is waited for; then a warp
+// takes every eighth part, eight loads in flight, with the dims over its lanes.
+template <int kQ, int D, int kTile>
+__global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_constant__ DecodeArgs a, int heads_max,
+                                                                 int by_row) {
+    constexpr int kWarps = kJoinThreads / 32, E = D / 32, kBatch = 8;
+    __shared__ int64_t sh[32];
     __shared__ float s_o[kWarps][D];
-    __shared__ float s_red[2][kWarps];
+    __shared__ float2 s_ml[kWarps];
+    __shared__ int64_t s_row[2];
+    __shared__ int s_bh[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int c = blockIdx.x, head = blockIdx.y;
-    grid_dep_wait();
-    const int4 join = __ldcg(a.joins + c);
-    const int n = join.z;
-    const int h = join.y / a.chunks, chunk = join.y - h * a.chunks;
-    if (n == 0 || head >= min(a.heads, a.G - chunk * a.heads)) return;
-    auto slot_of = [&](int i) { return ((int64_t)(c + i) * 2 + (i == 0 ? 1 : 0)) * heads_max + head; };
-    float mx = -INFINITY;
-    for (int i = tid; i < n; i += kJoinThreads) mx = fmaxf(mx, __ldcg(a.stats + slot_of(i) * 2));
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    if (lane == 0) s_red[0][warp] = mx;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_red[0][w]);
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f;
-    for (int i = tid; i < n; i += kJoinThreads) {
-        const float2 s = __ldcg(reinterpret_cast<const float2*>(a.stats + slot_of(i) * 2));
-        const float w = exp2_fast(s.x - ref);
-        s_w[i] = w;
-        sum += w * s.y;
+    const int chunk = blockIdx.x % a.chunks, cand = blockIdx.x / a.chunks, head = blockIdx.y;
+    // Every path waits for the decode grid before it ends: the next kernel on
+    // the stream waits for this one alone.
+    if (head >= min(a.heads, a.G - chunk * a.heads)) {
+        grid_dep_wait();
+        return;
     }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (lane == 0) s_red[1][warp] = sum;
-    __syncthreads();
-    sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += s_red[1][w];
-    float o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < n; i += kWarps) {
-        const float* p = a.parts + slot_of(i) * D;
-        const float w = s_w[i];
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            const float2 y = __ldcg(reinterpret_cast<const float2*>(p + 64 * (e / 2) + 2 * lane));
-            o[e] += w * y.x;
-            o[e + 1] += w * y.y;
+    const Units x = count_units<kTile, kJoinThreads>(a, sh);
+    const int64_t ctas = min((int64_t)a.groups, x.total);
+    if (by_row) {
+        const int b = cand / a.kv_heads;
+        if (b >= x.b_lo && b < x.b_hi) {
+            int64_t begin = x.before;
+            for (int i = x.b_lo; i < b; ++i)
+                begin += (int64_t)row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + i))) * a.kv_heads;
+            const int tiles = row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + b)));
+            s_bh[0] = b;
+            s_bh[1] = cand - b * a.kv_heads;
+            s_row[0] = begin + (int64_t)s_bh[1] * tiles;
+            s_row[1] = s_row[0] + tiles;
+        }
+    } else {
+        if (cand >= ctas) {
+            grid_dep_wait();
+            return;
+        }
+        const int64_t u = x.total * (cand + 1) / ctas - 1;
+        int b, tiles;
+        int64_t off;
+        if (locate<kTile>(a, x, u, b, off, tiles)) {
+            s_bh[0] = b;
+            s_bh[1] = (int)(off / tiles);
+            s_row[0] = u - off % tiles;
+            s_row[1] = s_row[0] + tiles;
         }
     }
-#pragma unroll
-    for (int e = 0; e < E; e += 2)
-        *reinterpret_cast<float2*>(&s_o[warp][64 * (e / 2) + 2 * lane]) = make_float2(o[e], o[e + 1]);
     __syncthreads();
-    const int64_t at = ((int64_t)join.x * a.kv_heads + h) * a.G + chunk * a.heads + head;
+    const int64_t c0 = owner_cta(s_row[0], x.total, ctas);
+    const int n = (int)(owner_cta(s_row[1] - 1, x.total, ctas) - c0) + 1;
+    const int b = s_bh[0], h = s_bh[1];
+    grid_dep_wait();
+    if (n == 1 || (!by_row && c0 != cand)) return;
+    float m = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int i0 = warp; i0 < n; i0 += kWarps * kBatch) {
+        float2 y[kBatch][E / 2], s[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int i = i0 + k * kWarps;
+            s[k] = make_float2(-INFINITY, 0.f);
+            if (i < n) {
+                const int64_t slot = (((c0 + i) * a.chunks + chunk) * 2 + (i == 0 ? 1 : 0)) * heads_max + head;
+                s[k] = __ldcg(reinterpret_cast<const float2*>(a.stats) + slot);
+#pragma unroll
+                for (int e = 0; e < E / 2; ++e)
+                    y[k][e] = __ldcg(reinterpret_cast<const float2*>(a.parts + slot * D) + 32 * e + lane);
+            }
+        }
+        float mx = m;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) mx = fmaxf(mx, s[k].x);
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        const float old = exp2_fast(m - ref);
+        l *= old;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= old;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            if (i0 + k * kWarps >= n) continue;
+            const float w = exp2_fast(s[k].x - ref);
+            l += w * s[k].y;
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) {
+                o[2 * e] += w * y[k][e].x;
+                o[2 * e + 1] += w * y[k][e].y;
+            }
+        }
+        m = mx;
+    }
+    if (lane == 0) s_ml[warp] = make_float2(m, l);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e)
+        *reinterpret_cast<float2*>(&s_o[warp][64 * e + 2 * lane]) = make_float2(o[2 * e], o[2 * e + 1]);
+    __syncthreads();
+    float mx = -INFINITY, sum = 0.f, f[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_ml[w].x);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        f[w] = exp2_fast(s_ml[w].x - ref);
+        sum += f[w] * s_ml[w].y;
+    }
+    const int64_t at = ((int64_t)b * a.kv_heads + h) * a.G + chunk * a.heads + head;
     const float inv = sum == 0.f ? 0.f : (a.v_scale ? __ldcg(a.v_scale + h) : 1.f) / sum;
     if (tid < D / 4) {
         float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float4 y = *reinterpret_cast<const float4*>(&s_o[w][4 * tid]);
-            r.x += y.x, r.y += y.y, r.z += y.z, r.w += y.w;
+            r.x += f[w] * y.x, r.y += f[w] * y.y, r.z += f[w] * y.z, r.w += f[w] * y.w;
         }
         store4<kQ>(a.out, at * D + 4 * tid, make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv));
     }
@@ -805,7 +923,12 @@ static EncodeTiled encode_fn() {
     return fn;
 }
 
-// [block][head][piece][token][bytes of a piece]; a box is one head's tokens of a block, at most 64
+// A box holds one head's tokens of a block, at most a tile's and 256.
+static int box_tokens(const zkv_pool* p) {
+    return std::min(p->block_size, tile_tokens(p->head_dim * element_bytes(p->dtype)));
+}
+
+// [block][head][piece][token][bytes of a piece]
 static bool encode_pool(uint64_t* to, const zkv_pool* p, void* base, int64_t block, int64_t token, int64_t head) {
     EncodeTiled fn = encode_fn();
     if (!fn) return false;
@@ -814,7 +937,7 @@ static bool encode_pool(uint64_t* to, const zkv_pool* p, void* base, int64_t blo
                                 (cuuint64_t)p->kv_heads, (cuuint64_t)p->n_blocks};
     const cuuint64_t strides[4] = {(cuuint64_t)(token * el), (cuuint64_t)inner, (cuuint64_t)(head * el),
                                    (cuuint64_t)(block * el)};
-    const cuuint32_t box[5] = {(cuuint32_t)(inner / el), (cuuint32_t)std::min(p->block_size, kTile),
+    const cuuint32_t box[5] = {(cuuint32_t)(inner / el), (cuuint32_t)box_tokens(p),
                                (cuuint32_t)(row / inner), 1, 1};
     const cuuint32_t es[5] = {1, 1, 1, 1, 1};
     const CUtensorMapDataType type = p->dtype == ZKV_DT_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -861,17 +984,16 @@ static Heads split_heads(int G) {
     return h;
 }
 
-// Units of a call at most, cut at the largest grid.
-static int64_t grid_bound(int batch, int kv_heads, int chunks, int64_t max_len) {
-    const int64_t tiles = std::max<int64_t>(1, (max_len + kTile - 1) / kTile);
-    const int64_t rows = (int64_t)batch * kv_heads * chunks;
-    return rows >= kMaxGrid ? kMaxGrid : std::min<int64_t>(kMaxGrid, rows * tiles);
+// CTAs of a chunk that a call can use: its units at most, and what the largest grid leaves a chunk.
+static int64_t most_groups(int batch, int kv_heads, int chunks, int64_t max_len, int tile) {
+    const int64_t tiles = std::max<int64_t>(1, (max_len + tile - 1) / tile);
+    const int64_t rows = (int64_t)batch * kv_heads, most = kMaxGrid / chunks;
+    return rows >= most ? most : std::min<int64_t>(most, rows * tiles);
 }
 
 template <int kQ, bool kF8, int D, int NT>
-static int launch_decode(DecodeArgs& a, int64_t bound, cudaStream_t st) {
+static int launch_decode(DecodeArgs& a, cudaStream_t st) {
     using C = Cfg<kQ, kF8, D, NT>;
-    const int grid = (int)std::min<int64_t>(bound, (int64_t)C::kPerSm * sm_count());
     static int raised[64] = {};  // devices whose shared-memory limit of this kernel was raised
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ZKV_ERR_LAUNCH;
@@ -881,22 +1003,30 @@ static int launch_decode(DecodeArgs& a, int64_t bound, cudaStream_t st) {
             return ZKV_ERR_LAUNCH;
         raised[dev] = 1;
     }
-    int rc = launch_pdl_kernel(pool_decode_kernel<kQ, kF8, D, NT>, dim3(grid), dim3(kThreads), C::kSmem, st, a);
-    if (rc == ZKV_OK)
-        rc = launch_pdl_kernel(pool_join_kernel<kQ, D>, dim3(grid, a.heads), dim3(kJoinThreads), 0, st, a, C::kHeadsMax);
+    const int64_t rows = (int64_t)a.batch * a.kv_heads;
+    const int64_t wave = std::max(1, C::kPerSm * sm_count() / a.chunks);
+    a.groups = (int)std::min(wave, most_groups(a.batch, a.kv_heads, a.chunks, a.whole ? 0 : a.cap, C::kTile));
+    int rc = launch_pdl_kernel(pool_decode_kernel<kQ, kF8, D, NT>, dim3(a.groups * a.chunks), dim3(kThreads), C::kSmem,
+                               st, a);
+    if (rc == ZKV_OK && !a.whole && a.groups > 1) {
+        const int by_row = rows <= a.groups;
+        const int cands = by_row ? (int)rows : a.groups;
+        rc = launch_pdl_kernel(pool_join_kernel<kQ, D, C::kTile>, dim3(cands * a.chunks, a.heads), dim3(kJoinThreads), 0,
+                               st, a, C::kHeadsMax, by_row);
+    }
     return rc;
 }
 
 template <int kQ, bool kF8>
-static int launch_shape(DecodeArgs& a, int D, int tiles, int64_t bound, cudaStream_t st) {
+static int launch_shape(DecodeArgs& a, int D, int tiles, cudaStream_t st) {
     if (tiles == 1) {
-        if (D == 64) return launch_decode<kQ, kF8, 64, 1>(a, bound, st);
-        if (D == 128) return launch_decode<kQ, kF8, 128, 1>(a, bound, st);
-        return launch_decode<kQ, kF8, 256, 1>(a, bound, st);
+        if (D == 64) return launch_decode<kQ, kF8, 64, 1>(a, st);
+        if (D == 128) return launch_decode<kQ, kF8, 128, 1>(a, st);
+        return launch_decode<kQ, kF8, 256, 1>(a, st);
     }
-    if (D == 64) return launch_decode<kQ, kF8, 64, 2>(a, bound, st);
-    if (D == 128) return launch_decode<kQ, kF8, 128, 2>(a, bound, st);
-    return launch_decode<kQ, kF8, 256, 2>(a, bound, st);
+    if (D == 64) return launch_decode<kQ, kF8, 64, 2>(a, st);
+    if (D == 128) return launch_decode<kQ, kF8, 128, 2>(a, st);
+    return launch_decode<kQ, kF8, 256, 2>(a, st);
 }
 
 static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -918,9 +1048,10 @@ extern "C" int zkv_pool_init(zkv_pool* p) {
 extern "C" size_t zkv_pool_decode_ws_bytes(int batch, int q_heads, int kv_heads, int head_dim, int64_t max_len) {
     if (batch < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || head_dim < 1 || max_len < 0) return 0;
     const pool::Heads h = pool::split_heads(q_heads / kv_heads);
-    const size_t grid = (size_t)pool::grid_bound(batch, kv_heads, h.chunks, max_len);
+    if (h.chunks > pool::kMaxGrid) return 0;
+    const size_t grid = (size_t)pool::most_groups(batch, kv_heads, h.chunks, max_len, 64) * h.chunks;
     const size_t rows = grid * 2 * 8 * h.tiles;
-    return pool::up256(grid * sizeof(int4)) + pool::up256(rows * 8) + pool::up256(rows * head_dim * 4) + 256;
+    return pool::up256(rows * 8) + pool::up256(rows * head_dim * 4) + 256;
 }
 
 extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int dtype, const zkv_pool* p,
@@ -935,34 +1066,37 @@ extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int
         return ZKV_ERR_ARG;
     if (p->dtype != ZKV_DT_F8E4M3 && p->dtype != dtype) return ZKV_ERR_ARG;
     if (batch == 0) return ZKV_OK;
-    if (!q || !lens || !out || !workspace || (!block_table && width > 0)) return ZKV_ERR_ARG;
+    if (!q || !lens || !out || (!block_table && width > 0)) return ZKV_ERR_ARG;
     if (!pool::aligned16(q) || q_row % 8 || q_head % 8 || !pool::aligned16(out)) return ZKV_ERR_ALIGN;
     if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return ZKV_ERR_ALIGN;
     const int64_t room = (int64_t)width * p->block_size;
-    const int64_t cap = std::min<int64_t>(max_len > 0 ? std::min(max_len, room) : room, INT32_MAX - 2 * pool::kTile);
-    if (ws_bytes < zkv_pool_decode_ws_bytes(batch, q_heads, p->kv_heads, p->head_dim, cap)) return ZKV_ERR_CAPACITY;
+    const int64_t cap = std::min<int64_t>(max_len > 0 ? std::min(max_len, room) : room, INT32_MAX - 512);
+    const bool whole = cap <= pool::kWholeTokens;
+    if (!workspace && !whole) return ZKV_ERR_ARG;
+    if (workspace && ws_bytes < zkv_pool_decode_ws_bytes(batch, q_heads, p->kv_heads, p->head_dim, cap)) return ZKV_ERR_CAPACITY;
     uint64_t any = 0;
     for (uint64_t w : p->maps) any |= w;
     if (!any) return ZKV_ERR_ARG;  // zkv_pool_init was not called
     const pool::Heads hs = pool::split_heads(q_heads / p->kv_heads);
-    const int64_t bound = pool::grid_bound(batch, p->kv_heads, hs.chunks, cap);
+    if (hs.chunks > pool::kMaxGrid) return ZKV_ERR_CAPACITY;
     pool::DecodeArgs a;
     std::memcpy(&a.tk, p->maps, sizeof(a.tk));
     std::memcpy(&a.tv, p->maps + 16, sizeof(a.tv));
     a.q = (const uint8_t*)q;
     a.k_scale = p->k_scale, a.v_scale = p->v_scale;
     a.lens = lens, a.table = block_table, a.out = out, a.lse = lse, a.status = status;
-    a.joins = (int4*)workspace;
-    a.stats = (float*)((uint8_t*)workspace + pool::up256(bound * sizeof(int4)));
-    a.parts = a.stats + pool::up256((size_t)bound * 16 * hs.tiles * 8) / 4;
+    a.stats = (float*)workspace;
+    const size_t rows = (size_t)pool::most_groups(batch, p->kv_heads, hs.chunks, cap, 64) * hs.chunks * 2 * 8 * hs.tiles;
+    a.parts = a.stats + pool::up256(rows * 8) / 4;
+    a.whole = whole, a.groups = 0;
     a.q_row = q_row * 2, a.q_head = q_head * 2;
     a.table_ld = table_ld, a.n_blocks = p->n_blocks, a.cap = (int)cap;
     a.batch = batch, a.kv_heads = p->kv_heads, a.G = q_heads / p->kv_heads, a.chunks = hs.chunks, a.heads = hs.heads;
-    a.shift = pool::log2_of(p->block_size), a.lg_box = std::min(a.shift, 6), a.width = width, a.window = window;
+    a.shift = pool::log2_of(p->block_size), a.lg_box = pool::log2_of(pool::box_tokens(p)), a.window = window;
     a.scale = scale, a.softcap = softcap;
     cudaStream_t st = (cudaStream_t)stream;
-    if (p->dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, false>(a, p->head_dim, hs.tiles, bound, st);
-    if (p->dtype == ZKV_DT_F16) return pool::launch_shape<ZKV_DT_F16, false>(a, p->head_dim, hs.tiles, bound, st);
-    if (dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, true>(a, p->head_dim, hs.tiles, bound, st);
-    return pool::launch_shape<ZKV_DT_F16, true>(a, p->head_dim, hs.tiles, bound, st);
+    if (p->dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, false>(a, p->head_dim, hs.tiles, st);
+    if (p->dtype == ZKV_DT_F16) return pool::launch_shape<ZKV_DT_F16, false>(a, p->head_dim, hs.tiles, st);
+    if (dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, true>(a, p->head_dim, hs.tiles, st);
+    return pool::launch_shape<ZKV_DT_F16, true>(a, p->head_dim, hs.tiles, st);
 }

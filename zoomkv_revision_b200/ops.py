@@ -1115,6 +1115,7 @@ def rq_popcount_topk(cand, lay: RqLayout, planes, qparams, K: int, *, C: int | N
 
 # ----------------------------------------------------------------- pooled KV cache
 _POOL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
+POOL_WHOLE_TOKENS = 256   # up to this bound of the lengths pool_decode needs no workspace
 _INT32 = torch.int32
 
 
@@ -1127,7 +1128,7 @@ class KVPool:
     allocated: it holds the tensors, their addresses and strides."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "struct", "ref", "dtype", "device", "kv_heads", "head_dim",
-                 "block_size", "n_blocks")
+                 "block_size", "n_blocks", "float_like", "byte_like")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _cuda(("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale))
@@ -1163,12 +1164,13 @@ class KVPool:
         self.struct = _lib.ZkvPool(_p(k), _p(v), *strides(k), *strides(v), n, S, H, D, _POOL_DTYPES[k.dtype],
                                    _p(k_scale), _p(v_scale))
         self.ref = ctypes.addressof(self.struct)
+        self.float_like, self.byte_like = k.new_empty(0, dtype=torch.float32), k.new_empty(0, dtype=torch.uint8)
         check(lib().zkv_pool_init(self.ref), "zkv_pool_init")
 
 
 def _ints32(**tensors):
     """int32, contiguous CUDA tensors of one device (None is left out)."""
-    dev = None
+    dev = -1
     for name, t in tensors.items():
         if t is None:
             continue
@@ -1176,22 +1178,27 @@ def _ints32(**tensors):
             raise TypeError(f"{name} must be torch.int32; got {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-        if not t.is_cuda:
+        at = t.get_device()
+        if at < 0:
             raise ValueError(f"{name} must be a CUDA tensor")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        if dev < 0:
+            dev = at
+        elif at != dev:
             raise ValueError("tensors must be on one device")
 
 
-def _block_table(block_table, batch, dev):
-    if block_table.dtype is not _INT32:
-        raise TypeError(f"block_table must be torch.int32; got {block_table.dtype}")
-    if block_table.dim() != 2 or block_table.shape[0] != batch or block_table.device != dev:
+def _block_table(t, batch, dev):
+    """(row stride, width) of an int32 [batch, width] table."""
+    if t.dtype is not _INT32:
+        raise TypeError(f"block_table must be torch.int32; got {t.dtype}")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != batch or t.device != dev:
         raise ValueError("block_table must be [batch, width] on the device of lens")
-    width = block_table.shape[1]
-    ld = block_table.stride(0) if batch > 1 else width
-    if (width > 1 and block_table.stride(1) != 1) or ld < width:
+    width = shape[1]
+    ld, one = t.stride()
+    if batch <= 1:
+        ld = width
+    if (width > 1 and one != 1) or ld < width:
         raise ValueError("block_table rows must be contiguous and not overlap")
     return ld, width
 
@@ -1256,8 +1263,9 @@ def pool_release(done, lens, block_table, free_blocks, n_free, block_size: int, 
 
 
 def _whole_rows(t):
-    """t with its last dim contiguous and 16-byte rows (a copy where it has not)."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0:
+    """t [n, heads, dim] with contiguous dims and 16-byte rows (a copy where it has not)."""
+    row, head, one = t.stride()
+    if one == 1 and not (t.data_ptr() | 2 * row | 2 * head) & 15:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -1283,8 +1291,11 @@ def pool_write(k, v, slots, pool: KVPool, *, status=None):
     if k.device != dev or v.device != dev or slots.device != dev:
         raise ValueError("tensors must be on the pool's device")
     k, v = _whole_rows(k), _whole_rows(v)
-    check(lib().zkv_pool_write(_p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _POOL_DTYPES[dt],
-                               _p(slots), n, pool.ref, _p(status), _stream(k)), "zkv_pool_write")
+    ks, vs = k.stride(), v.stride()
+    rc = lib().zkv_pool_write(k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _POOL_DTYPES[dt],
+                              slots.data_ptr(), n, pool.ref, None if status is None else status.data_ptr(), _stream(k))
+    if rc:
+        check(rc, "zkv_pool_write")
 
 
 def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int = 0, softcap: float = 0.0,
@@ -1301,36 +1312,49 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     log, -inf for a request without tokens, whose out is 0).  workspace:
     uint8 CUDA tensor of pool_decode_ws_bytes(...) bytes, scratch only
     (default: allocated per call from torch's caching allocator)."""
-    B, Hq, D = q.shape[0], q.shape[-2], q.shape[-1]
-    if D != pool.head_dim or Hq % pool.kv_heads or q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[1] != 1):
+    shape = q.shape
+    B, Hq, D = shape[0], shape[-2], shape[-1]
+    if D != pool.head_dim or Hq % pool.kv_heads or len(shape) not in (3, 4) or (len(shape) == 4 and shape[1] != 1):
         raise ValueError(f"q must be [B, (1,) q_heads, {pool.head_dim}] with q_heads a multiple of {pool.kv_heads}; got "
-                         f"{tuple(q.shape)}")
-    dt = q.dtype
-    if dt not in (torch.bfloat16, torch.float16) or (pool.dtype != dt and pool.dtype != torch.float8_e4m3fn):
+                         f"{tuple(shape)}")
+    dt, dev = q.dtype, pool.device
+    code = _POOL_DTYPES.get(dt, 2)
+    if code == 2 or (pool.dtype != dt and pool.dtype != torch.float8_e4m3fn):
         raise TypeError(f"q {dt} does not fit a {pool.dtype} pool")
-    dev = pool.device
     if q.device != dev or lens.device != dev:
         raise ValueError("tensors must be on the pool's device")
-    _ints32(lens=lens, status=status)
-    if lens.numel() != B:
-        raise ValueError("lens must have one value per request")
+    if lens.dtype is not _INT32 or (status is not None and status.dtype is not _INT32):
+        raise TypeError("lens and status must be torch.int32")
+    if lens.numel() != B or not lens.is_contiguous():
+        raise ValueError("lens must be contiguous, one value per request")
     ld, width = _block_table(block_table, B, dev)
-    q3 = _whole_rows(q if q.dim() == 3 else q[:, 0])
+    q3 = _whole_rows(q if len(shape) == 3 else q[:, 0])
     if out is None:
-        out = torch.empty(q.shape, dtype=dt, device=dev)
-    elif out.shape != q.shape or out.dtype != dt or not out.is_contiguous() or out.device != dev:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != dt or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be contiguous, shaped and typed like q")
     if lse is None:
         if return_lse:
-            lse = torch.empty(B, Hq, dtype=torch.float32, device=dev)
+            lse = pool.float_like.new_empty((B, Hq))
     elif lse.dtype != torch.float32 or lse.numel() != B * Hq or not lse.is_contiguous() or lse.device != dev:
         raise ValueError("lse must be contiguous fp32 [B, q_heads]")
-    if workspace is None:
-        workspace = torch.empty(pool_decode_ws_bytes(B, Hq, pool, width, max_len), dtype=torch.uint8, device=dev)
-    check(lib().zkv_pool_decode(_p(q3), q3.stride(0), q3.stride(1), _POOL_DTYPES[dt], pool.ref, _p(lens),
-                                _p(block_table), ld, width, B, Hq, D ** -0.5 if scale is None else float(scale),
-                                int(window), float(softcap), int(max_len), _p(out), _p(lse), _p(status),
-                                _p(workspace), workspace.numel(), _stream(q)), "zkv_pool_decode")
+    room = width * pool.block_size
+    if 0 < max_len < room:
+        room = max_len
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel()
+    elif room > POOL_WHOLE_TOKENS:
+        ws_bytes = lib().zkv_pool_decode_ws_bytes(B, Hq, pool.kv_heads, D, room)
+        workspace = pool.byte_like.new_empty(ws_bytes)
+        ws = workspace.data_ptr()
+    stride = q3.stride()
+    rc = lib().zkv_pool_decode(q3.data_ptr(), stride[0], stride[1], code, pool.ref, lens.data_ptr(),
+                               block_table.data_ptr(), ld, width, B, Hq, D ** -0.5 if scale is None else scale, window,
+                               softcap, max_len, out.data_ptr(), None if lse is None else lse.data_ptr(),
+                               None if status is None else status.data_ptr(), ws, ws_bytes, _stream(q))
+    if rc:
+        check(rc, "zkv_pool_decode")
     return (out, lse) if return_lse else out
 
 
