@@ -758,12 +758,11 @@ int zkv_pool_write(const void* k, int64_t k_token, int64_t k_head, const void* v
  *   max_len: a bound of lens known to the host (0: width * block_size); a
  *   longer or negative length is cut to the bound or 0, and a block id
  *   outside the pool leaves its tokens out, both with ZKV_ERR_RANGE
- *   workspace: device, 256-byte aligned, >= zkv_pool_decode_ws_bytes
- *   (scratch only, no state between calls); not needed where the bound of the
- *   lengths is at most ZKV_POOL_WHOLE_TOKENS (may be NULL then).
+ *   workspace: device, 256-byte aligned, >= zkv_pool_decode_ws_bytes (0:
+ *   none is needed, NULL will do; also 0 for bad arguments), scratch only, no
+ *   state between calls
  *   q_heads / kv_heads <= 5120.                                           */
-#define ZKV_POOL_WHOLE_TOKENS 256
-size_t zkv_pool_decode_ws_bytes(int batch, int q_heads, int kv_heads, int head_dim, int64_t max_len);
+size_t zkv_pool_decode_ws_bytes(const zkv_pool* pool, int batch, int q_heads, int window, int64_t max_len);
 int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int dtype, const zkv_pool* pool,
                     const int32_t* lens, const int32_t* block_table, int64_t table_ld, int width, int batch,
                     int q_heads, float scale, int window, float softcap, int64_t max_len, void* out, float* lse,

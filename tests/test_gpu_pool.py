@@ -116,10 +116,16 @@ def check_decode(q, k, v, ks, vs, lens, table, out, lse, scale, window=0, softca
         assert bool((le <= lt).all()), f"lse of request {b}: {float((le / lt).max()):.2f} of the tolerance"
 
 
-def run_decode(seed, lens, S, H, G, D, qt, pt, layout, window=0, softcap=0.0, scale=None, max_len=0, spare=3, **kw):
+def run_decode(seed, lens, S, H, G, D, qt, pt, layout, window=0, softcap=0.0, scale=None, max_len=0, spare=3, wide=None,
+               **kw):
+    """wide: a table of so many more columns that the bound of the lengths lets the rows be cut by units (None: both ways)."""
+    if wide is None:
+        run_decode(seed, lens, S, H, G, D, qt, pt, layout, window, softcap, scale, max_len, spare, True, **kw)
     need = sum((n + S - 1) // S for n in lens)
     n_blocks = need + spare
     width = max(1, max((n + S - 1) // S for n in lens)) + 1
+    if wide and not 0 < window < 10000:
+        width += (80 << 20) // (2 * len(lens) * H * D * S * (1 if pt == F8 else 2))
     k, v, ks, vs = make_pool(seed, n_blocks, S, H, D, pt, layout)
     table = make_table(seed + 1, lens, S, n_blocks, width)
     lo = [max(0, n - window) if window else 0 for n in lens]
@@ -206,8 +212,17 @@ def test_decode_is_deterministic_and_takes_dirty_workspaces():
     q = torch.randn(4, 8, 128, generator=gen(3), device=DEV).to(BF)
     pool = ops.KVPool(k, v)
     first = None
+    wide = torch.full((4, 9000), -1, dtype=torch.int32, device=DEV)   # a bound of the lengths that cuts the rows by units
+    wide[:, :600] = table
     for fill in (0, 255, 127, 1):
         ws = torch.full((ops.pool_decode_ws_bytes(4, 8, pool, 600),), fill, dtype=torch.uint8, device=DEV)
+        assert ws.numel() == 0
+        got = ops.pool_decode(q, pool, i32(lens), table, return_lse=True, workspace=ws)
+        check_decode(q, k, v, ks, vs, lens, table, *got, 128 ** -0.5)
+    for fill in (0, 255, 127, 1):
+        ws = torch.full((ops.pool_decode_ws_bytes(4, 8, pool, 9000),), fill, dtype=torch.uint8, device=DEV)
+        assert ws.numel() > 0
+        table = wide
         got = ops.pool_decode(q, pool, i32(lens), table, return_lse=True, workspace=ws)
         first = first or got
         assert all(torch.equal(x, y) for x, y in zip(first, got))
@@ -314,10 +329,11 @@ def test_decode_query_range_over_fp8(mag):
     check_decode(q, k, v, ks, vs, [200, 77], table, out, lse, 0.1 / mag)
 
 
-def test_decode_on_another_stream_and_in_a_graph():
+@pytest.mark.parametrize("width", [80, 20000])
+def test_decode_on_another_stream_and_in_a_graph(width):
     lens = [1000, 17, 0, 640]
     k, v, _, _ = make_pool(51, 120, 16, 2, 128, BF, "hnd")
-    table = make_table(52, lens, 16, 120, 80)
+    table = make_table(52, lens, 16, 120, width)
     q = torch.randn(4, 8, 128, generator=gen(53), device=DEV).to(BF)
     pool, n = ops.KVPool(k, v), i32(lens)
     torch.cuda.synchronize()
@@ -326,7 +342,7 @@ def test_decode_on_another_stream_and_in_a_graph():
         out, lse = ops.pool_decode(q, pool, n, table, return_lse=True)
     side.synchronize()
     check_decode(q, k, v, None, None, lens, table, out, lse, 128 ** -0.5)
-    ws = torch.empty(ops.pool_decode_ws_bytes(4, 8, pool, 80), dtype=torch.uint8, device=DEV)
+    ws = torch.empty(ops.pool_decode_ws_bytes(4, 8, pool, width), dtype=torch.uint8, device=DEV)
     g_out, g_lse = torch.empty_like(out), torch.empty_like(lse)
     with torch.cuda.stream(side):
         ops.pool_decode(q, pool, n, table, out=g_out, lse=g_lse, workspace=ws)
@@ -335,7 +351,7 @@ def test_decode_on_another_stream_and_in_a_graph():
     with torch.cuda.graph(graph):
         ops.pool_decode(q, pool, n, table, out=g_out, lse=g_lse, workspace=ws)
     lens2 = [999, 40, 3, 700]     # the lengths are read on the GPU: a replay sees the new ones
-    table.copy_(make_table(54, lens2, 16, 120, 80))
+    table.copy_(make_table(54, lens2, 16, 120, width))
     n.copy_(i32(lens2))
     graph.replay()
     torch.cuda.synchronize()
@@ -621,8 +637,9 @@ def test_refusals():
     for kw in (dict(window=-1), dict(softcap=-1.0), dict(softcap=math.nan), dict(max_len=-1)):
         with pytest.raises(RuntimeError):
             ops.pool_decode(q, pool, lens, table, **kw)
+    wide = torch.zeros(2, 10 ** 5, dtype=torch.int32, device=DEV)
     with pytest.raises(RuntimeError, match="limit"):
-        ops.pool_decode(q, pool, lens, table, workspace=torch.empty(16, dtype=torch.uint8, device=DEV))
+        ops.pool_decode(q, pool, lens, wide, workspace=torch.empty(256, dtype=torch.uint8, device=DEV))
     with pytest.raises(TypeError):
         ops.KVPool(k, v.half())
     with pytest.raises(ValueError):

@@ -49,7 +49,8 @@ def decode(p, q=0x1000, q_row=1024, q_head=128, dtype=0, lens=0x1000, table=0x10
     (dict(batch=-1), ARG), (dict(width=-1), ARG), (dict(ld=3), ARG), (dict(heads=7), ARG), (dict(heads=0), ARG),
     (dict(window=-1), ARG), (dict(softcap=-1.0), ARG), (dict(softcap=float("nan")), ARG), (dict(max_len=-1), ARG),
     (dict(dtype=1), ARG), (dict(dtype=2), ARG), (dict(q=0x1008), ALIGN), (dict(q_row=1020), ALIGN),
-    (dict(q_head=132), ALIGN), (dict(ws=0x1010), ALIGN), (dict(ws_bytes=8), CAPACITY), (dict(batch=0), OK),
+    (dict(q_head=132), ALIGN), (dict(ws=0x1010), ALIGN), (dict(width=10 ** 6, ld=10 ** 6, ws_bytes=8), CAPACITY),
+    (dict(heads=2 * 5121), CAPACITY), (dict(batch=0), OK),
 ])
 def test_decode_arguments(bad, code):
     assert decode(pool(), **bad) == code
@@ -76,9 +77,13 @@ def test_write_plan_release_arguments():
 
 
 def test_workspace_sizes():
-    f = _lib.lib().zkv_pool_decode_ws_bytes
-    assert f(-1, 8, 2, 128, 10) == 0 and f(1, 7, 2, 128, 10) == 0 and f(1, 8, 2, 128, -1) == 0
-    assert f(1, 8, 2, 128, 0) > 0 and f(64, 32, 8, 128, 131072) >= f(1, 32, 8, 128, 131072)
+    lib, p = _lib.lib(), pool()
+    f = lambda *x: lib.zkv_pool_decode_ws_bytes(ctypes.addressof(p), *x)  # noqa: E731
+    assert f(-1, 8, 0, 10 ** 6) == 0 and f(1, 7, 0, 10 ** 6) == 0 and f(1, 8, -1, 10 ** 6) == 0 and f(1, 8, 0, -1) == 0
+    assert lib.zkv_pool_decode_ws_bytes(None, 1, 8, 0, 10 ** 6) == 0
+    # short bounds need none; long ones a part's size for each CTA of the largest grid, whatever the batch
+    assert f(1, 8, 0, 256) == 0 and f(4096, 8, 0, 256) == 0 and f(64, 8, 100, 10 ** 6) == 0
+    assert 0 < f(1, 8, 0, 10 ** 6) <= f(64, 8, 0, 10 ** 6) == f(6400, 8, 0, 10 ** 6) < 16 << 20
 
 
 def test_python_checks_need_no_gpu():

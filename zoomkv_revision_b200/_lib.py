@@ -167,7 +167,7 @@ _SIGNATURES = {
                          _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     "zkv_pool_write": [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i32, _c_void_p, _i64, _c_void_p, _c_void_p,
                        _c_void_p],
-    "zkv_pool_decode_ws_bytes": [_i32, _i32, _i32, _i32, _i64],
+    "zkv_pool_decode_ws_bytes": [_c_void_p, _i32, _i32, _i32, _i64],
     "zkv_pool_decode": [_c_void_p, _i64, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _i32, _f32,
                         _i32, _f32, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p],
     "zkv_version": [],

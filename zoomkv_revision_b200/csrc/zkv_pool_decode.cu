@@ -13,8 +13,11 @@
 //    so uneven requests, one long request and many short ones are spread the
 //    same way and the host needs no length.  A row (request, kv head) that
 //    ends in another CTA than it began in leaves partials (m, l, o), which
-//    pool_join_kernel joins in CTA order.  Where no request can have more than
-//    kWholeTokens tokens the rows are cut whole and one launch does.
+//    pool_join_kernel joins in CTA order.  Where the host's bound of the
+//    lengths leaves little to balance (see plan_call) the rows are not cut by
+//    units: a CTA takes whole rows, or a cluster of CTAs shares one row and
+//    joins through distributed shared memory; one launch does, with no scan
+//    and no workspace.
 //  * One producer warp per CTA walks the range: block ids from the table, one
 //    5-D TMA copy per block and tensor (dims | tokens | 128-byte pieces | head
 //    | block; any strides, so both memory orders), a ring of stages.  An id
@@ -55,16 +58,17 @@ namespace pool {
 constexpr int kConsumers = 4;                   // warps that share a tile's tokens
 constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxGrid = 320;                   // CTAs that a workspace is sized for
-constexpr int kWholeTokens = ZKV_POOL_WHOLE_TOKENS;  // longest request of a call whose rows are not split
+constexpr int kWholeTokens = 256;               // requests up to this length are never cut
+constexpr int kMaxRanks = 16;                   // CTAs of a cluster that shares a row
 constexpr uint64_t kWaitNs = 2000000000ull;     // limit of each wait inside a CTA
 
 // What a unit is, written by the producer beside its stage.
-struct Unit {
+struct alignas(16) Unit {
     int b, h;         // request, kv head
     int tile0;        // first token
     int lo, len;      // tokens [lo, len) of the request are attended
     int flags;        // kFirst, kLast of the row in this CTA; kEnd: the CTA's last unit
-    int part;         // -1: the row is this CTA's alone; else its partial slot
+    int part;         // -1: the row is this CTA's alone; 0, 1: its partial slot; 2: a cluster's
     int bad;          // boxes of the tile that are not in the pool
 };
 constexpr int kFirst = 1, kLast = 2, kEnd = 4;
@@ -88,8 +92,12 @@ struct DecodeArgs {
     int64_t table_ld, n_blocks;
     int cap;        // longest length
     int batch, kv_heads, G, chunks, heads;  // heads: query heads of a chunk (the last one may have fewer)
-    int groups;     // CTAs of a chunk; CTA x: chunk x % chunks of range x / chunks
-    int whole;      // rows are not split
+    int abreast;    // kv heads of a row: their CTAs walk one range side by side
+    int head_rows;  // rows of a request: kv_heads / abreast
+    int side;       // CTAs of a range: abreast * chunks; CTA x: member x % side of range x / side
+    int groups;     // ranges
+    int whole;      // rows are not cut by units
+    int ranks;      // CTAs (a cluster) that share a row, if `whole`
     int shift, lg_box, window;
     float scale, softcap;
 };
@@ -105,7 +113,7 @@ struct Cfg {
     static constexpr int kKv = kTile * kRow;                     // K (or V) of a stage
     static constexpr int kHeadsMax = 8 * NT;
     static constexpr int kQPitch = D * 2 + 16;
-    static constexpr int kQSlot = kHeadsMax * kQPitch;
+    static constexpr int kQSlot = kHeadsMax * kQPitch;  // a multiple of 16
     static constexpr int kFixed = 1024 + 1024;                   // alignment; barriers, units, statistics
     static constexpr int kStage = 2 * kKv + kQSlot + (int)sizeof(Unit);
     static constexpr int kMl = 2 * kConsumers * kHeadsMax * 8;
@@ -120,6 +128,7 @@ struct Cfg {
     // n-tiles of O that fit into a stage's K and V when the warps are joined
     static constexpr int kJoinTiles = (2 * kKv) / (kConsumers * 8 * D * 4) < NT ? (2 * kKv) / (kConsumers * 8 * D * 4) : NT;
     static_assert(kJoinTiles >= 1 && NT % kJoinTiles == 0, "join buffer");
+    static_assert(kHeadsMax * D * 4 <= kStages * kQSlot, "a cluster's part takes the queries' place");
 };
 
 // ------------------------------------------------------------ device helpers
@@ -244,7 +253,7 @@ __device__ __forceinline__ Units count_units(const DecodeArgs& a, int64_t* sh) {
     u.b_hi = min(a.batch, u.b_lo + per);
     u.mine = 0;
     for (int b = u.b_lo; b < u.b_hi; ++b)
-        u.mine += (int64_t)row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + b))) * a.kv_heads;
+        u.mine += (int64_t)row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + b))) * a.head_rows;
     u.before = block_sum_before(u.mine, sh, &u.total);
     return u;
 }
@@ -255,7 +264,7 @@ __device__ __forceinline__ bool locate(const DecodeArgs& a, const Units& x, int6
     off = u - x.before;
     for (b = x.b_lo;; ++b) {
         tiles = row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + b)));
-        const int64_t n = (int64_t)tiles * a.kv_heads;
+        const int64_t n = (int64_t)tiles * a.head_rows;
         if (off < n || b + 1 >= x.b_hi) return true;
         off -= n;
     }
@@ -333,7 +342,7 @@ struct Row {
     // at base + at[i] and base + kKv + at[i] (in a swizzled box, `piece` bytes
     // from one 128-byte piece to the next); its tokens [v0[i], v1[i]) count.
     __device__ __forceinline__ void step(const DecodeArgs& a, uint32_t base, const uint32_t (&at)[C::kSub], uint32_t piece,
-                                         const int (&v0)[C::kSub], const int (&v1)[C::kSub]) {
+                                         const int (&v0)[C::kSub], const int (&v1)[C::kSub], bool partial) {
         const int lane = threadIdx.x & 31, g = lane >> 2;
         constexpr int kPerPiece = C::kInner / 16;  // 16-byte chunks of a row in a piece
         constexpr int kSub = C::kSub;
@@ -343,19 +352,13 @@ struct Row {
         auto chunk = [&](uint32_t from, int tok, int sw, int c) {
             return from + (uint32_t)(c / kPerPiece) * piece + tok * C::kInner + (((c % kPerPiece) ^ sw) << 4);
         };
-        float x[kSub][NT][4];
-        // two chains of products at least, so that one does not wait for the other
-        constexpr int kChains = kSub == 1 ? 2 : 1;
-        float x2[kChains == 2 ? NT : 1][4];
+        float x[kSub][NT][4], x2[kSub][NT][4];  // two chains of products each, so that one does not wait for the other
 #pragma unroll
         for (int i = 0; i < kSub; ++i)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[i][n][e] = 0.f;
-                    if (kChains == 2) x2[n][e] = 0.f;
-                }
+                for (int e = 0; e < 4; ++e) x[i][n][e] = x2[i][n][e] = 0.f;
 #pragma unroll
         for (int s = 0; s < D / 16; s += 2)
 #pragma unroll
@@ -375,16 +378,9 @@ struct Row {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     mma16816<kMmaBf16>(x[i][n], a0, q[s][n][0], q[s][n][1]);
-                    if constexpr (kChains == 2) mma16816<kMmaBf16>(x2[n], a1, q[s + 1][n][0], q[s + 1][n][1]);
-                    else mma16816<kMmaBf16>(x[i][n], a1, q[s + 1][n][0], q[s + 1][n][1]);
+                    mma16816<kMmaBf16>(x2[i][n], a1, q[s + 1][n][0], q[s + 1][n][1]);
                 }
             }
-        if constexpr (kChains == 2) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[0][n][e] += x2[n][e];
-        }
         // x[i][n][0..3]: (token g, head 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
         float alpha[NT][2];
         bool moved = false;
@@ -395,13 +391,23 @@ struct Row {
             for (int i = 0; i < kSub; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float y = x[i][n][e] * f[n][e & 1];
+                    float y = (x[i][n][e] + x2[i][n][e]) * f[n][e & 1];
                     if (a.softcap > 0.f) y = a.softcap * 1.4426950408889634f * tanhf(y / a.softcap);
-                    const int tok = e < 2 ? g : g + 8;
-                    if (tok < v0[i] || tok >= v1[i]) y = -INFINITY;
                     x[i][n][e] = y;
-                    mx[e & 1] = fmaxf(mx[e & 1], y);
                 }
+            if (partial) {
+#pragma unroll
+                for (int i = 0; i < kSub; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int tok = e < 2 ? g : g + 8;
+                        if (tok < v0[i] || tok >= v1[i]) x[i][n][e] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < kSub; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e & 1] = fmaxf(mx[e & 1], x[i][n][e]);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
@@ -446,35 +452,36 @@ struct Row {
                     }
                 }
             const uint32_t vs = base + C::kKv + at[i];
-            if constexpr (kF8) {
+            // four tiles of dims at a time, their hi products before their lo ones, so that none waits for the one before
+            const int tok_v = (lane & 7) + ((lane >> 4) << 3), off_v = (lane >> 3) & 1, sw_v = tok_v & 7;
 #pragma unroll
-                for (int j = 0; j < C::kMTiles; j += 2) {
-                    uint32_t r[4];
-                    ldsm4_t(chunk(vs, tok_k, sw_k, j + off_k), r);
+            for (int j = 0; j < C::kMTiles; j += 4) {
+                uint32_t v[4][4];
+                if constexpr (kF8) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const uint32_t w0 = __byte_perm(r[2 * k], 0, 0x3120);  // (dim 2g: tokens 2t, 2t+1), (dim 2g+1)
-                        const uint32_t w1 = __byte_perm(r[2 * k + 1], 0, 0x3120);
-                        const uint32_t v[4] = {e4m3x2_to_f16x2((uint16_t)w0), e4m3x2_to_f16x2((uint16_t)(w0 >> 16)),
-                                               e4m3x2_to_f16x2((uint16_t)w1), e4m3x2_to_f16x2((uint16_t)(w1 >> 16))};
+                    for (int k = 0; k < 4; k += 2) {
+                        uint32_t r[4];
+                        ldsm4_t(chunk(vs, tok_k, sw_k, j + k + off_k), r);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            mma16816<false>(o[j + k][n], v, hi[n][0], hi[n][1]);
-                            if constexpr (C::kTwoParts) mma16816<false>(o[j + k][n], v, lo[n][0], lo[n][1]);
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t y = __byte_perm(r[w], 0, 0x3120);  // (dim 2g: tokens 2t, 2t+1), (dim 2g+1)
+                            v[k + w / 2][2 * (w & 1)] = e4m3x2_to_f16x2((uint16_t)y);
+                            v[k + w / 2][2 * (w & 1) + 1] = e4m3x2_to_f16x2((uint16_t)(y >> 16));
                         }
                     }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) ldsm4_t(chunk(vs, tok_v, sw_v, 2 * (j + k) + off_v), v[k]);
                 }
-            } else {
-                const int tok_v = (lane & 7) + ((lane >> 4) << 3), off_v = (lane >> 3) & 1, sw_v = tok_v & 7;
 #pragma unroll
-                for (int j = 0; j < C::kMTiles; ++j) {
-                    uint32_t v[4];
-                    ldsm4_t(chunk(vs, tok_v, sw_v, 2 * j + off_v), v);
+                for (int k = 0; k < 4; ++k)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma16816<kMmaBf16>(o[j][n], v, hi[n][0], hi[n][1]);
-                        if constexpr (C::kTwoParts) mma16816<kMmaBf16>(o[j][n], v, lo[n][0], lo[n][1]);
-                    }
+                    for (int n = 0; n < NT; ++n) mma16816<kMmaBf16>(o[j + k][n], v[k], hi[n][0], hi[n][1]);
+                if constexpr (C::kTwoParts) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma16816<kMmaBf16>(o[j + k][n], v[k], lo[n][0], lo[n][1]);
                 }
             }
         }
@@ -524,15 +531,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         mbar_init(&epi, kConsumers);
         mbar_fence_init();
     }
-    const int chunk = blockIdx.x % a.chunks;
-    const int64_t c = blockIdx.x / a.chunks;
+    const int rank = blockIdx.x % a.ranks, block = blockIdx.x / a.ranks;
+    const int member = block % a.side, chunk = member % a.chunks, abreast = member / a.chunks;
+    const int64_t c = block / a.side;
     const int n_heads = min(a.heads, a.G - chunk * a.heads);
     grid_dep_wait();
     grid_dep_launch_next();  // the join kernel may become resident; it waits for this grid
     // ---- this CTA's range [u0, u1): of units, or of rows where those are not split
     int64_t u0, u1;
     if (a.whole) {
-        const int64_t rows = (int64_t)a.batch * a.kv_heads;
+        const int64_t rows = (int64_t)a.batch * a.head_rows;
         u0 = rows * c / a.groups;
         u1 = rows * (c + 1) / a.groups;
         __syncthreads();
@@ -554,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
 
     if (warp == kConsumers) {
         // ---------------------------------------------------- producer
-        int b = a.whole ? (int)(u0 / a.kv_heads) : s_b;
+        int b = a.whole ? (int)(u0 / a.head_rows) : s_b;
         int next = __ldcg(a.lens + b);  // the length of the next request to begin, asked for one request ahead
         int len, lo, tile_first, tiles;
         auto begin_request = [&]() {
@@ -566,21 +574,28 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             if (b + 1 < a.batch) next = __ldcg(a.lens + b + 1);
         };
         begin_request();
-        int h = a.whole ? (int)(u0 % a.kv_heads) : (int)(s_off / tiles);
-        int tile = a.whole ? 0 : (int)(s_off % tiles);
-        int64_t row_begin = u0 - tile;  // unit at which the row begins (its number, where rows are whole)
+        int hr = a.whole ? (int)(u0 % a.head_rows) : (int)(s_off / tiles);  // row of the request
+        int tile = a.whole ? (int)((int64_t)tiles * rank / a.ranks) : (int)(s_off % tiles);
+        bool none = false;  // more CTAs than tiles: this one has an empty unit
+        if (a.ranks > 1) {
+            tiles = (int)((int64_t)tiles * (rank + 1) / a.ranks);
+            none = tile == tiles;
+            if (none) tiles = tile + 1;
+        }
+        int64_t row_begin = a.whole ? u0 : u0 - tile;  // unit at which the row begins (its number, where rows are whole)
         int ids = -1, ids_next = -1, ids_b = -1, ids_at = 0;
         int n_row = 0;                  // rows begun in this CTA
         const int boxes = C::kTile >> a.lg_box, box_bytes = C::kRow << a.lg_box;
         bool ok = true, end = false;
         int done = 0;
         for (; !end; ++done) {
-            const int stage = done % C::kStages;
+            const int stage = done % C::kStages, h = hr * a.abreast + abreast;
             const bool first = done == 0 || tile == 0;
             end = a.whole ? tile == tiles - 1 && row_begin + 1 == u1 : u0 + done + 1 == u1;
             const bool last = end || tile == tiles - 1;
             int part = -1;
             if (!a.whole) part = row_begin < u0 ? 0 : row_begin + tiles > u1 ? 1 : -1;
+            else if (a.ranks > 1) part = 2;
             // ---- block ids of the tile: 32 entries of the table at a time, the next 32 on their way
             const int tile0 = (tile_first + tile) * C::kTile;
             const int entry = tile0 >> a.shift;
@@ -596,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             }
             const int id = __shfl_sync(0xffffffffu, ids, (entry - ids_at + lane) & 31);  // lane j: box j
             const int tok = tile0 + (lane << a.lg_box);
-            const bool wanted = lane < boxes && tok < len && tok + (1 << a.lg_box) > lo;
+            const bool wanted = lane < boxes && tok < len && tok + (1 << a.lg_box) > lo && !none;
             const bool there = wanted && id >= 0 && id < a.n_blocks;
             if (wanted && !there) raise_status(a.status, ZKV_ERR_RANGE);
             const unsigned copy = __ballot_sync(0xffffffffu, there), bad = __ballot_sync(0xffffffffu, wanted && !there);
@@ -610,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
                 x.h = h;
                 x.tile0 = tile0;
                 x.lo = lo;
-                x.len = len;
+                x.len = none ? 0 : len;
                 x.flags = (first ? kFirst : 0) | (last ? kLast : 0) | (end ? kEnd : 0);
                 x.part = part;
                 x.bad = (int)bad;
@@ -633,8 +648,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             if (++tile == tiles) {
                 tile = 0;
                 row_begin += a.whole ? 1 : tiles;
-                if (++h == a.kv_heads) {
-                    h = 0;
+                if (++hr == a.head_rows) {
+                    hr = 0;
                     if (++b < a.batch) begin_request();
                 }
             }
@@ -650,10 +665,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     uint32_t epi_phase = 0;
     int n_row = 0;
     const int g = lane >> 2, t = lane & 3;
-    bool end = false;
+    // a cluster's part of a row: this CTA's only one, so the queries and the first half of ml are free when it is done
+    float* const cl_o = reinterpret_cast<float*>(qs);  // [heads][D]
+    float2* const cl_ml = ml;                          // [heads]
+    bool end = false, alive = true;
     for (int i = 0; !end; ++i) {
         const int stage = i % C::kStages;
-        if (!__all_sync(0xffffffffu, wait_for(full + stage, (uint32_t)((i / C::kStages) & 1), a.status))) return;
+        if (!__all_sync(0xffffffffu, wait_for(full + stage, (uint32_t)((i / C::kStages) & 1), a.status))) {
+            alive = false;
+            break;
+        }
         const Unit x = units[stage];
         end = x.flags & kEnd;
         uint8_t* const base = kv + stage * 2 * C::kKv;
@@ -680,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
 #pragma unroll
                 for (int k = 0; k < C::kSub; ++k) row.clear_rows(base + C::kKv + at[k], piece, v0[k], v1[k]);
             }
-            row.step(a, smem_u32(base), at, piece, v0, v1);
+            row.step(a, smem_u32(base), at, piece, v0, v1, partial);
             if (partial) proxy_fence();
         }
         if (!(x.flags & kLast)) {
@@ -707,14 +728,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             epi_phase ^= 1;
             return got;
         };
-        if (!meet()) return;  // statistics written, stage read by all
+        if (!meet()) {  // statistics written, stage read by all
+            alive = false;
+            break;
+        }
         float* buf = reinterpret_cast<float*>(base);
         const float v_scale = kF8 && a.v_scale ? __ldcg(a.v_scale + x.h) : 1.f;
         const int64_t head0 = ((int64_t)x.b * a.kv_heads + x.h) * a.G + chunk * a.heads;
         const int64_t slot = (int64_t)blockIdx.x * 2 + x.part;
 #pragma unroll
         for (int r = 0; r < NT; r += C::kJoinTiles) {
-            if (r > 0 && !meet()) return;
+            if (r > 0 && alive) alive = meet();
 #pragma unroll
             for (int n = 0; n < C::kJoinTiles; ++n) {
                 float fac[2];
@@ -744,7 +768,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
                     }
                 }
             }
-            if (!meet()) return;
+            if (alive) alive = meet();
+            if (!alive) continue;
             for (int idx = tid; idx < 8 * C::kJoinTiles * (D / 4); idx += 32 * kConsumers) {
                 const int hl = idx / (D / 4), d = 4 * (idx % (D / 4)), head = 8 * r + hl;
                 if (head >= n_heads) continue;
@@ -765,16 +790,61 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
                     const float inv = sum == 0.f ? 0.f : v_scale / sum;
                     store4<kQ>(a.out, (head0 + head) * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
                     if (a.lse && d == 0) a.lse[head0 + head] = (mx + log2f(sum)) * 0.6931471805599453f;
+                } else if (x.part == 2) {
+                    *reinterpret_cast<float4*>(cl_o + head * D + d) = o;
+                    if (d == 0) cl_ml[head] = make_float2(mx, sum);
                 } else {
                     *reinterpret_cast<float4*>(a.parts + (slot * C::kHeadsMax + head) * D + d) = o;
                     if (d == 0) *reinterpret_cast<float2*>(a.stats + (slot * C::kHeadsMax + head) * 2) = make_float2(mx, sum);
                 }
             }
         }
+        if (!alive) break;
         proxy_fence();  // the stage was written by these threads; the next copy into it is the async proxy's
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + stage);
     }
+    if (a.ranks == 1) return;
+    // ---- the row's parts, by the cluster's ranks in order; every CTA meets here whatever became of its waits
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int h = (int)(c % a.head_rows);
+    const int64_t head0 = c * a.G + chunk * a.heads;  // (request, kv head) is the row's number: one head abreast
+    for (int idx = tid * a.ranks + rank; alive && idx < n_heads * (D / 4); idx += 32 * kConsumers * a.ranks) {
+        const int head = idx / (D / 4), d = 4 * (idx % (D / 4));
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r0 = 0; r0 < a.ranks; r0 += 4) {
+            float2 s[4];
+            float4 y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                s[k] = make_float2(-INFINITY, 0.f);
+                y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r0 + k < a.ranks) {
+                    s[k] = *cluster.map_shared_rank(cl_ml + head, r0 + k);
+                    y[k] = *cluster.map_shared_rank(reinterpret_cast<float4*>(cl_o + head * D + d), r0 + k);
+                }
+            }
+            float mx = m;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx = fmaxf(mx, s[k].x);
+            const float ref = mx == -INFINITY ? 0.f : mx, old = exp2_fast(m - ref);
+            l *= old, o.x *= old, o.y *= old, o.z *= old, o.w *= old;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float w = exp2_fast(s[k].x - ref);
+                l += w * s[k].y;
+                o.x += w * y[k].x, o.y += w * y[k].y, o.z += w * y[k].z, o.w += w * y[k].w;
+            }
+            m = mx;
+        }
+        const float v_scale = kF8 && a.v_scale ? __ldcg(a.v_scale + h) : 1.f;
+        const float inv = l == 0.f ? 0.f : v_scale / l;
+        store4<kQ>(a.out, (head0 + head) * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        if (a.lse && d == 0) a.lse[head0 + head] = (m + log2f(l)) * 0.6931471805599453f;
+    }
+    cluster.sync();  // no CTA leaves while another reads its part
 }
 
 // ------------------------------------------------------------ joining split rows
@@ -796,7 +866,7 @@ __global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_co
     __shared__ int64_t s_row[2];
     __shared__ int s_bh[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int chunk = blockIdx.x % a.chunks, cand = blockIdx.x / a.chunks, head = blockIdx.y;
+    const int member = blockIdx.x % a.side, chunk = member % a.chunks, cand = blockIdx.x / a.side, head = blockIdx.y;
     // Every path waits for the decode grid before it ends: the next kernel on
     // the stream waits for this one alone.
     if (head >= min(a.heads, a.G - chunk * a.heads)) {
@@ -806,14 +876,14 @@ __global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_co
     const Units x = count_units<kTile, kJoinThreads>(a, sh);
     const int64_t ctas = min((int64_t)a.groups, x.total);
     if (by_row) {
-        const int b = cand / a.kv_heads;
+        const int b = cand / a.head_rows;
         if (b >= x.b_lo && b < x.b_hi) {
             int64_t begin = x.before;
             for (int i = x.b_lo; i < b; ++i)
-                begin += (int64_t)row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + i))) * a.kv_heads;
+                begin += (int64_t)row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + i))) * a.head_rows;
             const int tiles = row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + b)));
             s_bh[0] = b;
-            s_bh[1] = cand - b * a.kv_heads;
+            s_bh[1] = cand - b * a.head_rows;
             s_row[0] = begin + (int64_t)s_bh[1] * tiles;
             s_row[1] = s_row[0] + tiles;
         }
@@ -835,7 +905,7 @@ __global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_co
     __syncthreads();
     const int64_t c0 = owner_cta(s_row[0], x.total, ctas);
     const int n = (int)(owner_cta(s_row[1] - 1, x.total, ctas) - c0) + 1;
-    const int b = s_bh[0], h = s_bh[1];
+    const int b = s_bh[0], h = s_bh[1] * a.abreast + member / a.chunks;
     grid_dep_wait();
     if (n == 1 || (!by_row && c0 != cand)) return;
     float m = -INFINITY, l = 0.f, o[E];
@@ -848,7 +918,7 @@ __global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_co
             const int i = i0 + k * kWarps;
             s[k] = make_float2(-INFINITY, 0.f);
             if (i < n) {
-                const int64_t slot = (((c0 + i) * a.chunks + chunk) * 2 + (i == 0 ? 1 : 0)) * heads_max + head;
+                const int64_t slot = (((c0 + i) * a.side + member) * 2 + (i == 0 ? 1 : 0)) * heads_max + head;
                 s[k] = __ldcg(reinterpret_cast<const float2*>(a.stats) + slot);
 #pragma unroll
                 for (int e = 0; e < E / 2; ++e)
@@ -984,34 +1054,86 @@ static Heads split_heads(int G) {
     return h;
 }
 
-// CTAs of a chunk that a call can use: its units at most, and what the largest grid leaves a chunk.
-static int64_t most_groups(int batch, int kv_heads, int chunks, int64_t max_len, int tile) {
+// Ranges that a call can use, `side` CTAs each: its units at most, and what the largest grid has room for.
+static int64_t most_groups(int batch, int head_rows, int side, int64_t max_len, int tile) {
     const int64_t tiles = std::max<int64_t>(1, (max_len + tile - 1) / tile);
-    const int64_t rows = (int64_t)batch * kv_heads, most = kMaxGrid / chunks;
+    const int64_t rows = (int64_t)batch * head_rows, most = kMaxGrid / side;
     return rows >= most ? most : std::min<int64_t>(most, rows * tiles);
+}
+
+// Rows of partials in the workspace: two parts of a chunk's heads per CTA of the largest grid.
+static size_t part_rows(int batch, int kv_heads, const Heads& h, int64_t max_len) {
+    return (size_t)most_groups(batch, kv_heads, h.chunks, max_len, 64) * h.chunks * 2 * 8 * h.tiles;
+}
+
+// How a call's rows are cut, from what the host knows: the bound of the lengths.
+struct Cut {
+    bool whole;    // not by units
+    int ranks;     // CTAs of a cluster that share a row, if `whole`
+    int abreast;   // kv heads walked side by side, if not
+};
+#ifndef ZKV_CLUSTER_BYTES
+#define ZKV_CLUSTER_BYTES (64 << 20)
+#endif
+#ifndef ZKV_RANK_TILES
+#define ZKV_RANK_TILES 1
+#endif
+static Cut plan_call(int batch, int kv_heads, int chunks, int row_bytes, int window, int64_t cap, int per_sm) {
+    Cut c{false, 1, 8};
+    const int tile = tile_tokens(row_bytes);
+    const int64_t longest = window > 0 ? std::min<int64_t>(cap, window) : cap;
+    const int64_t rows = (int64_t)batch * kv_heads * chunks;
+    const int64_t tiles = (longest + tile - 1) / tile + (window > 0 ? 1 : 0);
+    c.whole = longest <= kWholeTokens || 2 * (int64_t)batch * kv_heads * longest * row_bytes <= ZKV_CLUSTER_BYTES;
+    if (c.whole) {
+        const int64_t wave = (int64_t)per_sm * sm_count();
+        while (c.ranks < kMaxRanks && rows * c.ranks * 2 <= wave && c.ranks * 2 * ZKV_RANK_TILES <= tiles) c.ranks *= 2;
+    }
+    while (kv_heads % c.abreast || c.abreast * chunks > kMaxGrid) --c.abreast;
+    return c;
 }
 
 template <int kQ, bool kF8, int D, int NT>
 static int launch_decode(DecodeArgs& a, cudaStream_t st) {
     using C = Cfg<kQ, kF8, D, NT>;
-    static int raised[64] = {};  // devices whose shared-memory limit of this kernel was raised
+    const auto kernel = pool_decode_kernel<kQ, kF8, D, NT>;
+    static int raised[64] = {};  // devices whose limits of this kernel were raised
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ZKV_ERR_LAUNCH;
     if (!raised[dev]) {
-        if (cudaFuncSetAttribute((const void*)pool_decode_kernel<kQ, kF8, D, NT>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+        if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
+                cudaSuccess ||
+            cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
             return ZKV_ERR_LAUNCH;
         raised[dev] = 1;
     }
-    const int64_t rows = (int64_t)a.batch * a.kv_heads;
-    const int64_t wave = std::max(1, C::kPerSm * sm_count() / a.chunks);
-    a.groups = (int)std::min(wave, most_groups(a.batch, a.kv_heads, a.chunks, a.whole ? 0 : a.cap, C::kTile));
-    int rc = launch_pdl_kernel(pool_decode_kernel<kQ, kF8, D, NT>, dim3(a.groups * a.chunks), dim3(kThreads), C::kSmem,
-                               st, a);
+    const Cut cut = plan_call(a.batch, a.kv_heads, a.chunks, C::kRow, a.window, a.cap, C::kPerSm);
+    a.whole = cut.whole, a.ranks = cut.ranks, a.abreast = cut.whole ? 1 : cut.abreast;
+    a.head_rows = a.kv_heads / a.abreast, a.side = a.abreast * a.chunks;
+    if (!a.whole && !a.parts) return ZKV_ERR_ARG;
+    const int64_t rows = (int64_t)a.batch * a.head_rows;
+    const int64_t wave = std::max(1, C::kPerSm * sm_count() / a.side);
+    if (a.ranks > 1) a.groups = (int)rows;
+    else a.groups = (int)std::min(wave, most_groups(a.batch, a.head_rows, a.side, a.whole ? 0 : a.cap, C::kTile));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.groups * a.side * a.ranks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)a.ranks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.ranks > 1 ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return ZKV_ERR_LAUNCH;
+    int rc = launch_status();
     if (rc == ZKV_OK && !a.whole && a.groups > 1) {
         const int by_row = rows <= a.groups;
         const int cands = by_row ? (int)rows : a.groups;
-        rc = launch_pdl_kernel(pool_join_kernel<kQ, D, C::kTile>, dim3(cands * a.chunks, a.heads), dim3(kJoinThreads), 0,
+        rc = launch_pdl_kernel(pool_join_kernel<kQ, D, C::kTile>, dim3(cands * a.side, a.heads), dim3(kJoinThreads), 0,
                                st, a, C::kHeadsMax, by_row);
     }
     return rc;
@@ -1045,13 +1167,18 @@ extern "C" int zkv_pool_init(zkv_pool* p) {
     return ZKV_OK;
 }
 
-extern "C" size_t zkv_pool_decode_ws_bytes(int batch, int q_heads, int kv_heads, int head_dim, int64_t max_len) {
-    if (batch < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || head_dim < 1 || max_len < 0) return 0;
-    const pool::Heads h = pool::split_heads(q_heads / kv_heads);
-    if (h.chunks > pool::kMaxGrid) return 0;
-    const size_t grid = (size_t)pool::most_groups(batch, kv_heads, h.chunks, max_len, 64) * h.chunks;
-    const size_t rows = grid * 2 * 8 * h.tiles;
-    return pool::up256(rows * 8) + pool::up256(rows * head_dim * 4) + 256;
+// CTAs of the decode kernel on an SM do not change which calls are cut by units, so any value does here.
+static bool needs_parts(const zkv_pool* p, int batch, const pool::Heads& h, int window, int64_t cap) {
+    return !pool::plan_call(batch, p->kv_heads, h.chunks, p->head_dim * pool::element_bytes(p->dtype), window, cap, 1).whole;
+}
+
+extern "C" size_t zkv_pool_decode_ws_bytes(const zkv_pool* p, int batch, int q_heads, int window, int64_t max_len) {
+    if (pool::check_pool(p) != ZKV_OK || batch < 0 || q_heads < 1 || q_heads % p->kv_heads || window < 0 || max_len < 0)
+        return 0;
+    const pool::Heads h = pool::split_heads(q_heads / p->kv_heads);
+    if (h.chunks > pool::kMaxGrid || !needs_parts(p, batch, h, window, max_len)) return 0;
+    const size_t rows = pool::part_rows(batch, p->kv_heads, h, max_len);
+    return pool::up256(rows * 8) + pool::up256(rows * p->head_dim * 4);
 }
 
 extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int dtype, const zkv_pool* p,
@@ -1071,24 +1198,22 @@ extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int
     if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return ZKV_ERR_ALIGN;
     const int64_t room = (int64_t)width * p->block_size;
     const int64_t cap = std::min<int64_t>(max_len > 0 ? std::min(max_len, room) : room, INT32_MAX - 512);
-    const bool whole = cap <= pool::kWholeTokens;
-    if (!workspace && !whole) return ZKV_ERR_ARG;
-    if (workspace && ws_bytes < zkv_pool_decode_ws_bytes(batch, q_heads, p->kv_heads, p->head_dim, cap)) return ZKV_ERR_CAPACITY;
+    const pool::Heads hs = pool::split_heads(q_heads / p->kv_heads);
+    if (hs.chunks > pool::kMaxGrid) return ZKV_ERR_CAPACITY;
+    const bool parts = needs_parts(p, batch, hs, window, cap);
+    if (parts && !workspace) return ZKV_ERR_ARG;
+    if (parts && ws_bytes < zkv_pool_decode_ws_bytes(p, batch, q_heads, window, cap)) return ZKV_ERR_CAPACITY;
     uint64_t any = 0;
     for (uint64_t w : p->maps) any |= w;
     if (!any) return ZKV_ERR_ARG;  // zkv_pool_init was not called
-    const pool::Heads hs = pool::split_heads(q_heads / p->kv_heads);
-    if (hs.chunks > pool::kMaxGrid) return ZKV_ERR_CAPACITY;
     pool::DecodeArgs a;
     std::memcpy(&a.tk, p->maps, sizeof(a.tk));
     std::memcpy(&a.tv, p->maps + 16, sizeof(a.tv));
     a.q = (const uint8_t*)q;
     a.k_scale = p->k_scale, a.v_scale = p->v_scale;
     a.lens = lens, a.table = block_table, a.out = out, a.lse = lse, a.status = status;
-    a.stats = (float*)workspace;
-    const size_t rows = (size_t)pool::most_groups(batch, p->kv_heads, hs.chunks, cap, 64) * hs.chunks * 2 * 8 * hs.tiles;
-    a.parts = a.stats + pool::up256(rows * 8) / 4;
-    a.whole = whole, a.groups = 0;
+    a.stats = parts ? (float*)workspace : nullptr;
+    a.parts = parts ? a.stats + pool::up256(pool::part_rows(batch, p->kv_heads, hs, cap) * 8) / 4 : nullptr;
     a.q_row = q_row * 2, a.q_head = q_head * 2;
     a.table_ld = table_ld, a.n_blocks = p->n_blocks, a.cap = (int)cap;
     a.batch = batch, a.kv_heads = p->kv_heads, a.G = q_heads / p->kv_heads, a.chunks = hs.chunks, a.heads = hs.heads;

@@ -1115,7 +1115,6 @@ def rq_popcount_topk(cand, lay: RqLayout, planes, qparams, K: int, *, C: int | N
 
 # ----------------------------------------------------------------- pooled KV cache
 _POOL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
-POOL_WHOLE_TOKENS = 256   # up to this bound of the lengths pool_decode needs no workspace
 _INT32 = torch.int32
 
 
@@ -1128,7 +1127,7 @@ class KVPool:
     allocated: it holds the tensors, their addresses and strides."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "struct", "ref", "dtype", "device", "kv_heads", "head_dim",
-                 "block_size", "n_blocks", "float_like", "byte_like")
+                 "block_size", "n_blocks", "float_like", "byte_like", "ws_sizes")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _cuda(("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale))
@@ -1164,6 +1163,7 @@ class KVPool:
         self.struct = _lib.ZkvPool(_p(k), _p(v), *strides(k), *strides(v), n, S, H, D, _POOL_DTYPES[k.dtype],
                                    _p(k_scale), _p(v_scale))
         self.ref = ctypes.addressof(self.struct)
+        self.ws_sizes = {}
         self.float_like, self.byte_like = k.new_empty(0, dtype=torch.float32), k.new_empty(0, dtype=torch.uint8)
         check(lib().zkv_pool_init(self.ref), "zkv_pool_init")
 
@@ -1311,7 +1311,8 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     Returns out like q, with return_lse (out, lse [B, q_heads] fp32, natural
     log, -inf for a request without tokens, whose out is 0).  workspace:
     uint8 CUDA tensor of pool_decode_ws_bytes(...) bytes, scratch only
-    (default: allocated per call from torch's caching allocator)."""
+    (default: allocated per call, where one is needed, from torch's caching
+    allocator)."""
     shape = q.shape
     B, Hq, D = shape[0], shape[-2], shape[-1]
     if D != pool.head_dim or Hq % pool.kv_heads or len(shape) not in (3, 4) or (len(shape) == 4 and shape[1] != 1):
@@ -1338,16 +1339,14 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
             lse = pool.float_like.new_empty((B, Hq))
     elif lse.dtype != torch.float32 or lse.numel() != B * Hq or not lse.is_contiguous() or lse.device != dev:
         raise ValueError("lse must be contiguous fp32 [B, q_heads]")
-    room = width * pool.block_size
-    if 0 < max_len < room:
-        room = max_len
     ws, ws_bytes = None, 0
     if workspace is not None:
         ws, ws_bytes = workspace.data_ptr(), workspace.numel()
-    elif room > POOL_WHOLE_TOKENS:
-        ws_bytes = lib().zkv_pool_decode_ws_bytes(B, Hq, pool.kv_heads, D, room)
-        workspace = pool.byte_like.new_empty(ws_bytes)
-        ws = workspace.data_ptr()
+    else:
+        ws_bytes = pool_decode_ws_bytes(B, Hq, pool, width, max_len, window)
+        if ws_bytes:
+            workspace = pool.byte_like.new_empty(ws_bytes)
+            ws = workspace.data_ptr()
     stride = q3.stride()
     rc = lib().zkv_pool_decode(q3.data_ptr(), stride[0], stride[1], code, pool.ref, lens.data_ptr(),
                                block_table.data_ptr(), ld, width, B, Hq, D ** -0.5 if scale is None else scale, window,
@@ -1358,8 +1357,15 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     return (out, lse) if return_lse else out
 
 
-def pool_decode_ws_bytes(batch: int, q_heads: int, pool: KVPool, width: int, max_len: int = 0) -> int:
-    """Bytes of workspace that pool_decode needs for a block table of `width` columns."""
-    room = width * pool.block_size
-    return int(lib().zkv_pool_decode_ws_bytes(batch, q_heads, pool.kv_heads, pool.head_dim,
-                                              min(max_len, room) if max_len > 0 else room))
+def pool_decode_ws_bytes(batch: int, q_heads: int, pool: KVPool, width: int, max_len: int = 0, window: int = 0) -> int:
+    """Bytes of workspace that pool_decode needs for a block table of `width` columns; 0: none."""
+    key = (batch, q_heads, width, max_len, window)
+    got = pool.ws_sizes.get(key)
+    if got is None:
+        room = width * pool.block_size
+        got = int(lib().zkv_pool_decode_ws_bytes(pool.ref, batch, q_heads, window,
+                                                 min(max_len, room) if max_len > 0 else room))
+        if len(pool.ws_sizes) > 256:   # a bound that moves with every step
+            pool.ws_sizes.clear()
+        pool.ws_sizes[key] = got
+    return got
