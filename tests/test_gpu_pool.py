@@ -214,18 +214,21 @@ def test_decode_is_deterministic_and_takes_dirty_workspaces():
     first = None
     wide = torch.full((4, 9000), -1, dtype=torch.int32, device=DEV)   # a bound of the lengths that cuts the rows by units
     wide[:, :600] = table
-    for fill in (0, 255, 127, 1):
-        ws = torch.full((ops.pool_decode_ws_bytes(4, 8, pool, 600),), fill, dtype=torch.uint8, device=DEV)
-        assert ws.numel() == 0
-        got = ops.pool_decode(q, pool, i32(lens), table, return_lse=True, workspace=ws)
-        check_decode(q, k, v, ks, vs, lens, table, *got, 128 ** -0.5)
+    short = [3900, 1, 0, 257]                                        # one that does not: no workspace
+    assert ops.pool_decode_ws_bytes(4, 8, pool, 244) == 0
+    for _ in range(3):
+        got = ops.pool_decode(q, pool, i32(short), table[:, :244], return_lse=True)
+        first = first or got
+        assert all(torch.equal(x, y) for x, y in zip(first, got))
+    check_decode(q, k, v, ks, vs, short, table, *first, 128 ** -0.5)
+    first = None
     for fill in (0, 255, 127, 1):
         ws = torch.full((ops.pool_decode_ws_bytes(4, 8, pool, 9000),), fill, dtype=torch.uint8, device=DEV)
         assert ws.numel() > 0
-        table = wide
-        got = ops.pool_decode(q, pool, i32(lens), table, return_lse=True, workspace=ws)
+        got = ops.pool_decode(q, pool, i32(lens), wide, return_lse=True, workspace=ws)
         first = first or got
         assert all(torch.equal(x, y) for x, y in zip(first, got))
+    check_decode(q, k, v, ks, vs, lens, wide, *first, 128 ** -0.5)
 
 
 def test_decode_strides_and_out():

@@ -60,6 +60,11 @@ constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxGrid = 320;                   // CTAs that a workspace is sized for
 constexpr int kWholeTokens = 256;               // requests up to this length are never cut
 constexpr int kMaxRanks = 16;                   // CTAs of a cluster that shares a row
+// Up to kWholeBytes of K and V and kRankTiles tiles a CTA the cluster's one launch is ahead of ranges and a join (8 kv
+// heads of 128, bf16: one request of 4096 10.0 us on the GPU both ways, of 8192 13.7 against 12.2 and 6 us less to
+// issue, of 16384 20.7 against 14.7; 16 of 1000 13.0 against 18.0, 4 of 4096 13.7 against 15.2).
+constexpr int64_t kWholeBytes = 64 << 20;
+constexpr int kRankTiles = 8;
 constexpr uint64_t kWaitNs = 2000000000ull;     // limit of each wait inside a CTA
 
 // What a unit is, written by the producer beside its stage.
@@ -114,11 +119,12 @@ struct Cfg {
     static constexpr int kHeadsMax = 8 * NT;
     static constexpr int kQPitch = D * 2 + 16;
     static constexpr int kQSlot = kHeadsMax * kQPitch;  // a multiple of 16
-    static constexpr int kFixed = 1024 + 1024;                   // alignment; barriers, units, statistics
+    static constexpr int kFixed = 1024;                          // alignment of the swizzled boxes
     static constexpr int kStage = 2 * kKv + kQSlot + (int)sizeof(Unit);
     static constexpr int kMl = 2 * kConsumers * kHeadsMax * 8;
-    static constexpr int kHalf = 232448 / 2 - 1024;              // shared memory of one of two CTAs on an SM
-    static constexpr int kWhole = 232448 - 1024;
+    static constexpr int kOther = 1024 + 512;                    // an SM's reserve for a CTA; its static variables
+    static constexpr int kHalf = 233472 / 2 - kOther;            // shared memory of one of two CTAs on an SM
+    static constexpr int kWhole = 233472 - kOther;
     static constexpr int kPerSm = (kHalf - kFixed - kMl) / kStage >= 3 ? 2 : 1;
     static constexpr int kFit = ((kPerSm == 2 ? kHalf : kWhole) - kFixed - kMl) / kStage;
     static constexpr int kStages = kFit < 8 ? kFit : 8;
@@ -257,22 +263,38 @@ __device__ __forceinline__ Units count_units(const DecodeArgs& a, int64_t* sh) {
     u.before = block_sum_before(u.mine, sh, &u.total);
     return u;
 }
-// The request of unit `u` and the unit's number in it, by the one thread that holds it.
+// The request of unit `u`, the unit's number in it and the request's length, by the one thread that holds it.
 template <int kTile>
-__device__ __forceinline__ bool locate(const DecodeArgs& a, const Units& x, int64_t u, int& b, int64_t& off, int& tiles) {
+__device__ __forceinline__ bool locate(const DecodeArgs& a, const Units& x, int64_t u, int& b, int64_t& off, int& len) {
     if (u < x.before || u >= x.before + x.mine) return false;
     off = u - x.before;
     for (b = x.b_lo;; ++b) {
-        tiles = row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + b)));
-        const int64_t n = (int64_t)tiles * a.head_rows;
+        len = __ldcg(a.lens + b);
+        const int64_t n = (int64_t)row_tiles<kTile>(a, request_len(a, len)) * a.head_rows;
         if (off < n || b + 1 >= x.b_hi) return true;
         off -= n;
     }
 }
-// CTA (of `ctas`) that has unit u of `total`: ranges are [total c / ctas, total (c + 1) / ctas).
-__device__ __forceinline__ int64_t owner_cta(int64_t u, int64_t total, int64_t ctas) {
-    return ((u + 1) * ctas - 1) / total;
+
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {  // x >= 0, y > 0; in 32 bits where they allow it
+    return (uint64_t)(x | y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
 }
+
+// The list cut into equal ranges, the first `longer` of them one unit longer.
+struct Ranges {
+    int64_t count, size, longer;
+
+    __device__ __forceinline__ Ranges(const DecodeArgs& a, int64_t total) {
+        count = min((int64_t)a.groups, total);
+        size = quotient(total, count);
+        longer = total - size * count;
+    }
+    __device__ __forceinline__ int64_t begin(int64_t c) const { return c * size + min(c, longer); }
+    __device__ __forceinline__ int64_t owner(int64_t u) const {
+        const int64_t split = longer * (size + 1);
+        return u < split ? quotient(u, size + 1) : longer + quotient(u - split, size);
+    }
+};
 
 // ------------------------------------------------------------ consumers
 template <int kQ, bool kF8, int D, int NT>
@@ -521,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     __shared__ uint64_t full[C::kStages], empty[C::kStages], epi;
     __shared__ int64_t sh[32];
     __shared__ int64_t s_off;
-    __shared__ int s_b;
+    __shared__ int s_b, s_len;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < C::kStages; ++i) {
@@ -530,6 +552,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         }
         mbar_init(&epi, kConsumers);
         mbar_fence_init();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.tk)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.tv)) : "memory");
     }
     const int rank = blockIdx.x % a.ranks, block = blockIdx.x / a.ranks;
     const int member = block % a.side, chunk = member % a.chunks, abreast = member / a.chunks;
@@ -541,20 +565,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     int64_t u0, u1;
     if (a.whole) {
         const int64_t rows = (int64_t)a.batch * a.head_rows;
-        u0 = rows * c / a.groups;
-        u1 = rows * (c + 1) / a.groups;
+        u0 = quotient(rows * c, a.groups);
+        u1 = quotient(rows * (c + 1), a.groups);
         __syncthreads();
         if (u0 == u1) return;
     } else {
         const Units x = count_units<C::kTile, kThreads>(a, sh);
-        const int64_t ctas = min((int64_t)a.groups, x.total);
-        if (c >= ctas) return;
-        u0 = x.total * c / ctas;
-        u1 = x.total * (c + 1) / ctas;
-        int b, tiles;
+        const Ranges cuts(a, x.total);
+        if (c >= cuts.count) return;
+        u0 = cuts.begin(c);
+        u1 = cuts.begin(c + 1);
+        int b, len;
         int64_t off;
-        if (locate<C::kTile>(a, x, u0, b, off, tiles)) {
+        if (locate<C::kTile>(a, x, u0, b, off, len)) {
             s_b = b;
+            s_len = len;
             s_off = off;
         }
         __syncthreads();
@@ -562,8 +587,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
 
     if (warp == kConsumers) {
         // ---------------------------------------------------- producer
-        int b = a.whole ? (int)(u0 / a.head_rows) : s_b;
-        int next = __ldcg(a.lens + b);  // the length of the next request to begin, asked for one request ahead
+        int b = a.whole ? (int)quotient(u0, a.head_rows) : s_b;
+        int next = a.whole ? __ldcg(a.lens + b) : s_len;  // the next request's length, asked for one request ahead
         int len, lo, tile_first, tiles;
         auto begin_request = [&]() {
             if (next < 0 || next > a.cap) raise_status(a.status, ZKV_ERR_RANGE);
@@ -574,11 +599,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             if (b + 1 < a.batch) next = __ldcg(a.lens + b + 1);
         };
         begin_request();
-        int hr = a.whole ? (int)(u0 % a.head_rows) : (int)(s_off / tiles);  // row of the request
-        int tile = a.whole ? (int)((int64_t)tiles * rank / a.ranks) : (int)(s_off % tiles);
+        int hr, tile;  // row of the request, tile of the row
+        if (a.whole) {
+            hr = (int)(u0 - (int64_t)b * a.head_rows);
+            tile = (int)((uint32_t)tiles * (uint32_t)rank / (uint32_t)a.ranks);
+        } else {
+            hr = (int)quotient(s_off, tiles);
+            tile = (int)(s_off - (int64_t)hr * tiles);
+        }
         bool none = false;  // more CTAs than tiles: this one has an empty unit
         if (a.ranks > 1) {
-            tiles = (int)((int64_t)tiles * (rank + 1) / a.ranks);
+            tiles = (int)((uint32_t)tiles * (uint32_t)(rank + 1) / (uint32_t)a.ranks);
             none = tile == tiles;
             if (none) tiles = tile + 1;
         }
@@ -848,14 +879,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
 }
 
 // ------------------------------------------------------------ joining split rows
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 128;  // few enough to wait beside two decode CTAs
 
 // The parts of a split row, in CTA order: slot 1 of its first CTA, slot 0 of
 // the others.  One block per (candidate row, chunk; query head of the chunk):
 // the candidates are the rows if there are no more of them than CTAs, else the
 // rows in which a CTA's range ends.  Which parts there are follows from the
 // lengths, so it is known before the decode grid is waited for; then a warp
-// takes every eighth part, eight loads in flight, with the dims over its lanes.
+// takes every fourth part, eight loads in flight, with the dims over its lanes.
 template <int kQ, int D, int kTile>
 __global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_constant__ DecodeArgs a, int heads_max,
                                                                  int by_row) {
@@ -874,7 +905,7 @@ __global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_co
         return;
     }
     const Units x = count_units<kTile, kJoinThreads>(a, sh);
-    const int64_t ctas = min((int64_t)a.groups, x.total);
+    const Ranges cuts(a, x.total);
     if (by_row) {
         const int b = cand / a.head_rows;
         if (b >= x.b_lo && b < x.b_hi) {
@@ -888,23 +919,24 @@ __global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_co
             s_row[1] = s_row[0] + tiles;
         }
     } else {
-        if (cand >= ctas) {
+        if (cand >= cuts.count) {
             grid_dep_wait();
             return;
         }
-        const int64_t u = x.total * (cand + 1) / ctas - 1;
-        int b, tiles;
+        const int64_t u = cuts.begin(cand + 1) - 1;
+        int b, len;
         int64_t off;
-        if (locate<kTile>(a, x, u, b, off, tiles)) {
+        if (locate<kTile>(a, x, u, b, off, len)) {
+            const int tiles = row_tiles<kTile>(a, request_len(a, len));
             s_bh[0] = b;
-            s_bh[1] = (int)(off / tiles);
-            s_row[0] = u - off % tiles;
+            s_bh[1] = (int)quotient(off, tiles);
+            s_row[0] = u - (off - (int64_t)s_bh[1] * tiles);
             s_row[1] = s_row[0] + tiles;
         }
     }
     __syncthreads();
-    const int64_t c0 = owner_cta(s_row[0], x.total, ctas);
-    const int n = (int)(owner_cta(s_row[1] - 1, x.total, ctas) - c0) + 1;
+    const int64_t c0 = cuts.owner(s_row[0]);
+    const int n = (int)(cuts.owner(s_row[1] - 1) - c0) + 1;
     const int b = s_bh[0], h = s_bh[1] * a.abreast + member / a.chunks;
     grid_dep_wait();
     if (n == 1 || (!by_row && c0 != cand)) return;
@@ -1072,23 +1104,17 @@ struct Cut {
     int ranks;     // CTAs of a cluster that share a row, if `whole`
     int abreast;   // kv heads walked side by side, if not
 };
-#ifndef ZKV_CLUSTER_BYTES
-#define ZKV_CLUSTER_BYTES (64 << 20)
-#endif
-#ifndef ZKV_RANK_TILES
-#define ZKV_RANK_TILES 1
-#endif
-static Cut plan_call(int batch, int kv_heads, int chunks, int row_bytes, int window, int64_t cap, int per_sm) {
+static Cut plan_call(int batch, int kv_heads, int chunks, int row_bytes, int window, int64_t cap) {
     Cut c{false, 1, 8};
     const int tile = tile_tokens(row_bytes);
     const int64_t longest = window > 0 ? std::min<int64_t>(cap, window) : cap;
     const int64_t rows = (int64_t)batch * kv_heads * chunks;
     const int64_t tiles = (longest + tile - 1) / tile + (window > 0 ? 1 : 0);
-    c.whole = longest <= kWholeTokens || 2 * (int64_t)batch * kv_heads * longest * row_bytes <= ZKV_CLUSTER_BYTES;
-    if (c.whole) {
-        const int64_t wave = (int64_t)per_sm * sm_count();
-        while (c.ranks < kMaxRanks && rows * c.ranks * 2 <= wave && c.ranks * 2 * ZKV_RANK_TILES <= tiles) c.ranks *= 2;
-    }
+    const int64_t bytes = 2 * (int64_t)batch * kv_heads * longest * row_bytes;
+    const int64_t wave = 2 * sm_count();  // (one CTA an SM, as 256 dims have it, takes two turns)
+    while (c.ranks < kMaxRanks && rows * c.ranks * 2 <= wave && c.ranks * 2 <= tiles) c.ranks *= 2;
+    c.whole = longest <= kWholeTokens || (bytes <= kWholeBytes && tiles <= c.ranks * kRankTiles);
+    if (!c.whole) c.ranks = 1;
     while (kv_heads % c.abreast || c.abreast * chunks > kMaxGrid) --c.abreast;
     return c;
 }
@@ -1107,7 +1133,7 @@ static int launch_decode(DecodeArgs& a, cudaStream_t st) {
             return ZKV_ERR_LAUNCH;
         raised[dev] = 1;
     }
-    const Cut cut = plan_call(a.batch, a.kv_heads, a.chunks, C::kRow, a.window, a.cap, C::kPerSm);
+    const Cut cut = plan_call(a.batch, a.kv_heads, a.chunks, C::kRow, a.window, a.cap);
     a.whole = cut.whole, a.ranks = cut.ranks, a.abreast = cut.whole ? 1 : cut.abreast;
     a.head_rows = a.kv_heads / a.abreast, a.side = a.abreast * a.chunks;
     if (!a.whole && !a.parts) return ZKV_ERR_ARG;
@@ -1167,9 +1193,8 @@ extern "C" int zkv_pool_init(zkv_pool* p) {
     return ZKV_OK;
 }
 
-// CTAs of the decode kernel on an SM do not change which calls are cut by units, so any value does here.
 static bool needs_parts(const zkv_pool* p, int batch, const pool::Heads& h, int window, int64_t cap) {
-    return !pool::plan_call(batch, p->kv_heads, h.chunks, p->head_dim * pool::element_bytes(p->dtype), window, cap, 1).whole;
+    return !pool::plan_call(batch, p->kv_heads, h.chunks, p->head_dim * pool::element_bytes(p->dtype), window, cap).whole;
 }
 
 extern "C" size_t zkv_pool_decode_ws_bytes(const zkv_pool* p, int batch, int q_heads, int window, int64_t max_len) {
