@@ -103,7 +103,7 @@ struct DecodeArgs {
     int groups;     // ranges
     int whole;      // rows are not cut by units
     int ranks;      // CTAs (a cluster) that share a row, if `whole`
-    int shift, lg_box, window;
+    int shift, lg_box, width, window;
     float scale, softcap;
 };
 
@@ -249,6 +249,7 @@ __device__ __forceinline__ int row_tiles(const DecodeArgs& a, int len) {
 // requests [b_lo, b_hi), whose units are [before, before + mine).
 struct Units {
     int b_lo, b_hi;
+    int len;  // of request b_lo
     int64_t before, mine, total;
 };
 template <int kTile, int kN>
@@ -258,7 +259,12 @@ __device__ __forceinline__ Units count_units(const DecodeArgs& a, int64_t* sh) {
     u.b_lo = min(a.batch, (int)threadIdx.x * per);
     u.b_hi = min(a.batch, u.b_lo + per);
     u.mine = 0;
-    for (int b = u.b_lo; b < u.b_hi; ++b)
+    u.len = 0;
+    if (u.b_lo < u.b_hi) {
+        u.len = __ldcg(a.lens + u.b_lo);
+        u.mine = (int64_t)row_tiles<kTile>(a, request_len(a, u.len)) * a.head_rows;
+    }
+    for (int b = u.b_lo + 1; b < u.b_hi; ++b)
         u.mine += (int64_t)row_tiles<kTile>(a, request_len(a, __ldcg(a.lens + b))) * a.head_rows;
     u.before = block_sum_before(u.mine, sh, &u.total);
     return u;
@@ -268,11 +274,12 @@ template <int kTile>
 __device__ __forceinline__ bool locate(const DecodeArgs& a, const Units& x, int64_t u, int& b, int64_t& off, int& len) {
     if (u < x.before || u >= x.before + x.mine) return false;
     off = u - x.before;
-    for (b = x.b_lo;; ++b) {
-        len = __ldcg(a.lens + b);
+    len = x.len;
+    for (b = x.b_lo;;) {
         const int64_t n = (int64_t)row_tiles<kTile>(a, request_len(a, len)) * a.head_rows;
         if (off < n || b + 1 >= x.b_hi) return true;
         off -= n;
+        len = __ldcg(a.lens + ++b);
     }
 }
 
@@ -559,6 +566,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     const int member = block % a.side, chunk = member % a.chunks, abreast = member / a.chunks;
     const int64_t c = block / a.side;
     const int n_heads = min(a.heads, a.G - chunk * a.heads);
+    // the arguments' constant-cache lines, while the previous grid ends
+    asm volatile("" ::"l"(a.q), "l"(a.lens), "l"(a.parts), "l"(a.q_head), "r"(a.batch), "r"(a.groups), "f"(a.softcap));
     grid_dep_wait();
     grid_dep_launch_next();  // the join kernel may become resident; it waits for this grid
     // ---- this CTA's range [u0, u1): of units, or of rows where those are not split
@@ -598,6 +607,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             tiles = row_tiles<C::kTile>(a, len);
             if (b + 1 < a.batch) next = __ldcg(a.lens + b + 1);
         };
+        // a row that begins at token 0 needs the table's first entries: asked for beside its length
+        int ids = -1, ids_next = -1, ids_b = -1, ids_at = 0;
+        if (a.whole && a.ranks == 1 && a.window == 0) {
+            const int32_t* row = a.table + b * a.table_ld;
+            ids = lane < a.width ? __ldcg(row + lane) : -1;
+            ids_next = 32 + lane < a.width ? __ldcg(row + 32 + lane) : -1;
+            ids_b = b;
+        }
         begin_request();
         int hr, tile;  // row of the request, tile of the row
         if (a.whole) {
@@ -614,7 +631,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             if (none) tiles = tile + 1;
         }
         int64_t row_begin = a.whole ? u0 : u0 - tile;  // unit at which the row begins (its number, where rows are whole)
-        int ids = -1, ids_next = -1, ids_b = -1, ids_at = 0;
         int n_row = 0;                  // rows begun in this CTA
         const int boxes = C::kTile >> a.lg_box, box_bytes = C::kRow << a.lg_box;
         bool ok = true, end = false;
@@ -845,11 +861,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         const int head = idx / (D / 4), d = 4 * (idx % (D / 4));
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int r0 = 0; r0 < a.ranks; r0 += 4) {
-            float2 s[4];
-            float4 y[4];
+        for (int r0 = 0; r0 < a.ranks; r0 += 8) {
+            float2 s[8];
+            float4 y[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 8; ++k) {
                 s[k] = make_float2(-INFINITY, 0.f);
                 y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (r0 + k < a.ranks) {
@@ -859,11 +875,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             }
             float mx = m;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mx = fmaxf(mx, s[k].x);
+            for (int k = 0; k < 8; ++k) mx = fmaxf(mx, s[k].x);
             const float ref = mx == -INFINITY ? 0.f : mx, old = exp2_fast(m - ref);
             l *= old, o.x *= old, o.y *= old, o.z *= old, o.w *= old;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 8; ++k) {
                 const float w = exp2_fast(s[k].x - ref);
                 l += w * s[k].y;
                 o.x += w * y[k].x, o.y += w * y[k].y, o.z += w * y[k].z, o.w += w * y[k].w;
@@ -1242,7 +1258,7 @@ extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int
     a.q_row = q_row * 2, a.q_head = q_head * 2;
     a.table_ld = table_ld, a.n_blocks = p->n_blocks, a.cap = (int)cap;
     a.batch = batch, a.kv_heads = p->kv_heads, a.G = q_heads / p->kv_heads, a.chunks = hs.chunks, a.heads = hs.heads;
-    a.shift = pool::log2_of(p->block_size), a.lg_box = pool::log2_of(pool::box_tokens(p)), a.window = window;
+    a.shift = pool::log2_of(p->block_size), a.lg_box = pool::log2_of(pool::box_tokens(p)), a.width = width, a.window = window;
     a.scale = scale, a.softcap = softcap;
     cudaStream_t st = (cudaStream_t)stream;
     if (p->dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, false>(a, p->head_dim, hs.tiles, st);

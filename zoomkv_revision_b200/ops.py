@@ -1118,6 +1118,11 @@ _POOL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 _INT32 = torch.int32
 
 
+def _raw_stream(index: int) -> int:
+    """The raw handle of the current stream of CUDA device `index`."""
+    return torch.cuda.current_stream(index).cuda_stream if _RAW_STREAM is None else _RAW_STREAM(index)
+
+
 class KVPool:
     """One layer's pooled KV cache: k, v [n_blocks, block_size, kv_heads, head_dim]
     bf16, fp16 or float8_e4m3fn CUDA tensors, any strides with whole 16-byte
@@ -1127,7 +1132,7 @@ class KVPool:
     allocated: it holds the tensors, their addresses and strides."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "struct", "ref", "dtype", "device", "kv_heads", "head_dim",
-                 "block_size", "n_blocks", "float_like", "byte_like", "ws_sizes")
+                 "block_size", "n_blocks", "float_like", "byte_like", "ws_sizes", "index", "code")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _cuda(("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale))
@@ -1158,7 +1163,7 @@ class KVPool:
             return s
 
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self.index, self.code = k.dtype, k.device, k.get_device(), _POOL_DTYPES[k.dtype]
         self.n_blocks, self.block_size, self.kv_heads, self.head_dim = n, S, H, D
         self.struct = _lib.ZkvPool(_p(k), _p(v), *strides(k), *strides(v), n, S, H, D, _POOL_DTYPES[k.dtype],
                                    _p(k_scale), _p(v_scale))
@@ -1168,23 +1173,21 @@ class KVPool:
         check(lib().zkv_pool_init(self.ref), "zkv_pool_init")
 
 
-def _ints32(**tensors):
-    """int32, contiguous CUDA tensors of one device (None is left out)."""
+def _refuse_int32(names, tensors):
+    """The error for the first of `tensors` that is not int32, contiguous and on one CUDA device."""
     dev = -1
-    for name, t in tensors.items():
+    for name, t in zip(names, tensors):
         if t is None:
             continue
         if t.dtype is not _INT32:
             raise TypeError(f"{name} must be torch.int32; got {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-        at = t.get_device()
-        if at < 0:
+        if t.get_device() < 0:
             raise ValueError(f"{name} must be a CUDA tensor")
-        if dev < 0:
-            dev = at
-        elif at != dev:
+        if dev >= 0 and t.get_device() != dev:
             raise ValueError("tensors must be on one device")
+        dev = t.get_device()
 
 
 def _block_table(t, batch, dev):
@@ -1192,7 +1195,7 @@ def _block_table(t, batch, dev):
     if t.dtype is not _INT32:
         raise TypeError(f"block_table must be torch.int32; got {t.dtype}")
     shape = t.shape
-    if len(shape) != 2 or shape[0] != batch or t.device != dev:
+    if len(shape) != 2 or shape[0] != batch or t.get_device() != dev:
         raise ValueError("block_table must be [batch, width] on the device of lens")
     width = shape[1]
     ld, one = t.stride()
@@ -1217,25 +1220,31 @@ def pool_plan(lens, new_lens, block_table, free_blocks, n_free, block_size: int,
     lens_out / n_free_out default to lens / n_free in place.  A request that
     finds no room keeps its length and blocks; status [1] int32 then gets
     ZKV_ERR_CAPACITY (3).  Returns slots."""
-    _ints32(lens=lens, new_lens=new_lens, free_blocks=free_blocks, n_free=n_free, positions=positions, cu_new=cu_new,
-            lens_out=lens_out, n_free_out=n_free_out, status=status)
-    B = lens.numel()
-    ld, width = _block_table(block_table, B, lens.device)
-    if slots.dtype != torch.int64:
+    dev = lens.get_device()
+    for t in (lens, free_blocks, n_free, new_lens, positions, cu_new, lens_out, n_free_out, status):
+        if t is not None and (t.dtype is not _INT32 or t.get_device() != dev or dev < 0 or not t.is_contiguous()):
+            _refuse_int32(("lens", "free_blocks", "n_free", "new_lens", "positions", "cu_new", "lens_out", "n_free_out",
+                           "status"), (lens, free_blocks, n_free, new_lens, positions, cu_new, lens_out, n_free_out, status))
+    B, n_slots = lens.numel(), slots.numel()
+    ld, width = _block_table(block_table, B, dev)
+    if slots.dtype is not torch.int64:
         raise TypeError(f"slots must be torch.int64; got {slots.dtype}")
-    if not slots.is_contiguous() or slots.device != lens.device:
+    if not slots.is_contiguous() or slots.get_device() != dev:
         raise ValueError("slots must be contiguous, on the device of lens")
     if (new_lens is not None and new_lens.numel() != B) or (lens_out is not None and lens_out.numel() != B):
         raise ValueError("new_lens and lens_out must have one value per request")
-    if (positions is not None and positions.numel() < slots.numel()) or (cu_new is not None and cu_new.numel() < B + 1):
+    if (positions is not None and positions.numel() < n_slots) or (cu_new is not None and cu_new.numel() <= B):
         raise ValueError("positions needs one value per slot and cu_new [B + 1]")
-    if lens_out is None:
-        lens_out = lens
-    if n_free_out is None:
-        n_free_out = n_free
-    check(lib().zkv_pool_plan(_p(lens), _p(new_lens), B, block_size, _p(block_table), ld, width, _p(free_blocks),
-                              _p(n_free), free_blocks.numel(), _p(slots), _p(positions), slots.numel(), _p(cu_new),
-                              _p(lens_out), _p(n_free_out), _p(status), _stream(lens)), "zkv_pool_plan")
+    at, count = lens.data_ptr(), n_free.data_ptr()
+    rc = lib().zkv_pool_plan(at, None if new_lens is None else new_lens.data_ptr(), B, block_size, block_table.data_ptr(),
+                             ld, width, free_blocks.data_ptr(), count, free_blocks.numel(), slots.data_ptr(),
+                             None if positions is None else positions.data_ptr(), n_slots,
+                             None if cu_new is None else cu_new.data_ptr(),
+                             at if lens_out is None else lens_out.data_ptr(),
+                             count if n_free_out is None else n_free_out.data_ptr(),
+                             None if status is None else status.data_ptr(), _raw_stream(dev))
+    if rc:
+        check(rc, "zkv_pool_plan")
     return slots
 
 
@@ -1244,22 +1253,27 @@ def pool_release(done, lens, block_table, free_blocks, n_free, block_size: int, 
     """Pushes the blocks of the requests with done[b] on the free stack
     (free_blocks, n_free) and sets their lengths to 0.  done [B] bool;
     the others as in pool_plan; lens_out / n_free_out default to in place."""
-    _ints32(lens=lens, free_blocks=free_blocks, n_free=n_free, lens_out=lens_out, n_free_out=n_free_out, status=status)
+    dev = lens.get_device()
+    for t in (lens, free_blocks, n_free, lens_out, n_free_out, status):
+        if t is not None and (t.dtype is not _INT32 or t.get_device() != dev or dev < 0 or not t.is_contiguous()):
+            _refuse_int32(("lens", "free_blocks", "n_free", "lens_out", "n_free_out", "status"),
+                          (lens, free_blocks, n_free, lens_out, n_free_out, status))
     B = lens.numel()
-    ld, width = _block_table(block_table, B, lens.device)
-    if done.dtype != torch.bool:
+    ld, width = _block_table(block_table, B, dev)
+    if done.dtype is not torch.bool:
         raise TypeError(f"done must be torch.bool; got {done.dtype}")
-    if done.numel() != B or not done.is_contiguous() or done.device != lens.device:
+    if done.numel() != B or not done.is_contiguous() or done.get_device() != dev:
         raise ValueError("done must be contiguous [B], on the device of lens")
     if lens_out is not None and lens_out.numel() != B:
         raise ValueError("lens_out must have one value per request")
-    if lens_out is None:
-        lens_out = lens
-    if n_free_out is None:
-        n_free_out = n_free
-    check(lib().zkv_pool_release(_p(done), _p(lens), B, block_size, _p(block_table), ld, width, _p(free_blocks),
-                                 _p(n_free), free_blocks.numel(), _p(lens_out), _p(n_free_out), _p(status),
-                                 _stream(lens)), "zkv_pool_release")
+    at, count = lens.data_ptr(), n_free.data_ptr()
+    rc = lib().zkv_pool_release(done.data_ptr(), at, B, block_size, block_table.data_ptr(), ld, width,
+                                free_blocks.data_ptr(), count, free_blocks.numel(),
+                                at if lens_out is None else lens_out.data_ptr(),
+                                count if n_free_out is None else n_free_out.data_ptr(),
+                                None if status is None else status.data_ptr(), _raw_stream(dev))
+    if rc:
+        check(rc, "zkv_pool_release")
 
 
 def _whole_rows(t):
@@ -1275,25 +1289,25 @@ def pool_write(k, v, slots, pool: KVPool, *, status=None):
     [n_tokens, kv_heads, head_dim] bf16 or fp16 (the pool's type; any of the
     two for an e4m3 pool, which stores e4m3(row / scale), saturated at 448);
     slots [n_tokens] int64 of pool_plan, -1 = none."""
-    if k.shape != v.shape or k.dim() != 3 or k.shape[1] != pool.kv_heads or k.shape[2] != pool.head_dim:
-        raise ValueError(f"k and v must be [n_tokens, {pool.kv_heads}, {pool.head_dim}]; got {tuple(k.shape)} and "
+    shape = k.shape
+    if v.shape != shape or len(shape) != 3 or shape[1] != pool.kv_heads or shape[2] != pool.head_dim:
+        raise ValueError(f"k and v must be [n_tokens, {pool.kv_heads}, {pool.head_dim}]; got {tuple(shape)} and "
                          f"{tuple(v.shape)}")
-    dt = k.dtype
-    if v.dtype != dt or dt not in (torch.bfloat16, torch.float16) or (pool.dtype != dt and
-                                                                      pool.dtype != torch.float8_e4m3fn):
+    dt, n = k.dtype, shape[0]
+    code = _POOL_DTYPES.get(dt, 2)
+    if v.dtype is not dt or code == 2 or (pool.dtype is not dt and pool.code != 2):
         raise TypeError(f"k {dt} and v {v.dtype} do not go into a {pool.dtype} pool")
-    if slots.dtype != torch.int64:
-        raise TypeError(f"slots must be torch.int64; got {slots.dtype}")
-    n = k.shape[0]
+    if slots.dtype is not torch.int64 or (status is not None and status.dtype is not _INT32):
+        raise TypeError("slots must be torch.int64 and status torch.int32")
     if slots.numel() < n or not slots.is_contiguous():
         raise ValueError("slots must be contiguous, one per token")
-    dev = pool.device
-    if k.device != dev or v.device != dev or slots.device != dev:
+    dev = pool.index
+    if k.get_device() != dev or v.get_device() != dev or slots.get_device() != dev:
         raise ValueError("tensors must be on the pool's device")
     k, v = _whole_rows(k), _whole_rows(v)
     ks, vs = k.stride(), v.stride()
-    rc = lib().zkv_pool_write(k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _POOL_DTYPES[dt],
-                              slots.data_ptr(), n, pool.ref, None if status is None else status.data_ptr(), _stream(k))
+    rc = lib().zkv_pool_write(k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code, slots.data_ptr(), n, pool.ref,
+                              None if status is None else status.data_ptr(), _raw_stream(dev))
     if rc:
         check(rc, "zkv_pool_write")
 
@@ -1318,11 +1332,11 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     if D != pool.head_dim or Hq % pool.kv_heads or len(shape) not in (3, 4) or (len(shape) == 4 and shape[1] != 1):
         raise ValueError(f"q must be [B, (1,) q_heads, {pool.head_dim}] with q_heads a multiple of {pool.kv_heads}; got "
                          f"{tuple(shape)}")
-    dt, dev = q.dtype, pool.device
+    dt, dev = q.dtype, pool.index
     code = _POOL_DTYPES.get(dt, 2)
-    if code == 2 or (pool.dtype != dt and pool.dtype != torch.float8_e4m3fn):
+    if code == 2 or (pool.dtype is not dt and pool.code != 2):
         raise TypeError(f"q {dt} does not fit a {pool.dtype} pool")
-    if q.device != dev or lens.device != dev:
+    if q.get_device() != dev or lens.get_device() != dev:
         raise ValueError("tensors must be on the pool's device")
     if lens.dtype is not _INT32 or (status is not None and status.dtype is not _INT32):
         raise TypeError("lens and status must be torch.int32")
@@ -1332,12 +1346,13 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     q3 = _whole_rows(q if len(shape) == 3 else q[:, 0])
     if out is None:
         out = q.new_empty(shape)
-    elif out.shape != shape or out.dtype != dt or not out.is_contiguous() or out.device != dev:
+    elif out.shape != shape or out.dtype is not dt or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError("out must be contiguous, shaped and typed like q")
     if lse is None:
         if return_lse:
             lse = pool.float_like.new_empty((B, Hq))
-    elif lse.dtype != torch.float32 or lse.numel() != B * Hq or not lse.is_contiguous() or lse.device != dev:
+    elif (lse.dtype is not torch.float32 or lse.numel() != B * Hq or not lse.is_contiguous()
+          or lse.get_device() != dev):
         raise ValueError("lse must be contiguous fp32 [B, q_heads]")
     ws, ws_bytes = None, 0
     if workspace is not None:
@@ -1351,7 +1366,7 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     rc = lib().zkv_pool_decode(q3.data_ptr(), stride[0], stride[1], code, pool.ref, lens.data_ptr(),
                                block_table.data_ptr(), ld, width, B, Hq, D ** -0.5 if scale is None else scale, window,
                                softcap, max_len, out.data_ptr(), None if lse is None else lse.data_ptr(),
-                               None if status is None else status.data_ptr(), ws, ws_bytes, _stream(q))
+                               None if status is None else status.data_ptr(), ws, ws_bytes, _raw_stream(dev))
     if rc:
         check(rc, "zkv_pool_decode")
     return (out, lse) if return_lse else out
