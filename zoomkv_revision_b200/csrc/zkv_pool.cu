@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(kMaxThreads) pool_plan_kernel(const __grid_con
     const int tid = threadIdx.x, nt = blockDim.x;
     const int S = 1 << a.shift;
     int code = 0;
+    pdl_begin();
     int64_t n_free = *a.n_free;
     if (n_free < 0 || n_free > a.n_blocks) {
         code = ZKV_ERR_RANGE;
@@ -196,6 +197,7 @@ __global__ void __launch_bounds__(kMaxThreads) pool_release_kernel(const __grid_
     const int tid = threadIdx.x, nt = blockDim.x;
     const int S = 1 << a.shift;
     int code = 0;
+    pdl_begin();
     int64_t n_free = *a.n_free;
     if (n_free < 0 || n_free > a.n_blocks) {
         code = ZKV_ERR_RANGE;
@@ -295,7 +297,8 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 // rounding (the products are off by 3 * 2^-24 at most), rounding is monotone,
 // so where both ends give one code the quotient has that code; else (a
 // quotient that close to the middle of two codes) it is divided.  The
-// division in every element made 8191 tokens of 8 x 128 take 13.2 us.
+// division in every element made 8191 tokens of 8 x 128 take 13.2 us
+// (10.7 without, in L2).
 struct Divisor {
     float scale, low, high;
     bool plain;  // the reciprocal is not a normal number: divide
@@ -321,13 +324,17 @@ struct Divisor {
 };
 
 constexpr int kWriteThreads = 256;
-constexpr int kWriteUnroll = 4;
 
 // One 16-byte store per item (token, head, part of the row); K at blockIdx.y
-// 0, V at 1.  A thread's kWriteUnroll source loads are in flight together.
-// kMode 0: 16-bit copy; 1: bf16 -> e4m3; 2: fp16 -> e4m3 (two loads an item).
+// 0, V at 1.  kMode 0: 16-bit copy, two items a thread; 1: bf16 -> e4m3, one
+// item (two loads); 2: fp16 -> e4m3.  32 source bytes a thread, all loads
+// before the first store: with 128 the grid is one wave that reads, converts
+// and writes in step (cold, 8191 tokens of 8 x 128 to e4m3 14.7 us, with 32
+// 11.1 us, its bytes alone 7.7; 16384 tokens bf16 22.7 and 22.6, bytes 20.6).
 template <int kMode>
 __global__ void __launch_bounds__(kWriteThreads) pool_write_kernel(const __grid_constant__ WriteArgs a) {
+    pdl_begin();
+    constexpr int kWriteUnroll = kMode ? 1 : 2;
     const int y = blockIdx.y;
     constexpr int kLoads = kMode ? 2 : 1;
     const int64_t first = (int64_t)blockIdx.x * (kWriteThreads * kWriteUnroll) + threadIdx.x;
@@ -347,7 +354,7 @@ __global__ void __launch_bounds__(kWriteThreads) pool_write_kernel(const __grid_
         const uint4* p = reinterpret_cast<const uint4*>(a.src[y] + tok * a.src_token[y] + head[u] * a.src_head[y]) +
                          part * kLoads;
 #pragma unroll
-        for (int l = 0; l < kLoads; ++l) x[u][l] = __ldg(p + l);
+        for (int l = 0; l < kLoads; ++l) x[u][l] = p[l];
     }
     bool bad = false;
 #pragma unroll
@@ -366,7 +373,7 @@ __global__ void __launch_bounds__(kWriteThreads) pool_write_kernel(const __grid_
         if constexpr (kMode == 0) {
             out = x[u][0];
         } else {
-            const Divisor by(sc ? __ldg(sc + head[u]) : 1.f);
+            const Divisor by(sc ? __ldcg(sc + head[u]) : 1.f);
             out.x = by.e4m3<kMode == 1>(x[u][0].x, x[u][0].y);
             out.y = by.e4m3<kMode == 1>(x[u][0].z, x[u][0].w);
             out.z = by.e4m3<kMode == 1>(x[u][1].x, x[u][1].y);
@@ -386,7 +393,7 @@ static int launch_cluster(const void* fn, int batch, int64_t work, size_t smem, 
     const int threads = (int)std::min<int64_t>(kMaxThreads, (want + 31) / 32 * 32);
     if (ctas == 16 && cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
         return ZKV_ERR_LAUNCH;
-    return launch_clustered(fn, ctas, threads, ctas, smem, st, args);
+    return launch_clustered(fn, ctas, threads, ctas, smem, st, args, true);
 }
 
 }  // namespace pool
@@ -458,14 +465,10 @@ extern "C" int zkv_pool_write(const void* k, int64_t k_token, int64_t k_head, co
     a.pool_tokens = p->n_blocks * p->block_size;
     a.items = (n_tokens * p->kv_heads) << lg;
     a.heads = p->kv_heads, a.lg_parts = lg, a.shift = pool::log2_of(p->block_size);
-    const int64_t per = pool::kWriteThreads * pool::kWriteUnroll;
+    const int64_t per = pool::kWriteThreads * (el == 2 ? 2 : 1);
     const dim3 grid((unsigned)((a.items + per - 1) / per), 2);
-    cudaStream_t st = (cudaStream_t)stream;
-    if (el == 2)
-        pool::pool_write_kernel<0><<<grid, pool::kWriteThreads, 0, st>>>(a);
-    else if (dtype == ZKV_DT_BF16)
-        pool::pool_write_kernel<1><<<grid, pool::kWriteThreads, 0, st>>>(a);
-    else
-        pool::pool_write_kernel<2><<<grid, pool::kWriteThreads, 0, st>>>(a);
-    return launch_status();
+    const auto kernel = el == 2                 ? pool::pool_write_kernel<0>
+                        : dtype == ZKV_DT_BF16 ? pool::pool_write_kernel<1>
+                                               : pool::pool_write_kernel<2>;
+    return launch_pdl_kernel(kernel, grid, dim3(pool::kWriteThreads), 0, (cudaStream_t)stream, a);
 }
