@@ -193,6 +193,18 @@ def test_decode_many_requests():
     run_decode(711, [(91 * i) % 40 for i in range(1500)], 16, 1, 2, 64, BF, F8, "nhd")
 
 
+def test_decode_empty_batch_and_endless_window():
+    k, v, _, _ = make_pool(725, 4, 16, 2, 128, BF, "hnd")
+    pool = ops.KVPool(k, v)
+    out, lse = ops.pool_decode(torch.empty(0, 8, 128, dtype=BF, device=DEV), pool, i32([]),
+                               torch.empty(0, 4, dtype=torch.int32, device=DEV), return_lse=True)
+    assert out.shape == (0, 8, 128) and lse.shape == (0, 8)
+    q, table = torch.randn(1, 8, 128, generator=gen(726), device=DEV).to(BF), make_table(727, [50], 16, 4, 4)
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        out, lse = ops.pool_decode(q, pool, i32([50]), table, window=window, return_lse=True)
+        check_decode(q, k, v, None, None, [50], table, out, lse, 128 ** -0.5)
+
+
 def test_decode_all_empty():
     run_decode(720, [0, 0, 0], 16, 2, 4, 128, BF, BF, "hnd")
     run_decode(721, [0], 16, 1, 1, 64, HF, F8, "hnd")

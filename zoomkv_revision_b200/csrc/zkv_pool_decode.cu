@@ -57,7 +57,7 @@ namespace pool {
 
 constexpr int kConsumers = 4;                   // warps that share a tile's tokens
 constexpr int kThreads = 32 * (kConsumers + 1);
-constexpr int kMaxGrid = 320;                   // CTAs that a workspace is sized for
+constexpr int kMaxGrid = 480;                   // CTAs that a workspace is sized for
 constexpr int kWholeTokens = 256;               // requests up to this length are never cut
 constexpr int kMaxRanks = 16;                   // CTAs of a cluster that shares a row
 // Up to kWholeBytes of K and V and kRankTiles tiles a CTA the cluster's one launch is ahead of ranges and a join (8 kv
@@ -123,10 +123,12 @@ struct Cfg {
     static constexpr int kStage = 2 * kKv + kQSlot + (int)sizeof(Unit);
     static constexpr int kMl = 2 * kConsumers * kHeadsMax * 8;
     static constexpr int kOther = 1024 + 512;                    // an SM's reserve for a CTA; its static variables
-    static constexpr int kHalf = 233472 / 2 - kOther;            // shared memory of one of two CTAs on an SM
-    static constexpr int kWhole = 233472 - kOther;
-    static constexpr int kPerSm = (kHalf - kFixed - kMl) / kStage >= 3 ? 2 : 1;
-    static constexpr int kFit = ((kPerSm == 2 ? kHalf : kWhole) - kFixed - kMl) / kStage;
+    static constexpr int stages_of(int ctas) { return (233472 / ctas - kOther - kFixed - kMl) / kStage; }
+    // CTAs of an SM: two where they keep three stages each.  64-byte rows take three of two stages (32 requests of 8192,
+    // 8 kv heads: 67.3 us with two, 54.4 with three); 128-byte rows gain nothing by it (95.0 and 91.8, uneven ones 174
+    // and 177).
+    static constexpr int kPerSm = kRow <= 64 && NT == 1 ? 3 : stages_of(2) >= 3 ? 2 : 1;
+    static constexpr int kFit = stages_of(kPerSm);
     static constexpr int kStages = kFit < 8 ? kFit : 8;
     static constexpr int kSmem = kStages * kStage + kFixed + kMl;
     static constexpr bool kTwoParts = !(kF8 && kQ == ZKV_DT_BF16);  // the probability as hi + lo
@@ -955,6 +957,7 @@ __global__ void __launch_bounds__(kJoinThreads) pool_join_kernel(const __grid_co
     const int n = (int)(cuts.owner(s_row[1] - 1) - c0) + 1;
     const int b = s_bh[0], h = s_bh[1] * a.abreast + member / a.chunks;
     grid_dep_wait();
+    grid_dep_launch_next();
     if (n == 1 || (!by_row && c0 != cand)) return;
     float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll

@@ -1354,6 +1354,8 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     elif (lse.dtype is not torch.float32 or lse.numel() != B * Hq or not lse.is_contiguous()
           or lse.get_device() != dev):
         raise ValueError("lse must be contiguous fp32 [B, q_heads]")
+    if window > 0x7fffffff:   # more than any length: every token (the C argument is 32 bits wide)
+        window = 0
     ws, ws_bytes = None, 0
     if workspace is not None:
         ws, ws_bytes = workspace.data_ptr(), workspace.numel()
