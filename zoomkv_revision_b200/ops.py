@@ -1132,7 +1132,7 @@ class KVPool:
     allocated: it holds the tensors, their addresses and strides."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "struct", "ref", "dtype", "device", "kv_heads", "head_dim",
-                 "block_size", "n_blocks", "float_like", "byte_like", "ws_sizes", "index", "code")
+                 "block_size", "n_blocks", "lse_like", "byte_like", "ws_sizes", "index", "code")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _cuda(("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale))
@@ -1169,7 +1169,7 @@ class KVPool:
                                    _p(k_scale), _p(v_scale))
         self.ref = ctypes.addressof(self.struct)
         self.ws_sizes = {}
-        self.float_like, self.byte_like = k.new_empty(0, dtype=torch.float32), k.new_empty(0, dtype=torch.uint8)
+        self.lse_like, self.byte_like = None, k.new_empty(0, dtype=torch.uint8)
         check(lib().zkv_pool_init(self.ref), "zkv_pool_init")
 
 
@@ -1345,12 +1345,15 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     ld, width = _block_table(block_table, B, dev)
     q3 = _whole_rows(q if len(shape) == 3 else q[:, 0])
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     elif out.shape != shape or out.dtype is not dt or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError("out must be contiguous, shaped and typed like q")
     if lse is None:
-        if return_lse:
-            lse = pool.float_like.new_empty((B, Hq))
+        if return_lse:   # (empty_like of a tensor of that shape is the quickest allocation there is)
+            like = pool.lse_like
+            if like is None or like.shape != (B, Hq):
+                like = pool.lse_like = torch.empty(B, Hq, dtype=torch.float32, device=pool.device)
+            lse = torch.empty_like(like)
     elif (lse.dtype is not torch.float32 or lse.numel() != B * Hq or not lse.is_contiguous()
           or lse.get_device() != dev):
         raise ValueError("lse must be contiguous fp32 [B, q_heads]")
