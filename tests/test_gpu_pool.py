@@ -180,6 +180,16 @@ def test_decode_softcap_and_scale(softcap):
     run_decode(603, [5, 64, 700], 16, 2, 4, 128, HF, HF, "hnd", scale=-0.1)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("qt,pt", [(BF, BF), (HF, HF), (BF, F8), (HF, F8)])
+def test_decode_few_rows(qt, pt, D):
+    """One to three rows: every CTA of the largest cluster has a part, or some have none."""
+    run_decode(650, [2100], 16, 1, 4, D, qt, pt, "hnd", wide=False)
+    run_decode(651, [1025, 7, 0], 32, 1, 12, D, qt, pt, "nhd", wide=False)
+    run_decode(652, [513], 64, 1, 33, D, qt, pt, "hnd", window=500, wide=False)
+    run_decode(653, [3000, 2999], 128, 1, 1, D, qt, pt, "nhd", wide=False)
+
+
 def test_decode_long_and_uneven():
     run_decode(700, [40001], 16, 2, 4, 128, BF, BF, "hnd")
     run_decode(701, [1, 20000, 3, 0, 9999, 64, 64, 12345], 16, 2, 4, 128, BF, BF, "nhd")
