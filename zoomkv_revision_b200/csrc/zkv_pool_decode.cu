@@ -73,10 +73,11 @@ struct alignas(16) Unit {
     int tile0;        // first token
     int lo, len;      // tokens [lo, len) of the request are attended
     int flags;        // kFirst, kLast of the row in this CTA; kEnd: the CTA's last unit
-    int part;         // -1: the row is this CTA's alone; 0, 1: its partial slot; 2: a cluster's
+    int part;         // kAlone: the row is this CTA's alone; 0, 1: its partial slot; kShared: a cluster's
     int bad;          // boxes of the tile that are not in the pool
 };
 constexpr int kFirst = 1, kLast = 2, kEnd = 4;
+constexpr int kAlone = -1, kShared = 2;
 
 // Tokens of a tile, for a row of `bytes` bytes.
 __host__ __device__ constexpr int tile_tokens(int bytes) { return bytes >= 256 ? 64 : 64 * 256 / bytes; }
@@ -122,12 +123,18 @@ struct Cfg {
     static constexpr int kFixed = 1024;                          // alignment of the swizzled boxes
     static constexpr int kStage = 2 * kKv + kQSlot + (int)sizeof(Unit);
     static constexpr int kMl = 2 * kConsumers * kHeadsMax * 8;
-    static constexpr int kOther = 1024 + 512;                    // an SM's reserve for a CTA; its static variables
+    static constexpr int kOther = 1024 + 448;                    // an SM's reserve for a CTA; its static variables
     static constexpr int stages_of(int ctas) { return (233472 / ctas - kOther - kFixed - kMl) / kStage; }
-    // CTAs of an SM: two where they keep three stages each.  64-byte rows take three of two stages (32 requests of 8192,
-    // 8 kv heads: 67.3 us with two, 54.4 with three); 128-byte rows gain nothing by it (95.0 and 91.8, uneven ones 174
-    // and 177).
-    static constexpr int kPerSm = kRow <= 64 && NT == 1 ? 3 : stages_of(2) >= 3 ? 2 : 1;
+    // Two n-tiles of heads read the query from shared memory for each product: its registers are worth another CTA on
+    // the SM (16 heads, 32 requests of 8192, 4 kv heads: e4m3 of 128 dims 74.4 -> 61.4 us, of 256 164 -> 144, bf16 of 128
+    // 98.5 -> 96.3).  512-byte rows have no room for a second CTA, one n-tile has registers to spare.
+    static constexpr bool kQShared = NT == 2 && kRow <= 256;
+    // CTAs of an SM: two where they keep three stages each, or three of two stages each.  64-byte rows of one n-tile take
+    // three (32 requests of 8192, 8 kv heads: 67.3 us with two, 54.4 with three); 128-byte rows gain nothing by it (95.0
+    // and 91.8, uneven ones 174 and 177).
+    static constexpr int kPerSm = (kRow <= 64 && NT == 1) || (kQShared && D <= 128) ? 3
+                                  : kQShared || stages_of(2) >= 3                    ? 2
+                                                                                     : 1;
     static constexpr int kFit = stages_of(kPerSm);
     static constexpr int kStages = kFit < 8 ? kFit : 8;
     static constexpr int kSmem = kStages * kStage + kFixed + kMl;
@@ -136,6 +143,7 @@ struct Cfg {
     // n-tiles of O that fit into a stage's K and V when the warps are joined
     static constexpr int kJoinTiles = (2 * kKv) / (kConsumers * 8 * D * 4) < NT ? (2 * kKv) / (kConsumers * 8 * D * 4) : NT;
     static_assert(kJoinTiles >= 1 && NT % kJoinTiles == 0, "join buffer");
+    static_assert(kStages >= 2, "a ring");
     static_assert(kHeadsMax * D * 4 <= kStages * kQSlot, "a cluster's part takes the queries' place");
 };
 
@@ -313,53 +321,94 @@ struct Row {
     float m[NT][2], l[NT][2];   // log2 units; heads 2t, 2t+1 of n-tile (t = lane % 4); l: this lane's tokens
     float f[NT][2];             // score factor of those heads, log2 units (natural under a soft cap)
     float o[C::kMTiles][NT][4];
-    uint32_t q[D / 16][NT][2];  // B fragments of Q^T
+    uint32_t q_at;              // the queries' place, this lane's part
+    uint32_t q[C::kQShared ? 1 : D / 16][NT][2];  // B fragments of Q^T, where they are not read from there each time
+
+    // A bf16 query to fp16, for e4m3 rows: scaled down by the power of two of its largest element; up: the way back.
+    static __device__ __forceinline__ float down_scale(float largest, float& up) {
+        int e = (int)(__float_as_uint(largest) >> 23) - 127;  // in [2^e, 2^(e+1))
+        e = largest > 0.f ? (e < -126 ? -126 : (e > 126 ? 126 : e)) : 0;
+        up = __uint_as_float((uint32_t)(127 + e) << 23);
+        return __uint_as_float((uint32_t)(127 - e) << 23);
+    }
+
+    // The same in the queries' place in shared memory: four heads a warp, eight lanes a head; `up` behind the head's row.
+    static __device__ __forceinline__ void narrow_shared(uint8_t* qs) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        uint8_t* row = qs + (4 * warp + (lane >> 3)) * C::kQPitch;
+        uint4* at = reinterpret_cast<uint4*>(row) + (lane & 7);
+        uint4 w[D / 64];
+        float largest = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+            w[i] = at[8 * i];
+            const uint32_t* x = reinterpret_cast<const uint32_t*>(&w[i]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 y = unpack2<true>(x[k]);
+                largest = fmaxf(largest, fmaxf(fabsf(y.x), fabsf(y.y)));
+            }
+        }
+#pragma unroll
+        for (int off = 4; off >= 1; off >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, off));
+        float up;
+        const float down = down_scale(largest, up);
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+            uint32_t* x = reinterpret_cast<uint32_t*>(&w[i]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 y = unpack2<true>(x[k]);
+                x[k] = pack2<false>(y.x * down, y.y * down);
+            }
+            at[8 * i] = w[i];
+        }
+        if ((lane & 7) == 0) *reinterpret_cast<float*>(row + 2 * D) = up;
+    }
 
     __device__ __forceinline__ void init(const DecodeArgs& a, const uint8_t* qs, int n_heads, float k_scale) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         const float base = a.scale * k_scale * (a.softcap > 0.f ? 1.f : 1.4426950408889634f);
+        q_at = smem_u32(qs) + g * C::kQPitch + (kF8 ? 8 : 4) * t;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int head = 8 * n + g;
-            const uint8_t* row = qs + head * C::kQPitch;
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+            f[n][0] = f[n][1] = base;
+            if constexpr (C::kQShared) {
+                if constexpr (kF8 && kQ == ZKV_DT_BF16)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        f[n][e] *= *reinterpret_cast<const float*>(qs + (8 * n + 2 * t + e) * C::kQPitch + 2 * D);
+                continue;
+            }
+            const bool in = 8 * n + g < n_heads;
+            float largest = 0.f;
 #pragma unroll
             for (int s = 0; s < D / 16; ++s) {
-                if constexpr (kF8) {  // k index 2t, 2t+1, 2t+8, 2t+9 <- dims 4t .. 4t+3, as the e4m3 rows are read
-                    const uint2 w = *reinterpret_cast<const uint2*>(row + 32 * s + 8 * t);
-                    q[s][n][0] = head < n_heads ? w.x : 0u;
-                    q[s][n][1] = head < n_heads ? w.y : 0u;
-                } else {
-                    q[s][n][0] = head < n_heads ? *reinterpret_cast<const uint32_t*>(row + 32 * s + 4 * t) : 0u;
-                    q[s][n][1] = head < n_heads ? *reinterpret_cast<const uint32_t*>(row + 32 * s + 16 + 4 * t) : 0u;
+                query_at(n, s, q[s][n]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (!in) q[s][n][i] = 0u;
+                    const float2 y = unpack2<true>(q[s][n][i]);
+                    if (kF8 && kQ == ZKV_DT_BF16) largest = fmaxf(largest, fmaxf(fabsf(y.x), fabsf(y.y)));
                 }
             }
-            f[n][0] = f[n][1] = base;
             if constexpr (kF8 && kQ == ZKV_DT_BF16) {
-                float mx = 0.f;
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                float up;
+                const float down = down_scale(largest, up);
 #pragma unroll
                 for (int s = 0; s < D / 16; ++s)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float2 x = unpack2<true>(q[s][n][i]);
-                        mx = fmaxf(mx, fmaxf(fabsf(x.x), fabsf(x.y)));
-                    }
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                int e = (int)(__float_as_uint(mx) >> 23) - 127;  // mx in [2^e, 2^(e+1))
-                e = mx > 0.f ? (e < -126 ? -126 : (e > 126 ? 126 : e)) : 0;
-                const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-                for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float2 x = unpack2<true>(q[s][n][i]);
-                        q[s][n][i] = pack2<false>(x.x * down, x.y * down);
+                        const float2 y = unpack2<true>(q[s][n][i]);
+                        q[s][n][i] = pack2<false>(y.x * down, y.y * down);
                     }
                 f[n][0] *= __shfl_sync(0xffffffffu, up, 8 * t);
                 f[n][1] *= __shfl_sync(0xffffffffu, up, 8 * t + 4);
             }
-            m[n][0] = m[n][1] = -INFINITY;
-            l[n][0] = l[n][1] = 0.f;
         }
 #pragma unroll
         for (int j = 0; j < C::kMTiles; ++j)
@@ -367,6 +416,18 @@ struct Row {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
+    }
+
+    // The B fragment of Q^T for 16 dims of n-tile n.  Over e4m3 rows k index 2t, 2t+1, 2t+8, 2t+9 stands for dims
+    // 4t .. 4t+3, as those rows are read.
+    __device__ __forceinline__ void query_at(int n, int s, uint32_t (&b)[2]) const {
+        const uint32_t at = q_at + n * 8 * C::kQPitch + 32 * s;
+        if constexpr (kF8) {
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(b[0]), "=r"(b[1]) : "r"(at) : "memory");
+        } else {
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(b[0]) : "r"(at) : "memory");
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(b[1]) : "r"(at + 16) : "memory");
+        }
     }
 
     // The warp's tokens of a tile, 16 a product: product i's K and V rows begin
@@ -383,15 +444,32 @@ struct Row {
         auto chunk = [&](uint32_t from, int tok, int sw, int c) {
             return from + (uint32_t)(c / kPerPiece) * piece + tok * C::kInner + (((c % kPerPiece) ^ sw) << 4);
         };
-        float x[kSub][NT][4], x2[kSub][NT][4];  // two chains of products each, so that one does not wait for the other
+        // two chains of products at least, so that one does not wait for the other
+        constexpr bool kSplit = kSub == 1 || !C::kQShared;
+        float x[kSub][NT][4], x2[kSplit ? kSub : 1][NT][4];
 #pragma unroll
         for (int i = 0; i < kSub; ++i)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[i][n][e] = x2[i][n][e] = 0.f;
+                for (int e = 0; e < 4; ++e) {
+                    x[i][n][e] = 0.f;
+                    if constexpr (kSplit) x2[i][n][e] = 0.f;
+                }
 #pragma unroll
-        for (int s = 0; s < D / 16; s += 2)
+        for (int s = 0; s < D / 16; s += 2) {
+            uint32_t qf[2][NT][2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (C::kQShared) {
+                        query_at(n, s + k, qf[k][n]);
+                    } else {
+                        qf[k][n][0] = q[s + k][n][0];
+                        qf[k][n][1] = q[s + k][n][1];
+                    }
+                }
 #pragma unroll
             for (int i = 0; i < kSub; ++i) {
                 uint32_t a0[4], a1[4];
@@ -408,10 +486,20 @@ struct Row {
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    mma16816<kMmaBf16>(x[i][n], a0, q[s][n][0], q[s][n][1]);
-                    mma16816<kMmaBf16>(x2[i][n], a1, q[s + 1][n][0], q[s + 1][n][1]);
+                    mma16816<kMmaBf16>(x[i][n], a0, qf[0][n][0], qf[0][n][1]);
+                    if constexpr (kSplit) mma16816<kMmaBf16>(x2[i][n], a1, qf[1][n][0], qf[1][n][1]);
+                    else mma16816<kMmaBf16>(x[i][n], a1, qf[1][n][0], qf[1][n][1]);
                 }
             }
+        }
+        if constexpr (kSplit) {
+#pragma unroll
+            for (int i = 0; i < kSub; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[i][n][e] += x2[i][n][e];
+        }
         // x[i][n][0..3]: (token g, head 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
         float alpha[NT][2];
         bool moved = false;
@@ -422,7 +510,7 @@ struct Row {
             for (int i = 0; i < kSub; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float y = (x[i][n][e] + x2[i][n][e]) * f[n][e & 1];
+                    float y = x[i][n][e] * f[n][e & 1];
                     if (a.softcap > 0.f) y = a.softcap * 1.4426950408889634f * tanhf(y / a.softcap);
                     x[i][n][e] = y;
                 }
@@ -568,6 +656,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     const int member = block % a.side, chunk = member % a.chunks, abreast = member / a.chunks;
     const int64_t c = block / a.side;
     const int n_heads = min(a.heads, a.G - chunk * a.heads);
+    if constexpr (C::kQShared) {  // the places of heads that the chunk has not: products of zeros
+        const int per = (C::kHeadsMax - n_heads) * (D / 8);
+        for (int i = tid; i < C::kStages * per; i += kThreads)
+            *reinterpret_cast<uint4*>(qs + i / per * C::kQSlot + (n_heads + i % per / (D / 8)) * C::kQPitch +
+                                      i % (D / 8) * 16) = make_uint4(0, 0, 0, 0);
+    }
     // the arguments' constant-cache lines, while the previous grid ends
     asm volatile("" ::"l"(a.q), "l"(a.lens), "l"(a.parts), "l"(a.q_head), "r"(a.batch), "r"(a.groups), "f"(a.softcap));
     grid_dep_wait();
@@ -642,9 +736,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             const bool first = done == 0 || tile == 0;
             end = a.whole ? tile == tiles - 1 && row_begin + 1 == u1 : u0 + done + 1 == u1;
             const bool last = end || tile == tiles - 1;
-            int part = -1;
-            if (!a.whole) part = row_begin < u0 ? 0 : row_begin + tiles > u1 ? 1 : -1;
-            else if (a.ranks > 1) part = 2;
+            int part = kAlone;
+            if (!a.whole) part = row_begin < u0 ? 0 : row_begin + tiles > u1 ? 1 : kAlone;
+            else if (a.ranks > 1) part = kShared;
             // ---- block ids of the tile: 32 entries of the table at a time, the next 32 on their way
             const int tile0 = (tile_first + tile) * C::kTile;
             const int entry = tile0 >> a.shift;
@@ -717,6 +811,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     // a cluster's part of a row: this CTA's only one, so the queries and the first half of ml are free when it is done
     float* const cl_o = reinterpret_cast<float*>(qs);  // [heads][D]
     float2* const cl_ml = ml;                          // [heads]
+    auto meet = [&]() -> bool {  // the four warps, at most kWaitNs
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&epi);
+        const bool got = __all_sync(0xffffffffu, wait_for(&epi, epi_phase, a.status));
+        epi_phase ^= 1;
+        return got;
+    };
     bool end = false, alive = true;
     for (int i = 0; !end; ++i) {
         const int stage = i % C::kStages;
@@ -728,7 +829,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         end = x.flags & kEnd;
         uint8_t* const base = kv + stage * 2 * C::kKv;
         if (x.flags & kFirst) {
-            row.init(a, qs + (n_row % C::kStages) * C::kQSlot, n_heads, kF8 && a.k_scale ? __ldcg(a.k_scale + x.h) : 1.f);
+            uint8_t* const q_row = qs + (n_row % C::kStages) * C::kQSlot;
+            if constexpr (C::kQShared && kF8 && kQ == ZKV_DT_BF16) {
+                row.narrow_shared(q_row);
+                alive = meet();
+                if (!alive) break;
+            }
+            row.init(a, q_row, n_heads, kF8 && a.k_scale ? __ldcg(a.k_scale + x.h) : 1.f);
             ++n_row;
         }
         // 16 tokens lie in one box (a box has 16 or more)
@@ -770,13 +877,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
                 s += __shfl_xor_sync(0xffffffffu, s, 16);
                 if (g == 0) mine_ml[warp * C::kHeadsMax + 8 * n + 2 * t + e] = make_float2(row.m[n][e], s);
             }
-        auto meet = [&]() -> bool {  // the four warps, at most kWaitNs
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&epi);
-            const bool got = __all_sync(0xffffffffu, wait_for(&epi, epi_phase, a.status));
-            epi_phase ^= 1;
-            return got;
-        };
         if (!meet()) {  // statistics written, stage read by all
             alive = false;
             break;
@@ -835,11 +935,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
                                                                       (d ^ (((hl >> 1) & 3) << 3)));
                     o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
                 }
-                if (x.part < 0) {
+                if (x.part == kAlone) {
                     const float inv = sum == 0.f ? 0.f : v_scale / sum;
                     store4<kQ>(a.out, (head0 + head) * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
                     if (a.lse && d == 0) a.lse[head0 + head] = (mx + log2f(sum)) * 0.6931471805599453f;
-                } else if (x.part == 2) {
+                } else if (x.part == kShared) {
                     *reinterpret_cast<float4*>(cl_o + head * D + d) = o;
                     if (d == 0) cl_ml[head] = make_float2(mx, sum);
                 } else {
