@@ -125,7 +125,7 @@ def run_decode(seed, lens, S, H, G, D, qt, pt, layout, window=0, softcap=0.0, sc
     n_blocks = need + spare
     width = max(1, max((n + S - 1) // S for n in lens)) + 1
     if wide and not 0 < window < 10000:
-        width += (80 << 20) // (2 * len(lens) * H * D * S * (1 if pt == F8 else 2))
+        width += (160 << 20) // (2 * len(lens) * H * D * S * (1 if pt == F8 else 2))
     k, v, ks, vs = make_pool(seed, n_blocks, S, H, D, pt, layout)
     table = make_table(seed + 1, lens, S, n_blocks, width)
     lo = [max(0, n - window) if window else 0 for n in lens]
@@ -234,7 +234,7 @@ def test_decode_is_deterministic_and_takes_dirty_workspaces():
     q = torch.randn(4, 8, 128, generator=gen(3), device=DEV).to(BF)
     pool = ops.KVPool(k, v)
     first = None
-    wide = torch.full((4, 9000), -1, dtype=torch.int32, device=DEV)   # a bound of the lengths that cuts the rows by units
+    wide = torch.full((4, 20000), -1, dtype=torch.int32, device=DEV)   # a bound of the lengths that cuts the rows by units
     wide[:, :600] = table
     short = [3900, 1, 0, 257]                                        # one that does not: no workspace
     assert ops.pool_decode_ws_bytes(4, 8, pool, 244) == 0
@@ -245,7 +245,7 @@ def test_decode_is_deterministic_and_takes_dirty_workspaces():
     check_decode(q, k, v, ks, vs, short, table, *first, 128 ** -0.5)
     first = None
     for fill in (0, 255, 127, 1):
-        ws = torch.full((ops.pool_decode_ws_bytes(4, 8, pool, 9000),), fill, dtype=torch.uint8, device=DEV)
+        ws = torch.full((ops.pool_decode_ws_bytes(4, 8, pool, 20000),), fill, dtype=torch.uint8, device=DEV)
         assert ws.numel() > 0
         got = ops.pool_decode(q, pool, i32(lens), wide, return_lse=True, workspace=ws)
         first = first or got

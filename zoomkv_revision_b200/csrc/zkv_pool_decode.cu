@@ -59,11 +59,13 @@ constexpr int kConsumers = 4;                   // warps that share a tile's tok
 constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxGrid = 480;                   // CTAs that a workspace is sized for
 constexpr int kWholeTokens = 256;               // requests up to this length are never cut
+constexpr int kMaxChunks = 320;                 // of 16 query heads per kv head
 constexpr int kMaxRanks = 16;                   // CTAs of a cluster that shares a row
-// Up to kWholeBytes of K and V and kRankTiles tiles a CTA the cluster's one launch is ahead of ranges and a join (8 kv
-// heads of 128, bf16: one request of 4096 10.0 us on the GPU both ways, of 8192 13.7 against 12.2 and 6 us less to
-// issue, of 16384 20.7 against 14.7; 16 of 1000 13.0 against 18.0, 4 of 4096 13.7 against 15.2).
-constexpr int64_t kWholeBytes = 64 << 20;
+// Up to kWholeBytes of K and V, and kRankTiles tiles a CTA or twice that where the CTAs fill their waves to 4/5, whole
+// rows in one launch are ahead of ranges and a join, which 4 us more issue (8 kv heads of 128, bf16, us on the GPU, whole
+// and ranges: 1 request of 4096 9.8 and 10.0, 1 of 16384 21.0 and 19.4, 16 of 1000 12.9 and 18.0, 64 of 480 25.2 and 30.7,
+// 32 of 1000 24.5 and 30.9, 40 of 800 34.3 and 31.0, 16 up to 1900 19.3 and 17.7, 64 up to 1000 36.0 and 33.4).
+constexpr int64_t kWholeBytes = 128 << 20;
 constexpr int kRankTiles = 8;
 constexpr uint64_t kWaitNs = 2000000000ull;     // limit of each wait inside a CTA
 
@@ -1232,7 +1234,9 @@ static Cut plan_call(int batch, int kv_heads, int chunks, int row_bytes, int win
     const int64_t bytes = 2 * (int64_t)batch * kv_heads * longest * row_bytes;
     const int64_t wave = 2 * sm_count();  // (one CTA an SM, as 256 dims have it, takes two turns)
     while (c.ranks < kMaxRanks && rows * c.ranks * 2 <= wave && c.ranks * 2 <= tiles) c.ranks *= 2;
-    c.whole = longest <= kWholeTokens || (bytes <= kWholeBytes && tiles <= c.ranks * kRankTiles);
+    const int64_t ctas = rows * c.ranks, slots = (ctas + wave - 1) / wave * wave;
+    const int most = 5 * ctas >= 4 * slots ? 2 * kRankTiles : kRankTiles;
+    c.whole = longest <= kWholeTokens || (bytes <= kWholeBytes && tiles <= c.ranks * most);
     if (!c.whole) c.ranks = 1;
     while (kv_heads % c.abreast || c.abreast * chunks > kMaxGrid) --c.abreast;
     return c;
@@ -1320,7 +1324,7 @@ extern "C" size_t zkv_pool_decode_ws_bytes(const zkv_pool* p, int batch, int q_h
     if (pool::check_pool(p) != ZKV_OK || batch < 0 || q_heads < 1 || q_heads % p->kv_heads || window < 0 || max_len < 0)
         return 0;
     const pool::Heads h = pool::split_heads(q_heads / p->kv_heads);
-    if (h.chunks > pool::kMaxGrid || !needs_parts(p, batch, h, window, max_len)) return 0;
+    if (h.chunks > pool::kMaxChunks || !needs_parts(p, batch, h, window, max_len)) return 0;
     const size_t rows = pool::part_rows(batch, p->kv_heads, h, max_len);
     return pool::up256(rows * 8) + pool::up256(rows * p->head_dim * 4);
 }
@@ -1343,7 +1347,7 @@ extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int
     const int64_t room = (int64_t)width * p->block_size;
     const int64_t cap = std::min<int64_t>(max_len > 0 ? std::min(max_len, room) : room, INT32_MAX - 512);
     const pool::Heads hs = pool::split_heads(q_heads / p->kv_heads);
-    if (hs.chunks > pool::kMaxGrid) return ZKV_ERR_CAPACITY;
+    if (hs.chunks > pool::kMaxChunks) return ZKV_ERR_CAPACITY;
     const bool parts = needs_parts(p, batch, hs, window, cap);
     if (parts && !workspace) return ZKV_ERR_ARG;
     if (parts && ws_bytes < zkv_pool_decode_ws_bytes(p, batch, q_heads, window, cap)) return ZKV_ERR_CAPACITY;
