@@ -137,8 +137,10 @@ struct Cfg {
     static constexpr int kPerSm = (kRow <= 64 && NT == 1) || (kQShared && D <= 128) ? 3
                                   : kQShared || stages_of(2) >= 3                    ? 2
                                                                                      : 1;
+    // As many stages as fit, but two for 256-byte rows of one n-tile: their warps keep up, and more reads in flight only
+    // slow the memory down (8 requests of 32768 165.2 us with three, 159.4 with two; 128-byte rows 162.8 and 173).
     static constexpr int kFit = stages_of(kPerSm);
-    static constexpr int kStages = kFit < 8 ? kFit : 8;
+    static constexpr int kStages = kRow == 256 && !kF8 && NT == 1 ? 2 : kFit < 8 ? kFit : 8;
     static constexpr int kSmem = kStages * kStage + kFixed + kMl;
     static constexpr bool kTwoParts = !(kF8 && kQ == ZKV_DT_BF16);  // the probability as hi + lo
     static constexpr int kMTiles = D / 16;
@@ -179,12 +181,21 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// K and V rows are read once a call: they leave L2 before what the call uses again (one request of 131071 85.0 -> 83.7 us,
+// 12 query heads a kv head 111.6 -> 106.9).
+__device__ __forceinline__ uint64_t evict_first_policy() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int token, int head, int block,
-                                            uint64_t* bar) {
+                                            uint64_t* bar, uint64_t policy) {
     asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-        "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(token), "r"(0), "r"(head), "r"(block), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], "
+        "[%1, {%2, %3, %4, %5, %6}], [%7], %8;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(token), "r"(0), "r"(head), "r"(block), "r"(smem_u32(bar)),
+        "l"(policy)
         : "memory");
 }
 
@@ -730,6 +741,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         }
         int64_t row_begin = a.whole ? u0 : u0 - tile;  // unit at which the row begins (its number, where rows are whole)
         int n_row = 0;                  // rows begun in this CTA
+        const uint64_t policy = evict_first_policy();
         const int boxes = C::kTile >> a.lg_box, box_bytes = C::kRow << a.lg_box;
         bool ok = true, end = false;
         int done = 0;
@@ -781,8 +793,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
                 const uint32_t dst = smem_u32(kv + stage * 2 * C::kKv) + lane * box_bytes;
                 // a box is a whole block, or a tile's tokens of one
                 const int in_block = a.shift > a.lg_box ? tile0 & ((1 << a.shift) - 1) : 0;
-                tma_load_5d(dst, &a.tk, in_block, h, id, full + stage);
-                tma_load_5d(dst + C::kKv, &a.tv, in_block, h, id, full + stage);
+                tma_load_5d(dst, &a.tk, in_block, h, id, full + stage, policy);
+                tma_load_5d(dst + C::kKv, &a.tv, in_block, h, id, full + stage, policy);
             }
             if (first && lane >= 32 - C::kHeadsMax && lane - (32 - C::kHeadsMax) < n_heads) {
                 const int j = lane - (32 - C::kHeadsMax);
