@@ -849,7 +849,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
                 alive = meet();
                 if (!alive) break;
             }
-            row.init(a, q_row, n_heads, kF8 && a.k_scale ? __ldcg(a.k_scale + x.h) : 1.f);
+            row.init(a, q_row, n_heads, kF8 && a.k_scale ? a.k_scale[x.h] : 1.f);
             ++n_row;
         }
         // 16 tokens lie in one box (a box has 16 or more)
@@ -896,7 +896,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             break;
         }
         float* buf = reinterpret_cast<float*>(base);
-        const float v_scale = kF8 && a.v_scale ? __ldcg(a.v_scale + x.h) : 1.f;
+        const float v_scale = kF8 && a.v_scale ? a.v_scale[x.h] : 1.f;
         const int64_t head0 = ((int64_t)x.b * a.kv_heads + x.h) * a.G + chunk * a.heads;
         const int64_t slot = (int64_t)blockIdx.x * 2 + x.part;
 #pragma unroll
