@@ -215,6 +215,18 @@ def test_decode_empty_batch_and_endless_window():
         check_decode(q, k, v, None, None, [50], table, out, lse, 128 ** -0.5)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("qt,pt", [(BF, BF), (HF, HF), (BF, F8), (HF, F8)])
+def test_decode_many_short_rows(qt, pt, D):
+    """Rows of a tile at most, few and more than the GPU's places: a warp's own."""
+    run_decode(740, [0, 1, 5, 15, 16], 16, 2, 4, D, qt, pt, "hnd", wide=False)
+    run_decode(741, [i % 14 for i in range(700)], 16, 2, 4, D, qt, pt, "nhd", wide=False)
+    run_decode(742, [(7 * i) % 49 for i in range(700)], 16, 1, 16, D, qt, pt, "hnd", wide=False, softcap=20.0)
+    run_decode(743, [i % 65 for i in range(350)], 64, 2, 17, D, qt, pt, "nhd", wide=False, max_len=64)
+    run_decode(744, [i % 30 for i in range(300)], 32, 4, 1, D, qt, pt, "hnd", wide=False)
+    run_decode(745, [200 - i % 200 for i in range(610)], 256, 1, 9, D, qt, pt, "hnd", wide=False, max_len=200)
+
+
 def test_decode_all_empty():
     run_decode(720, [0, 0, 0], 16, 2, 4, 128, BF, BF, "hnd")
     run_decode(721, [0], 16, 1, 1, 64, HF, F8, "hnd")

@@ -60,6 +60,7 @@ constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxGrid = 480;                   // CTAs that a workspace is sized for
 constexpr int kWholeTokens = 256;               // requests up to this length are never cut
 constexpr int kMaxChunks = 320;                 // of 16 query heads per kv head
+constexpr int kMaxStages = 8;                   // of a CTA's ring (a multiple of kConsumers)
 constexpr int kMaxRanks = 16;                   // CTAs of a cluster that shares a row
 // Up to kWholeBytes of K and V, and kRankTiles tiles a CTA or twice that where the CTAs fill their waves to 4/5, whole
 // rows in one launch are ahead of ranges and a join, which 4 us more issue (8 kv heads of 128, bf16, us on the GPU, whole
@@ -67,6 +68,7 @@ constexpr int kMaxRanks = 16;                   // CTAs of a cluster that shares
 // 32 of 1000 24.5 and 30.9, 40 of 800 34.3 and 31.0, 16 up to 1900 19.3 and 17.7, 64 up to 1000 36.0 and 33.4).
 constexpr int64_t kWholeBytes = 128 << 20;
 constexpr int kRankTiles = 8;
+constexpr int kSoloRows = 2;                    // rows a CTA from which on a warp takes one of more than one product alone
 constexpr uint64_t kWaitNs = 2000000000ull;     // limit of each wait inside a CTA
 
 // What a unit is, written by the producer beside its stage.
@@ -106,6 +108,7 @@ struct DecodeArgs {
     int groups;     // ranges
     int whole;      // rows are not cut by units
     int ranks;      // CTAs (a cluster) that share a row, if `whole`
+    int stages, half;  // kSolo: the ring's stages, two times `half` bytes each, K and V
     int shift, lg_box, width, window;
     float scale, softcap;
 };
@@ -140,8 +143,9 @@ struct Cfg {
     // As many stages as fit, but two for 256-byte rows of one n-tile: their warps keep up, and more reads in flight only
     // slow the memory down (8 requests of 32768 165.2 us with three, 159.4 with two; 128-byte rows 162.8 and 173).
     static constexpr int kFit = stages_of(kPerSm);
-    static constexpr int kStages = kRow == 256 && !kF8 && NT == 1 ? 2 : kFit < 8 ? kFit : 8;
-    static constexpr int kSmem = kStages * kStage + kFixed + kMl;
+    static constexpr int kStages = kRow == 256 && !kF8 && NT == 1 ? 2 : kFit < kMaxStages ? kFit : kMaxStages;
+    static constexpr int kRing = kFit * kStage;                   // bytes of a ring at most
+    static constexpr int smem_of(int ring) { return ring + kFixed + kMl; }
     static constexpr bool kTwoParts = !(kF8 && kQ == ZKV_DT_BF16);  // the probability as hi + lo
     static constexpr int kMTiles = D / 16;
     // n-tiles of O that fit into a stage's K and V when the warps are joined
@@ -326,6 +330,26 @@ struct Ranges {
     }
 };
 
+// A place in a ring and the phase of its barrier in this round.
+struct Turn {
+    int stage = 0;
+    uint32_t phase = 0;
+
+    __device__ __forceinline__ void next(int stages) {
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+    __device__ __forceinline__ void skip(int stages, int n) {  // n <= stages
+        stage += n;
+        if (stage >= stages) {
+            stage -= stages;
+            phase ^= 1;
+        }
+    }
+};
+
 // ------------------------------------------------------------ consumers
 template <int kQ, bool kF8, int D, int NT>
 struct Row {
@@ -345,10 +369,10 @@ struct Row {
         return __uint_as_float((uint32_t)(127 - e) << 23);
     }
 
-    // The same in the queries' place in shared memory: four heads a warp, eight lanes a head; `up` behind the head's row.
-    static __device__ __forceinline__ void narrow_shared(uint8_t* qs) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        uint8_t* row = qs + (4 * warp + (lane >> 3)) * C::kQPitch;
+    // The same in the queries' place in shared memory: four heads at a time, eight lanes a head; `up` behind the head's row.
+    static __device__ __forceinline__ void narrow_shared(uint8_t* qs, int quarter) {
+        const int lane = threadIdx.x & 31;
+        uint8_t* row = qs + (4 * quarter + (lane >> 3)) * C::kQPitch;
         uint4* at = reinterpret_cast<uint4*>(row) + (lane & 7);
         uint4 w[D / 64];
         float largest = 0.f;
@@ -444,9 +468,9 @@ struct Row {
     }
 
     // The warp's tokens of a tile, 16 a product: product i's K and V rows begin
-    // at base + at[i] and base + kKv + at[i] (in a swizzled box, `piece` bytes
+    // at base + at[i] and base + half + at[i] (in a swizzled box, `piece` bytes
     // from one 128-byte piece to the next); its tokens [v0[i], v1[i]) count.
-    __device__ __forceinline__ void step(const DecodeArgs& a, uint32_t base, const uint32_t (&at)[C::kSub], uint32_t piece,
+    __device__ __forceinline__ void step(const DecodeArgs& a, uint32_t base, uint32_t half, const uint32_t (&at)[C::kSub], uint32_t piece,
                                          const int (&v0)[C::kSub], const int (&v1)[C::kSub], bool partial) {
         const int lane = threadIdx.x & 31, g = lane >> 2;
         constexpr int kPerPiece = C::kInner / 16;  // 16-byte chunks of a row in a piece
@@ -583,7 +607,7 @@ struct Row {
                         lo[n][r] = transposed(pack2<kMmaBf16>(p0 - back.x, p1 - back.y));
                     }
                 }
-            const uint32_t vs = base + C::kKv + at[i];
+            const uint32_t vs = base + half + at[i];
             // four tiles of dims at a time, their hi products before their lo ones, so that none waits for the one before
             const int tok_v = (lane & 7) + ((lane >> 4) << 3), off_v = (lane >> 3) & 1, sw_v = tok_v & 7;
 #pragma unroll
@@ -619,6 +643,37 @@ struct Row {
         }
     }
 
+    // The sum of a head's exponentials over the warp's tokens.
+    __device__ __forceinline__ float total(int n, int e) const {
+        float s = l[n][e];
+        s += __shfl_xor_sync(0xffffffffu, s, 4);
+        s += __shfl_xor_sync(0xffffffffu, s, 8);
+        s += __shfl_xor_sync(0xffffffffu, s, 16);
+        return s;
+    }
+
+    // O of n-tile n times a factor per head to `to` [8][D].  Dims of a head are permuted by its pair's number, so that the
+    // 32 lanes meet 32 banks.
+    __device__ __forceinline__ void put(float* to, int n, const float (&fac)[2]) const {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        float* p = to + 2 * t * D;
+#pragma unroll
+        for (int j = 0; j < C::kMTiles; ++j) {
+            const float* x = o[j][n];
+            if constexpr (kF8) {
+                const int d = (16 * j + 2 * g) ^ (t << 3);
+                *reinterpret_cast<float2*>(p + d) = make_float2(x[0] * fac[0], x[2] * fac[0]);
+                *reinterpret_cast<float2*>(p + D + d) = make_float2(x[1] * fac[1], x[3] * fac[1]);
+            } else {
+                const int d = (16 * j + g) ^ (t << 3), d8 = (16 * j + g + 8) ^ (t << 3);
+                p[d] = x[0] * fac[0];
+                p[D + d] = x[1] * fac[1];
+                p[d8] = x[2] * fac[0];
+                p[D + d8] = x[3] * fac[1];
+            }
+        }
+    }
+
     // V rows of tokens outside [v0, v1) to zero: their probability is 0, but 0 times what an unwritten row may hold
     // (NaN, infinities) is not.
     __device__ __forceinline__ void clear_rows(uint8_t* vs, uint32_t piece, int v0, int v1) {
@@ -640,38 +695,44 @@ __device__ __forceinline__ void store4(void* out, int64_t i, float4 x) {
         make_uint2(pack2<kBf16>(x.x, x.y), pack2<kBf16>(x.z, x.w));
 }
 
-template <int kQ, bool kF8, int D, int NT>
+// kSolo: every row is one unit and one warp's, so the four warps of a CTA have
+// four rows in hand and none waits for another.  For rows of a tile at most,
+// where the four warps' chain and join take 1.9 us a row whatever it holds: 256
+// requests of 1 token, 8 kv heads of 128, 17.1 -> 9.1 us, 131 of 8 tokens, 16 kv
+// heads of 256, 54.4 -> 17.2.
+template <int kQ, bool kF8, int D, int NT, bool kSolo>
 __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     pool_decode_kernel(const __grid_constant__ DecodeArgs a) {
     using C = Cfg<kQ, kF8, D, NT>;
+    const int stages = kSolo ? a.stages : C::kStages, half = kSolo ? a.half : C::kKv;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
     uint8_t* kv = smem;                                                  // [stages] K, V
-    uint8_t* qs = kv + C::kStages * 2 * C::kKv;                          // [stages] query heads, by row
-    Unit* units = reinterpret_cast<Unit*>(qs + C::kStages * C::kQSlot);  // [stages]
-    float2* ml = reinterpret_cast<float2*>(units + C::kStages);          // [2][warps][heads]
-    __shared__ uint64_t full[C::kStages], empty[C::kStages], epi;
+    uint8_t* qs = kv + stages * 2 * half;                            // [stages] query heads, by row
+    Unit* units = reinterpret_cast<Unit*>(qs + stages * C::kQSlot);    // [stages]
+    float2* ml = reinterpret_cast<float2*>(units + stages);            // [2][warps][heads]
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], epi;
     __shared__ int64_t sh[32];
     __shared__ int64_t s_off;
     __shared__ int s_b, s_len;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        for (int i = 0; i < C::kStages; ++i) {
+        for (int i = 0; i < stages; ++i) {
             mbar_init(full + i, 1);
-            mbar_init(empty + i, kConsumers);
+            mbar_init(empty + i, kSolo ? 1 : kConsumers);
         }
         mbar_init(&epi, kConsumers);
         mbar_fence_init();
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.tk)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.tv)) : "memory");
     }
-    const int rank = blockIdx.x % a.ranks, block = blockIdx.x / a.ranks;
+    const int rank = kSolo ? 0 : blockIdx.x % a.ranks, block = kSolo ? blockIdx.x : blockIdx.x / a.ranks;
     const int member = block % a.side, chunk = member % a.chunks, abreast = member / a.chunks;
     const int64_t c = block / a.side;
     const int n_heads = min(a.heads, a.G - chunk * a.heads);
     if constexpr (C::kQShared) {  // the places of heads that the chunk has not: products of zeros
         const int per = (C::kHeadsMax - n_heads) * (D / 8);
-        for (int i = tid; i < C::kStages * per; i += kThreads)
+        for (int i = tid; i < stages * per; i += kThreads)
             *reinterpret_cast<uint4*>(qs + i / per * C::kQSlot + (n_heads + i % per / (D / 8)) * C::kQPitch +
                                       i % (D / 8) * 16) = make_uint4(0, 0, 0, 0);
     }
@@ -681,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     grid_dep_launch_next();  // the join kernel may become resident; it waits for this grid
     // ---- this CTA's range [u0, u1): of units, or of rows where those are not split
     int64_t u0, u1;
-    if (a.whole) {
+    if (kSolo || a.whole) {
         const int64_t rows = (int64_t)a.batch * a.head_rows;
         u0 = quotient(rows * c, a.groups);
         u1 = quotient(rows * (c + 1), a.groups);
@@ -705,8 +766,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
 
     if (warp == kConsumers) {
         // ---------------------------------------------------- producer
-        int b = a.whole ? (int)quotient(u0, a.head_rows) : s_b;
-        int next = a.whole ? __ldcg(a.lens + b) : s_len;  // the next request's length, asked for one request ahead
+        int b = kSolo || a.whole ? (int)quotient(u0, a.head_rows) : s_b;
+        int next = kSolo || a.whole ? __ldcg(a.lens + b) : s_len;  // the next request's length, asked for one request ahead
         int len, lo, tile_first, tiles;
         auto begin_request = [&]() {
             if (next < 0 || next > a.cap) raise_status(a.status, ZKV_ERR_RANGE);
@@ -726,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         }
         begin_request();
         int hr, tile;  // row of the request, tile of the row
-        if (a.whole) {
+        if (kSolo || a.whole) {
             hr = (int)(u0 - (int64_t)b * a.head_rows);
             tile = (int)((uint32_t)tiles * (uint32_t)rank / (uint32_t)a.ranks);
         } else {
@@ -734,24 +795,25 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             tile = (int)(s_off - (int64_t)hr * tiles);
         }
         bool none = false;  // more CTAs than tiles: this one has an empty unit
-        if (a.ranks > 1) {
+        if (!kSolo && a.ranks > 1) {
             tiles = (int)((uint32_t)tiles * (uint32_t)(rank + 1) / (uint32_t)a.ranks);
             none = tile == tiles;
             if (none) tiles = tile + 1;
         }
-        int64_t row_begin = a.whole ? u0 : u0 - tile;  // unit at which the row begins (its number, where rows are whole)
-        int n_row = 0;                  // rows begun in this CTA
+        int64_t row_begin = kSolo || a.whole ? u0 : u0 - tile;  // unit at which the row begins (its number, where rows are whole)
+        Turn at, q_at;  // of the stages; of the queries' places, a row's the next
+        q_at.stage = stages - 1;
         const uint64_t policy = evict_first_policy();
         const int boxes = C::kTile >> a.lg_box, box_bytes = C::kRow << a.lg_box;
         bool ok = true, end = false;
         int done = 0;
         for (; !end; ++done) {
-            const int stage = done % C::kStages, h = hr * a.abreast + abreast;
+            const int stage = at.stage, h = hr * a.abreast + abreast;
             const bool first = done == 0 || tile == 0;
-            end = a.whole ? tile == tiles - 1 && row_begin + 1 == u1 : u0 + done + 1 == u1;
+            end = kSolo || a.whole ? tile == tiles - 1 && row_begin + 1 == u1 : u0 + done + 1 == u1;
             const bool last = end || tile == tiles - 1;
             int part = kAlone;
-            if (!a.whole) part = row_begin < u0 ? 0 : row_begin + tiles > u1 ? 1 : kAlone;
+            if (!kSolo && !a.whole) part = row_begin < u0 ? 0 : row_begin + tiles > u1 ? 1 : kAlone;
             else if (a.ranks > 1) part = kShared;
             // ---- block ids of the tile: 32 entries of the table at a time, the next 32 on their way
             const int tile0 = (tile_first + tile) * C::kTile;
@@ -772,9 +834,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             const bool there = wanted && id >= 0 && id < a.n_blocks;
             if (wanted && !there) raise_status(a.status, ZKV_ERR_RANGE);
             const unsigned copy = __ballot_sync(0xffffffffu, there), bad = __ballot_sync(0xffffffffu, wanted && !there);
-            if (first) ++n_row;
-            const int q_slot = (n_row - 1) % C::kStages;
-            if (done >= C::kStages) ok = wait_for(empty + stage, (uint32_t)((done / C::kStages - 1) & 1), a.status);
+            if (first) q_at.next(stages);
+            if (done >= stages) ok = wait_for(empty + stage, at.phase ^ 1, a.status);
             if (!__all_sync(0xffffffffu, ok)) break;
             if (lane == 0) {
                 Unit& x = units[stage];
@@ -790,21 +851,22 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             }
             __syncwarp();
             if (there) {
-                const uint32_t dst = smem_u32(kv + stage * 2 * C::kKv) + lane * box_bytes;
+                const uint32_t dst = smem_u32(kv + stage * 2 * half) + lane * box_bytes;
                 // a box is a whole block, or a tile's tokens of one
                 const int in_block = a.shift > a.lg_box ? tile0 & ((1 << a.shift) - 1) : 0;
                 tma_load_5d(dst, &a.tk, in_block, h, id, full + stage, policy);
-                tma_load_5d(dst + C::kKv, &a.tv, in_block, h, id, full + stage, policy);
+                tma_load_5d(dst + half, &a.tv, in_block, h, id, full + stage, policy);
             }
             if (first && lane >= 32 - C::kHeadsMax && lane - (32 - C::kHeadsMax) < n_heads) {
                 const int j = lane - (32 - C::kHeadsMax);
-                bulk_g2s(qs + q_slot * C::kQSlot + j * C::kQPitch,
+                bulk_g2s(qs + q_at.stage * C::kQSlot + j * C::kQPitch,
                          a.q + b * a.q_row + (int64_t)(h * a.G + chunk * a.heads + j) * a.q_head, D * 2, full + stage);
             }
             // ---- next unit
+            at.next(stages);
             if (++tile == tiles) {
                 tile = 0;
-                row_begin += a.whole ? 1 : tiles;
+                row_begin += kSolo || a.whole ? 1 : tiles;
                 if (++hr == a.head_rows) {
                     hr = 0;
                     if (++b < a.batch) begin_request();
@@ -812,8 +874,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             }
         }
         if (!ok)  // a consumer gave up: the copies on their way land in this CTA's memory, so wait for them
-            for (int i = max(0, done - C::kStages); i < done; ++i)
-                wait_for(full + i % C::kStages, (uint32_t)((i / C::kStages) & 1), a.status);
+            for (int i = max(0, done - stages); i < done; ++i)
+                wait_for(full + i % stages, (uint32_t)((i / stages) & 1), a.status);
         return;
     }
 
@@ -832,49 +894,92 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         epi_phase ^= 1;
         return got;
     };
-    bool end = false, alive = true;
-    for (int i = 0; !end; ++i) {
-        const int stage = i % C::kStages;
-        if (!__all_sync(0xffffffffu, wait_for(full + stage, (uint32_t)((i / C::kStages) & 1), a.status))) {
+    bool alive = true;
+    Turn at, q_at;
+    q_at.stage = stages - 1;
+    // a warp sees every unit, its 1/4 of the tokens, or (solo) every fourth unit, all of them
+    constexpr int parts = kSolo ? kConsumers : 1;
+    const int part0 = kSolo ? 0 : warp;
+    const int mine = kSolo ? (int)(u1 - u0) - warp : 1;
+    if (kSolo) at.skip(stages, warp);
+    bool end = mine <= 0;
+    for (int i = 0; !end; ++i, kSolo ? at.skip(stages, kConsumers) : at.next(stages)) {
+        const int stage = at.stage;
+        if (!__all_sync(0xffffffffu, wait_for(full + stage, at.phase, a.status))) {
             alive = false;
             break;
         }
         const Unit x = units[stage];
-        end = x.flags & kEnd;
-        uint8_t* const base = kv + stage * 2 * C::kKv;
+        end = kSolo ? mine <= (i + 1) * kConsumers : (x.flags & kEnd) != 0;
+        uint8_t* const base = kv + stage * 2 * half;
         if (x.flags & kFirst) {
-            uint8_t* const q_row = qs + (n_row % C::kStages) * C::kQSlot;
+            q_at.next(stages);
+            uint8_t* const q_row = qs + (kSolo ? stage : q_at.stage) * C::kQSlot;
             if constexpr (C::kQShared && kF8 && kQ == ZKV_DT_BF16) {
-                row.narrow_shared(q_row);
-                alive = meet();
+                for (int p = 0; p < parts; ++p) row.narrow_shared(q_row, part0 + p);
+                __syncwarp();
+                if (!kSolo) alive = meet();
                 if (!alive) break;
             }
             row.init(a, q_row, n_heads, kF8 && a.k_scale ? a.k_scale[x.h] : 1.f);
             ++n_row;
         }
-        // 16 tokens lie in one box (a box has 16 or more)
-        uint32_t at[C::kSub];
-        int v0[C::kSub], v1[C::kSub];
-        bool any = false, partial = false;
+#pragma unroll 1
+        for (int p = 0; p < parts; ++p) {
+            // 16 tokens lie in one box (a box has 16 or more)
+            uint32_t from[C::kSub];
+            int v0[C::kSub], v1[C::kSub];
+            bool any = false, partial = false;
 #pragma unroll
-        for (int k = 0; k < C::kSub; ++k) {
-            const int in_tile = 16 * (C::kSub * warp + k), box = in_tile >> a.lg_box;
-            at[k] = (uint32_t)((box << a.lg_box) * C::kRow + (in_tile - (box << a.lg_box)) * C::kInner);
-            v0[k] = max(x.lo - x.tile0 - in_tile, 0);
-            v1[k] = (x.bad >> box) & 1 ? 0 : min(x.len - x.tile0 - in_tile, 16);
-            any |= v0[k] < v1[k];
-            partial |= v0[k] > 0 || v1[k] < 16;
-        }
-        if (any) {
+            for (int k = 0; k < C::kSub; ++k) {
+                const int in_tile = 16 * (C::kSub * (part0 + p) + k), box = in_tile >> a.lg_box;
+                from[k] = (uint32_t)((box << a.lg_box) * C::kRow + (in_tile - (box << a.lg_box)) * C::kInner);
+                v0[k] = max(x.lo - x.tile0 - in_tile, 0);
+                v1[k] = (x.bad >> box) & 1 ? 0 : min(x.len - x.tile0 - in_tile, 16);
+                any |= v0[k] < v1[k];
+                partial |= v0[k] > 0 || v1[k] < 16;
+            }
+            if (!any) continue;
             const uint32_t piece = (uint32_t)C::kInner << a.lg_box;
             if (partial) {
 #pragma unroll
-                for (int k = 0; k < C::kSub; ++k) row.clear_rows(base + C::kKv + at[k], piece, v0[k], v1[k]);
+                for (int k = 0; k < C::kSub; ++k) row.clear_rows(base + half + from[k], piece, v0[k], v1[k]);
             }
-            row.step(a, smem_u32(base), at, piece, v0, v1, partial);
+            row.step(a, smem_u32(base), half, from, piece, v0, v1, partial);
             if (partial) proxy_fence();
         }
         if (!(x.flags & kLast)) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + stage);
+            continue;
+        }
+        float* buf = reinterpret_cast<float*>(base);
+        const float v_scale = kF8 && a.v_scale ? a.v_scale[x.h] : 1.f;
+        const int64_t head0 = ((int64_t)x.b * a.kv_heads + x.h) * a.G + chunk * a.heads;
+        if constexpr (kSolo) {  // the row is this warp's: through its stage to whole lines of the output
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float inv[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float sum = row.total(n, e);
+                    const int head = 8 * n + 2 * t + e;
+                    inv[e] = sum == 0.f ? 0.f : v_scale / sum;
+                    if (a.lse && g == 0 && head < n_heads)
+                        a.lse[head0 + head] = (row.m[n][e] + log2f(sum)) * 0.6931471805599453f;
+                }
+                row.put(buf, n, inv);
+                __syncwarp();
+                for (int idx = lane; idx < 8 * (D / 4); idx += 32) {
+                    const int hl = idx / (D / 4), d = 4 * (idx % (D / 4));
+                    if (8 * n + hl >= n_heads) continue;
+                    const float4 y = *reinterpret_cast<const float4*>(buf + hl * D + (d ^ (((hl >> 1) & 3) << 3)));
+                    store4<kQ>(a.out, (head0 + 8 * n + hl) * D + d, y);
+                }
+                __syncwarp();
+            }
+            proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + stage);
             continue;
@@ -885,19 +990,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float s = row.l[n][e];
-                s += __shfl_xor_sync(0xffffffffu, s, 4);
-                s += __shfl_xor_sync(0xffffffffu, s, 8);
-                s += __shfl_xor_sync(0xffffffffu, s, 16);
+                const float s = row.total(n, e);
                 if (g == 0) mine_ml[warp * C::kHeadsMax + 8 * n + 2 * t + e] = make_float2(row.m[n][e], s);
             }
         if (!meet()) {  // statistics written, stage read by all
             alive = false;
             break;
         }
-        float* buf = reinterpret_cast<float*>(base);
-        const float v_scale = kF8 && a.v_scale ? a.v_scale[x.h] : 1.f;
-        const int64_t head0 = ((int64_t)x.b * a.kv_heads + x.h) * a.G + chunk * a.heads;
         const int64_t slot = (int64_t)blockIdx.x * 2 + x.part;
 #pragma unroll
         for (int r = 0; r < NT; r += C::kJoinTiles) {
@@ -913,23 +1012,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
                         mx = fmaxf(mx, mine_ml[w * C::kHeadsMax + 8 * (r + n) + 2 * t + e].x);
                     fac[e] = exp2_fast(row.m[r + n][e] - (mx == -INFINITY ? 0.f : mx));
                 }
-                // dims of a head are permuted by its pair's number, so that the 32 lanes meet 32 banks
-                float* p = buf + (warp * 8 * C::kJoinTiles + 8 * n + 2 * t) * D;
-#pragma unroll
-                for (int j = 0; j < C::kMTiles; ++j) {
-                    const float* o = row.o[j][r + n];
-                    if constexpr (kF8) {
-                        const int d = (16 * j + 2 * g) ^ (t << 3);
-                        *reinterpret_cast<float2*>(p + d) = make_float2(o[0] * fac[0], o[2] * fac[0]);
-                        *reinterpret_cast<float2*>(p + D + d) = make_float2(o[1] * fac[1], o[3] * fac[1]);
-                    } else {
-                        const int d = (16 * j + g) ^ (t << 3), d8 = (16 * j + g + 8) ^ (t << 3);
-                        p[d] = o[0] * fac[0];
-                        p[D + d] = o[1] * fac[1];
-                        p[d8] = o[2] * fac[0];
-                        p[D + d8] = o[3] * fac[1];
-                    }
-                }
+                row.put(buf + (warp * 8 * C::kJoinTiles + 8 * n) * D, r + n, fac);
             }
             if (alive) alive = meet();
             if (!alive) continue;
@@ -967,7 +1050,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + stage);
     }
-    if (a.ranks == 1) return;
+    if (kSolo || a.ranks == 1) return;
     // ---- the row's parts, by the cluster's ranks in order; every CTA meets here whatever became of its waits
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
@@ -1254,32 +1337,25 @@ static Cut plan_call(int batch, int kv_heads, int chunks, int row_bytes, int win
     return c;
 }
 
-template <int kQ, bool kF8, int D, int NT>
-static int launch_decode(DecodeArgs& a, cudaStream_t st) {
-    using C = Cfg<kQ, kF8, D, NT>;
-    const auto kernel = pool_decode_kernel<kQ, kF8, D, NT>;
-    static int raised[64] = {};  // devices whose limits of this kernel were raised
+// A decode kernel's launch, its limits raised on its first one on a device.
+template <int kQ, bool kF8, int D, int NT, bool kSolo>
+static int launch_kernel(const DecodeArgs& a, int grid, int smem, cudaStream_t st) {
+    const auto kernel = pool_decode_kernel<kQ, kF8, D, NT, kSolo>;
+    static int raised[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ZKV_ERR_LAUNCH;
     if (!raised[dev]) {
-        if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
+        using C = Cfg<kQ, kF8, D, NT>;
+        if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem_of(C::kRing)) !=
                 cudaSuccess ||
             cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
             return ZKV_ERR_LAUNCH;
         raised[dev] = 1;
     }
-    const Cut cut = plan_call(a.batch, a.kv_heads, a.chunks, C::kRow, a.window, a.cap);
-    a.whole = cut.whole, a.ranks = cut.ranks, a.abreast = cut.whole ? 1 : cut.abreast;
-    a.head_rows = a.kv_heads / a.abreast, a.side = a.abreast * a.chunks;
-    if (!a.whole && !a.parts) return ZKV_ERR_ARG;
-    const int64_t rows = (int64_t)a.batch * a.head_rows;
-    const int64_t wave = std::max(1, C::kPerSm * sm_count() / a.side);
-    if (a.ranks > 1) a.groups = (int)rows;
-    else a.groups = (int)std::min(wave, most_groups(a.batch, a.head_rows, a.side, a.whole ? 0 : a.cap, C::kTile));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.groups * a.side * a.ranks));
+    cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1290,7 +1366,34 @@ static int launch_decode(DecodeArgs& a, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = a.ranks > 1 ? 2 : 1;
     if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return ZKV_ERR_LAUNCH;
-    int rc = launch_status();
+    return launch_status();
+}
+
+template <int kQ, bool kF8, int D, int NT>
+static int launch_decode(DecodeArgs& a, cudaStream_t st) {
+    using C = Cfg<kQ, kF8, D, NT>;
+    const Cut cut = plan_call(a.batch, a.kv_heads, a.chunks, C::kRow, a.window, a.cap);
+    a.whole = cut.whole, a.ranks = cut.ranks, a.abreast = cut.whole ? 1 : cut.abreast;
+    a.head_rows = a.kv_heads / a.abreast, a.side = a.abreast * a.chunks;
+    if (!a.whole && !a.parts) return ZKV_ERR_ARG;
+    const int64_t rows = (int64_t)a.batch * a.head_rows;
+    const int64_t wave = std::max(1, C::kPerSm * sm_count() / a.side);
+    if (a.ranks > 1) a.groups = (int)rows;
+    else a.groups = (int)std::min(wave, most_groups(a.batch, a.head_rows, a.side, a.whole ? 0 : a.cap, C::kTile));
+    const int grid = a.groups * a.side * a.ranks;
+    if (a.whole && a.ranks == 1 && a.window == 0 && a.cap <= C::kTile &&
+        (a.cap <= 16 * C::kSub || rows >= kSoloRows * wave)) {
+        // Stages of what a row can have, in whole boxes and products.  Their number is a multiple of the warps': a stage
+        // is then always the same warp's, which has seen its last phase end (a parity alone does not tell a phase from
+        // the one after the next).
+        const int unit = std::max(1 << a.lg_box, 16 * C::kSub);
+        a.half = std::max(1, (a.cap + unit - 1) / unit) * unit * C::kRow;
+        const int stage = 2 * a.half + C::kQSlot + (int)sizeof(Unit);
+        a.stages = std::min(kMaxStages, C::kRing / stage / kConsumers * kConsumers);
+        if (a.stages >= kConsumers)
+            return launch_kernel<kQ, kF8, D, NT, true>(a, grid, C::smem_of(a.stages * stage), st);
+    }
+    int rc = launch_kernel<kQ, kF8, D, NT, false>(a, grid, C::smem_of(C::kStages * C::kStage), st);
     if (rc == ZKV_OK && !a.whole && a.groups > 1) {
         const int by_row = rows <= a.groups;
         const int cands = by_row ? (int)rows : a.groups;
