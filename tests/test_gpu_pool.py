@@ -227,6 +227,14 @@ def test_decode_many_short_rows(qt, pt, D):
     run_decode(745, [200 - i % 200 for i in range(610)], 256, 1, 9, D, qt, pt, "hnd", wide=False, max_len=200)
 
 
+@pytest.mark.parametrize("D,G", [(256, 4), (256, 16), (128, 16)])
+@pytest.mark.parametrize("qt,pt", [(BF, BF), (HF, HF), (BF, F8), (HF, F8)])
+@pytest.mark.parametrize("B", [297, 1100])
+def test_decode_rows_of_a_tile(B, qt, pt, D, G):
+    """Room for two or three rows in a CTA: as many warps work, each on rows of its own."""
+    run_decode(750, [(11 * i) % 65 for i in range(B)], 16, 1, G, D, qt, pt, "nhd", wide=False, max_len=64)
+
+
 def test_decode_all_empty():
     run_decode(720, [0, 0, 0], 16, 2, 4, 128, BF, BF, "hnd")
     run_decode(721, [0], 16, 1, 1, 64, HF, F8, "hnd")

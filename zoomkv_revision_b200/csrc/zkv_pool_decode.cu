@@ -60,7 +60,7 @@ constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxGrid = 480;                   // CTAs that a workspace is sized for
 constexpr int kWholeTokens = 256;               // requests up to this length are never cut
 constexpr int kMaxChunks = 320;                 // of 16 query heads per kv head
-constexpr int kMaxStages = 8;                   // of a CTA's ring (a multiple of kConsumers)
+constexpr int kMaxStages = 8;                   // of a CTA's ring (kSolo: a multiple of its working warps)
 constexpr int kMaxRanks = 16;                   // CTAs of a cluster that shares a row
 // Up to kWholeBytes of K and V, and kRankTiles tiles a CTA or twice that where the CTAs fill their waves to 4/5, whole
 // rows in one launch are ahead of ranges and a join, which 4 us more issue (8 kv heads of 128, bf16, us on the GPU, whole
@@ -108,7 +108,7 @@ struct DecodeArgs {
     int groups;     // ranges
     int whole;      // rows are not cut by units
     int ranks;      // CTAs (a cluster) that share a row, if `whole`
-    int stages, half;  // kSolo: the ring's stages, two times `half` bytes each, K and V
+    int stages, half, workers;  // kSolo: the ring's stages, two times `half` bytes each, K and V; warps that take rows
     int shift, lg_box, width, window;
     float scale, softcap;
 };
@@ -330,7 +330,7 @@ struct Ranges {
     }
 };
 
-// A place in a ring and the phase of its barrier in this round.
+// A place in a ring and the parity that its barrier completes next.
 struct Turn {
     int stage = 0;
     uint32_t phase = 0;
@@ -699,7 +699,9 @@ __device__ __forceinline__ void store4(void* out, int64_t i, float4 x) {
 // four rows in hand and none waits for another.  For rows of a tile at most,
 // where the four warps' chain and join take 1.9 us a row whatever it holds: 256
 // requests of 1 token, 8 kv heads of 128, 17.1 -> 9.1 us, 131 of 8 tokens, 16 kv
-// heads of 256, 54.4 -> 17.2.
+// heads of 256, 54.4 -> 17.2.  Where the ring has room for two or three stages
+// only, as many warps work: 256 requests of 40 tokens, 8 kv heads of 256, 41.4
+// -> 27.4, with 16 query heads each 74.1 -> 46.7.
 template <int kQ, bool kF8, int D, int NT, bool kSolo>
 __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     pool_decode_kernel(const __grid_constant__ DecodeArgs a) {
@@ -900,17 +902,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     // a warp sees every unit, its 1/4 of the tokens, or (solo) every fourth unit, all of them
     constexpr int parts = kSolo ? kConsumers : 1;
     const int part0 = kSolo ? 0 : warp;
-    const int mine = kSolo ? (int)(u1 - u0) - warp : 1;
+    const int workers = kSolo ? a.workers : 1;
+    const int mine = kSolo ? (warp < workers ? (int)(u1 - u0) - warp : 0) : 1;
     if (kSolo) at.skip(stages, warp);
     bool end = mine <= 0;
-    for (int i = 0; !end; ++i, kSolo ? at.skip(stages, kConsumers) : at.next(stages)) {
+    for (int i = 0; !end; ++i, kSolo ? at.skip(stages, workers) : at.next(stages)) {
         const int stage = at.stage;
         if (!__all_sync(0xffffffffu, wait_for(full + stage, at.phase, a.status))) {
             alive = false;
             break;
         }
         const Unit x = units[stage];
-        end = kSolo ? mine <= (i + 1) * kConsumers : (x.flags & kEnd) != 0;
+        end = kSolo ? mine <= (i + 1) * workers : (x.flags & kEnd) != 0;
         uint8_t* const base = kv + stage * 2 * half;
         if (x.flags & kFirst) {
             q_at.next(stages);
@@ -1383,15 +1386,16 @@ static int launch_decode(DecodeArgs& a, cudaStream_t st) {
     const int grid = a.groups * a.side * a.ranks;
     if (a.whole && a.ranks == 1 && a.window == 0 && a.cap <= C::kTile &&
         (a.cap <= 16 * C::kSub || rows >= kSoloRows * wave)) {
-        // Stages of what a row can have, in whole boxes and products.  Their number is a multiple of the warps': a stage
-        // is then always the same warp's, which has seen its last phase end (a parity alone does not tell a phase from
-        // the one after the next).
+        // Stages of what a row can have, in whole boxes and products; two or more fit, a stage being no larger than the
+        // other kernel's.  Their number is a multiple of the working warps': a stage is then always the same warp's,
+        // which has seen its last phase end (a parity alone does not tell a phase from the one after the next).
         const int unit = std::max(1 << a.lg_box, 16 * C::kSub);
         a.half = std::max(1, (a.cap + unit - 1) / unit) * unit * C::kRow;
         const int stage = 2 * a.half + C::kQSlot + (int)sizeof(Unit);
-        a.stages = std::min(kMaxStages, C::kRing / stage / kConsumers * kConsumers);
-        if (a.stages >= kConsumers)
-            return launch_kernel<kQ, kF8, D, NT, true>(a, grid, C::smem_of(a.stages * stage), st);
+        const int fit = std::min(kMaxStages, C::kRing / stage);
+        a.workers = std::min(kConsumers, fit);
+        a.stages = fit / a.workers * a.workers;
+        return launch_kernel<kQ, kF8, D, NT, true>(a, grid, C::smem_of(a.stages * stage), st);
     }
     int rc = launch_kernel<kQ, kF8, D, NT, false>(a, grid, C::smem_of(C::kStages * C::kStage), st);
     if (rc == ZKV_OK && !a.whole && a.groups > 1) {
