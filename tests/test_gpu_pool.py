@@ -720,3 +720,26 @@ def test_refusals():
         ops.pool_plan(big, None, big.view(9000, 1), big, n, 16, slots)
     with pytest.raises(TypeError):
         ops.pool_release(i32([1, 0]), lens, table, free, n, 16)
+
+
+def test_refusals_of_host_memory():
+    """What the kernels would write lies on the pool's device."""
+    k, v, _, _ = make_pool(92, 4, 16, 2, 128, BF, "hnd")
+    pool = ops.KVPool(k, v)
+    q, lens, table = torch.zeros(2, 8, 128, dtype=BF, device=DEV), i32([1, 1]), i32([[0], [1]])
+    rows, slots = torch.zeros(2, 2, 128, dtype=BF, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV)
+    host = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.pool_decode(q, pool, lens, table, status=host)
+    with pytest.raises(TypeError):
+        ops.pool_decode(q, pool, lens, table, status=host.to(DEV).long())
+    with pytest.raises(ValueError):
+        ops.pool_write(rows, rows, slots, pool, status=host)
+    with pytest.raises(TypeError):
+        ops.pool_write(rows, rows, slots, pool, status=host.to(DEV).float())
+    n = ops.pool_decode_ws_bytes(2, 8, pool, 10 ** 5)
+    assert n > 0
+    for ws in (torch.empty(n, dtype=torch.uint8), torch.empty(n, dtype=torch.int8, device=DEV),
+               torch.empty(2 * n, dtype=torch.uint8, device=DEV)[::2]):
+        with pytest.raises(ValueError):
+            ops.pool_decode(q, pool, lens, torch.zeros(2, 10 ** 5, dtype=torch.int32, device=DEV), workspace=ws)

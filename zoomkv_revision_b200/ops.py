@@ -1276,6 +1276,13 @@ def pool_release(done, lens, block_table, free_blocks, n_free, block_size: int, 
         check(rc, "zkv_pool_release")
 
 
+def _status_word(t, dev):
+    if t.dtype is not _INT32:
+        raise TypeError(f"status must be torch.int32; got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError("status must be on the pool's device")
+
+
 def _whole_rows(t):
     """t [n, heads, dim] with contiguous dims and 16-byte rows (a copy where it has not)."""
     row, head, one = t.stride()
@@ -1297,13 +1304,15 @@ def pool_write(k, v, slots, pool: KVPool, *, status=None):
     code = _POOL_DTYPES.get(dt, 2)
     if v.dtype is not dt or code == 2 or (pool.dtype is not dt and pool.code != 2):
         raise TypeError(f"k {dt} and v {v.dtype} do not go into a {pool.dtype} pool")
-    if slots.dtype is not torch.int64 or (status is not None and status.dtype is not _INT32):
-        raise TypeError("slots must be torch.int64 and status torch.int32")
+    if slots.dtype is not torch.int64:
+        raise TypeError(f"slots must be torch.int64; got {slots.dtype}")
     if slots.numel() < n or not slots.is_contiguous():
         raise ValueError("slots must be contiguous, one per token")
     dev = pool.index
     if k.get_device() != dev or v.get_device() != dev or slots.get_device() != dev:
         raise ValueError("tensors must be on the pool's device")
+    if status is not None:
+        _status_word(status, dev)
     k, v = _whole_rows(k), _whole_rows(v)
     ks, vs = k.stride(), v.stride()
     rc = lib().zkv_pool_write(k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code, slots.data_ptr(), n, pool.ref,
@@ -1338,8 +1347,10 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
         raise TypeError(f"q {dt} does not fit a {pool.dtype} pool")
     if q.get_device() != dev or lens.get_device() != dev:
         raise ValueError("tensors must be on the pool's device")
-    if lens.dtype is not _INT32 or (status is not None and status.dtype is not _INT32):
-        raise TypeError("lens and status must be torch.int32")
+    if lens.dtype is not _INT32:
+        raise TypeError(f"lens must be torch.int32; got {lens.dtype}")
+    if status is not None:
+        _status_word(status, dev)
     if lens.numel() != B or not lens.is_contiguous():
         raise ValueError("lens must be contiguous, one value per request")
     ld, width = _block_table(block_table, B, dev)
@@ -1361,6 +1372,8 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
         window = 0
     ws, ws_bytes = None, 0
     if workspace is not None:
+        if workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.get_device() != dev:
+            raise ValueError("workspace must be contiguous torch.uint8 on the pool's device")
         ws, ws_bytes = workspace.data_ptr(), workspace.numel()
     else:
         ws_bytes = pool_decode_ws_bytes(B, Hq, pool, width, max_len, window)
