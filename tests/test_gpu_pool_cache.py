@@ -42,6 +42,19 @@ def test_decode_loop_over_the_pool_follows_a_dense_forward(graphs):
         assert (got - want).abs().max().item() <= 0.05 * want.abs().max().item(), i
 
 
+def test_a_request_may_fill_its_last_block():
+    cache = PoolCache(1, 1, 1, 64, 20)             # two blocks of 16
+    rows = torch.randn(30, 1, 64, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).to(torch.bfloat16)
+    cache.write(0, rows, rows, cache.plan(torch.tensor([30], dtype=torch.int32, device=DEV), 30, 30))
+    q = torch.randn(1, 2, 64, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV).to(torch.bfloat16)
+    out, wide = cache.attend(0, q), cache.attend(0, q, max_len=0)
+    cache.check()
+    x = rows[:, 0].double()
+    want = torch.softmax(q[0].double() @ x.T / 8, -1) @ x
+    for got in (out, wide):  # rounding of the output, and of probabilities and scores as 2^-10 of the largest value
+        assert bool(((got[0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * x.abs().max()).all())
+
+
 def test_too_few_blocks_are_reported():
     cache = PoolCache(1, 2, 1, 64, 64, n_blocks=5)
     slots = cache.plan(torch.tensor([40, 40], dtype=torch.int32, device=DEV), 80, 40)

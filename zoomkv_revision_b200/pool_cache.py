@@ -33,10 +33,11 @@ from . import ops
 
 class PoolCache:
     """layers x pools of n_blocks blocks of block_size tokens for up to
-    `batch` requests of up to max_length tokens (n_blocks: room for all of
-    them by default; fewer blocks serve more, shorter requests).  dtype
-    bfloat16, float16 or float8_e4m3fn, for which k_scale / v_scale
-    [layers, kv_heads] fp32 give what a stored 1.0 stands for (None: 1)."""
+    `batch` requests of up to max_length tokens, in whole blocks (n_blocks:
+    room for all of them by default; fewer blocks serve more, shorter
+    requests).  dtype bfloat16, float16 or float8_e4m3fn, for which
+    k_scale / v_scale [layers, kv_heads] fp32 give what a stored 1.0 stands
+    for (None: 1)."""
 
     def __init__(self, layers: int, batch: int, kv_heads: int, head_dim: int, max_length: int, *, n_blocks=None,
                  block_size: int = 16, dtype=torch.bfloat16, k_scale=None, v_scale=None, device="cuda"):
@@ -64,7 +65,7 @@ class PoolCache:
         n_slots in all and max_new for one request.  Returns the slot map [n_slots]."""
         slots = torch.empty(n_slots, dtype=torch.int64, device=self.k.device)
         ops.pool_plan(self.lens, new_lens, self.table, self.free, self.n_free, self.block_size, slots, status=self.status)
-        self.bound = min(self.bound + max_new, self.max_length)
+        self.bound = min(self.bound + max_new, self.width * self.block_size)
         self.slots = slots
         return slots
 
@@ -73,8 +74,11 @@ class PoolCache:
         ops.pool_write(k, v, slots, self.pools[layer], status=self.status)
 
     def attend(self, layer: int, q, **kw):
-        """Attention of q [batch, (1,) q_heads, head_dim] over each request's tokens (keywords of ops.pool_decode)."""
-        return ops.pool_decode(q, self.pools[layer], self.lens, self.table, max_len=self.bound, status=self.status, **kw)
+        """Attention of q [batch, (1,) q_heads, head_dim] over each request's tokens (keywords of ops.pool_decode;
+        max_len is the bound that plan keeps, so a call that is captured in a graph and replayed gives its own: 0 for
+        all of the table's room)."""
+        kw.setdefault("max_len", self.bound)
+        return ops.pool_decode(q, self.pools[layer], self.lens, self.table, status=self.status, **kw)
 
     def release(self, done, bound=None) -> None:
         """Ends the requests with done[b] ([batch] bool on the GPU).  bound: the longest that is left, where the host
