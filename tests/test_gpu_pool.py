@@ -180,6 +180,18 @@ def test_decode_softcap_and_scale(softcap):
     run_decode(603, [5, 64, 700], 16, 2, 4, 128, HF, HF, "hnd", scale=-0.1)
 
 
+@pytest.mark.parametrize("pt", [BF, F8])
+def test_decode_wide_softcap(pt):
+    """A cap far above the scores leaves them: c tanh(x / c) is off by x^3 / 3 c^2, under 2^-20 for |x| < 16 and c = 1e5,
+    so the tolerance is the one without a cap."""
+    lens, S, H, G, D = [1, 64, 700], 16, 2, 4, 128
+    k, v, ks, vs = make_pool(610, 60, S, H, D, pt, "hnd")
+    table = make_table(611, lens, S, 60, 44)
+    q = torch.randn(3, H * G, D, generator=gen(612), device=DEV).to(BF)
+    out, lse = ops.pool_decode(q, ops.KVPool(k, v, ks, vs), i32(lens), table, scale=0.03, softcap=1e5, return_lse=True)
+    check_decode(q, k, v, ks, vs, lens, table, out, lse, 0.03)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("qt,pt", [(BF, BF), (HF, HF), (BF, F8), (HF, F8)])
 def test_decode_few_rows(qt, pt, D):

@@ -233,6 +233,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// tanh to 2^-20 of itself: with t = exp(-2|u|), (1 - t) / (1 + t), where t's error of 2^-22 of itself leaves 2^-23; below
+// 1/4, where 1 - t cancels, Taylor's polynomial, whose next term is 2^-26.  tanhf of an exact quotient in every score
+// made 219 requests of 2917 e4m3 tokens, 1 kv head of 128, take 58.2 us (34.0 without a soft cap).
+__device__ __forceinline__ float tanh_fast(float u) {
+    const float w = fabsf(u), s = u * u, t = exp2_fast(-2.8853900817779268f * w);
+    const float p = -1.f / 3 + s * (2.f / 15 + s * (-17.f / 315 + s * (62.f / 2835)));
+    return w < 0.25f ? u + u * (s * p) : copysignf(__fdividef(1.f - t, 1.f + t), u);
+}
+
 // D(16x8 f32) += A(16x16, row) * B(16x8, col), both bf16 or both fp16
 template <bool kBf16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -356,7 +365,7 @@ struct Row {
     using C = Cfg<kQ, kF8, D, NT>;
     static constexpr bool kMmaBf16 = kQ == ZKV_DT_BF16 && !kF8;
     float m[NT][2], l[NT][2];   // log2 units; heads 2t, 2t+1 of n-tile (t = lane % 4); l: this lane's tokens
-    float f[NT][2];             // score factor of those heads, log2 units (natural under a soft cap)
+    float f[NT][2];             // score factor of those heads, log2 units (under a soft cap, natural ones of it)
     float o[C::kMTiles][NT][4];
     uint32_t q_at;              // the queries' place, this lane's part
     uint32_t q[C::kQShared ? 1 : D / 16][NT][2];  // B fragments of Q^T, where they are not read from there each time
@@ -447,6 +456,12 @@ struct Row {
                 f[n][1] *= __shfl_sync(0xffffffffu, up, 8 * t + 4);
             }
         }
+        if (a.softcap > 0.f)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)  // finite, so that a score of 0 stays one
+                    f[n][e] = fminf(fmaxf(f[n][e] / a.softcap, -3.4e38f), 3.4e38f);
 #pragma unroll
         for (int j = 0; j < C::kMTiles; ++j)
 #pragma unroll
@@ -548,7 +563,7 @@ struct Row {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float y = x[i][n][e] * f[n][e & 1];
-                    if (a.softcap > 0.f) y = a.softcap * 1.4426950408889634f * tanhf(y / a.softcap);
+                    if (a.softcap > 0.f) y = a.softcap * 1.4426950408889634f * tanh_fast(y);
                     x[i][n][e] = y;
                 }
             if (partial) {
