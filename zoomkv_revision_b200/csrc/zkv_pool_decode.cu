@@ -18,6 +18,8 @@
 //    units: a CTA takes whole rows, or a cluster of CTAs shares one row and
 //    joins through distributed shared memory; one launch does, with no scan
 //    and no workspace.
+//  * Where there are many short rows (or windows) a warp takes a row alone and
+//    loads it itself (pool_rows_kernel): nothing to join, nothing to wait for.
 //  * One producer warp per CTA walks the range: block ids from the table, one
 //    5-D TMA copy per block and tensor (dims | tokens | 128-byte pieces | head
 //    | block; any strides, so both memory orders), a ring of stages.  An id
@@ -60,7 +62,7 @@ constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxGrid = 480;                   // CTAs that a workspace is sized for
 constexpr int kWholeTokens = 256;               // requests up to this length are never cut
 constexpr int kMaxChunks = 320;                 // of 16 query heads per kv head
-constexpr int kMaxStages = 8;                   // of a CTA's ring (kSolo: a multiple of its working warps)
+constexpr int kMaxStages = 8;                   // of a CTA's ring
 constexpr int kMaxRanks = 16;                   // CTAs of a cluster that shares a row
 // Up to kWholeBytes of K and V, and kRankTiles tiles a CTA or twice that where the CTAs fill their waves to 4/5, whole
 // rows in one launch are ahead of ranges and a join, which 4 us more issue (8 kv heads of 128, bf16, us on the GPU, whole
@@ -68,7 +70,13 @@ constexpr int kMaxRanks = 16;                   // CTAs of a cluster that shares
 // 32 of 1000 24.5 and 30.9, 40 of 800 34.3 and 31.0, 16 up to 1900 19.3 and 17.7, 64 up to 1000 36.0 and 33.4).
 constexpr int64_t kWholeBytes = 128 << 20;
 constexpr int kRankTiles = 8;
-constexpr int kSoloRows = 2;                    // rows a CTA from which on a warp takes one of more than one product alone
+// A warp a row (pool_rows_kernel) or the CTA's four warps a row: alone where one product's tokens are all, where a row
+// is one load and every CTA has one, or where a CTA has two rows or more of up to kRowLoads loads (e4m3, whose chain is
+// the longer one, kRowLoadsF8), four of which are in flight (three with 8 heads).  256 requests, 8 kv heads of 128, bf16,
+// us with four warps and with one: 1 token 9.1 and 7.3, 100 26.6 and 25.6, 256 (6 loads) 45.5 and 46.9; e4m3 64 13.5 and
+// 12.8, 0..256 30.4 and 27.7, all 256 29.7 and 31.6; a window of 100 31.5 and 25.9; 64 requests of 40 7.0 and 5.7, up to
+// 200 12.3 and 14.5; 16 query heads, blocks of 128 (two in flight), 191 requests of 108..217 64.7 and 78.0.
+constexpr int kRowLoads = 5, kRowLoadsF8 = 8;
 constexpr uint64_t kWaitNs = 2000000000ull;     // limit of each wait inside a CTA
 
 // What a unit is, written by the producer beside its stage.
@@ -108,7 +116,7 @@ struct DecodeArgs {
     int groups;     // ranges
     int whole;      // rows are not cut by units
     int ranks;      // CTAs (a cluster) that share a row, if `whole`
-    int stages, half, workers;  // kSolo: the ring's stages, two times `half` bytes each, K and V; warps that take rows
+    int unit, workers, ahead;   // a warp a row: tokens of a stage, warps of a CTA, stages of a warp
     int shift, lg_box, width, window;
     float scale, softcap;
 };
@@ -140,11 +148,12 @@ struct Cfg {
     static constexpr int kPerSm = (kRow <= 64 && NT == 1) || (kQShared && D <= 128) ? 3
                                   : kQShared || stages_of(2) >= 3                    ? 2
                                                                                      : 1;
+    static constexpr int kRowWarps = kPerSm == 1 ? 8 : kConsumers;  // of a CTA whose warps take rows alone
     // As many stages as fit, but two for 256-byte rows of one n-tile: their warps keep up, and more reads in flight only
     // slow the memory down (8 requests of 32768 165.2 us with three, 159.4 with two; 128-byte rows 162.8 and 173).
     static constexpr int kFit = stages_of(kPerSm);
     static constexpr int kStages = kRow == 256 && !kF8 && NT == 1 ? 2 : kFit < kMaxStages ? kFit : kMaxStages;
-    static constexpr int kRing = kFit * kStage;                   // bytes of a ring at most
+    static constexpr int kRing = 233472 / kPerSm - kOther - kFixed - kMl;  // bytes of a ring at most
     static constexpr int smem_of(int ring) { return ring + kFixed + kMl; }
     static constexpr bool kTwoParts = !(kF8 && kQ == ZKV_DT_BF16);  // the probability as hi + lo
     static constexpr int kMTiles = D / 16;
@@ -701,6 +710,31 @@ struct Row {
         }
         __syncwarp();
     }
+
+    // Part `part` of a unit: 16 tokens a product, kSub products.
+    __device__ __forceinline__ void tokens(const DecodeArgs& a, const Unit& x, uint8_t* base, int half, int part) {
+        // 16 tokens lie in one box (a box has 16 or more)
+        uint32_t from[C::kSub];
+        int v0[C::kSub], v1[C::kSub];
+        bool any = false, partial = false;
+#pragma unroll
+        for (int k = 0; k < C::kSub; ++k) {
+            const int in_tile = 16 * (C::kSub * part + k), box = in_tile >> a.lg_box;
+            from[k] = (uint32_t)((box << a.lg_box) * C::kRow + (in_tile - (box << a.lg_box)) * C::kInner);
+            v0[k] = max(x.lo - x.tile0 - in_tile, 0);
+            v1[k] = (x.bad >> box) & 1 ? 0 : min(x.len - x.tile0 - in_tile, 16);
+            any |= v0[k] < v1[k];
+            partial |= v0[k] > 0 || v1[k] < 16;
+        }
+        if (!any) return;
+        const uint32_t piece = (uint32_t)C::kInner << a.lg_box;
+        if (partial) {
+#pragma unroll
+            for (int k = 0; k < C::kSub; ++k) clear_rows(base + half + from[k], piece, v0[k], v1[k]);
+        }
+        step(a, smem_u32(base), half, from, piece, v0, v1, partial);
+        if (partial) proxy_fence();
+    }
 };
 
 template <int kQ>
@@ -710,18 +744,11 @@ __device__ __forceinline__ void store4(void* out, int64_t i, float4 x) {
         make_uint2(pack2<kBf16>(x.x, x.y), pack2<kBf16>(x.z, x.w));
 }
 
-// kSolo: every row is one unit and one warp's, so the four warps of a CTA have
-// four rows in hand and none waits for another.  For rows of a tile at most,
-// where the four warps' chain and join take 1.9 us a row whatever it holds: 256
-// requests of 1 token, 8 kv heads of 128, 17.1 -> 9.1 us, 131 of 8 tokens, 16 kv
-// heads of 256, 54.4 -> 17.2.  Where the ring has room for two or three stages
-// only, as many warps work: 256 requests of 40 tokens, 8 kv heads of 256, 41.4
-// -> 27.4, with 16 query heads each 74.1 -> 46.7.
-template <int kQ, bool kF8, int D, int NT, bool kSolo>
+template <int kQ, bool kF8, int D, int NT>
 __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     pool_decode_kernel(const __grid_constant__ DecodeArgs a) {
     using C = Cfg<kQ, kF8, D, NT>;
-    const int stages = kSolo ? a.stages : C::kStages, half = kSolo ? a.half : C::kKv;
+    constexpr int stages = C::kStages, half = C::kKv;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
     uint8_t* kv = smem;                                                  // [stages] K, V
@@ -736,14 +763,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     if (tid == 0) {
         for (int i = 0; i < stages; ++i) {
             mbar_init(full + i, 1);
-            mbar_init(empty + i, kSolo ? 1 : kConsumers);
+            mbar_init(empty + i, kConsumers);
         }
         mbar_init(&epi, kConsumers);
         mbar_fence_init();
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.tk)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.tv)) : "memory");
     }
-    const int rank = kSolo ? 0 : blockIdx.x % a.ranks, block = kSolo ? blockIdx.x : blockIdx.x / a.ranks;
+    const int rank = blockIdx.x % a.ranks, block = blockIdx.x / a.ranks;
     const int member = block % a.side, chunk = member % a.chunks, abreast = member / a.chunks;
     const int64_t c = block / a.side;
     const int n_heads = min(a.heads, a.G - chunk * a.heads);
@@ -759,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     grid_dep_launch_next();  // the join kernel may become resident; it waits for this grid
     // ---- this CTA's range [u0, u1): of units, or of rows where those are not split
     int64_t u0, u1;
-    if (kSolo || a.whole) {
+    if (a.whole) {
         const int64_t rows = (int64_t)a.batch * a.head_rows;
         u0 = quotient(rows * c, a.groups);
         u1 = quotient(rows * (c + 1), a.groups);
@@ -783,8 +810,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
 
     if (warp == kConsumers) {
         // ---------------------------------------------------- producer
-        int b = kSolo || a.whole ? (int)quotient(u0, a.head_rows) : s_b;
-        int next = kSolo || a.whole ? __ldcg(a.lens + b) : s_len;  // the next request's length, asked for one request ahead
+        int b = a.whole ? (int)quotient(u0, a.head_rows) : s_b;
+        int next = a.whole ? __ldcg(a.lens + b) : s_len;  // the next request's length, asked for one request ahead
         int len, lo, tile_first, tiles;
         auto begin_request = [&]() {
             if (next < 0 || next > a.cap) raise_status(a.status, ZKV_ERR_RANGE);
@@ -804,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         }
         begin_request();
         int hr, tile;  // row of the request, tile of the row
-        if (kSolo || a.whole) {
+        if (a.whole) {
             hr = (int)(u0 - (int64_t)b * a.head_rows);
             tile = (int)((uint32_t)tiles * (uint32_t)rank / (uint32_t)a.ranks);
         } else {
@@ -812,12 +839,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             tile = (int)(s_off - (int64_t)hr * tiles);
         }
         bool none = false;  // more CTAs than tiles: this one has an empty unit
-        if (!kSolo && a.ranks > 1) {
+        if (a.ranks > 1) {
             tiles = (int)((uint32_t)tiles * (uint32_t)(rank + 1) / (uint32_t)a.ranks);
             none = tile == tiles;
             if (none) tiles = tile + 1;
         }
-        int64_t row_begin = kSolo || a.whole ? u0 : u0 - tile;  // unit at which the row begins (its number, where rows are whole)
+        int64_t row_begin = a.whole ? u0 : u0 - tile;  // unit at which the row begins (its number, where rows are whole)
         Turn at, q_at;  // of the stages; of the queries' places, a row's the next
         q_at.stage = stages - 1;
         const uint64_t policy = evict_first_policy();
@@ -827,10 +854,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         for (; !end; ++done) {
             const int stage = at.stage, h = hr * a.abreast + abreast;
             const bool first = done == 0 || tile == 0;
-            end = kSolo || a.whole ? tile == tiles - 1 && row_begin + 1 == u1 : u0 + done + 1 == u1;
+            end = a.whole ? tile == tiles - 1 && row_begin + 1 == u1 : u0 + done + 1 == u1;
             const bool last = end || tile == tiles - 1;
             int part = kAlone;
-            if (!kSolo && !a.whole) part = row_begin < u0 ? 0 : row_begin + tiles > u1 ? 1 : kAlone;
+            if (!a.whole) part = row_begin < u0 ? 0 : row_begin + tiles > u1 ? 1 : kAlone;
             else if (a.ranks > 1) part = kShared;
             // ---- block ids of the tile: 32 entries of the table at a time, the next 32 on their way
             const int tile0 = (tile_first + tile) * C::kTile;
@@ -883,7 +910,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
             at.next(stages);
             if (++tile == tiles) {
                 tile = 0;
-                row_begin += kSolo || a.whole ? 1 : tiles;
+                row_begin += a.whole ? 1 : tiles;
                 if (++hr == a.head_rows) {
                     hr = 0;
                     if (++b < a.batch) begin_request();
@@ -914,58 +941,28 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
     bool alive = true;
     Turn at, q_at;
     q_at.stage = stages - 1;
-    // a warp sees every unit, its 1/4 of the tokens, or (solo) every fourth unit, all of them
-    constexpr int parts = kSolo ? kConsumers : 1;
-    const int part0 = kSolo ? 0 : warp;
-    const int workers = kSolo ? a.workers : 1;
-    const int mine = kSolo ? (warp < workers ? (int)(u1 - u0) - warp : 0) : 1;
-    if (kSolo) at.skip(stages, warp);
-    bool end = mine <= 0;
-    for (int i = 0; !end; ++i, kSolo ? at.skip(stages, workers) : at.next(stages)) {
+    for (bool end = false; !end; at.next(stages)) {
         const int stage = at.stage;
         if (!__all_sync(0xffffffffu, wait_for(full + stage, at.phase, a.status))) {
             alive = false;
             break;
         }
         const Unit x = units[stage];
-        end = kSolo ? mine <= (i + 1) * workers : (x.flags & kEnd) != 0;
+        end = (x.flags & kEnd) != 0;
         uint8_t* const base = kv + stage * 2 * half;
         if (x.flags & kFirst) {
             q_at.next(stages);
-            uint8_t* const q_row = qs + (kSolo ? stage : q_at.stage) * C::kQSlot;
+            uint8_t* const q_row = qs + q_at.stage * C::kQSlot;
             if constexpr (C::kQShared && kF8 && kQ == ZKV_DT_BF16) {
-                for (int p = 0; p < parts; ++p) row.narrow_shared(q_row, part0 + p);
+                row.narrow_shared(q_row, warp);
                 __syncwarp();
-                if (!kSolo) alive = meet();
+                alive = meet();
                 if (!alive) break;
             }
             row.init(a, q_row, n_heads, kF8 && a.k_scale ? a.k_scale[x.h] : 1.f);
             ++n_row;
         }
-#pragma unroll 1
-        for (int p = 0; p < parts; ++p) {
-            // 16 tokens lie in one box (a box has 16 or more)
-            uint32_t from[C::kSub];
-            int v0[C::kSub], v1[C::kSub];
-            bool any = false, partial = false;
-#pragma unroll
-            for (int k = 0; k < C::kSub; ++k) {
-                const int in_tile = 16 * (C::kSub * (part0 + p) + k), box = in_tile >> a.lg_box;
-                from[k] = (uint32_t)((box << a.lg_box) * C::kRow + (in_tile - (box << a.lg_box)) * C::kInner);
-                v0[k] = max(x.lo - x.tile0 - in_tile, 0);
-                v1[k] = (x.bad >> box) & 1 ? 0 : min(x.len - x.tile0 - in_tile, 16);
-                any |= v0[k] < v1[k];
-                partial |= v0[k] > 0 || v1[k] < 16;
-            }
-            if (!any) continue;
-            const uint32_t piece = (uint32_t)C::kInner << a.lg_box;
-            if (partial) {
-#pragma unroll
-                for (int k = 0; k < C::kSub; ++k) row.clear_rows(base + half + from[k], piece, v0[k], v1[k]);
-            }
-            row.step(a, smem_u32(base), half, from, piece, v0, v1, partial);
-            if (partial) proxy_fence();
-        }
+        row.tokens(a, x, base, half, warp);
         if (!(x.flags & kLast)) {
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + stage);
@@ -974,34 +971,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         float* buf = reinterpret_cast<float*>(base);
         const float v_scale = kF8 && a.v_scale ? a.v_scale[x.h] : 1.f;
         const int64_t head0 = ((int64_t)x.b * a.kv_heads + x.h) * a.G + chunk * a.heads;
-        if constexpr (kSolo) {  // the row is this warp's: through its stage to whole lines of the output
-            __syncwarp();
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float inv[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float sum = row.total(n, e);
-                    const int head = 8 * n + 2 * t + e;
-                    inv[e] = sum == 0.f ? 0.f : v_scale / sum;
-                    if (a.lse && g == 0 && head < n_heads)
-                        a.lse[head0 + head] = (row.m[n][e] + log2f(sum)) * 0.6931471805599453f;
-                }
-                row.put(buf, n, inv);
-                __syncwarp();
-                for (int idx = lane; idx < 8 * (D / 4); idx += 32) {
-                    const int hl = idx / (D / 4), d = 4 * (idx % (D / 4));
-                    if (8 * n + hl >= n_heads) continue;
-                    const float4 y = *reinterpret_cast<const float4*>(buf + hl * D + (d ^ (((hl >> 1) & 3) << 3)));
-                    store4<kQ>(a.out, (head0 + 8 * n + hl) * D + d, y);
-                }
-                __syncwarp();
-            }
-            proxy_fence();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty + stage);
-            continue;
-        }
         // ---- the row's end: join the warps in the stage's K and V
         float2* mine_ml = ml + (n_row & 1) * kConsumers * C::kHeadsMax;
 #pragma unroll
@@ -1068,7 +1037,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + stage);
     }
-    if (kSolo || a.ranks == 1) return;
+    if (a.ranks == 1) return;
     // ---- the row's parts, by the cluster's ranks in order; every CTA meets here whatever became of its waits
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
@@ -1109,6 +1078,174 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
         if (a.lse && d == 0) a.lse[head0 + head] = (m + log2f(l)) * 0.6931471805599453f;
     }
     cluster.sync();  // no CTA leaves while another reads its part
+}
+
+// ------------------------------------------------------------ a warp a row
+// Short rows, many of them: a warp takes whole rows alone and loads them itself,
+// `unit` tokens at a time into its own stages, so no warp waits for another and
+// no row is joined.  Where four warps share a row, their chain and join take
+// 1.9 us a row whatever it holds.  The reads in flight are the CTA's warps', a
+// load each; its stages' owner never changes, so a parity always tells its
+// phases apart.  256 requests, four warps a row and one: 1 token, 8 kv heads of
+// 128, bf16 17.1 -> 7.3 us, the last 8 of 17 tokens 18.3 -> 10.4, 17 tokens' last
+// 8 with 16 query heads of 256 76.4 -> 30.3, 100 e4m3 tokens with 12 of 256
+// 68.4 -> 41.8; 191 requests of 108..217, 16 kv heads of 256, 116 -> 98.
+template <int kQ, bool kF8, int D, int NT>
+__global__ void __launch_bounds__(32 * Cfg<kQ, kF8, D, NT>::kRowWarps, Cfg<kQ, kF8, D, NT>::kPerSm)
+    pool_rows_kernel(const __grid_constant__ DecodeArgs a) {
+    using C = Cfg<kQ, kF8, D, NT>;
+    extern __shared__ uint8_t smem_raw[];
+    const int stages = a.workers * a.ahead, half = a.unit * C::kRow;
+    uint8_t* kv = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));  // [stages] K, V
+    uint8_t* qs = kv + stages * 2 * half;                              // [stages] query heads, by row
+    Unit* units = reinterpret_cast<Unit*>(qs + stages * C::kQSlot);    // [stages]
+    __shared__ uint64_t full[kMaxStages];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    if (tid == 0) {
+        for (int i = 0; i < stages; ++i) mbar_init(full + i, 1);
+        mbar_fence_init();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.tk)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.tv)) : "memory");
+    }
+    const int chunk = blockIdx.x % a.side, c = blockIdx.x / a.side;
+    const int n_heads = min(a.heads, a.G - chunk * a.heads);
+    if constexpr (C::kQShared) {  // the places of heads that the chunk has not: products of zeros
+        const int per = (C::kHeadsMax - n_heads) * (D / 8);
+        for (int i = tid; i < stages * per; i += 32 * C::kRowWarps)
+            *reinterpret_cast<uint4*>(qs + i / per * C::kQSlot + (n_heads + i % per / (D / 8)) * C::kQPitch +
+                                      i % (D / 8) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    grid_dep_wait();
+    grid_dep_launch_next();
+    __syncthreads();
+    const int64_t rows = (int64_t)a.batch * a.kv_heads, stride = (int64_t)a.workers * a.groups;
+    int64_t r = (int64_t)warp * a.groups + c;  // a CTA's rows are far apart, of requests of different lengths
+    if (warp >= a.workers || r >= rows) return;
+    kv += warp * a.ahead * 2 * half;
+    qs += warp * a.ahead * C::kQSlot;
+    units += warp * a.ahead;
+    uint64_t* const bars = full + warp * a.ahead;
+
+    // ---- the next unit to load: its row, first token, block ids (lane j: box j) and the length of the row after
+    const int box = 1 << a.lg_box, grain = max(box, 16 * C::kSub);
+    const uint64_t policy = evict_first_policy();
+    int b = (int)quotient(r, a.kv_heads), h = 0, len = 0, lo = 0, tok = 0, id = -1, next = __ldcg(a.lens + b);
+    bool first = true;
+    auto enter = [&]() {
+        b = (int)quotient(r, a.kv_heads);
+        h = (int)(r - (int64_t)b * a.kv_heads);
+        if (next < 0 || next > a.cap) raise_status(a.status, ZKV_ERR_RANGE);
+        len = request_len(a, next);
+        lo = first_token(a, len);
+        tok = lo & ~(grain - 1);
+        first = true;
+        if (r + stride < rows) next = __ldcg(a.lens + quotient(r + stride, a.kv_heads));
+    };
+    auto wanted = [&]() {
+        const int off = lane << a.lg_box;
+        return off < a.unit && off < len - tok && off + box > lo - tok;
+    };
+    auto ask = [&]() { id = wanted() ? __ldcg(a.table + b * a.table_ld + (tok >> a.shift) + lane) : -1; };
+    int issued = 0;
+    Turn put_at, put_q;
+    put_q.stage = a.ahead - 1;
+    auto issue = [&]() {
+        const int stage = put_at.stage;
+        const bool want = wanted(), there = want && id >= 0 && id < a.n_blocks;
+        if (want && !there) raise_status(a.status, ZKV_ERR_RANGE);
+        const unsigned copy = __ballot_sync(0xffffffffu, there), bad = __ballot_sync(0xffffffffu, want && !there);
+        const bool last = tok + a.unit >= len;
+        if (first) put_q.next(a.ahead);
+        if (lane == 0) {
+            Unit& x = units[stage];
+            x.b = b;
+            x.h = h;
+            x.tile0 = tok;
+            x.lo = lo;
+            x.len = len;
+            x.flags = (first ? kFirst : 0) | (last ? kLast : 0);
+            x.part = put_q.stage;
+            x.bad = (int)bad;
+            mbar_arrive_expect_tx(bars + stage,
+                                  (uint32_t)(__popc(copy) * 2 * (C::kRow << a.lg_box) + (first ? n_heads * D * 2 : 0)));
+        }
+        __syncwarp();
+        if (there) {
+            const uint32_t dst = smem_u32(kv + stage * 2 * half) + lane * (C::kRow << a.lg_box);
+            const int in_block = a.shift > a.lg_box ? tok & ((1 << a.shift) - 1) : 0;
+            tma_load_5d(dst, &a.tk, in_block, h, id, bars + stage, policy);
+            tma_load_5d(dst + half, &a.tv, in_block, h, id, bars + stage, policy);
+        }
+        if (first && lane >= 32 - C::kHeadsMax && lane - (32 - C::kHeadsMax) < n_heads) {
+            const int j = lane - (32 - C::kHeadsMax);
+            bulk_g2s(qs + put_q.stage * C::kQSlot + j * C::kQPitch,
+                     a.q + b * a.q_row + (int64_t)(h * a.G + chunk * a.heads + j) * a.q_head, D * 2, bars + stage);
+        }
+        put_at.next(a.ahead);
+        ++issued;
+        if (last) r += stride;
+        if (last && r < rows) enter();
+        else {
+            tok += a.unit;
+            first = false;
+        }
+        if (r < rows) ask();
+    };
+    enter();
+    ask();
+    for (int i = 0; i < a.ahead && r < rows; ++i) issue();
+
+    Row<kQ, kF8, D, NT> row;
+    Turn at;
+    int done = 0;
+    for (; done < issued; ++done, at.next(a.ahead)) {
+        const int stage = at.stage;
+        if (!__all_sync(0xffffffffu, wait_for(bars + stage, at.phase, a.status))) break;
+        const Unit x = units[stage];
+        uint8_t* const base = kv + stage * 2 * half;
+        if (x.flags & kFirst) {
+            uint8_t* const q_row = qs + x.part * C::kQSlot;
+            if constexpr (C::kQShared && kF8 && kQ == ZKV_DT_BF16) {
+                for (int p = 0; p < kConsumers; ++p) row.narrow_shared(q_row, p);
+                __syncwarp();
+            }
+            row.init(a, q_row, n_heads, kF8 && a.k_scale ? a.k_scale[x.h] : 1.f);
+        }
+#pragma unroll 1
+        for (int p = 0; p * 16 * C::kSub < a.unit; ++p) row.tokens(a, x, base, half, p);
+        if (x.flags & kLast) {  // through the stage to whole lines of the output
+            float* buf = reinterpret_cast<float*>(base);
+            const float v_scale = kF8 && a.v_scale ? a.v_scale[x.h] : 1.f;
+            const int64_t head0 = ((int64_t)x.b * a.kv_heads + x.h) * a.G + chunk * a.heads;
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float inv[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float sum = row.total(n, e);
+                    const int head = 8 * n + 2 * t + e;
+                    inv[e] = sum == 0.f ? 0.f : v_scale / sum;
+                    if (a.lse && g == 0 && head < n_heads)
+                        a.lse[head0 + head] = (row.m[n][e] + log2f(sum)) * 0.6931471805599453f;
+                }
+                row.put(buf, n, inv);
+                __syncwarp();
+                for (int idx = lane; idx < 8 * (D / 4); idx += 32) {
+                    const int hl = idx / (D / 4), d = 4 * (idx % (D / 4));
+                    if (8 * n + hl >= n_heads) continue;
+                    const float4 y = *reinterpret_cast<const float4*>(buf + hl * D + (d ^ (((hl >> 1) & 3) << 3)));
+                    store4<kQ>(a.out, (head0 + 8 * n + hl) * D + d, y);
+                }
+                __syncwarp();
+            }
+        }
+        proxy_fence();  // the stage was read and written by these threads; the next copy into it is the async proxy's
+        __syncwarp();
+        if (r < rows) issue();
+    }
+    for (; done < issued; ++done, at.next(a.ahead))  // a wait gave up: the copies on their way land in this CTA's memory
+        wait_for(bars + at.stage, at.phase, a.status);
 }
 
 // ------------------------------------------------------------ joining split rows
@@ -1356,14 +1493,14 @@ static Cut plan_call(int batch, int kv_heads, int chunks, int row_bytes, int win
 }
 
 // A decode kernel's launch, its limits raised on its first one on a device.
-template <int kQ, bool kF8, int D, int NT, bool kSolo>
+template <int kQ, bool kF8, int D, int NT, bool kRows>
 static int launch_kernel(const DecodeArgs& a, int grid, int smem, cudaStream_t st) {
-    const auto kernel = pool_decode_kernel<kQ, kF8, D, NT, kSolo>;
+    using C = Cfg<kQ, kF8, D, NT>;
+    const auto kernel = kRows ? pool_rows_kernel<kQ, kF8, D, NT> : pool_decode_kernel<kQ, kF8, D, NT>;
     static int raised[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ZKV_ERR_LAUNCH;
     if (!raised[dev]) {
-        using C = Cfg<kQ, kF8, D, NT>;
         if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem_of(C::kRing)) !=
                 cudaSuccess ||
             cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
@@ -1372,7 +1509,7 @@ static int launch_kernel(const DecodeArgs& a, int grid, int smem, cudaStream_t s
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kRows ? 32 * C::kRowWarps : kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -1399,18 +1536,23 @@ static int launch_decode(DecodeArgs& a, cudaStream_t st) {
     if (a.ranks > 1) a.groups = (int)rows;
     else a.groups = (int)std::min(wave, most_groups(a.batch, a.head_rows, a.side, a.whole ? 0 : a.cap, C::kTile));
     const int grid = a.groups * a.side * a.ranks;
-    if (a.whole && a.ranks == 1 && a.window == 0 && a.cap <= C::kTile &&
-        (a.cap <= 16 * C::kSub || rows >= kSoloRows * wave)) {
-        // Stages of what a row can have, in whole boxes and products; two or more fit, a stage being no larger than the
-        // other kernel's.  Their number is a multiple of the working warps': a stage is then always the same warp's,
-        // which has seen its last phase end (a parity alone does not tell a phase from the one after the next).
-        const int unit = std::max(1 << a.lg_box, 16 * C::kSub);
-        a.half = std::max(1, (a.cap + unit - 1) / unit) * unit * C::kRow;
-        const int stage = 2 * a.half + C::kQSlot + (int)sizeof(Unit);
-        const int fit = std::min(kMaxStages, C::kRing / stage);
-        a.workers = std::min(kConsumers, fit);
-        a.stages = fit / a.workers * a.workers;
-        return launch_kernel<kQ, kF8, D, NT, true>(a, grid, C::smem_of(a.stages * stage), st);
+    if (a.whole && a.ranks == 1) {
+        // A warp a row: in equal loads of whole boxes and products, of which four fit into the ring (or two or three, if a
+        // box is too large for that: it is a tile's at most, so two always fit).
+        const int longest = a.window > 0 ? std::min(a.cap, a.window) : a.cap;
+        const int grain = std::max(1 << a.lg_box, 16 * C::kSub), other = C::kQSlot + (int)sizeof(Unit);
+        const int most = std::min(C::kTile, std::max(grain, (C::kRing / 4 - other) / (2 * C::kRow) / grain * grain));
+        const int loads = std::max(1, (longest + most - 1) / most);
+        const int unit = std::max(1, ((longest + loads - 1) / loads + grain - 1) / grain) * grain;
+        const int stage = 2 * unit * C::kRow + other, fit = std::min(kMaxStages, C::kRing / stage);
+        if (longest <= 16 * C::kSub ||
+            (loads == 1 ? rows >= wave
+                        : rows >= 2 * wave && loads <= (kF8 ? kRowLoadsF8 : kRowLoads) && fit >= (NT == 1 ? 3 : 4))) {
+            a.unit = unit;
+            a.workers = std::min(C::kRowWarps, fit);
+            a.ahead = fit / a.workers;
+            return launch_kernel<kQ, kF8, D, NT, true>(a, grid, C::smem_of(a.workers * a.ahead * stage), st);
+        }
     }
     int rc = launch_kernel<kQ, kF8, D, NT, false>(a, grid, C::smem_of(C::kStages * C::kStage), st);
     if (rc == ZKV_OK && !a.whole && a.groups > 1) {
