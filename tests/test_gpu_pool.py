@@ -247,6 +247,38 @@ def test_decode_rows_of_a_tile(B, qt, pt, D, G):
     run_decode(750, [(11 * i) % 65 for i in range(B)], 16, 1, G, D, qt, pt, "nhd", wide=False, max_len=64)
 
 
+@pytest.mark.parametrize("D,qt,pt,G", [(64, BF, F8, 8), (64, HF, HF, 16), (128, BF, BF, 4), (128, BF, F8, 20),
+                                       (256, HF, HF, 4), (256, BF, F8, 12)])
+@pytest.mark.parametrize("S,window", [(16, 0), (16, 7), (32, 100), (128, 0), (128, 65)])
+def test_decode_many_rows_of_several_loads(S, window, D, qt, pt, G):
+    """More rows than warps, up to 200 tokens or a window at any offset in a block; lengths 0 and 1 among them."""
+    lens = [(37 * i) % 201 for i in range(500)] + [0, 1, 200]
+    run_decode(760, lens, S, 2, G, D, qt, pt, "hnd" if S == 32 else "nhd", window=window, softcap=10.0 if S == 32 else 0.0,
+               wide=False, max_len=200)
+
+
+def test_decode_rows_of_several_loads_report_bad_ids():
+    lens = [100] * 700
+    k, v, _, _ = make_pool(770, 700 * 7, 16, 2, 64, BF, "hnd")
+    table = make_table(771, lens, 16, 700 * 7, 7)
+    q = torch.randn(700, 8, 64, generator=gen(772), device=DEV).to(BF)
+    pool, status = ops.KVPool(k, v), i32([0])
+    good = ops.pool_decode(q, pool, i32(lens), table, status=status)
+    assert int(status) == 0
+    table[5, 6] = 700 * 7
+    table[9, 0] = -1
+    cut = lens.copy()
+    cut[5] = 96                                    # the tokens of a bad id at the end do not count
+    out = ops.pool_decode(q, pool, i32(lens), table, status=status)
+    assert int(status) == ERR_RANGE
+    want = ops.pool_decode(q, pool, i32(cut), table)
+    same = [b for b in range(700) if b not in (5, 9)]
+    assert torch.equal(out[same], good[same]) and torch.equal(out[5], want[5]) and not torch.equal(out[9], good[9])
+    status.zero_()
+    ops.pool_decode(q, pool, i32([-1] + lens[1:]), table[:, :7], status=status)
+    assert int(status) == ERR_RANGE
+
+
 def test_decode_all_empty():
     run_decode(720, [0, 0, 0], 16, 2, 4, 128, BF, BF, "hnd")
     run_decode(721, [0], 16, 1, 1, 64, HF, F8, "hnd")
