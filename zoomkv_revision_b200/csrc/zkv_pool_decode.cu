@@ -40,8 +40,12 @@
 //
 // Roundings: scores, statistics and accumulators are fp32.  The probability
 // enters the second product as two 16-bit parts (p = hi + lo, 16 bits of
-// mantissa for bf16), so that it adds nothing visible to the output's own
-// rounding; over e4m3 blocks with bf16 output one fp16 part (11 bits) does.
+// mantissa for bf16), so that it adds little to the output's own rounding of 8
+// or 11 bits; over e4m3 blocks with bf16 output one fp16 part (11 bits) does.
+// Where those parts are fp16, p is 2^15 exp(x - max), at most half of what
+// fp16 holds: full 11 bits down to 2^-29 of the largest and something down to
+// 2^-40, where exp(x - max) itself would be gone at 2^-25 (17.3 below the
+// largest score, which a first token that draws all attention reaches).
 // e4m3 blocks are widened to fp16, exactly; a bf16 query is scaled by the
 // power of two that puts its largest element into [1, 2) first, which leaves
 // it exact in fp16 but for elements below 2^-14 of the largest.
@@ -373,6 +377,8 @@ template <int kQ, bool kF8, int D, int NT>
 struct Row {
     using C = Cfg<kQ, kF8, D, NT>;
     static constexpr bool kMmaBf16 = kQ == ZKV_DT_BF16 && !kF8;
+    // exponentials are 2^kLift of themselves: o and a lane's l too, while the warp's total and what it puts are not
+    static constexpr float kLift = kMmaBf16 ? 0.f : 15.f, kDown = kMmaBf16 ? 1.f : 1.f / 32768;
     float m[NT][2], l[NT][2];   // log2 units; heads 2t, 2t+1 of n-tile (t = lane % 4); l: this lane's tokens
     float f[NT][2];             // score factor of those heads, log2 units (under a soft cap, natural ones of it)
     float o[C::kMTiles][NT][4];
@@ -599,10 +605,11 @@ struct Row {
                 moved |= mx[c] != m[n][c];
                 m[n][c] = mx[c];
                 float sum = 0.f;
+                const float from = ref - kLift;
 #pragma unroll
                 for (int i = 0; i < kSub; ++i) {
-                    x[i][n][c] = exp2_fast(x[i][n][c] - ref);
-                    x[i][n][c + 2] = exp2_fast(x[i][n][c + 2] - ref);
+                    x[i][n][c] = exp2_fast(x[i][n][c] - from);
+                    x[i][n][c + 2] = exp2_fast(x[i][n][c + 2] - from);
                     sum += x[i][n][c] + x[i][n][c + 2];
                 }
                 l[n][c] = l[n][c] * alpha[n][c] + sum;
@@ -673,13 +680,14 @@ struct Row {
         s += __shfl_xor_sync(0xffffffffu, s, 4);
         s += __shfl_xor_sync(0xffffffffu, s, 8);
         s += __shfl_xor_sync(0xffffffffu, s, 16);
-        return s;
+        return s * kDown;
     }
 
     // O of n-tile n times a factor per head to `to` [8][D].  Dims of a head are permuted by its pair's number, so that the
     // 32 lanes meet 32 banks.
-    __device__ __forceinline__ void put(float* to, int n, const float (&fac)[2]) const {
+    __device__ __forceinline__ void put(float* to, int n, const float (&factor)[2]) const {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const float fac[2] = {factor[0] * kDown, factor[1] * kDown};
         float* p = to + 2 * t * D;
 #pragma unroll
         for (int j = 0; j < C::kMTiles; ++j) {
