@@ -45,3 +45,24 @@ def test_tokens_far_below_a_sink(shape, qt, pt, D, G):
     out, lse = ops.pool_decode(q, ops.KVPool(k, v), i32(lens), table, max_len=bound, return_lse=True, status=status)
     assert int(status) == 0
     check_decode(q, k, v, None, None, lens, table, out, lse, D ** -0.5)
+
+
+@pytest.mark.parametrize("small", [2.0 ** -16, 2.0 ** -20, 2.0 ** -27])
+@pytest.mark.parametrize("G", [4, 12])
+@pytest.mark.parametrize("lens", [[300, 77], [i % 60 for i in range(700)]])
+def test_small_query_elements_over_fp8(lens, G, small):
+    """A bf16 query's largest element meets zeros, the others are `small` of it and make the scores."""
+    S, D = 16, 128
+    n_blocks = sum(-(-n // S) for n in lens) + 1
+    g = gen(3)
+    k = torch.randn(n_blocks, S, 1, D, generator=g, device=DEV) * 100
+    k[..., 0] = 0
+    k = narrow(k, F8)
+    v = narrow(torch.randn(n_blocks, S, 1, D, generator=g, device=DEV), F8)
+    table = make_table(4, lens, S, n_blocks, -(-max(lens) // S))
+    q = torch.randn(len(lens), G, D, generator=g, device=DEV) * small
+    q[..., 0] = 1.3
+    q = q.to(BF)
+    scale = 0.004 / small
+    out, lse = ops.pool_decode(q, ops.KVPool(k, v), i32(lens), table, scale=scale, return_lse=True)
+    check_decode(q, k, v, None, None, lens, table, out, lse, scale)

@@ -47,8 +47,8 @@
 // 2^-40, where exp(x - max) itself would be gone at 2^-25 (17.3 below the
 // largest score, which a first token that draws all attention reaches).
 // e4m3 blocks are widened to fp16, exactly; a bf16 query is scaled by the
-// power of two that puts its largest element into [1, 2) first, which leaves
-// it exact in fp16 but for elements below 2^-14 of the largest.
+// power of two that puts its largest element into [2^15, 2^16) first, which
+// leaves it exact in fp16 but for elements below 2^-32 of the largest.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -385,10 +385,11 @@ struct Row {
     uint32_t q_at;              // the queries' place, this lane's part
     uint32_t q[C::kQShared ? 1 : D / 16][NT][2];  // B fragments of Q^T, where they are not read from there each time
 
-    // A bf16 query to fp16, for e4m3 rows: scaled down by the power of two of its largest element; up: the way back.
+    // A bf16 query to fp16, for e4m3 rows: scaled by the power of two that puts its largest element into [2^15, 2^16)
+    // (65280 at most), so that the small ones keep their bits; up: the way back.  Both factors are normal numbers.
     static __device__ __forceinline__ float down_scale(float largest, float& up) {
-        int e = (int)(__float_as_uint(largest) >> 23) - 127;  // in [2^e, 2^(e+1))
-        e = largest > 0.f ? (e < -126 ? -126 : (e > 126 ? 126 : e)) : 0;
+        int e = (int)(__float_as_uint(largest) >> 23) - 127 - 15;  // in [2^(e+15), 2^(e+16))
+        e = largest > 0.f ? (e < -126 ? -126 : (e > 113 ? 113 : e)) : 0;
         up = __uint_as_float((uint32_t)(127 + e) << 23);
         return __uint_as_float((uint32_t)(127 - e) << 23);
     }
