@@ -1,0 +1,43 @@
+"""GPU: the pooled cache at its bounds: prompts without a bound, replayed
+plans, and a decode loop that runs out of room."""
+import pytest
+import torch
+
+from zoomkv_revision_b200 import decode_loop as DL
+from zoomkv_revision_b200.pool_cache import PoolCache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF = torch.bfloat16
+SMALL = DL.Shape(hidden=256, layers=2, heads=6, kv_heads=2, head_dim=128, ffn=512, vocab=1000)
+
+
+def rows(seed, *shape):
+    return torch.randn(shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).to(BF)
+
+
+def dense(q, kv):
+    """q [heads, dim] over kv [tokens, dim] as K and V, one kv head."""
+    x = kv.double()
+    return torch.softmax(q.double() @ x.T * q.shape[-1] ** -0.5, -1) @ x
+
+
+def near(got, want, kv):
+    """Rounding of the output, and of probabilities and scores as 2^-10 of the largest value."""
+    return bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * kv.double().abs().max()).all())
+
+
+def test_prompts_planned_without_a_bound_are_attended_whole():
+    cache = PoolCache(1, 2, 1, 64, 640)
+    n = [600, 17]
+    kv = rows(1, sum(n), 1, 64)
+    slots = cache.plan(torch.tensor(n, dtype=torch.int32, device=DEV), sum(n))
+    assert cache.bound >= max(n)
+    cache.write(0, kv, kv, slots)
+    q = rows(2, 2, 4, 64)
+    out = cache.attend(0, q)
+    cache.check()
+    for b, part in enumerate((kv[:600, 0], kv[600:, 0])):
+        assert near(out[b], dense(q[b], part), part)
+    cache.plan(None, 2)                                # one token each
+    assert cache.lens.tolist() == [601, 18] and cache.bound >= 601

@@ -60,11 +60,14 @@ class PoolCache:
         self.slots = None                    # of the step that is being written
 
     # ------------------------------------------------------------------ a serving step
-    def plan(self, new_lens, n_slots: int, max_new: int = 1):
+    def plan(self, new_lens, n_slots: int, max_new=None):
         """Blocks and slots for the step's new tokens: new_lens [batch] int32 on the GPU (None: one each), at most
-        n_slots in all and max_new for one request.  Returns the slot map [n_slots]."""
+        n_slots in all and max_new for one request (None: what n_slots allows; a step of single tokens from new_lens
+        gives 1).  Returns the slot map [n_slots]."""
         slots = torch.empty(n_slots, dtype=torch.int64, device=self.k.device)
         ops.pool_plan(self.lens, new_lens, self.table, self.free, self.n_free, self.block_size, slots, status=self.status)
+        if max_new is None:
+            max_new = 1 if new_lens is None else n_slots
         self.bound = min(self.bound + max_new, self.width * self.block_size)
         self.slots = slots
         return slots
