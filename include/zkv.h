@@ -755,8 +755,10 @@ int zkv_pool_write(const void* k, int64_t k_token, int64_t k_head, const void* v
  *   q [batch][q_heads][head_dim] at b*q_row + j*q_head (16-byte rows), `dtype`
  *   bf16 or fp16, the pool's own type unless the pool is e4m3; out dense in
  *   `dtype`; lse [batch][q_heads] fp32 or NULL
- *   max_len: a bound of lens known to the host (0: width * block_size); a
- *   longer or negative length is cut to the bound or 0, and a block id
+ *   max_len: the host's guess of the longest request (0: width * block_size),
+ *   from which the work's cut and the workspace follow; the result is the
+ *   same tokens' with any guess, and a guess far too short costs time.
+ *   A length outside [0, width * block_size] is cut to that, and a block id
  *   outside the pool leaves its tokens out, both with ZKV_ERR_RANGE
  *   workspace: device, 256-byte aligned, >= zkv_pool_decode_ws_bytes (0:
  *   none is needed, NULL will do; also 0 for bad arguments), scratch only, no

@@ -41,3 +41,24 @@ def test_prompts_planned_without_a_bound_are_attended_whole():
         assert near(out[b], dense(q[b], part), part)
     cache.plan(None, 2)                                # one token each
     assert cache.lens.tolist() == [601, 18] and cache.bound >= 601
+
+
+def test_a_replayed_plan_is_attended_whole():
+    """A captured plan and write move the lengths at every replay, and the host's bound only once."""
+    cache = PoolCache(1, 1, 1, 64, 512)
+    kv = torch.zeros(1, 1, 64, dtype=BF, device=DEV)
+    all_rows = rows(3, 200, 1, 64)
+    cache.write(0, kv, kv, cache.plan(None, 1))
+    cache.release(torch.tensor([True], device=DEV), bound=0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.write(0, kv, kv, cache.plan(None, 1))
+    for t in range(200):
+        kv.copy_(all_rows[t: t + 1])
+        graph.replay()
+    assert cache.lens.tolist() == [200]
+    q = rows(4, 1, 4, 64)
+    out = cache.attend(0, q)
+    cache.check()
+    assert near(out[0], dense(q[0], all_rows[:, 0]), all_rows)

@@ -1,0 +1,40 @@
+"""GPU: bounds, limits and reports of the pooled KV cache's operators."""
+import pytest
+import torch
+
+from test_gpu_pool import BF, DEV, check_decode, gen, i32, make_pool, make_table
+from zoomkv_revision_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("spare", [0, 20000])
+@pytest.mark.parametrize("max_len", [1, 64, 300, 100000])
+def test_max_len_never_cuts(max_len, spare):
+    """Requests that are longer than the host believes, on every path that the belief chooses."""
+    for lens, H, G, D, window in (([300, 0, 2000, 17], 2, 4, 128, 0), ([37 * i % 201 for i in range(700)], 1, 4, 64, 0),
+                                  ([4000], 1, 4, 128, 0), ([37 * i % 201 for i in range(700)], 1, 12, 128, 100)):
+        n_blocks = sum(-(-n // 16) for n in lens)
+        k, v, _, _ = make_pool(1, n_blocks, 16, H, D, BF, "hnd")
+        table = make_table(2, lens, 16, n_blocks, -(-max(lens) // 16) + spare)
+        q = torch.randn(len(lens), H * G, D, generator=gen(3), device=DEV).to(BF)
+        status = i32([0])
+        out, lse = ops.pool_decode(q, ops.KVPool(k, v), i32(lens), table, window=window, max_len=max_len, return_lse=True,
+                                   status=status)
+        assert int(status) == 0
+        check_decode(q, k, v, None, None, lens, table, out, lse, D ** -0.5, window)
+
+
+def test_max_len_never_cuts_split_rows():
+    """A belief that has the rows cut by units (over 128 MiB of K and V), and twice the tokens."""
+    lens = [3000 - 17 * i for i in range(32)]
+    n_blocks = sum(-(-n // 16) for n in lens)
+    k, v, _, _ = make_pool(4, n_blocks, 16, 8, 128, BF, "hnd")
+    table = make_table(5, lens, 16, n_blocks, 200)
+    pool = ops.KVPool(k, v)
+    assert ops.pool_decode_ws_bytes(32, 32, pool, 200, 1500) > 0
+    q = torch.randn(32, 32, 128, generator=gen(6), device=DEV).to(BF)
+    status = i32([0])
+    out, lse = ops.pool_decode(q, pool, i32(lens), table, max_len=1500, return_lse=True, status=status)
+    assert int(status) == 0
+    check_decode(q, k, v, None, None, lens, table, out, lse, 128 ** -0.5)

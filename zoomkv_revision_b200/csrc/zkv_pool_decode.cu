@@ -13,8 +13,8 @@
 //    so uneven requests, one long request and many short ones are spread the
 //    same way and the host needs no length.  A row (request, kv head) that
 //    ends in another CTA than it began in leaves partials (m, l, o), which
-//    pool_join_kernel joins in CTA order.  Where the host's bound of the
-//    lengths leaves little to balance (see plan_call) the rows are not cut by
+//    pool_join_kernel joins in CTA order.  Where the host's guess of the
+//    longest request leaves little to balance (see plan_call) the rows are not cut by
 //    units: a CTA takes whole rows, or a cluster of CTAs shares one row and
 //    joins through distributed shared memory; one launch does, with no scan
 //    and no workspace.
@@ -112,7 +112,7 @@ struct DecodeArgs {
     float* stats;   // [grid][2][heads][2] its m, l
     int64_t q_row, q_head;  // bytes
     int64_t table_ld, n_blocks;
-    int cap;        // longest length
+    int cap;        // the longest length that the table holds
     int batch, kv_heads, G, chunks, heads;  // heads: query heads of a chunk (the last one may have fewer)
     int abreast;    // kv heads of a row: their CTAs walk one range side by side
     int head_rows;  // rows of a request: kv_heads / abreast
@@ -1478,16 +1478,17 @@ static size_t part_rows(int batch, int kv_heads, const Heads& h, int64_t max_len
     return (size_t)most_groups(batch, kv_heads, h.chunks, max_len, 64) * h.chunks * 2 * 8 * h.tiles;
 }
 
-// How a call's rows are cut, from what the host knows: the bound of the lengths.
+// How a call's rows are cut, from what the host knows: a guess of the longest request.  Every way is right for every
+// length; a guess far too short leaves long rows to one CTA, or a cluster, each.
 struct Cut {
     bool whole;    // not by units
     int ranks;     // CTAs of a cluster that share a row, if `whole`
     int abreast;   // kv heads walked side by side, if not
 };
-static Cut plan_call(int batch, int kv_heads, int chunks, int row_bytes, int window, int64_t cap) {
+static Cut plan_call(int batch, int kv_heads, int chunks, int row_bytes, int window, int64_t guess) {
     Cut c{false, 1, 8};
     const int tile = tile_tokens(row_bytes);
-    const int64_t longest = window > 0 ? std::min<int64_t>(cap, window) : cap;
+    const int64_t longest = window > 0 ? std::min<int64_t>(guess, window) : guess;
     const int64_t rows = (int64_t)batch * kv_heads * chunks;
     const int64_t tiles = (longest + tile - 1) / tile + (window > 0 ? 1 : 0);
     const int64_t bytes = 2 * (int64_t)batch * kv_heads * longest * row_bytes;
@@ -1534,21 +1535,21 @@ static int launch_kernel(const DecodeArgs& a, int grid, int smem, cudaStream_t s
 }
 
 template <int kQ, bool kF8, int D, int NT>
-static int launch_decode(DecodeArgs& a, cudaStream_t st) {
+static int launch_decode(DecodeArgs& a, int guess, cudaStream_t st) {
     using C = Cfg<kQ, kF8, D, NT>;
-    const Cut cut = plan_call(a.batch, a.kv_heads, a.chunks, C::kRow, a.window, a.cap);
+    const Cut cut = plan_call(a.batch, a.kv_heads, a.chunks, C::kRow, a.window, guess);
     a.whole = cut.whole, a.ranks = cut.ranks, a.abreast = cut.whole ? 1 : cut.abreast;
     a.head_rows = a.kv_heads / a.abreast, a.side = a.abreast * a.chunks;
     if (!a.whole && !a.parts) return ZKV_ERR_ARG;
     const int64_t rows = (int64_t)a.batch * a.head_rows;
     const int64_t wave = std::max(1, C::kPerSm * sm_count() / a.side);
     if (a.ranks > 1) a.groups = (int)rows;
-    else a.groups = (int)std::min(wave, most_groups(a.batch, a.head_rows, a.side, a.whole ? 0 : a.cap, C::kTile));
+    else a.groups = (int)std::min(wave, most_groups(a.batch, a.head_rows, a.side, a.whole ? 0 : guess, C::kTile));
     const int grid = a.groups * a.side * a.ranks;
     if (a.whole && a.ranks == 1) {
         // A warp a row: in equal loads of whole boxes and products, of which four fit into the ring (or two or three, if a
         // box is too large for that: it is a tile's at most, so two always fit).
-        const int longest = a.window > 0 ? std::min(a.cap, a.window) : a.cap;
+        const int longest = a.window > 0 ? std::min(guess, a.window) : guess;
         const int grain = std::max(1 << a.lg_box, 16 * C::kSub), other = C::kQSlot + (int)sizeof(Unit);
         const int most = std::min(C::kTile, std::max(grain, (C::kRing / 4 - other) / (2 * C::kRow) / grain * grain));
         const int loads = std::max(1, (longest + most - 1) / most);
@@ -1574,15 +1575,15 @@ static int launch_decode(DecodeArgs& a, cudaStream_t st) {
 }
 
 template <int kQ, bool kF8>
-static int launch_shape(DecodeArgs& a, int D, int tiles, cudaStream_t st) {
+static int launch_shape(DecodeArgs& a, int guess, int D, int tiles, cudaStream_t st) {
     if (tiles == 1) {
-        if (D == 64) return launch_decode<kQ, kF8, 64, 1>(a, st);
-        if (D == 128) return launch_decode<kQ, kF8, 128, 1>(a, st);
-        return launch_decode<kQ, kF8, 256, 1>(a, st);
+        if (D == 64) return launch_decode<kQ, kF8, 64, 1>(a, guess, st);
+        if (D == 128) return launch_decode<kQ, kF8, 128, 1>(a, guess, st);
+        return launch_decode<kQ, kF8, 256, 1>(a, guess, st);
     }
-    if (D == 64) return launch_decode<kQ, kF8, 64, 2>(a, st);
-    if (D == 128) return launch_decode<kQ, kF8, 128, 2>(a, st);
-    return launch_decode<kQ, kF8, 256, 2>(a, st);
+    if (D == 64) return launch_decode<kQ, kF8, 64, 2>(a, guess, st);
+    if (D == 128) return launch_decode<kQ, kF8, 128, 2>(a, guess, st);
+    return launch_decode<kQ, kF8, 256, 2>(a, guess, st);
 }
 
 static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -1601,8 +1602,8 @@ extern "C" int zkv_pool_init(zkv_pool* p) {
     return ZKV_OK;
 }
 
-static bool needs_parts(const zkv_pool* p, int batch, const pool::Heads& h, int window, int64_t cap) {
-    return !pool::plan_call(batch, p->kv_heads, h.chunks, p->head_dim * pool::element_bytes(p->dtype), window, cap).whole;
+static bool needs_parts(const zkv_pool* p, int batch, const pool::Heads& h, int window, int64_t guess) {
+    return !pool::plan_call(batch, p->kv_heads, h.chunks, p->head_dim * pool::element_bytes(p->dtype), window, guess).whole;
 }
 
 extern "C" size_t zkv_pool_decode_ws_bytes(const zkv_pool* p, int batch, int q_heads, int window, int64_t max_len) {
@@ -1630,12 +1631,13 @@ extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int
     if (!pool::aligned16(q) || q_row % 8 || q_head % 8 || !pool::aligned16(out)) return ZKV_ERR_ALIGN;
     if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return ZKV_ERR_ALIGN;
     const int64_t room = (int64_t)width * p->block_size;
-    const int64_t cap = std::min<int64_t>(max_len > 0 ? std::min(max_len, room) : room, INT32_MAX - 512);
+    const int64_t cap = std::min<int64_t>(room, INT32_MAX - 512);
+    const int64_t guess = max_len > 0 ? std::min(max_len, cap) : cap;
     const pool::Heads hs = pool::split_heads(q_heads / p->kv_heads);
     if (hs.chunks > pool::kMaxChunks) return ZKV_ERR_CAPACITY;
-    const bool parts = needs_parts(p, batch, hs, window, cap);
+    const bool parts = needs_parts(p, batch, hs, window, guess);
     if (parts && !workspace) return ZKV_ERR_ARG;
-    if (parts && ws_bytes < zkv_pool_decode_ws_bytes(p, batch, q_heads, window, cap)) return ZKV_ERR_CAPACITY;
+    if (parts && ws_bytes < zkv_pool_decode_ws_bytes(p, batch, q_heads, window, guess)) return ZKV_ERR_CAPACITY;
     uint64_t any = 0;
     for (uint64_t w : p->maps) any |= w;
     if (!any) return ZKV_ERR_ARG;  // zkv_pool_init was not called
@@ -1646,15 +1648,15 @@ extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int
     a.k_scale = p->k_scale, a.v_scale = p->v_scale;
     a.lens = lens, a.table = block_table, a.out = out, a.lse = lse, a.status = status;
     a.stats = parts ? (float*)workspace : nullptr;
-    a.parts = parts ? a.stats + pool::up256(pool::part_rows(batch, p->kv_heads, hs, cap) * 8) / 4 : nullptr;
+    a.parts = parts ? a.stats + pool::up256(pool::part_rows(batch, p->kv_heads, hs, guess) * 8) / 4 : nullptr;
     a.q_row = q_row * 2, a.q_head = q_head * 2;
     a.table_ld = table_ld, a.n_blocks = p->n_blocks, a.cap = (int)cap;
     a.batch = batch, a.kv_heads = p->kv_heads, a.G = q_heads / p->kv_heads, a.chunks = hs.chunks, a.heads = hs.heads;
     a.shift = pool::log2_of(p->block_size), a.lg_box = pool::log2_of(pool::box_tokens(p)), a.width = width, a.window = window;
     a.scale = scale, a.softcap = softcap;
     cudaStream_t st = (cudaStream_t)stream;
-    if (p->dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, false>(a, p->head_dim, hs.tiles, st);
-    if (p->dtype == ZKV_DT_F16) return pool::launch_shape<ZKV_DT_F16, false>(a, p->head_dim, hs.tiles, st);
-    if (dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, true>(a, p->head_dim, hs.tiles, st);
-    return pool::launch_shape<ZKV_DT_F16, true>(a, p->head_dim, hs.tiles, st);
+    if (p->dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, false>(a, (int)guess, p->head_dim, hs.tiles, st);
+    if (p->dtype == ZKV_DT_F16) return pool::launch_shape<ZKV_DT_F16, false>(a, (int)guess, p->head_dim, hs.tiles, st);
+    if (dtype == ZKV_DT_BF16) return pool::launch_shape<ZKV_DT_BF16, true>(a, (int)guess, p->head_dim, hs.tiles, st);
+    return pool::launch_shape<ZKV_DT_F16, true>(a, (int)guess, p->head_dim, hs.tiles, st);
 }

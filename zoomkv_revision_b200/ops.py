@@ -1330,7 +1330,8 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     request (the new one among them, written by pool_write); block_table
     [B, width] int32.  Softmax over the last `window` tokens (0: all) of
     scale * q.k (default 1 / sqrt(head_dim)), soft-capped if softcap > 0.
-    max_len: a bound of lens that the host knows (0: width * block_size).
+    max_len: the host's guess of the longest request (0: width * block_size);
+    it chooses how the work is cut, never what is attended.
     Returns out like q, with return_lse (out, lse [B, q_heads] fp32, natural
     log, -inf for a request without tokens, whose out is 0).  workspace:
     uint8 CUDA tensor of pool_decode_ws_bytes(...) bytes, scratch only

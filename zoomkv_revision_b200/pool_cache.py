@@ -56,7 +56,7 @@ class PoolCache:
         self.free = torch.arange(self.n_blocks, **ints)
         self.n_free = torch.full((1,), self.n_blocks, **ints)
         self.status = torch.zeros(1, **ints)
-        self.bound = 0                       # no request is longer, as far as the host knows
+        self.bound = 0                       # no request is longer, as far as the host knows (a replayed plan does not tell it)
         self.slots = None                    # of the step that is being written
 
     # ------------------------------------------------------------------ a serving step
@@ -78,8 +78,8 @@ class PoolCache:
 
     def attend(self, layer: int, q, **kw):
         """Attention of q [batch, (1,) q_heads, head_dim] over each request's tokens (keywords of ops.pool_decode;
-        max_len is the bound that plan keeps, so a call that is captured in a graph and replayed gives its own: 0 for
-        all of the table's room)."""
+        max_len, which chooses how the work is cut, is the bound that plan keeps; a call that is captured in a graph for
+        longer requests gives its own, 0 for all of the table's room)."""
         kw.setdefault("max_len", self.bound)
         return ops.pool_decode(q, self.pools[layer], self.lens, self.table, status=self.status, **kw)
 
