@@ -62,3 +62,45 @@ def test_a_replayed_plan_is_attended_whole():
     out = cache.attend(0, q)
     cache.check()
     assert near(out[0], dense(q[0], all_rows[:, 0]), all_rows)
+
+
+@pytest.mark.parametrize("n_blocks", [None, 8])
+def test_a_decode_loop_that_runs_out_of_room_is_told(n_blocks):
+    """3 requests of 20 tokens: 64 tokens fit the table, 32 tokens each fit 8 blocks (two each, then 6 + 3 > 8)."""
+    B, prompt, s = 3, 20, SMALL
+    w = DL.Weights(s, DEV, seed=1, std=0.05)
+    cache = PoolCache(s.layers, B, s.kv_heads, s.head_dim, 64, n_blocks=n_blocks)
+    loop = DL.DecodeLoop(s, w, cache, B, 200, DEV, use_graphs=False, temperature=0.0)
+    tok = loop.prefill(torch.randint(0, s.vocab, (B, prompt), generator=torch.Generator().manual_seed(7)).to(DEV))
+    room = 64 if n_blocks is None else 32
+    for _ in range(room - prompt):
+        tok = loop.step(tok)
+    cache.check()
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        loop.step(tok)
+    assert cache.lens.tolist() == [room] * B           # nothing was appended
+    cache.check()
+
+
+def test_a_prompt_that_does_not_fit_is_refused():
+    cache = PoolCache(1, 2, 1, 64, 64)
+    x = rows(5, 2, 65, 1, 64)
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        cache.prefill_update_kv_cache(None, x, x, 0, 0)
+    assert cache.lens.tolist() == [0, 0]
+    cache.prefill_update_kv_cache(None, x[:, :64], x[:, :64], 0, 0)
+    cache.check()
+    assert cache.lens.tolist() == [64, 64]
+
+
+def test_released_places_serve_the_hooks_again():
+    """A release that leaves the host without a bound: the hooks ask the GPU instead of refusing."""
+    cache = PoolCache(1, 2, 1, 64, 64)
+    x = rows(6, 2, 60, 1, 64)
+    for _ in range(4):
+        cache.prefill_update_kv_cache(None, x, x, 0, 0)
+        cache.decode_update_kv_cache(x[:, :1], x[:, :1], 0)
+        assert cache.lens.tolist() == [61, 61]
+        cache.release(torch.tensor([True, True], device=DEV))
+    cache.check()
+    assert cache.lens.tolist() == [0, 0] and int(cache.n_free) == cache.n_blocks

@@ -18,7 +18,8 @@ A serving step:
 The cache hooks of the decode loop (prefill_update_kv_cache, sync,
 decode_update_kv_cache, compute; model_hub/LLM.py:208-294 of the reference's
 runtime calls them) are there too, so that decode_loop.DecodeLoop runs over
-it with a batch of equal prompts.  The reference has no pooled cache.
+it with a batch of equal prompts; they raise when a token has no room, where a
+server's own steps find out by `check`.  The reference has no pooled cache.
 
     python -m zoomkv_revision_b200.pool_cache          # a small serving run
 """
@@ -98,6 +99,21 @@ class PoolCache:
             raise RuntimeError(f"pool cache: {ops.lib().zkv_status_string(code).decode()}")
 
     # ------------------------------------------------------------------ hooks of the decode loop
+    def _make_room(self, new: int) -> None:
+        """Raises if `new` more tokens of every request do not fit: the loop's caller has no status to look at.  Where the
+        host's bound leaves a doubt the GPU is asked, and the bound is what it says; not in a graph capture, whose replays
+        only `check` can judge."""
+        def blocks(n):
+            return -(-n // self.block_size)
+
+        if blocks(self.bound + new) <= min(self.width, self.n_blocks // self.batch) or torch.cuda.is_current_stream_capturing():
+            return
+        lens, n_free = self.lens.tolist(), int(self.n_free.item())
+        self.bound = max(lens)
+        if blocks(self.bound + new) > self.width or sum(blocks(n + new) - blocks(n) for n in lens) > n_free:
+            raise RuntimeError(f"KV write is outside the cache: {new} more tokens for requests of up to {self.bound}, of "
+                               f"{self.width * self.block_size} each; {n_free} of {self.n_blocks} blocks are free")
+
     def prefill_update_kv_cache(self, query_states, key_states, value_states, layer_idx: int, batch_idx: int):
         """Appends a prompt to every request: key_states, value_states [batch, T, kv_heads, head_dim]."""
         del query_states
@@ -105,6 +121,7 @@ class PoolCache:
         if B != self.batch or batch_idx != 0:
             raise ValueError(f"prompts come for the whole batch of {self.batch} at once; got {B} from {batch_idx} on")
         if layer_idx == 0:
+            self._make_room(T)
             self.plan(torch.full((B,), T, dtype=torch.int32, device=self.k.device), B * T, T)
         self.write(layer_idx, key_states.reshape(B * T, *key_states.shape[2:]),
                    value_states.reshape(B * T, *value_states.shape[2:]), self.slots)
@@ -116,6 +133,7 @@ class PoolCache:
     def decode_update_kv_cache(self, key_states, value_states, layer_idx: int):
         """Appends one token to every request: [batch, 1, kv_heads, head_dim]."""
         if layer_idx == 0:
+            self._make_room(1)
             self.plan(None, self.batch, 1)
         self.write(layer_idx, key_states[:, 0], value_states[:, 0], self.slots)
 
