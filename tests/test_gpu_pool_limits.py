@@ -1,4 +1,6 @@
 """GPU: bounds, limits and reports of the pooled KV cache's operators."""
+import threading
+
 import pytest
 import torch
 
@@ -38,3 +40,34 @@ def test_max_len_never_cuts_split_rows():
     out, lse = ops.pool_decode(q, pool, i32(lens), table, max_len=1500, return_lse=True, status=status)
     assert int(status) == 0
     check_decode(q, k, v, None, None, lens, table, out, lse, 128 ** -0.5)
+
+
+def run_plan_and_release(batch):
+    """One token for each of `batch` empty requests, and their release."""
+    lens, n_free = i32([0] * batch), i32([batch])
+    table = torch.full((batch, 1), -1, dtype=torch.int32, device=DEV)
+    free = torch.arange(batch, device=DEV).int()
+    slots = torch.empty(batch, dtype=torch.int64, device=DEV)
+    ops.pool_plan(lens, None, table, free, n_free, 16, slots)
+    assert sorted(slots.tolist()) == [16 * i for i in range(batch)]
+    ops.pool_release(torch.ones(batch, dtype=torch.bool, device=DEV), lens, table, free, n_free, 16)
+    assert int(n_free) == batch and not bool(lens.any())
+
+
+def test_batches_of_every_size_from_several_threads():
+    """A small batch of one thread does not lower what a large one of another needs."""
+    failed = []
+
+    def work(batch):
+        try:
+            run_plan_and_release(batch)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    run_plan_and_release(8192)
+    for batch in (8, 8192, 3):
+        t = threading.Thread(target=work, args=(batch,))
+        t.start()
+        t.join()
+        run_plan_and_release(8192)
+    assert not failed

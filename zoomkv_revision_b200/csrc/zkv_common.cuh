@@ -9,6 +9,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "../../include/zkv.h"
 
 namespace cg = cooperative_groups;
@@ -983,8 +985,30 @@ int raw_quest_topk(const void* q, int G, const void* cmin, const void* cmax, con
 // (zkv_peer_set_wait_ms; 5 s by default).
 uint64_t peer_wait_ns();
 
+// Let `fn` be launched with `smem` bytes of dynamic shared memory on the
+// current device.  The limit belongs to the process, and setting it can lower
+// it, so the largest one set is kept for all threads (per source file, as the
+// kernels are).
+static bool raise_smem_limit(const void* fn, size_t smem) {
+    constexpr int kFns = 8, kDevs = 64;
+    static std::mutex mutex;
+    static const void* fns[kFns] = {};
+    static size_t set[kFns][kDevs] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevs) return false;
+    const std::lock_guard<std::mutex> lock(mutex);
+    int i = 0;
+    while (i < kFns && fns[i] && fns[i] != fn) ++i;
+    if (i == kFns) return false;
+    fns[i] = fn;
+    if (smem <= set[i][dev]) return true;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
+    set[i][dev] = smem;
+    return true;
+}
+
 // Launch `nblocks` CTAs of `nthreads` in clusters of CS (cudaLaunchKernelExC),
-// raising the kernel's dynamic shared-memory limit once per (kernel, device).
+// raising the kernel's dynamic shared-memory limit where it has to be.
 // `pdl`: programmatic dependent launch -- the grid may be scheduled while the
 // previous kernel on the stream finishes; the kernel must execute
 // griddepcontrol.wait before it reads anything an earlier kernel writes.
@@ -1004,30 +1028,7 @@ static int launch_clustered(const void* fn, int nblocks, int nthreads, int CS, s
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 2 : 1;
-    // raise the dynamic shared-memory limit once per (kernel, device, size)
-    static thread_local const void* last_fn[8] = {};
-    static thread_local size_t last_smem[8] = {};
-    static thread_local int last_dev[8] = {-1, -1, -1, -1, -1, -1, -1, -1};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    int slot = -1;
-    for (int i = 0; i < 8; ++i)
-        if (last_fn[i] == fn && last_dev[i] == dev) slot = i;
-    if (slot < 0 || last_smem[slot] < smem) {
-        if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-            return ZKV_ERR_LAUNCH;
-        if (slot < 0) {
-            for (int i = 0; i < 8; ++i)
-                if (!last_fn[i]) {
-                    slot = i;
-                    break;
-                }
-            if (slot < 0) slot = 0;
-        }
-        last_fn[slot] = fn;
-        last_dev[slot] = dev;
-        last_smem[slot] = smem;
-    }
+    if (!raise_smem_limit(fn, smem)) return ZKV_ERR_LAUNCH;
     if (cudaLaunchKernelExC(&cfg, fn, args) != cudaSuccess) return ZKV_ERR_LAUNCH;
     return cudaGetLastError() == cudaSuccess ? ZKV_OK : ZKV_ERR_LAUNCH;
 }
