@@ -949,6 +949,12 @@ __device__ __forceinline__ float quest_half(uint4 qv, uint4 mnv, uint4 mxv) {
 }  // namespace zkv
 
 static inline int launch_status() { return cudaGetLastError() == cudaSuccess ? ZKV_OK : ZKV_ERR_LAUNCH; }
+// A refused call's error stays the thread's last one until it is taken, and the next caller that looks (a launch here or
+// in PyTorch) would take it for its own.
+static inline int launch_refused() {
+    cudaGetLastError();
+    return ZKV_ERR_LAUNCH;
+}
 
 // Launch a kernel that begins with pdl_begin() with programmatic dependent
 // launch allowed: it may become resident while the previous kernel on the
@@ -966,7 +972,7 @@ static int launch_pdl_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, si
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...) != cudaSuccess) return ZKV_ERR_LAUNCH;
+    if (cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...) != cudaSuccess) return launch_refused();
     return launch_status();
 }
 
@@ -1028,7 +1034,7 @@ static int launch_clustered(const void* fn, int nblocks, int nthreads, int CS, s
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 2 : 1;
-    if (!raise_smem_limit(fn, smem)) return ZKV_ERR_LAUNCH;
-    if (cudaLaunchKernelExC(&cfg, fn, args) != cudaSuccess) return ZKV_ERR_LAUNCH;
-    return cudaGetLastError() == cudaSuccess ? ZKV_OK : ZKV_ERR_LAUNCH;
+    if (!raise_smem_limit(fn, smem)) return launch_refused();
+    if (cudaLaunchKernelExC(&cfg, fn, args) != cudaSuccess) return launch_refused();
+    return launch_status();
 }

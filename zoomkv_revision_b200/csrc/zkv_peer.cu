@@ -207,12 +207,12 @@ extern "C" int zkv_peer_open(const void* handle, void** ptr) {
 
 extern "C" int zkv_peer_close(void* ptr) {
     if (!ptr) return ZKV_ERR_ARG;
-    return cudaIpcCloseMemHandle(ptr) == cudaSuccess ? ZKV_OK : ZKV_ERR_LAUNCH;
+    return cudaIpcCloseMemHandle(ptr) == cudaSuccess ? ZKV_OK : launch_refused();
 }
 
 extern "C" int zkv_peer_free(void* ptr) {
     if (!ptr) return ZKV_ERR_ARG;
-    return cudaFree(ptr) == cudaSuccess ? ZKV_OK : ZKV_ERR_LAUNCH;
+    return cudaFree(ptr) == cudaSuccess ? ZKV_OK : launch_refused();
 }
 
 static int peer_put_launch(const zkv_peer_seg* segs, int n_seg, void* const* peer_base, int64_t flag_off, int rank,

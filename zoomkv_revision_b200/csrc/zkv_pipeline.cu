@@ -139,7 +139,7 @@ extern "C" int zkv_reference_select(const void* q, int G, const zkv_ref_layer* L
         return s;
     if (raw_q_out &&
         cudaMemcpyAsync(raw_q_out, raw_q, (size_t)rows * kHeadDim * 2, cudaMemcpyDeviceToDevice, st) != cudaSuccess)
-        return ZKV_ERR_LAUNCH;
+        return launch_refused();
     return ZKV_OK;
 }
 

@@ -392,7 +392,7 @@ static int launch_cluster(const void* fn, int batch, int64_t work, size_t smem, 
     const int ctas = want <= 2 * kMaxThreads ? 1 : want <= 32768 ? 8 : 16;
     const int threads = (int)std::min<int64_t>(kMaxThreads, (want + 31) / 32 * 32);
     if (ctas == 16 && cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-        return ZKV_ERR_LAUNCH;
+        return launch_refused();
     return launch_clustered(fn, ctas, threads, ctas, smem, st, args, true);
 }
 

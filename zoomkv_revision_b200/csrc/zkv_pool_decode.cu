@@ -1509,12 +1509,12 @@ static int launch_kernel(const DecodeArgs& a, int grid, int smem, cudaStream_t s
     const auto kernel = kRows ? pool_rows_kernel<kQ, kF8, D, NT> : pool_decode_kernel<kQ, kF8, D, NT>;
     static int raised[64] = {};
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ZKV_ERR_LAUNCH;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return launch_refused();
     if (!raised[dev]) {
         if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem_of(C::kRing)) !=
                 cudaSuccess ||
             cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-            return ZKV_ERR_LAUNCH;
+            return launch_refused();
         raised[dev] = 1;
     }
     cudaLaunchConfig_t cfg = {};
@@ -1530,7 +1530,7 @@ static int launch_kernel(const DecodeArgs& a, int grid, int smem, cudaStream_t s
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = a.ranks > 1 ? 2 : 1;
-    if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return ZKV_ERR_LAUNCH;
+    if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return launch_refused();
     return launch_status();
 }
 
@@ -1598,7 +1598,7 @@ extern "C" int zkv_pool_init(zkv_pool* p) {
     if (rc != ZKV_OK) return rc;
     if (!pool::encode_pool(p->maps, p, p->k, p->k_block, p->k_token, p->k_head) ||
         !pool::encode_pool(p->maps + 16, p, p->v, p->v_block, p->v_token, p->v_head))
-        return ZKV_ERR_LAUNCH;
+        return launch_refused();
     return ZKV_OK;
 }
 

@@ -925,7 +925,7 @@ static int launch_pdl(const void* fn, int grid, int threads, size_t smem, cudaSt
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelExC(&cfg, fn, args) != cudaSuccess) return ZKV_ERR_LAUNCH;
+    if (cudaLaunchKernelExC(&cfg, fn, args) != cudaSuccess) return launch_refused();
     return cudaGetLastError() == cudaSuccess ? ZKV_OK : ZKV_ERR_LAUNCH;
 }
 
@@ -960,7 +960,7 @@ static int decode_raw(const void* q, const zkv_raw_layer* layer, int rows, int G
         return ZKV_ERR_ALIGN;
     Args a;
     memset(&a, 0, sizeof(a));
-    if (!cached_maps(&a.tk, &a.tv, L.keys, L.values, (int64_t)rows * cap)) return ZKV_ERR_LAUNCH;
+    if (!cached_maps(&a.tk, &a.tv, L.keys, L.values, (int64_t)rows * cap)) return launch_refused();
     a.q = (const uint16_t*)q;
     a.cmin = (const uint16_t*)L.chunk_min;
     a.cmax = (const uint16_t*)L.chunk_max;
@@ -1017,7 +1017,7 @@ static int decode_raw(const void* q, const zkv_raw_layer* layer, int rows, int G
 
     static bool attr_set[64] = {};
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ZKV_ERR_LAUNCH;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return launch_refused();
     if (!attr_set[dev]) {
         if (cudaFuncSetAttribute(raw_score_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)score_smem()) != cudaSuccess ||
@@ -1025,7 +1025,7 @@ static int decode_raw(const void* q, const zkv_raw_layer* layer, int rows, int G
                                  (int)select_smem()) != cudaSuccess ||
             cudaFuncSetAttribute(raw_attend_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)attend_smem()) != cudaSuccess)
-            return ZKV_ERR_LAUNCH;
+            return launch_refused();
         attr_set[dev] = true;
     }
     void* args[] = {&a};
@@ -1147,7 +1147,7 @@ static int decode_raw_split(const void* q, const zkv_raw_layer* layer, const zkv
     if (sp->bytes < x.bytes) return ZKV_ERR_CAPACITY;  // the exchange buffers are too small for this shape
     Args a;
     memset(&a, 0, sizeof(a));
-    if (!cached_maps(&a.tk, &a.tv, L.keys, L.values, (int64_t)rows * cap)) return ZKV_ERR_LAUNCH;
+    if (!cached_maps(&a.tk, &a.tv, L.keys, L.values, (int64_t)rows * cap)) return launch_refused();
     a.q = (const uint16_t*)q;
     a.cmin = (const uint16_t*)L.chunk_min;
     a.cmax = (const uint16_t*)L.chunk_max;
@@ -1196,13 +1196,13 @@ static int decode_raw_split(const void* q, const zkv_raw_layer* layer, const zkv
 
     static bool attr_set[64] = {};
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ZKV_ERR_LAUNCH;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return launch_refused();
     if (!attr_set[dev]) {
         if (cudaFuncSetAttribute(raw_score_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)split_score_smem()) != cudaSuccess ||
             cudaFuncSetAttribute(raw_attend_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)attend_smem()) != cudaSuccess)
-            return ZKV_ERR_LAUNCH;
+            return launch_refused();
         attr_set[dev] = true;
     }
     void* args[] = {&a};
@@ -1250,11 +1250,11 @@ int raw_quest_topk(const void* q, int G, const void* cmin, const void* cmax, con
     a.raw_q_out = raw_q_out;
     static bool attr_set[64] = {};
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ZKV_ERR_LAUNCH;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return launch_refused();
     if (!attr_set[dev]) {
         if (cudaFuncSetAttribute(raw_score_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)score_smem()) != cudaSuccess)
-            return ZKV_ERR_LAUNCH;
+            return launch_refused();
         attr_set[dev] = true;
     }
     void* args[] = {&a};
