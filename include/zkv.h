@@ -726,9 +726,10 @@ int zkv_pool_plan(const int32_t* lens, const int32_t* new_lens, int batch, int b
 
 /* Pushes the blocks of the requests with done[b] != 0 on the free stack, in
  * request and then block order, and sets their lengths to 0 (their table rows
- * stay as they are).  A push past n_blocks (a block released twice) is left
- * out and reported as ZKV_ERR_CAPACITY.  lens_out / n_free_out may be lens /
- * n_free.  batch <= 8192.                                                  */
+ * stay as they are).  A block id outside [0, n_blocks) is left out and
+ * reported as ZKV_ERR_RANGE, a push past n_blocks (a block released twice) as
+ * ZKV_ERR_CAPACITY.  free_blocks past *n_free_out may hold anything.
+ * lens_out / n_free_out may be lens / n_free.  batch <= 8192.              */
 int zkv_pool_release(const uint8_t* done, const int32_t* lens, int batch, int block_size, const int32_t* block_table,
                      int64_t table_ld, int width, int32_t* free_blocks, const int32_t* n_free, int64_t n_blocks,
                      int32_t* lens_out, int32_t* n_free_out, int32_t* status, void* stream);

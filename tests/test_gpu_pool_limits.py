@@ -4,7 +4,7 @@ import threading
 import pytest
 import torch
 
-from test_gpu_pool import BF, DEV, check_decode, gen, i32, make_pool, make_table
+from test_gpu_pool import (BF, DEV, ERR_RANGE, check_decode, gen, i32, make_pool, make_table, plan_inputs)
 from zoomkv_revision_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +71,31 @@ def test_batches_of_every_size_from_several_threads():
         t.join()
         run_plan_and_release(8192)
     assert not failed
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("B,ctx", [(1, 100), (5, 200), (3, 20000), (1300, 90)])
+def test_release_leaves_bad_ids_out(B, ctx, in_place):
+    """An id outside the pool goes on no stack: the next plan would give its request a place that is none."""
+    import random
+    S, r = 16, random.Random(B)
+    lens, _, table, free, n_free = plan_inputs(B, B, S, ctx, 1)
+    lens = [max(n, 1) for n in lens]
+    n_blocks = len(free)
+    done = [r.random() < 0.8 or b == 0 for b in range(B)]
+    for b in range(B):
+        for j in range(-(-lens[b] // S)):
+            if table[b][j] < 0 or r.random() < 0.1 or (b, j) == (0, 0):
+                table[b][j] = r.choice([-1, n_blocks, 2 ** 31 - 1, -2 ** 31])
+    want = free[:n_free]
+    for b in range(B):
+        if done[b]:
+            want += [i for i in table[b][: -(-lens[b] // S)] if 0 <= i < n_blocks]
+    t_lens, t_free, t_n, status = i32(lens), i32(free), i32([n_free]), i32([0])
+    lo, no = (None, None) if in_place else (torch.empty_like(t_lens), torch.empty_like(t_n))
+    ops.pool_release(torch.tensor(done, device=DEV), t_lens, i32(table), t_free, t_n, S, lens_out=lo, n_free_out=no,
+                     status=status)
+    assert int(status) == ERR_RANGE
+    assert (t_lens if in_place else lo).tolist() == [0 if d else n for d, n in zip(done, lens)]
+    assert int(t_n if in_place else no) == len(want)
+    assert t_free[: len(want)].tolist() == want

@@ -6,7 +6,8 @@
 // token (per block).  Both run as ONE cluster: every CTA makes the sums for
 // itself (a few values per thread), the cluster meets once, and then its CTAs
 // share the tokens, so the outputs may be the inputs' own buffers without a
-// second launch or a counter in memory.
+// second launch or a counter in memory.  Release meets once more, to leave out
+// ids that are not the pool's.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -190,6 +191,7 @@ struct ReleaseArgs {
 __global__ void __launch_bounds__(kMaxThreads) pool_release_kernel(const __grid_constant__ ReleaseArgs a) {
     extern __shared__ int32_t sm[];
     __shared__ int64_t sh[32];
+    __shared__ int s_bad;              // rank 0's: ids outside the pool
     int32_t* s_start = sm;             // [batch] blocks pushed before a request
     int32_t* s_len = s_start + a.batch;  // [batch] its new length
     cg::cluster_group cluster = cg::this_cluster();
@@ -203,6 +205,7 @@ __global__ void __launch_bounds__(kMaxThreads) pool_release_kernel(const __grid_
         code = ZKV_ERR_RANGE;
         n_free = n_free < 0 ? 0 : a.n_blocks;
     }
+    if (tid == 0) s_bad = 0;
     int64_t start0 = 0;
     for (int b0 = 0; b0 < a.batch; b0 += nt) {
         const int b = b0 + tid;
@@ -228,12 +231,11 @@ __global__ void __launch_bounds__(kMaxThreads) pool_release_kernel(const __grid_
         start0 = room;
     }
     cluster.sync();  // every CTA has read lens and n_free
-    if (rank == 0) {
+    if (rank == 0)
         for (int b = tid; b < a.batch; b += nt) a.lens_out[b] = s_len[b];
-        if (tid == 0) *a.n_free_out = (int)(n_free + start0);
-    }
     // Four places of the stack a turn, from a multiple of four on: one search, 16-byte stores.
     const int64_t end = n_free + start0;
+    int bad = 0;
     for (int64_t w0 = (n_free & ~3) + ((int64_t)rank * nt + tid) * 4; w0 < end; w0 += (int64_t)ranks * nt * 4) {
         const int i0 = (int)(w0 - n_free);  // -3 .. : below 0 only in the first group
         int b = owner_of(s_start, a.batch, i0 > 0 ? i0 : 0);
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(kMaxThreads) pool_release_kernel(const __grid_
         for (int e = 0; e < 4; ++e) id[e] = from[e] ? *from[e] : 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (from[e] && (uint32_t)id[e] >= (uint32_t)a.n_blocks) code = ZKV_ERR_RANGE;
+            if (from[e] && (uint32_t)id[e] >= (uint32_t)a.n_blocks) ++bad;
         if (a.vectors && from[0] && from[3]) {
             *reinterpret_cast<int4*>(a.free_blocks + w0) = make_int4(id[0], id[1], id[2], id[3]);
         } else {
@@ -258,7 +260,27 @@ __global__ void __launch_bounds__(kMaxThreads) pool_release_kernel(const __grid_
                 if (from[e]) a.free_blocks[w0 + e] = id[e];
         }
     }
+    if (bad) {
+        code = ZKV_ERR_RANGE;
+        atomicAdd(cluster.map_shared_rank(&s_bad, 0), bad);
+    }
     if (code) raise_status(a.status, code);
+    cluster.sync();  // every id is on the stack and judged
+    if (rank != 0) return;
+    int64_t top = end;
+    if (s_bad) {  // rare: the ids of the pool move up over the others, in order
+        top = n_free;
+        for (int64_t i0 = n_free; i0 < end; i0 += nt) {
+            const int64_t i = i0 + tid;
+            const int id = i < end ? __ldcg(a.free_blocks + i) : -1;
+            const bool keep = (uint32_t)id < (uint32_t)a.n_blocks;
+            int64_t total;
+            const int64_t at = top + block_sum_before(keep, sh, &total);
+            if (keep) a.free_blocks[at] = id;
+            top += total;
+        }
+    }
+    if (tid == 0) *a.n_free_out = (int)top;
 }
 
 // ---------------------------------------------------------------- write
