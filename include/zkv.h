@@ -761,9 +761,10 @@ int zkv_pool_write(const void* k, int64_t k_token, int64_t k_head, const void* v
  *   same tokens' with any guess, and a guess far too short costs time.
  *   A length outside [0, width * block_size] is cut to that, and a block id
  *   outside the pool leaves its tokens out, both with ZKV_ERR_RANGE
- *   workspace: device, 256-byte aligned, >= zkv_pool_decode_ws_bytes (0:
- *   none is needed, NULL will do; also 0 for bad arguments), scratch only, no
- *   state between calls
+ *   workspace: device, 256-byte aligned, >= zkv_pool_decode_ws_bytes of the
+ *   same max_len, width * block_size where that is 0 or more (0: none is
+ *   needed, NULL will do; also 0 for bad arguments); scratch only, no state
+ *   between calls.  The size for max_len 0 does for every table and max_len
  *   q_heads / kv_heads <= 5120.                                           */
 size_t zkv_pool_decode_ws_bytes(const zkv_pool* pool, int batch, int q_heads, int window, int64_t max_len);
 int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int dtype, const zkv_pool* pool,

@@ -66,6 +66,7 @@ constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxGrid = 480;                   // CTAs that a workspace is sized for
 constexpr int kWholeTokens = 256;               // requests up to this length are never cut
 constexpr int kMaxChunks = 320;                 // of 16 query heads per kv head
+constexpr int64_t kMaxLen = INT32_MAX - 512;    // tokens of a request; 32 bits hold a tile past them
 constexpr int kMaxStages = 8;                   // of a CTA's ring
 constexpr int kMaxRanks = 16;                   // CTAs of a cluster that shares a row
 // Up to kWholeBytes of K and V, and kRankTiles tiles a CTA or twice that where the CTAs fill their waves to 4/5, whole
@@ -1610,8 +1611,9 @@ extern "C" size_t zkv_pool_decode_ws_bytes(const zkv_pool* p, int batch, int q_h
     if (pool::check_pool(p) != ZKV_OK || batch < 0 || q_heads < 1 || q_heads % p->kv_heads || window < 0 || max_len < 0)
         return 0;
     const pool::Heads h = pool::split_heads(q_heads / p->kv_heads);
-    if (h.chunks > pool::kMaxChunks || !needs_parts(p, batch, h, window, max_len)) return 0;
-    const size_t rows = pool::part_rows(batch, p->kv_heads, h, max_len);
+    const int64_t guess = max_len > 0 ? max_len : pool::kMaxLen;  // the table is not known here: the most that any needs
+    if (h.chunks > pool::kMaxChunks || !needs_parts(p, batch, h, window, guess)) return 0;
+    const size_t rows = pool::part_rows(batch, p->kv_heads, h, guess);
     return pool::up256(rows * 8) + pool::up256(rows * p->head_dim * 4);
 }
 
@@ -1631,11 +1633,11 @@ extern "C" int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int
     if (!pool::aligned16(q) || q_row % 8 || q_head % 8 || !pool::aligned16(out)) return ZKV_ERR_ALIGN;
     if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return ZKV_ERR_ALIGN;
     const int64_t room = (int64_t)width * p->block_size;
-    const int64_t cap = std::min<int64_t>(room, INT32_MAX - 512);
+    const int64_t cap = std::min<int64_t>(room, pool::kMaxLen);
     const int64_t guess = max_len > 0 ? std::min(max_len, cap) : cap;
     const pool::Heads hs = pool::split_heads(q_heads / p->kv_heads);
     if (hs.chunks > pool::kMaxChunks) return ZKV_ERR_CAPACITY;
-    const bool parts = needs_parts(p, batch, hs, window, guess);
+    const bool parts = needs_parts(p, batch, hs, window, guess);  // not with guess 0, a table of no columns
     if (parts && !workspace) return ZKV_ERR_ARG;
     if (parts && ws_bytes < zkv_pool_decode_ws_bytes(p, batch, q_heads, window, guess)) return ZKV_ERR_CAPACITY;
     uint64_t any = 0;

@@ -1396,9 +1396,9 @@ def pool_decode_ws_bytes(batch: int, q_heads: int, pool: KVPool, width: int, max
     key = (batch, q_heads, width, max_len, window)
     got = pool.ws_sizes.get(key)
     if got is None:
-        room = width * pool.block_size
-        got = int(lib().zkv_pool_decode_ws_bytes(pool.ref, batch, q_heads, window,
-                                                 min(max_len, room) if max_len > 0 else room))
+        room = width * pool.block_size   # (of a table without columns there is nothing to cut)
+        got = room and int(lib().zkv_pool_decode_ws_bytes(pool.ref, batch, q_heads, window,
+                                                          min(max_len, room) if max_len > 0 else room))
         if len(pool.ws_sizes) > 256:   # a bound that moves with every step
             pool.ws_sizes.clear()
         pool.ws_sizes[key] = got
