@@ -9,7 +9,8 @@
  *     stride argument is named; strides are in elements.
  *   - head_dim is 128 and the Quest chunk (= KIVI key group = page) is 16
  *     tokens, as in the production ZoomKV configuration.
- *   - `stream` is a cudaStream_t (NULL = legacy default stream).
+ *   - `stream` is a cudaStream_t (NULL = legacy default stream) of the current
+ *     device, on which the tensors lie: a launch goes to the current device.
  *   - Every entry point returns ZKV_OK (0) or a ZKV_ERR_* code; launches are
  *     asynchronous, so a device-side failure (bounded wait expired) is
  *     reported through the optional `status` word the caller passes.

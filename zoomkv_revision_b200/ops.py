@@ -38,10 +38,12 @@ pool_decode / pool_release             no counterpart)
 Errors follow the reference: wrong dtype -> TypeError, wrong shape / range ->
 ValueError / RuntimeError, and a non-zero C status -> RuntimeError.  There
 is no CPU path: every op requires CUDA tensors and the compiled library.
+An op runs on its tensors' device, whatever the current device is.
 """
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -60,13 +62,45 @@ __all__ = [
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+class _AnotherDevice(RuntimeError):
+    """The tensors' device is not the current one, on which a launch on the default stream (a handle of 0) would run."""
+
+    def __init__(self, index: int):
+        super().__init__(f"the tensors are on cuda:{index}, the current device is cuda:{_current_device()}")
+        self.index = index
+
+
+def _raw_stream(index: int) -> int:
+    """The current stream (its raw handle) of CUDA device `index`, which has to be the current device."""
+    if _current_device() != index:
+        raise _AnotherDevice(index)
+    return torch.cuda.current_stream(index).cuda_stream if _RAW_STREAM is None else _RAW_STREAM(index)
 
 
 def _stream(t: torch.Tensor) -> int:
     """The current CUDA stream of t's device (its raw handle)."""
-    if _RAW_STREAM is not None and t.device.index is not None:
-        return _RAW_STREAM(t.device.index)
-    return torch.cuda.current_stream(t.device).cuda_stream
+    index = t.device.index
+    return torch.cuda.current_stream(t.device).cuda_stream if index is None else _raw_stream(index)
+
+
+def _on_its_device(op):
+    """`op` with its tensors' device made current where it is not.  An operator asks for its stream when it launches, so
+    nothing has run on a GPU when it is begun again.  (The pooled cache's operators, whose calls are shorter than what this
+    wrapper adds is worth, look for themselves.)"""
+
+    @functools.wraps(op)
+    def call(*args, **kwargs):
+        try:
+            return op(*args, **kwargs)
+        except _AnotherDevice as e:
+            index = e.index
+        with torch.cuda.device(index):
+            return op(*args, **kwargs)
+
+    return call
 
 
 def _cuda(*ts):
@@ -92,6 +126,7 @@ def _p(t):
 
 
 # ----------------------------------------------------------------- Quest stage-1
+@_on_its_device
 def quest_chunk_score(raw_q, chunk_min, chunk_max, scores_out, n_chunks, chunk_valid=None):
     """scores_out[b,h,c] = sum_d max(q*max, q*min) for c < n_chunks (in place).
 
@@ -126,6 +161,7 @@ def quest_chunk_score(raw_q, chunk_min, chunk_max, scores_out, n_chunks, chunk_v
                                 n_chunks, n_max, _stream(raw_q)), "zkv_quest_score")
 
 
+@_on_its_device
 def quest_chunk_score_gqa(q, chunk_min, chunk_max, scores_out, n_chunks, chunk_valid=None):
     """quest_chunk_score with the GQA mean folded into the kernel: q
     [bs, 1, kv*G, 128] bf16 (the decode query) instead of raw_q."""
@@ -152,6 +188,7 @@ def quest_chunk_score_gqa(q, chunk_min, chunk_max, scores_out, n_chunks, chunk_v
 
 
 # ----------------------------------------------------------------- top-k
+@_on_its_device
 def float_topk(scores: torch.Tensor, k: int, out: torch.Tensor | None = None) -> torch.Tensor:
     """Top-k indices [B, k] int64 of fp32 [B, L] (ties -> lowest index, ascending)."""
     _cuda(("scores", scores))
@@ -182,6 +219,7 @@ def float_topk_3d(scores: torch.Tensor, k: int, out: torch.Tensor | None = None)
     return o.view(bs, kv, k)
 
 
+@_on_its_device
 def radix_topk_3d(vals: torch.Tensor, k: int) -> torch.Tensor:
     """Top-k indices of int32 [bs, kv, L] (ties -> lowest index, ascending)."""
     _cuda(("vals", vals))
@@ -196,6 +234,7 @@ def radix_topk_3d(vals: torch.Tensor, k: int) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------- CDS
+@_on_its_device
 def partial_chunk_density_scores_cuda(chunk_ids, chunk_centroids, raw_q, out_scores, kernel=None):
     """out_scores[b,h,j] = centroid[b,h,chunk_ids[b,h,j]] . raw_q[b,h] (fp32; -1e30 if invalid)."""
     del kernel
@@ -215,6 +254,7 @@ def partial_chunk_density_scores_cuda(chunk_ids, chunk_centroids, raw_q, out_sco
                                   _stream(ids)), "zkv_chunk_density")
 
 
+@_on_its_device
 def dense_mask_from_topk_cuda(positions, mask, kernel=None):
     """mask.fill_(False); mask.scatter_(2, positions, True) in one launch."""
     del kernel
@@ -229,6 +269,7 @@ def dense_mask_from_topk_cuda(positions, mask, kernel=None):
 
 
 # ----------------------------------------------------------------- KIVI stage-2
+@_on_its_device
 def partial_chunk_kivi_qk_dense_sparse_cuda(chunk_ids, dense_mask, packed_K, chunk_min, chunk_max, raw_q,
                                             dense_topk, sparse_topk, group_size, out_scores, out_indices,
                                             kernel=None):
@@ -275,6 +316,7 @@ def partial_chunk_kivi_qk_dense_sparse_cuda(chunk_ids, dense_mask, packed_K, chu
                             out_scores.shape[2], _stream(ids)), "zkv_kivi_qk")
 
 
+@_on_its_device
 def float_topk_gather_concat_3d(scores, lut, skipped, out, k):
     """out[:,:,:k] = lut[top_k(scores)]; out[:,:,k:k+sk] = skipped.  Returns out."""
     _cuda(("scores", scores), ("lut", lut), ("skipped", skipped), ("out", out))
@@ -305,6 +347,7 @@ def reference_select_ws_bytes(rows: int, n_chunks: int, nk: int, n_dense: int) -
     return int(lib().zkv_reference_select_ws_bytes(rows, n_chunks, nk, n_dense))
 
 
+@_on_its_device
 def reference_select(q, chunk_min, chunk_max, centroid, chunk_valid, packed, n_chunks: int, n_valid_chunks: int,
                      nk: int, n_dense: int, dense_topk: int, sparse_topk: int, k: int, skipped, final_out, workspace,
                      raw_q_out=None):
@@ -342,6 +385,7 @@ def reference_select(q, chunk_min, chunk_max, centroid, chunk_valid, packed, n_c
 
 
 # ----------------------------------------------------------------- merge
+@_on_its_device
 def lse_merge_cuda(attn_out_a, lse_a, attn_out_b, lse_b):
     """Merge two attention partials ([bs,1,heads,dim] + lse [bs,heads,1])."""
     if not attn_out_a.is_cuda:
@@ -359,6 +403,7 @@ def lse_merge_cuda(attn_out_a, lse_a, attn_out_b, lse_b):
     return out.to(attn_out_a.dtype)
 
 
+@_on_its_device
 def lse_merge_n(parts: torch.Tensor, lses: torch.Tensor, out: torch.Tensor, lse_out: torch.Tensor | None = None):
     """parts [n, rows, dim] fp32, lses [n, rows] -> out [rows, dim] bf16 (+ lse_out [rows])."""
     _dtype("parts", parts, torch.float32)
@@ -370,6 +415,7 @@ def lse_merge_n(parts: torch.Tensor, lses: torch.Tensor, out: torch.Tensor, lse_
 
 
 # ----------------------------------------------------------------- encode
+@_on_its_device
 def kivi_encode_chunks(keys, chunk_min, chunk_max, chunk_centroid, chunk_valid, packed, chunk_start: int,
                        kscale=None):
     """Write metadata + KIVI codes of the aligned chunks of `keys` [bs,kv,T,128]
@@ -390,6 +436,7 @@ def kivi_encode_chunks(keys, chunk_min, chunk_max, chunk_centroid, chunk_valid, 
           "zkv_kivi_encode")
 
 
+@_on_its_device
 def vquant_encode(values, vcodes_t, vmeta, tok_start: int):
     """Per-token 4-bit values of `values` [bs,kv,T,128] into the page buffers
     vcodes_t [bs,kv,n_pages,128,2] int32 / vmeta [bs,kv,n_pages,2,4,16] bf16."""
@@ -403,6 +450,7 @@ def vquant_encode(values, vcodes_t, vmeta, tok_start: int):
 
 
 # ----------------------------------------------------------------- attention
+@_on_its_device
 def attn_rows(q, keys, values, *, seg0=(0, 0), sel=None, sel_offset=0, seg1=(0, 0), scale=None, out=None, lse=None,
               split=0, status=None):
     """Decode attention of q [bs,1,H*G,128] over the raw rows of keys/values
@@ -444,6 +492,7 @@ def _pinned_src(src_k, src_v):
     _require(src_k.is_contiguous() and src_v.is_contiguous(), "src caches must be contiguous")
 
 
+@_on_its_device
 def h2d_gather_kv(src_k_caches, src_v_caches, selected_indices, dst_k_caches, dst_v_caches, status=None):
     """dst[b,h,j] = src[b,h,selected_indices[b,h,j]] for j < topk, K and V.
 
@@ -474,6 +523,7 @@ def h2d_gather_kv(src_k_caches, src_v_caches, selected_indices, dst_k_caches, ds
                                   _stream(dst_k_caches)), "zkv_h2d_gather_kv")
 
 
+@_on_its_device
 def h2d_gather_kv_packed(src_k_caches, src_v_caches, dst_k_packed, dst_v_packed, indices_packed, cu_seqlens_topk,
                          cu_seqlens_k, sl_end: int, global_k: int, status=None):
     """Variable-K gather into a flash-attention varlen packed buffer.
@@ -506,6 +556,7 @@ def h2d_gather_kv_packed(src_k_caches, src_v_caches, dst_k_packed, dst_v_packed,
                                          _stream(dst_k_packed)), "zkv_h2d_gather_kv_packed")
 
 
+@_on_its_device
 def h2d_gather_rows(src_k, src_v, sel, dst_k, dst_v, *, n_sel=None, src_offset=0, dst_offset=0, status=None):
     """Offload-tier gather with offsets: dst[b,h,dst_offset+j] =
     src[b,h,sel[b,h,j]+src_offset] for j < n_sel.  src_* host-pinned
@@ -565,6 +616,7 @@ def page_decode_plan(rows: int, n_c: int, nk: int, cluster: int = 0, split=None,
     return {"split": True, "parts": parts, "launches": 3 if parts > 1 else 2}
 
 
+@_on_its_device
 def page_decode(q, layer: PageLayer, n_c: int, nk: int, n_near: int, *, n_sink: int = 0, near_start: int = 0,
                 scale=None, out=None, lse=None, sel_out=None, status=None, cluster=0, split=None, workspace=None):
     """Fused page-mode decode: q [bs,1,H*G,128] -> out [bs,1,H*G,128].
@@ -611,6 +663,7 @@ def page_decode(q, layer: PageLayer, n_c: int, nk: int, n_near: int, *, n_sink: 
     return out
 
 
+@_on_its_device
 def page_attend(q, layer: PageLayer, sel, sel_lo: int, sel_hi: int, *, n_sink: int = 0, near_start: int = 0,
                 n_near: int = 0, scale=None, out=None, out_f32=None, lse=None, status=None, cluster=0):
     """Attention over externally selected pages (sequence split): sel
@@ -633,6 +686,7 @@ def page_attend(q, layer: PageLayer, sel, sel_lo: int, sel_hi: int, *, n_sink: i
     return out_f32 if out_f32 is not None else out
 
 
+@_on_its_device
 def page_decode_scored(q, layer: PageLayer, scores, n_c: int, nk: int, own_lo: int, own_hi: int, parts: int,
                        out_f32, lse, *, n_sink: int = 0, near_start: int = 0, n_near: int = 0, scale=None,
                        sel_out=None, status=None, cluster=0):
@@ -691,6 +745,7 @@ def page_decode_raw_ws_bytes(rows: int, n_c: int, nk: int, n_sink: int, n_near: 
     return int(lib().zkv_page_decode_raw_ws_bytes(int(rows), int(n_c), int(nk), int(n_sink), int(n_near)))
 
 
+@_on_its_device
 def page_decode_raw(q, layer: RawLayer, n_c: int, nk: int, n_near: int, *, n_sink: int = 0, near_start: int = 0,
                     scale=None, out=None, lse=None, sel_out=None, status=None, workspace=None):
     """Page mode over raw rows: q [bs,1,H*G,128] -> out [bs,1,H*G,128] bf16.
@@ -738,6 +793,7 @@ def raw_split_range(n_c: int, world: int, rank: int):
     return lo.value, hi.value
 
 
+@_on_its_device
 def page_decode_raw_split(q, layer: RawLayer, split, n_c: int, nk: int, n_near: int, *, n_sink: int = 0,
                           near_start: int = 0, scale=None, out=None, lse=None, sel_out=None, status=None,
                           workspace=None):
@@ -797,6 +853,7 @@ class LargeLayer:
         self.struct = _lib.ZkvQuestLarge(_p(large_min), _p(large_max), _p(large_valid), large_min.shape[2])
 
 
+@_on_its_device
 def quest_large_minmax(chunk_min, chunk_max, valid_end: int, factor: int, large_min, large_max, large_valid,
                        g_lo: int = 0, g_hi=None):
     """_update_large_chunk_minmax (polar_cache_kivi_quest_density_seperate_
@@ -812,6 +869,7 @@ def quest_large_minmax(chunk_min, chunk_max, valid_end: int, factor: int, large_
                                        _stream(chunk_min)), "zkv_quest_large_minmax")
 
 
+@_on_its_device
 def page_decode_raw_hier(q, layer: RawLayer, large: LargeLayer, n_c: int, factor: int, nk_large: int, nk_small: int,
                          n_near: int, *, n_sink: int = 0, near_start: int = 0, scale=None, out=None, lse=None,
                          sel_out=None, status=None, workspace=None):
@@ -848,6 +906,7 @@ def page_decode_raw_hier(q, layer: RawLayer, large: LargeLayer, n_c: int, factor
 
 
 # ----------------------------------------------------------------- decode-loop caller
+@_on_its_device
 def rmsnorm(x, w, eps: float, out=None):
     """Row-wise RMSNorm of x [..., dim] bf16 with weight w [dim] (fp32 inside)."""
     _dtype("x", x, torch.bfloat16)
@@ -858,6 +917,7 @@ def rmsnorm(x, w, eps: float, out=None):
     return out
 
 
+@_on_its_device
 def qk_norm_rope(qkv, q_norm, k_norm, cos, sin, pos, hq: int, hkv: int, eps: float, q, k, v):
     """qkv [rows, (hq + 2 hkv) * 128] -> q / k (per-head RMSNorm + rotate-half
     RoPE at position pos[0], a device int64) and v, into the given buffers."""
@@ -867,6 +927,7 @@ def qk_norm_rope(qkv, q_norm, k_norm, cos, sin, pos, hq: int, hkv: int, eps: flo
                                  float(eps), _p(q), _p(k), _p(v), _stream(qkv)), "zkv_qk_norm_rope")
 
 
+@_on_its_device
 def silu_mul(gu, out):
     """out [rows, ffn] = silu(gu[:, :ffn]) * gu[:, ffn:] (bf16, fp32 inside)."""
     _contig("gu", gu)
@@ -875,6 +936,7 @@ def silu_mul(gu, out):
     return out
 
 
+@_on_its_device
 def gqa_mean(q, heads: int, out=None):
     """raw_q [bs, H, 128] bf16 = GQA mean of q [bs, 1, H*G, 128] (fp32 sum in
     head order / G, as the fused kernels compute it)."""
@@ -967,6 +1029,7 @@ class RqLayout:
         return ctypes.byref(self._s)
 
 
+@_on_its_device
 def rq_encode(keys, signs, lay: RqLayout, tok_start: int = 0):
     """Encode keys [rows, T, 128] (or [bs, H, T, 128]) bf16 into `lay` at
     tokens [tok_start, tok_start + T) and add them to lay.hist."""
@@ -1000,6 +1063,7 @@ def batch_encode(Y, signs):
     return codebook, weight, packed, counts
 
 
+@_on_its_device
 def rq_query(q, signs, group: int = 4, *, planes: bool = False):
     """q [bs, 1, H*G, 128] or [rows, G, 128] bf16 -> dict(q_blocks [rows,128],
     q_norm [rows], q_mean [rows,128] bf16; planes [rows,4,16] u8 and qparams
@@ -1035,6 +1099,7 @@ def _targets_tensor(targets):
     return t, t.numel()
 
 
+@_on_its_device
 def get_cache_cnt_fused(q_blocks, lay: RqLayout, kv_len: int, targets, out=None):
     """cache_cnt [rows, kv_len] int32 (update_cache_cnt with the bucket order
     computed from q_blocks)."""
@@ -1047,6 +1112,7 @@ def get_cache_cnt_fused(q_blocks, lay: RqLayout, kv_len: int, targets, out=None)
     return out
 
 
+@_on_its_device
 def collision_topk(q_blocks, lay: RqLayout, kv_len: int, targets, C: int, idx_out=None, cnt_out=None):
     """Top-C keys by collision count (ties to the lower index), ascending
     index order: [rows, C] int64."""
@@ -1059,6 +1125,7 @@ def collision_topk(q_blocks, lay: RqLayout, kv_len: int, targets, C: int, idx_ou
     return idx_out
 
 
+@_on_its_device
 def partial_rerank_cuda(coarse_indices, lay: RqLayout, q_blocks, q_norm, mag_centers=None, final_topk: int = 0,
                         scores_out=None, final_out=None):
     """4-bit RaBitQ scores [rows, C] bf16 of coarse_indices [rows, C] (the
@@ -1082,6 +1149,7 @@ def partial_rerank_cuda(coarse_indices, lay: RqLayout, q_blocks, q_norm, mag_cen
     return (scores_out, final_out) if final_topk > 0 else scores_out
 
 
+@_on_its_device
 def coarse_2bit_score_cuda(lay: RqLayout, q_signs, q_mags, kv_len: int, out=None):
     """int32 [rows, kv_len] 2-bit-plane popcount scores (coarse_2bit_score.cu)."""
     rows = q_signs.numel() // 16
@@ -1092,6 +1160,7 @@ def coarse_2bit_score_cuda(lay: RqLayout, q_signs, q_mags, kv_len: int, out=None
     return out
 
 
+@_on_its_device
 def rq_popcount_topk(cand, lay: RqLayout, planes, qparams, K: int, *, C: int | None = None, keys=None,
                      q_mean=None, est_out=None):
     """Popcount-estimate rerank: keep the K best of cand [rows, C] (None = keys
@@ -1116,12 +1185,6 @@ def rq_popcount_topk(cand, lay: RqLayout, planes, qparams, K: int, *, C: int | N
 # ----------------------------------------------------------------- pooled KV cache
 _POOL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 _INT32 = torch.int32
-
-
-def _raw_stream(index: int) -> int:
-    """The raw handle of the current stream of CUDA device `index`."""
-    return torch.cuda.current_stream(index).cuda_stream if _RAW_STREAM is None else _RAW_STREAM(index)
-
 
 class KVPool:
     """One layer's pooled KV cache: k, v [n_blocks, block_size, kv_heads, head_dim]
@@ -1235,6 +1298,10 @@ def pool_plan(lens, new_lens, block_table, free_blocks, n_free, block_size: int,
         raise ValueError("new_lens and lens_out must have one value per request")
     if (positions is not None and positions.numel() < n_slots) or (cu_new is not None and cu_new.numel() <= B):
         raise ValueError("positions needs one value per slot and cu_new [B + 1]")
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return pool_plan(lens, new_lens, block_table, free_blocks, n_free, block_size, slots, positions=positions,
+                             cu_new=cu_new, lens_out=lens_out, n_free_out=n_free_out, status=status)
     at, count = lens.data_ptr(), n_free.data_ptr()
     rc = lib().zkv_pool_plan(at, None if new_lens is None else new_lens.data_ptr(), B, block_size, block_table.data_ptr(),
                              ld, width, free_blocks.data_ptr(), count, free_blocks.numel(), slots.data_ptr(),
@@ -1266,6 +1333,10 @@ def pool_release(done, lens, block_table, free_blocks, n_free, block_size: int, 
         raise ValueError("done must be contiguous [B], on the device of lens")
     if lens_out is not None and lens_out.numel() != B:
         raise ValueError("lens_out must have one value per request")
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return pool_release(done, lens, block_table, free_blocks, n_free, block_size, lens_out=lens_out,
+                                n_free_out=n_free_out, status=status)
     at, count = lens.data_ptr(), n_free.data_ptr()
     rc = lib().zkv_pool_release(done.data_ptr(), at, B, block_size, block_table.data_ptr(), ld, width,
                                 free_blocks.data_ptr(), count, free_blocks.numel(),
@@ -1313,6 +1384,9 @@ def pool_write(k, v, slots, pool: KVPool, *, status=None):
         raise ValueError("tensors must be on the pool's device")
     if status is not None:
         _status_word(status, dev)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return pool_write(k, v, slots, pool, status=status)
     k, v = _whole_rows(k), _whole_rows(v)
     ks, vs = k.stride(), v.stride()
     rc = lib().zkv_pool_write(k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code, slots.data_ptr(), n, pool.ref,
@@ -1355,6 +1429,10 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     if lens.numel() != B or not lens.is_contiguous():
         raise ValueError("lens must be contiguous, one value per request")
     ld, width = _block_table(block_table, B, dev)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return pool_decode(q, pool, lens, block_table, scale=scale, window=window, softcap=softcap, max_len=max_len,
+                               out=out, lse=lse, return_lse=return_lse, status=status, workspace=workspace)
     q3 = _whole_rows(q if len(shape) == 3 else q[:, 0])
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)

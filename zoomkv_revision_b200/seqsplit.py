@@ -322,7 +322,7 @@ def decode_step_p2p(q, layer: ops.PageLayer, pg: PeerGroup, *, n_sink: int = 0, 
     instead of returning a merge of stale partials; it synchronises the
     stream once per step, and is skipped while the stream is being captured
     into a CUDA graph (check the group after replaying the graph)."""
-    stream = torch.cuda.current_stream(q.device).cuda_stream
+    stream = ops._stream(q)   # the group's device is the process's current one
     if pg.n_loc > 0:
         cmin, cmax, valid = layer.tensors[0], layer.tensors[1], layer.tensors[2]
         ops.quest_chunk_score_gqa(q, cmin, cmax, pg.local, pg.n_loc, valid)
