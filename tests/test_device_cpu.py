@@ -47,6 +47,7 @@ class Tensor:
 
 class Pool:
     kv_heads, head_dim, block_size, dtype, code, index, ref, ws_sizes = 2, 128, 16, torch.bfloat16, 0, 1, 0, {}
+    status_at = 0
 
 
 @pytest.fixture

@@ -99,3 +99,24 @@ def test_release_leaves_bad_ids_out(B, ctx, in_place):
     assert (t_lens if in_place else lo).tolist() == [0 if d else n for d, n in zip(done, lens)]
     assert int(t_n if in_place else no) == len(want)
     assert t_free[: len(want)].tolist() == want
+
+
+def test_failures_reach_the_pool_s_own_status():
+    """A call without a status word of its own reports to the pool's."""
+    k, v, _, _ = make_pool(7, 4, 16, 2, 64, BF, "hnd")
+    pool = ops.KVPool(k, v)
+    q = torch.randn(1, 8, 64, generator=gen(8), device=DEV).to(BF)
+    ops.pool_decode(q, pool, i32([20]), i32([[0, 1]]))
+    pool.check()
+    ops.pool_decode(q, pool, i32([20]), i32([[0, 4]]))
+    with pytest.raises(RuntimeError, match="range"):
+        pool.check()
+    pool.check()                                   # the report is given once
+    rows = torch.zeros(1, 2, 64, dtype=BF, device=DEV)
+    ops.pool_write(rows, rows, torch.tensor([64], device=DEV), pool)
+    with pytest.raises(RuntimeError, match="range"):
+        pool.check()
+    status = i32([0])                              # a caller's own word: the pool's stays as it is
+    ops.pool_write(rows, rows, torch.tensor([64], device=DEV), pool, status=status)
+    assert int(status) == ERR_RANGE
+    pool.check()

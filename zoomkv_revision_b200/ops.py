@@ -1192,10 +1192,11 @@ class KVPool:
     rows (a head-before-token pool is passed as `t.transpose(1, 2)`).
     k_scale, v_scale [kv_heads] fp32: an e4m3 element stands for
     stored * scale of its head (None: 1).  Made once when the pool is
-    allocated: it holds the tensors, their addresses and strides."""
+    allocated: it holds the tensors, their addresses and strides, and a status
+    word for the calls that are given none (see check)."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "struct", "ref", "dtype", "device", "kv_heads", "head_dim",
-                 "block_size", "n_blocks", "lse_like", "byte_like", "ws_sizes", "index", "code")
+                 "block_size", "n_blocks", "lse_like", "byte_like", "ws_sizes", "index", "code", "status", "status_at")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _cuda(("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale))
@@ -1234,6 +1235,16 @@ class KVPool:
         self.ws_sizes = {}
         self.lse_like, self.byte_like = None, k.new_empty(0, dtype=torch.uint8)
         check(lib().zkv_pool_init(self.ref), "zkv_pool_init")
+        self.status = torch.zeros(1, dtype=_INT32, device=k.device)
+        self.status_at = self.status.data_ptr()
+
+    def check(self) -> None:
+        """Raises if a pool_write or pool_decode that was given no status word met a slot, block id or length outside the
+        pool or its table, or a wait that ran out, since the last check (waits for the GPU)."""
+        code = int(self.status.item())
+        if code:
+            self.status.zero_()
+            check(code, "pooled KV cache")
 
 
 def _refuse_int32(names, tensors):
@@ -1281,8 +1292,8 @@ def pool_plan(lens, new_lens, block_table, free_blocks, n_free, block_size: int,
     per new token in request order, -1 past the last and for a request that
     is not served); cu_new [B + 1] int32 (written: first token of a request).
     lens_out / n_free_out default to lens / n_free in place.  A request that
-    finds no room keeps its length and blocks; status [1] int32 then gets
-    ZKV_ERR_CAPACITY (3).  Returns slots."""
+    finds no room keeps its length and blocks, which its slots (-1) and length
+    show; status [1] int32 then gets ZKV_ERR_CAPACITY (3).  Returns slots."""
     dev = lens.get_device()
     for t in (lens, free_blocks, n_free, new_lens, positions, cu_new, lens_out, n_free_out, status):
         if t is not None and (t.dtype is not _INT32 or t.get_device() != dev or dev < 0 or not t.is_contiguous()):
@@ -1319,7 +1330,9 @@ def pool_release(done, lens, block_table, free_blocks, n_free, block_size: int, 
                  status=None):
     """Pushes the blocks of the requests with done[b] on the free stack
     (free_blocks, n_free) and sets their lengths to 0.  done [B] bool;
-    the others as in pool_plan; lens_out / n_free_out default to in place."""
+    the others as in pool_plan; lens_out / n_free_out default to in place.
+    Block ids outside the pool are left out, which n_free shows; status [1]
+    int32 then gets ZKV_ERR_RANGE (7)."""
     dev = lens.get_device()
     for t in (lens, free_blocks, n_free, lens_out, n_free_out, status):
         if t is not None and (t.dtype is not _INT32 or t.get_device() != dev or dev < 0 or not t.is_contiguous()):
@@ -1366,7 +1379,9 @@ def pool_write(k, v, slots, pool: KVPool, *, status=None):
     """K and V rows of new tokens into their slots of the pool: k, v
     [n_tokens, kv_heads, head_dim] bf16 or fp16 (the pool's type; any of the
     two for an e4m3 pool, which stores e4m3(row / scale), saturated at 448);
-    slots [n_tokens] int64 of pool_plan, -1 = none."""
+    slots [n_tokens] int64 of pool_plan, -1 = none.  status [1] int32 gets
+    ZKV_ERR_RANGE for a slot outside the pool (None: the pool's own word, which
+    pool.check() looks at)."""
     shape = k.shape
     if v.shape != shape or len(shape) != 3 or shape[1] != pool.kv_heads or shape[2] != pool.head_dim:
         raise ValueError(f"k and v must be [n_tokens, {pool.kv_heads}, {pool.head_dim}]; got {tuple(shape)} and "
@@ -1390,7 +1405,7 @@ def pool_write(k, v, slots, pool: KVPool, *, status=None):
     k, v = _whole_rows(k), _whole_rows(v)
     ks, vs = k.stride(), v.stride()
     rc = lib().zkv_pool_write(k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code, slots.data_ptr(), n, pool.ref,
-                              None if status is None else status.data_ptr(), _raw_stream(dev))
+                              pool.status_at if status is None else status.data_ptr(), _raw_stream(dev))
     if rc:
         check(rc, "zkv_pool_write")
 
@@ -1410,7 +1425,9 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     log, -inf for a request without tokens, whose out is 0).  workspace:
     uint8 CUDA tensor of pool_decode_ws_bytes(...) bytes, scratch only
     (default: allocated per call, where one is needed, from torch's caching
-    allocator)."""
+    allocator).  status [1] int32 gets ZKV_ERR_RANGE for a block id or length
+    outside the pool and its table, ZKV_ERR_TIMEOUT for a wait that ran out
+    (None: the pool's own word, which pool.check() looks at)."""
     shape = q.shape
     B, Hq, D = shape[0], shape[-2], shape[-1]
     if D != pool.head_dim or Hq % pool.kv_heads or len(shape) not in (3, 4) or (len(shape) == 4 and shape[1] != 1):
@@ -1463,7 +1480,7 @@ def pool_decode(q, pool: KVPool, lens, block_table, *, scale=None, window: int =
     rc = lib().zkv_pool_decode(q3.data_ptr(), stride[0], stride[1], code, pool.ref, lens.data_ptr(),
                                block_table.data_ptr(), ld, width, B, Hq, D ** -0.5 if scale is None else scale, window,
                                softcap, max_len, out.data_ptr(), None if lse is None else lse.data_ptr(),
-                               None if status is None else status.data_ptr(), ws, ws_bytes, _raw_stream(dev))
+                               pool.status_at if status is None else status.data_ptr(), ws, ws_bytes, _raw_stream(dev))
     if rc:
         check(rc, "zkv_pool_decode")
     return (out, lse) if return_lse else out
