@@ -927,9 +927,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<kQ, kF8, D, NT>::kPerSm)
                 }
             }
         }
-        if (!ok)  // a consumer gave up: the copies on their way land in this CTA's memory, so wait for them
-            for (int i = max(0, done - stages); i < done; ++i)
-                wait_for(full + i % stages, (uint32_t)((i / stages) & 1), a.status);
+        // a consumer may have given up: the copies on their way land in this CTA's memory, so it does not end before them
+        for (int i = max(0, done - stages); i < done; ++i)
+            wait_for(full + i % stages, (uint32_t)((i / stages) & 1), a.status);
         return;
     }
 
