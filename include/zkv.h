@@ -739,7 +739,7 @@ int zkv_pool_release(const uint8_t* done, const int32_t* lens, int batch, int bl
  * (block slots[i] / S, token slots[i] % S) of every head = the source row, or
  * for e4m3 blocks e4m3(row / scale[head]), rounded to nearest even and
  * saturated at +-448.  Slot -1 is skipped; any other slot outside the pool
- * too, with ZKV_ERR_RANGE.  Two tokens with one slot: either row may stay.
+ * too, with ZKV_ERR_RANGE.  Two tokens with one slot leave a mix of their rows.
  *   k, v  element (i, h, d) at i*token + h*head + d, 16-byte rows; `dtype`
  *   bf16 or fp16, the pool's own type unless the pool is e4m3             */
 int zkv_pool_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
@@ -752,8 +752,12 @@ int zkv_pool_write(const void* k, int64_t k_token, int64_t k_head, const void* v
  *   of cap(scale q . k_t),  cap(x) = softcap tanh(x / softcap) (0: x);
  *   window 0: every token.  lse = log of the sum of exponentials (natural).
  * A request without tokens gives out 0 and lse -inf.  Rows past `len` may
- * hold anything.  fp32 inside; the split over a long cache is decided on the
- * GPU from the lengths, and the parts are joined in a fixed order.
+ * hold anything; a V element of an attended token that is not finite leaves
+ * its dim of the output not finite, NaN perhaps where an infinity is due.
+ * fp32 inside but for the probabilities in the second product: 16 bits or
+ * more of each, 11 over e4m3 blocks with a bf16 query.  The split over a long
+ * cache is decided on the GPU from the lengths, and the parts are joined in a
+ * fixed order.
  *   q [batch][q_heads][head_dim] at b*q_row + j*q_head (16-byte rows), `dtype`
  *   bf16 or fp16, the pool's own type unless the pool is e4m3; out dense in
  *   `dtype`; lse [batch][q_heads] fp32 or NULL

@@ -28,9 +28,10 @@
 //    and O^T += V^T P^T (dims x heads) by mma.sync m16n8k16, so a group of up
 //    to 8 heads fills the 8 columns of one product, 16 heads two.  More heads
 //    are cut into chunks, whose CTAs walk the same range side by side, so that
-//    K and V come from HBM once and from L2 again.  tcgen05 needs 64 or 128
-//    rows of M per product and TMEM round trips for the softmax of a 16-token
-//    tile; at 4-16 heads and an HBM-bound tile it has nothing to win here.
+//    K and V come from HBM once and from L2 again.  Up to 8 heads the bytes
+//    bound the kernel with the tensor pipe active 15-19 % of the time, so
+//    tcgen05 (tokens as M, heads as N, the probabilities through shared
+//    memory) has nothing to win there; for many heads it was not tried.
 //  * A tile is 16 KiB of K (32 for 512-byte rows): what bounds a warp is the
 //    latency of its chain product - maximum - exponential - product, so rows of
 //    128 bytes get 32 tokens a warp and chain instead of 16, rows of 64 get 64
@@ -160,7 +161,10 @@ struct Cfg {
     static constexpr int kStages = kRow == 256 && !kF8 && NT == 1 ? 2 : kFit < kMaxStages ? kFit : kMaxStages;
     static constexpr int kRing = 233472 / kPerSm - kOther - kFixed - kMl;  // bytes of a ring at most
     static constexpr int smem_of(int ring) { return ring + kFixed + kMl; }
-    static constexpr bool kTwoParts = !(kF8 && kQ == ZKV_DT_BF16);  // the probability as hi + lo
+    // The probability as hi + lo, or hi alone over e4m3 blocks with bf16 output: 11 bits under a result of 8, whose error
+    // against 64 bits stays the same to three digits.  32 requests of 8192, one part and two: 8 kv heads of 128 with 4 heads
+    // each 92.9 and 93.9 us, 4 of 128 with 16 60.1 and 68.2, 4 of 256 with 16 142 and 151.
+    static constexpr bool kTwoParts = !(kF8 && kQ == ZKV_DT_BF16);
     static constexpr int kMTiles = D / 16;
     // n-tiles of O that fit into a stage's K and V when the warps are joined
     static constexpr int kJoinTiles = (2 * kKv) / (kConsumers * 8 * D * 4) < NT ? (2 * kKv) / (kConsumers * 8 * D * 4) : NT;
