@@ -66,3 +66,33 @@ def test_small_query_elements_over_fp8(lens, G, small):
     scale = 0.004 / small
     out, lse = ops.pool_decode(q, ops.KVPool(k, v), i32(lens), table, scale=scale, return_lse=True)
     check_decode(q, k, v, None, None, lens, table, out, lse, scale)
+
+
+@pytest.mark.parametrize("qt,pt", [(BF, BF), (HF, HF), (BF, F8), (HF, F8)])
+@pytest.mark.parametrize("shape", list(SHAPES))
+def test_scores_of_any_size(shape, qt, pt):
+    """One token a request scores 2^20 to 2^30, the others 0, or as much below 0: its V row is the output, bit for bit, and
+    its score, a power of two, the lse (1.4427 times which rounds by 2^-24, and back)."""
+    lens, spare, bound = SHAPES[shape]
+    S, D, G = 16, 128, 4
+    n_blocks = sum(-(-n // S) for n in lens)
+    g = gen(5)
+    k = torch.zeros(n_blocks, S, 1, D, device=DEV)
+    v = narrow(torch.randn(n_blocks, S, 1, D, generator=g, device=DEV), pt)
+    table = make_table(6, lens, S, n_blocks, -(-max(lens) // S) + spare)
+    at = torch.tensor([n * 2 // 3 for n in lens], device=DEV)
+    block = table[torch.arange(len(lens), device=DEV), at // S].long()
+    for sign in (1.0, -1.0):
+        if sign > 0:
+            k[block, at % S] = 8.0
+        else:
+            k.fill_(-8.0)
+            k[block, at % S] = 0.0
+        q = torch.full((len(lens), G, D), 1024.0, device=DEV).to(qt)     # scale times 2^(10 + 3 + 7)
+        pool = ops.KVPool(narrow(k, pt), v)
+        want = v.float()[block, at % S].to(qt).expand(len(lens), G, D)
+        for power in range(11):
+            out, lse = ops.pool_decode(q, pool, i32(lens), table, scale=2.0 ** power, max_len=bound, return_lse=True)
+            assert torch.equal(out, want), (sign, power)
+            score = 2.0 ** (20 + power) if sign > 0 else 0.0
+            assert bool(((lse - score).abs() <= 2.0 ** -22 * score).all()), (sign, power)

@@ -382,8 +382,9 @@ template <int kQ, bool kF8, int D, int NT>
 struct Row {
     using C = Cfg<kQ, kF8, D, NT>;
     static constexpr bool kMmaBf16 = kQ == ZKV_DT_BF16 && !kF8;
-    // exponentials are 2^kLift of themselves: o and a lane's l too, while the warp's total and what it puts are not
-    static constexpr float kLift = kMmaBf16 ? 0.f : 15.f, kDown = kMmaBf16 ? 1.f : 1.f / 32768;
+    // Exponentials are kLift of themselves, o and a lane's l too; the warp's total and what it puts are not.  By a product:
+    // 15 taken off the maximum rounds to 16 or 0 where scores pass 2^24, and 2^16 is infinite in fp16.
+    static constexpr float kLift = kMmaBf16 ? 1.f : 32768.f, kDown = 1.f / kLift;
     float m[NT][2], l[NT][2];   // log2 units; heads 2t, 2t+1 of n-tile (t = lane % 4); l: this lane's tokens
     float f[NT][2];             // score factor of those heads, log2 units (under a soft cap, natural ones of it)
     float o[C::kMTiles][NT][4];
@@ -611,11 +612,10 @@ struct Row {
                 moved |= mx[c] != m[n][c];
                 m[n][c] = mx[c];
                 float sum = 0.f;
-                const float from = ref - kLift;
 #pragma unroll
                 for (int i = 0; i < kSub; ++i) {
-                    x[i][n][c] = exp2_fast(x[i][n][c] - from);
-                    x[i][n][c + 2] = exp2_fast(x[i][n][c + 2] - from);
+                    x[i][n][c] = kLift * exp2_fast(x[i][n][c] - ref);
+                    x[i][n][c + 2] = kLift * exp2_fast(x[i][n][c + 2] - ref);
                     sum += x[i][n][c] + x[i][n][c + 2];
                 }
                 l[n][c] = l[n][c] * alpha[n][c] + sum;
