@@ -104,3 +104,22 @@ def test_released_places_serve_the_hooks_again():
         cache.release(torch.tensor([True, True], device=DEV))
     cache.check()
     assert cache.lens.tolist() == [0, 0] and int(cache.n_free) == cache.n_blocks
+
+
+def test_the_hooks_know_of_replayed_plans():
+    """Replays fill the cache without the host: the next hook has to look, not to trust its bound."""
+    cache = PoolCache(1, 1, 1, 64, 64)
+    x = rows(7, 1, 1, 1, 64)
+    cache.decode_update_kv_cache(x, x, 0)
+    cache.release(torch.tensor([True], device=DEV), bound=0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.decode_update_kv_cache(x, x, 0)
+    for _ in range(63):
+        graph.replay()
+    cache.decode_update_kv_cache(x, x, 0)              # the last place
+    assert cache.lens.tolist() == [64]
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        cache.decode_update_kv_cache(x, x, 0)
+    cache.check()

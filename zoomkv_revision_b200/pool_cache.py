@@ -58,6 +58,7 @@ class PoolCache:
         self.n_free = torch.full((1,), self.n_blocks, **ints)
         self.status = torch.zeros(1, **ints)
         self.bound = 0                       # no request is longer, as far as the host knows (a replayed plan does not tell it)
+        self.captured = False                # a plan was: replays may have moved the lengths
         self.slots = None                    # of the step that is being written
 
     # ------------------------------------------------------------------ a serving step
@@ -70,6 +71,7 @@ class PoolCache:
         if max_new is None:
             max_new = 1 if new_lens is None else n_slots
         self.bound = min(self.bound + max_new, self.width * self.block_size)
+        self.captured |= torch.cuda.is_current_stream_capturing()
         self.slots = slots
         return slots
 
@@ -101,12 +103,14 @@ class PoolCache:
     # ------------------------------------------------------------------ hooks of the decode loop
     def _make_room(self, new: int) -> None:
         """Raises if `new` more tokens of every request do not fit: the loop's caller has no status to look at.  Where the
-        host's bound leaves a doubt the GPU is asked, and the bound is what it says; not in a graph capture, whose replays
-        only `check` can judge."""
+        host's bound leaves a doubt, or a captured plan may have been replayed, the GPU is asked, and the bound is what it
+        says; not in a graph capture, whose replays only `check` can judge."""
         def blocks(n):
             return -(-n // self.block_size)
 
-        if blocks(self.bound + new) <= min(self.width, self.n_blocks // self.batch) or torch.cuda.is_current_stream_capturing():
+        if not self.captured and blocks(self.bound + new) <= min(self.width, self.n_blocks // self.batch):
+            return
+        if torch.cuda.is_current_stream_capturing():
             return
         lens, n_free = self.lens.tolist(), int(self.n_free.item())
         self.bound = max(lens)
