@@ -682,6 +682,7 @@ int zkv_peer_set_wait_ms(int ms);
 #define ZKV_DT_BF16 0
 #define ZKV_DT_F16 1
 #define ZKV_DT_F8E4M3 2 /* pool blocks only: value = stored * scale of its kv head */
+#define ZKV_DT_F32 3    /* outputs of zkv_fp8_linear only                          */
 
 typedef struct zkv_pool {
     void* k;                            /* element (block i, token t, head h, dim d) at      */
@@ -776,6 +777,68 @@ int zkv_pool_decode(const void* q, int64_t q_row, int64_t q_head, int dtype, con
                     const int32_t* lens, const int32_t* block_table, int64_t table_ld, int width, int batch,
                     int q_heads, float scale, int window, float softcap, int64_t max_len, void* out, float* lse,
                     int32_t* status, void* workspace, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------ 8-bit layers */
+
+/* A decoder layer's dense half in e4m3 with fp32 scales for blocks of 128 (no
+ * reference counterpart: the reference's layers are 16-bit, model_hub/qwen.py:
+ * 429-612).  A row of n elements has ceil(n / 128) blocks of 128 consecutive
+ * elements, the last perhaps shorter; element = stored * scale of its block.
+ * Block scales lie anywhere: token i, block b at i * scale_token + b *
+ * scale_block (elements); scale_token 1 is what the kernels read best.
+ *
+ * Quantising a block: scale = amax / 448 (fp32), stored = e4m3(fp32(x /
+ * scale)), both to nearest even; zeros where the scale is 0.  A block that
+ * holds an infinity or NaN reads back as NaN.
+ *   x     [tokens][dim] bf16 or fp16 (`dtype`), row i at i * x_ld
+ *   out   [tokens][dim] e4m3, row i at i * out_ld bytes
+ * dim a multiple of 16; rows start on 16 bytes.  Outputs overlap neither one
+ * another nor an input.                                                    */
+int zkv_quant_fp8(const void* x, int64_t x_ld, int dtype, int64_t tokens, int dim, void* out, int64_t out_ld,
+                  float* scale, int64_t scale_token, int64_t scale_block, void* stream);
+
+/* r = x + residual, rounded to their type and written to residual_out (which
+ * may be residual or x, with its row stride; both NULL: r = x), and the quantised RMSNorm
+ *   y = r * rsqrt(mean(r^2) + eps) * w      in fp32, not rounded before it is quantised.
+ * w [dim] of x's type.  dim <= 32768.                                      */
+int zkv_rmsnorm_fp8(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, void* residual_out,
+                    int64_t residual_out_ld, const void* w, int dtype, int64_t tokens, int dim, float eps, void* out,
+                    int64_t out_ld, float* scale, int64_t scale_token, int64_t scale_block, void* stream);
+
+/* A weight matrix [rows][k] in e4m3 with a scale for each block of 128 x 128,
+ * or two of one shape after one another (a gated block's gate and up halves,
+ * parts = 2: part p's row n at w + (p * rows + n) * ld), each with blocks of
+ * its own: scale [parts * ceil(rows / 128)][ceil(k / 128)].  k a multiple of
+ * 16, rows too where parts is 2.                                           */
+typedef struct zkv_fp8_weight {
+    const void* w;
+    const float* scale;
+    int64_t ld;       /* bytes from row to row, a multiple of 16            */
+    int64_t rows, k;  /* of one part                                        */
+    int64_t parts;    /* 1 or 2                                             */
+    uint64_t map[16]; /* tensor map of w, filled by zkv_fp8_weight_init      */
+} zkv_fp8_weight;
+
+/* Checks the fields of `w` and fills `map` (host only, no launch).  To be
+ * called once per weight, and again when a field above `map` changes.      */
+int zkv_fp8_weight_init(zkv_fp8_weight* w);
+
+/* out[i][n] = sum over blocks b of x_scale[i][b] * w.scale[n / 128][b] * (sum
+ * of the block's products), for w of one part.  Products and sums in fp32,
+ * one rounding to `dtype` (bf16, fp16 or fp32) at the end; the inner
+ * dimension may be summed in parts, joined in a fixed order.
+ *   x [tokens][k] e4m3, row i at i * x_ld bytes (16-byte rows)
+ *   out [tokens][rows], row i at i * out_ld elements
+ * `status` (may be NULL) gets ZKV_ERR_TIMEOUT for a wait that ran out.     */
+int zkv_fp8_linear(const void* x, int64_t x_ld, const float* x_scale, int64_t xs_token, int64_t xs_block, int64_t tokens,
+                   const zkv_fp8_weight* w, void* out, int64_t out_ld, int dtype, int32_t* status, void* stream);
+
+/* silu(g) * u, quantised in blocks of 128 features: g and u as
+ * zkv_fp8_linear gives them for the two parts of w, in fp32.
+ *   out [tokens][rows] e4m3, row i at i * out_ld bytes (16-byte rows)      */
+int zkv_fp8_swiglu(const void* x, int64_t x_ld, const float* x_scale, int64_t xs_token, int64_t xs_block, int64_t tokens,
+                   const zkv_fp8_weight* w, void* out, int64_t out_ld, float* out_scale, int64_t os_token,
+                   int64_t os_block, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

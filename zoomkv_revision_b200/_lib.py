@@ -82,6 +82,12 @@ class ZkvPool(ctypes.Structure):
                 ("v_scale", _c_void_p), ("maps", ctypes.c_uint64 * 32)]
 
 
+class ZkvFp8Weight(ctypes.Structure):
+    """Mirror of `zkv_fp8_weight` (include/zkv.h)."""
+    _fields_ = [("w", _c_void_p), ("scale", _c_void_p), ("ld", _i64), ("rows", _i64), ("k", _i64), ("parts", _i64),
+                ("map", ctypes.c_uint64 * 16)]
+
+
 _RQ = ctypes.POINTER(ZkvRqLayout)
 
 # name -> argtypes (restype is int status unless noted)
@@ -170,6 +176,14 @@ _SIGNATURES = {
     "zkv_pool_decode_ws_bytes": [_c_void_p, _i32, _i32, _i32, _i64],
     "zkv_pool_decode": [_c_void_p, _i64, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _i32, _f32,
                         _i32, _f32, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p],
+    "zkv_quant_fp8": [_c_void_p, _i64, _i32, _i64, _i32, _c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p],
+    "zkv_rmsnorm_fp8": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i32, _i64, _i32, _f32, _c_void_p,
+                        _i64, _c_void_p, _i64, _i64, _c_void_p],
+    "zkv_fp8_weight_init": [_c_void_p],
+    "zkv_fp8_linear": [_c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i32, _c_void_p,
+                       _c_void_p],
+    "zkv_fp8_swiglu": [_c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64,
+                       _c_void_p, _c_void_p],
     "zkv_version": [],
     "zkv_status_string": [_i32],
 }

@@ -1,0 +1,37 @@
+// zkv_fp8.cuh -- what the 8-bit kernels share: e4m3 with an fp32 scale for
+// each block of 128 elements.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "zkv_common.cuh"
+
+namespace zkv {
+namespace fp8 {
+
+constexpr int kBlock = 128;      // elements of a row that share a scale
+constexpr float kMax = 448.f;    // largest e4m3 value
+
+static inline int blocks_of(int64_t n) { return (int)((n + kBlock - 1) / kBlock); }
+static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The scale of a block from the bits of its largest magnitude.  Magnitudes
+// are compared as integers, so that a NaN counts as larger than an infinity
+// and neither is lost: the block then reads back as NaN.
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ float scale_of(uint32_t largest) { return __fdiv_rn(__uint_as_float(largest), kMax); }
+
+// e4m3 of the fp32 quotient, two roundings as defined; a block of zeros, or
+// one so small that its scale is 0, is stored as zeros.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float scale) {
+    if (scale == 0.f) return 0u;
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(a, scale), __fdiv_rn(b, scale)), __NV_SATFINITE,
+                                                 __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(c, scale), __fdiv_rn(d, scale)), __NV_SATFINITE,
+                                                 __NV_E4M3);
+    return lo | (hi << 16);
+}
+
+}  // namespace fp8
+}  // namespace zkv

@@ -33,6 +33,8 @@ coarse_2bit_score_cuda                 cache_hub/rerank/rerank.py:636-690
 rq_popcount_topk                       (1-bit x 4-bit popcount rerank + exact IP; no counterpart)
 KVPool / pool_plan / pool_write /      (pooled KV cache with block tables, requests of their own lengths;
 pool_decode / pool_release             no counterpart)
+quant_fp8 / rmsnorm_fp8 / Fp8Weight /  (a layer's dense half in e4m3 with block scales; no counterpart: the
+fp8_linear / fp8_swiglu                reference's layers are 16-bit, model_hub/qwen.py:429-612)
 =====================================  ==============================================
 
 Errors follow the reference: wrong dtype -> TypeError, wrong shape / range ->
@@ -58,6 +60,7 @@ __all__ = [
     "PageLayer", "page_attend", "RawLayer", "page_decode_raw", "page_decode_raw_ws_bytes", "gqa_mean", "reference_select", "reference_select_ws_bytes", "RqLayout", "rq_encode", "batch_encode", "rq_query", "get_cache_cnt_fused", "collision_topk",
     "partial_rerank_cuda", "coarse_2bit_score_cuda", "rq_popcount_topk", "MAG_CENTERS", "MAG_THRESHOLDS",
     "KVPool", "pool_plan", "pool_release", "pool_write", "pool_decode", "pool_decode_ws_bytes",
+    "quant_fp8", "rmsnorm_fp8", "Fp8Weight", "fp8_linear", "fp8_swiglu",
 ]
 
 
@@ -1498,3 +1501,293 @@ def pool_decode_ws_bytes(batch: int, q_heads: int, pool: KVPool, width: int, max
             pool.ws_sizes.clear()
         pool.ws_sizes[key] = got
     return got
+
+
+# ----------------------------------------------------------------- 8-bit layers
+_F8 = torch.float8_e4m3fn
+_F32 = torch.float32
+_OUT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 3}
+_QUANT_BLOCK = 128
+
+
+def _fp8_in(name, t, el):
+    """(t, rows, last dim, row stride) of rows [..., dim] that start on 16 bytes (a copy where they do not)."""
+    shape = t.shape
+    if not shape:
+        raise ValueError(f"{name} must have rows")
+    dim = shape[-1]
+    if t.is_contiguous():
+        rows, ld = t.numel() // dim if dim else 0, dim
+    elif len(shape) == 2 and t.stride(1) == 1 and t.stride(0) >= dim:
+        rows, ld = shape[0], t.stride(0)
+    else:
+        t = t.contiguous()
+        rows, ld = t.numel() // dim if dim else 0, dim
+    if (t.data_ptr() | ld * el) & 15:
+        if dim * el & 15:
+            raise ValueError(f"{name}: the last dim must be a multiple of 16; got {dim}")
+        t, ld = t.clone(memory_format=torch.contiguous_format), dim
+    return t, rows, dim, ld
+
+
+def _fp8_out(name, t, shape, dtype, dev, whole=True):
+    """The row stride of an output like `shape` (whole: its rows start on 16 bytes)."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}; got {t.dtype}")
+    if t.shape != shape or t.get_device() != dev:
+        raise ValueError(f"{name} must be {tuple(shape)} on the device of x; got {tuple(t.shape)}")
+    dim = shape[-1]
+    if t.is_contiguous():
+        ld = dim
+    elif len(shape) == 2 and t.stride(1) == 1 and t.stride(0) >= dim:
+        ld = t.stride(0)
+    else:
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+    if whole and (t.data_ptr() | ld * t.element_size()) & 15:
+        raise ValueError(f"{name} must have rows that start on 16 bytes")
+    return ld
+
+
+def _row_scales(name, t, rows, blocks, dev, out):
+    """(token stride, block stride) of fp32 [rows, blocks] scales."""
+    if t.dtype is not _F32:
+        raise TypeError(f"{name} must be torch.float32; got {t.dtype}")
+    if t.shape != (rows, blocks) or t.get_device() != dev:
+        raise ValueError(f"{name} must be [{rows}, {blocks}] on the device of x; got {tuple(t.shape)}")
+    token, block = t.stride()
+    if out:
+        if rows <= 1:
+            token = blocks * block
+        if blocks <= 1:
+            block = rows * token
+        if not ((block >= 1 and token >= blocks * block) or (token >= 1 and block >= rows * token)):
+            raise ValueError(f"{name} must not overlap itself")
+    return token, block
+
+
+def _new_scales(like, rows, blocks):
+    """Uninitialised scales [rows, blocks], block-major in memory as the products read them best."""
+    return torch.empty(blocks, rows, dtype=_F32, device=like.device).t()
+
+
+def quant_fp8(x, *, out=None, scale=None):
+    """x [..., dim] bf16 or fp16 to e4m3 with an fp32 scale for each block of
+    128 elements of a row (the last perhaps shorter): scale = amax / 448,
+    stored = e4m3(x / scale), zeros where the scale is 0.  A block that holds
+    an infinity or NaN reads back as NaN.  dim a multiple of 16.  Returns
+    (out like x, scale [rows, ceil(dim / 128)]); out and scale may be given,
+    scale with any strides, by default block-major in memory."""
+    code = _OUT_DTYPES.get(x.dtype, 3)
+    if code == 3:
+        raise TypeError(f"x must be bfloat16 or float16; got {x.dtype}")
+    dev = x.get_device()
+    if dev < 0:
+        raise ValueError("x must be a CUDA tensor")
+    x, rows, dim, ld = _fp8_in("x", x, 2)
+    blocks = -(-dim // _QUANT_BLOCK)
+    if out is None:
+        out = torch.empty(x.shape, dtype=_F8, device=x.device)
+    out_ld = _fp8_out("out", out, x.shape, _F8, dev)
+    if scale is None:
+        scale = _new_scales(x, rows, blocks)
+    st, sb = _row_scales("scale", scale, rows, blocks, dev, True)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return quant_fp8(x, out=out, scale=scale)
+    if rows:
+        rc = lib().zkv_quant_fp8(x.data_ptr(), ld, code, rows, dim, out.data_ptr(), out_ld, scale.data_ptr(), st, sb,
+                                 _raw_stream(dev))
+        if rc:
+            check(rc, "zkv_quant_fp8")
+    return out, scale
+
+
+def rmsnorm_fp8(x, w, eps: float, *, residual=None, residual_out=None, out=None, scale=None):
+    """RMSNorm of r = x + residual (x alone without one) in e4m3 with block
+    scales, as quant_fp8 of r * rsqrt(mean(r^2) + eps) * w in fp32.  x,
+    residual [..., dim] and w [dim] bf16 or fp16, one type.  r is rounded to
+    that type and kept in residual_out (default: residual, in place).
+    Returns (out, scale) as quant_fp8 does."""
+    dt = x.dtype
+    code = _OUT_DTYPES.get(dt, 3)
+    if code == 3:
+        raise TypeError(f"x must be bfloat16 or float16; got {dt}")
+    dev = x.get_device()
+    if dev < 0:
+        raise ValueError("x must be a CUDA tensor")
+    x, rows, dim, ld = _fp8_in("x", x, 2)
+    if w.dtype is not dt:
+        raise TypeError(f"w must be {dt}; got {w.dtype}")
+    if w.shape != (dim,) or w.get_device() != dev or not w.is_contiguous():
+        raise ValueError(f"w must be contiguous [{dim}] on the device of x")
+    if w.data_ptr() & 15:
+        w = w.clone()
+    res, res_ld, to, to_ld = None, 0, None, 0
+    if residual is not None:
+        if residual_out is None:
+            residual_out = residual
+        to_ld = _fp8_out("residual_out", residual_out, x.shape, dt, dev)
+        to = residual_out.data_ptr()
+        if residual is residual_out:
+            res, res_ld = to, to_ld
+        else:
+            if residual.dtype is not dt:
+                raise TypeError(f"residual must be {dt}; got {residual.dtype}")
+            if residual.shape != x.shape or residual.get_device() != dev:
+                raise ValueError(f"residual must be {tuple(x.shape)} on the device of x; got {tuple(residual.shape)}")
+            residual, _, _, res_ld = _fp8_in("residual", residual, 2)
+            res = residual.data_ptr()
+    elif residual_out is not None:
+        raise ValueError("residual_out belongs to a residual")
+    blocks = -(-dim // _QUANT_BLOCK)
+    if out is None:
+        out = torch.empty(x.shape, dtype=_F8, device=x.device)
+    out_ld = _fp8_out("out", out, x.shape, _F8, dev)
+    if scale is None:
+        scale = _new_scales(x, rows, blocks)
+    st, sb = _row_scales("scale", scale, rows, blocks, dev, True)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return rmsnorm_fp8(x, w, eps, residual=residual, residual_out=residual_out, out=out, scale=scale)
+    if rows:
+        rc = lib().zkv_rmsnorm_fp8(x.data_ptr(), ld, res, res_ld, to, to_ld, w.data_ptr(), code, rows, dim, eps,
+                                   out.data_ptr(), out_ld, scale.data_ptr(), st, sb, _raw_stream(dev))
+        if rc:
+            check(rc, "zkv_rmsnorm_fp8")
+    return out, scale
+
+
+class Fp8Weight:
+    """A product's weight matrix w [n, k] float8_e4m3fn with a scale for each
+    block of 128 x 128: scale [ceil(n / 128), ceil(k / 128)] fp32, element =
+    stored * scale.  parts = 2: the gate and up halves of a gated block, w
+    [2 f, k] with the gate's rows first, each half with blocks of its own:
+    scale [2 ceil(f / 128), ceil(k / 128)].  k a multiple of 16, f too.  Made
+    once when the weights are loaded: it holds the tensors, their addresses
+    and a status word (see check)."""
+
+    __slots__ = ("w", "scale", "parts", "rows", "k", "device", "index", "struct", "ref", "status", "status_at")
+
+    def __init__(self, w, scale, parts: int = 1):
+        _cuda(("w", w), ("scale", scale))
+        _dtype("w", w, _F8)
+        _dtype("scale", scale, _F32)
+        if parts not in (1, 2):
+            raise ValueError(f"parts must be 1 or 2; got {parts}")
+        if w.dim() != 2 or w.shape[0] % parts or not w.numel():
+            raise ValueError(f"w must be [n, k], n a multiple of parts; got {tuple(w.shape)}")
+        n, k = w.shape[0] // parts, w.shape[1]
+        if k % 16 or (parts == 2 and n % 16):
+            raise ValueError(f"k (and f of two parts) must be multiples of 16; got {tuple(w.shape)}")
+        want = (parts * -(-n // _QUANT_BLOCK), -(-k // _QUANT_BLOCK))
+        if tuple(scale.shape) != want or not scale.is_contiguous() or scale.device != w.device:
+            raise ValueError(f"scale must be contiguous {want} on the device of w; got {tuple(scale.shape)}")
+        if w.stride(1) != 1 or (w.shape[0] > 1 and w.stride(0) < k):
+            raise ValueError("w must have contiguous rows that do not overlap")
+        self.w, self.scale, self.parts, self.rows, self.k = w, scale, parts, n, k
+        self.device, self.index = w.device, w.get_device()
+        self.struct = _lib.ZkvFp8Weight(_p(w), _p(scale), w.stride(0) if w.shape[0] > 1 else k, n, k, parts)
+        self.ref = ctypes.addressof(self.struct)
+        check(lib().zkv_fp8_weight_init(self.ref), "zkv_fp8_weight_init")
+        self.status = torch.zeros(1, dtype=_INT32, device=w.device)
+        self.status_at = self.status.data_ptr()
+
+    @classmethod
+    def quantize(cls, w, parts: int = 1):
+        """The handle of 16- or 32-bit weights [n, k]: scale = amax / 448 of a block, stored = e4m3(w / scale).  For
+        loading: elementary operations, 16384 rows at a time."""
+        if w.dim() != 2 or w.shape[0] % parts:
+            raise ValueError(f"w must be [n, k], n a multiple of parts; got {tuple(w.shape)}")
+        n, k = w.shape[0] // parts, w.shape[1]
+        nb, kb, S = -(-n // _QUANT_BLOCK), -(-k // _QUANT_BLOCK), _QUANT_BLOCK
+        q = torch.empty(w.shape, dtype=_F8, device=w.device)
+        scale = torch.empty(parts * nb, kb, dtype=_F32, device=w.device)
+        for p in range(parts):
+            for r in range(0, n, 16384):
+                rows = min(16384, n - r)
+                tile = torch.zeros(-(-rows // S) * S, kb * S, dtype=_F32, device=w.device)
+                tile[:rows, :k] = w[p * n + r: p * n + r + rows]
+                tile = tile.view(-1, S, kb, S)
+                amax = tile.abs().amax(dim=(1, 3))
+                s = amax / torch.full_like(amax, 448.0)
+                scale[p * nb + r // S: p * nb + r // S + s.shape[0]] = s
+                s = s[:, None, :, None]
+                x = torch.where(s == 0, torch.zeros_like(tile), tile / s).clamp(-448.0, 448.0)
+                q[p * n + r: p * n + r + rows] = x.view(-1, kb * S)[:rows, :k].to(_F8)
+        return cls(q, scale, parts)
+
+    def dequantize(self):
+        """The weights as fp32 [n, k] (parts after one another)."""
+        n, S = self.rows, _QUANT_BLOCK
+        at = torch.arange(n, device=self.device) // S
+        at = torch.cat([at + p * -(-n // S) for p in range(self.parts)])
+        return self.w.float() * self.scale[at].repeat_interleave(S, 1)[:, : self.k]
+
+    def check(self) -> None:
+        """Raises if a wait inside a product with this weight ran out since the last check (waits for the GPU)."""
+        code = int(self.status.item())
+        if code:
+            self.status.zero_()
+            check(code, "8-bit product")
+
+
+def _fp8_product(x, x_scale, weight, parts):
+    """(x, rows, row stride, token stride, block stride of the scales) of a product's input."""
+    if x.dtype is not _F8:
+        raise TypeError(f"x must be float8_e4m3fn; got {x.dtype}")
+    if weight.parts != parts:
+        raise ValueError(f"the weight must have {parts} part(s); it has {weight.parts}")
+    if not x.shape or x.shape[-1] != weight.k or x.get_device() != weight.index:
+        raise ValueError(f"x must be [..., {weight.k}] on the weight's device; got {tuple(x.shape)}")
+    x, rows, dim, ld = _fp8_in("x", x, 1)
+    st, sb = _row_scales("x_scale", x_scale, rows, -(-dim // _QUANT_BLOCK), weight.index, False)
+    return x, rows, ld, st, sb
+
+
+def fp8_linear(x, x_scale, weight: Fp8Weight, *, out=None, dtype=torch.bfloat16):
+    """x [..., k] e4m3 with x_scale [rows, ceil(k / 128)] (of quant_fp8 or
+    rmsnorm_fp8, or any fp32 scales for blocks of 128, any strides) times
+    weight^T: out [..., n] bf16, fp16 or fp32 (`dtype`, or that of the given
+    out).  Sums in fp32, one rounding at the end."""
+    x, rows, ld, st, sb = _fp8_product(x, x_scale, weight, 1)
+    dev = weight.index
+    if out is None:
+        out = torch.empty(*x.shape[:-1], weight.rows, dtype=dtype, device=weight.device)
+    code = _OUT_DTYPES.get(out.dtype)
+    if code is None:
+        raise TypeError(f"out must be bfloat16, float16 or float32; got {out.dtype}")
+    out_ld = _fp8_out("out", out, x.shape[:-1] + (weight.rows,), out.dtype, dev, False)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return fp8_linear(x, x_scale, weight, out=out)
+    if rows:
+        rc = lib().zkv_fp8_linear(x.data_ptr(), ld, x_scale.data_ptr(), st, sb, rows, weight.ref, out.data_ptr(), out_ld,
+                                  code, weight.status_at, _raw_stream(dev))
+        if rc:
+            check(rc, "zkv_fp8_linear")
+    return out
+
+
+def fp8_swiglu(x, x_scale, weight: Fp8Weight, *, out=None, scale=None):
+    """silu(g) * u in e4m3 with block scales: g and u are x (as in fp8_linear)
+    times the two parts of `weight`, in fp32, and what is stored is quant_fp8
+    of their product without a rounding in between.  Returns (out [..., f],
+    scale [rows, ceil(f / 128)])."""
+    x, rows, ld, st, sb = _fp8_product(x, x_scale, weight, 2)
+    dev = weight.index
+    if out is None:
+        out = torch.empty(*x.shape[:-1], weight.rows, dtype=_F8, device=weight.device)
+    out_ld = _fp8_out("out", out, x.shape[:-1] + (weight.rows,), _F8, dev)
+    blocks = -(-weight.rows // _QUANT_BLOCK)
+    if scale is None:
+        scale = _new_scales(x, rows, blocks)
+    ot, ob = _row_scales("scale", scale, rows, blocks, dev, True)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return fp8_swiglu(x, x_scale, weight, out=out, scale=scale)
+    if rows:
+        rc = lib().zkv_fp8_swiglu(x.data_ptr(), ld, x_scale.data_ptr(), st, sb, rows, weight.ref, out.data_ptr(), out_ld,
+                                  scale.data_ptr(), ot, ob, weight.status_at, _raw_stream(dev))
+        if rc:
+            check(rc, "zkv_fp8_swiglu")
+    return out, scale
