@@ -996,7 +996,7 @@ uint64_t peer_wait_ns();
 // it, so the largest one set is kept for all threads (per source file, as the
 // kernels are).
 static bool raise_smem_limit(const void* fn, size_t smem) {
-    constexpr int kFns = 8, kDevs = 64;
+    constexpr int kFns = 16, kDevs = 64;
     static std::mutex mutex;
     static const void* fns[kFns] = {};
     static size_t set[kFns][kDevs] = {};

@@ -303,6 +303,349 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
     }
 }
 
+// ------------------------------------------------------------ many tokens
+// Tokens are the matrix rows: 256 of them and 256 features a tile (gated: 128
+// of each part), by a pair of CTAs whose tensor cores share the features'
+// operand, so that a CTA loads 32 KB for a block of the inner dimension
+// instead of 48 (96 bytes a clock at the full rate, more than L2 gives an SM).
+// A thread of the eight that read tensor memory has one token and 128
+// features in registers: both scales are its own, one packed product-and-sum
+// for two elements.  The two halves of tensor memory take the blocks in turn,
+// so that a tile's output is written while the next tile's first two blocks
+// are multiplied.
+template <bool kGated>
+struct Many {
+    static constexpr int kTokens = 256, kFeatures = 256;
+    // A warpgroup for the copies and products, two that read tensor memory, which take the registers that the first gives
+    // up: 128 x 64 + 256 x 208 of the 384 x 168 of the launch.
+    static constexpr int kThreads = 384;
+    static constexpr int kStages = kGated ? 6 : 5;
+    static constexpr int kStage = 2 * kTileBytes;  // 128 rows of tokens, 128 of features
+    static constexpr int kOut = (kGated ? 1 : 4) * kTileBytes;  // output staging; 16- and 32-bit: half for each warpgroup
+    static constexpr int kTop = kGated ? 1024 : 0;
+    // Scales come to shared memory a few blocks ahead, by a warp of their own: loaded one block ahead by the threads that
+    // use them, they took 1.1 us a block (4096 x 6144 x 4096: 220 us).
+    static constexpr int kSlots = kGated ? 4 : 3, kSlot = 528;  // 128 tokens, two of the weights
+    static constexpr int kSmem = 1024 + kStages * kStage + kOut + kTop + kSlots * kSlot + 256;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+struct ManyTiles {
+    int m, n;    // tiles of tokens and of features
+    int total;   // m * n
+    // Eight tiles of tokens by all tiles of features after one another: a wave reads few of either.
+    __device__ __forceinline__ void at(int t, int& tm, int& tn) const {
+        const int per = 8 * n, g = t / per, first = g * 8, high = min(8, m - first), r = t - g * per;
+        tm = first + r % high;
+        tn = r / high;
+    }
+};
+
+__device__ __forceinline__ void group_sync(int group) {
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+}
+
+// 16 bytes of row r of a swizzled tile of 128-byte rows.
+__device__ __forceinline__ uint32_t swizzled(uint32_t tile, int r, int chunk) {
+    return tile + r * 128 + ((chunk ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ void st_shared(uint32_t at, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ T ld_shared(uint32_t at) {
+    if (sizeof(T) == 2) {
+        uint16_t v;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+        return (T)v;
+    }
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return (T)v;
+}
+
+// One swizzled tile of 128 rows to an output whose rows do not start on 16 bytes: by a warpgroup, element by element.
+template <typename T>
+__device__ __forceinline__ void copy_out(const Product& a, uint32_t tile, int64_t token, int f, int columns) {
+    const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+    for (int r = warp; r < 128; r += 4) {
+        if (token + r >= a.tokens) break;
+        T* to = (T*)a.out + (token + r) * a.out_ld + f;
+        for (int c = lane; c < columns; c += 32) {
+            const int byte = c * (int)sizeof(T);
+            if (f + c < a.rows) to[c] = ld_shared<T>(swizzled(tile, r, byte >> 4) + (byte & 15));
+        }
+    }
+}
+
+template <bool kGated>
+__global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
+    many_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                const __grid_constant__ CUtensorMap out_map, Product a, ManyTiles tiles, bool mapped) {
+    using C = Many<kGated>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
+    uint8_t* const generic = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t out_at = base + C::kStages * C::kStage, top_at = out_at + C::kOut, slots = top_at + C::kTop,
+                   bars = slots + C::kSlots * C::kSlot;
+    const uint32_t full = bars, empty = full + 8 * C::kStages, sum_full = empty + 8 * C::kStages, sum_empty = sum_full + 16,
+                   slot_full = sum_empty + 16, slot_empty = slot_full + 8 * C::kSlots, tmem_at = slot_empty + 8 * C::kSlots;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = tc::cluster_rank();
+    const int n = a.k_blocks, pairs = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        auto bar = [&](uint32_t at) { return reinterpret_cast<uint64_t*>(generic + (at - base)); };
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(bar(full + 8 * i), 1);
+            mbar_init(bar(empty + 8 * i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(sum_full + 8 * i), 1);
+            mbar_init(bar(sum_empty + 8 * i), 16);  // 8 warps of both CTAs
+        }
+        for (int i = 0; i < C::kSlots; ++i) {
+            mbar_init(bar(slot_full + 8 * i), 32);
+            mbar_init(bar(slot_empty + 8 * i), 8);
+        }
+        mbar_fence_init();
+        tc::prefetch_map(&w_map);
+        tc::prefetch_map(&x_map);
+    }
+    if (warp == 1) tc::tmem_alloc_pair(tmem_at, 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::cluster_sync();  // both CTAs' barriers
+    tc::fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(generic + (tmem_at - base));
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+      if (warp == 0) {
+        if (lane == 0) {
+            const uint32_t leader = tc::in_cta(full, 0);
+            int got = 0;
+            bool ok = true;
+            for (int t = blockIdx.x >> 1; t < tiles.total && ok; t += pairs) {
+                int tm, tn;
+                tiles.at(t, tm, tn);
+                const int token = tm * C::kTokens + rank * 128;
+                for (int kb = 0; kb < n; ++kb, ++got) {
+                    const int s = got % C::kStages, turn = got / C::kStages;
+                    if (turn > 0 && !(ok = tc::wait_for(empty + 8 * s, (turn - 1) & 1, a.status))) break;
+                    const uint32_t at = base + s * C::kStage;
+                    if (rank == 0) tc::arrive_expect_tx(full + 8 * s, 2 * C::kStage);
+                    tc::tma_2d_pair(at, &x_map, kb * kBlock, token, leader + 8 * s);
+                    if (kGated)
+                        tc::tma_3d_pair(at + kTileBytes, &w_map, kb * kBlock, tn * kTile, (int)rank, leader + 8 * s);
+                    else
+                        tc::tma_3d_pair(at + kTileBytes, &w_map, kb * kBlock, (2 * tn + (int)rank) * kTile, 0, leader + 8 * s);
+                }
+            }
+            // both CTAs' copies have landed before either ends, whatever became of the others
+            if (rank == 0)
+                for (int i = got > C::kStages ? got - C::kStages : 0; i < got; ++i)
+                    if (!tc::wait_for(full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.status)) break;
+        }
+        __syncwarp();
+      } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t desc = tc::e4m3_desc(256, C::kFeatures);
+            int done = 0;
+            bool ok = true;
+            for (int t = blockIdx.x >> 1; t < tiles.total && ok; t += pairs) {
+                for (int kb = 0; kb < n; ++kb, ++done) {
+                    const int s = done % C::kStages, b = done & 1, turn = done >> 1;
+                    if (!(ok = tc::wait_for(full + 8 * s, (done / C::kStages) & 1, a.status))) break;
+                    if (turn > 0 && !(ok = tc::wait_for(sum_empty + 8 * b, (turn - 1) & 1, a.status))) break;
+                    tc::fence_after();
+                    const uint64_t x = tc::tile_desc(base + s * C::kStage), w = tc::tile_desc(base + s * C::kStage + kTileBytes);
+#pragma unroll
+                    for (int k = 0; k < kBlock / 32; ++k)
+                        tc::mma_e4m3_pair(tmem + b * C::kFeatures, x + 2 * k, w + 2 * k, desc, k > 0);
+                    tc::commit_pair(empty + 8 * s);
+                    tc::commit_pair(sum_full + 8 * b);
+                }
+            }
+            // the last products have ended before tensor memory is given back
+            if (done > 0) tc::wait_for(sum_full + 8 * ((done - 1) & 1), ((done - 1) >> 1) & 1, a.status);
+        }
+        __syncwarp();
+      } else if (warp == 2) {
+        const int64_t up = (int64_t)a.row_blocks * a.k_blocks;
+        int got = 0;
+        bool ok = true;
+        for (int t = blockIdx.x >> 1; t < tiles.total && ok; t += pairs) {
+            int tm, tn;
+            tiles.at(t, tm, tn);
+            const int64_t token = (int64_t)tm * C::kTokens + rank * 128 + lane;
+            const float* xs = a.x_scale + token * a.xs_token;
+            // lanes 0 and 1: the weights' scales of the two groups' features, or of the two parts
+            const int wb = kGated ? tn : min(2 * tn + lane, a.row_blocks - 1);
+            const float* ws = a.w_scale + (int64_t)wb * a.k_blocks + (kGated ? lane * up : 0);
+            for (int kb = 0; kb < n; ++kb, ++got) {
+                const int s = got % C::kSlots, turn = got / C::kSlots;
+                const uint32_t at = slots + s * C::kSlot;
+                ok = __all_sync(0xffffffffu, turn == 0 || tc::wait_for(slot_empty + 8 * s, (turn - 1) & 1, a.status));
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = token + 32 * i < a.tokens;
+                    tc::copy4(at + (lane + 32 * i) * 4, in ? xs + 32 * i * a.xs_token : a.x_scale, in);
+                }
+                if (lane < 2) tc::copy4(at + 512 + lane * 4, ws + kb, true);
+                tc::copy4_arrive(slot_full + 8 * s);
+                xs += a.xs_block;
+            }
+        }
+        tc::copy4_wait();
+      }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int group = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+        // this thread's columns of tensor memory: 128 of the group's, or 64 of each part
+        const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21) + (kGated ? 64 : 128) * group;
+        const uint32_t empty_at[2] = {tc::in_cta(sum_empty, 0), tc::in_cta(sum_empty + 8, 0)};
+        const uint32_t staging = out_at + group * 2 * kTileBytes;
+        const uint32_t top = top_at + row * 4;  // [2][128]: a group's largest magnitude of a token
+        const bool issues = threadIdx.x == 128 + 128 * group;
+        bool ok = true;
+        int done = 0;
+        for (int t = blockIdx.x >> 1; t < tiles.total; t += pairs) {
+            int tm, tn;
+            tiles.at(t, tm, tn);
+            const int64_t token0 = (int64_t)tm * C::kTokens + rank * 128, token = token0 + row;
+            const bool live = token < a.tokens;
+            uint64_t acc[64];
+#pragma unroll
+            for (int c = 0; c < 64; ++c) acc[c] = 0;
+            for (int kb = 0; kb < n; ++kb, ++done) {
+                const int b = done & 1, slot = done % C::kSlots;
+                const uint32_t scales = slots + slot * C::kSlot;
+                ok = __all_sync(0xffffffffu, ok && tc::wait_for(slot_full + 8 * slot, (done / C::kSlots) & 1, a.status) &&
+                                                 tc::wait_for(sum_full + 8 * b, (done >> 1) & 1, a.status));
+                tc::fence_after();
+                if (!ok) continue;
+                const float x = __uint_as_float(ld_shared<uint32_t>(scales + row * 4));
+                const float s0 = x * __uint_as_float(ld_shared<uint32_t>(scales + 512 + (kGated ? 0 : group * 4)));
+                const float s1 = kGated ? x * __uint_as_float(ld_shared<uint32_t>(scales + 516)) : s0;
+                __syncwarp();
+                if (lane == 0) tc::arrive(slot_empty + 8 * slot);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[32];
+                    tc::ld32(mine + b * C::kFeatures + (kGated ? (c & 1) * 32 + (c >> 1) * 128 : c * 32), v);
+                    tc::wait_ld();
+                    if (c == 3) {
+                        tc::fence_before();
+                        if (lane == 0) tc::arrive_cluster(empty_at[b]);
+                    }
+                    const uint32_t s = __float_as_uint(c < 2 ? s0 : s1);
+                    const uint64_t ss = tc::pack2(s, s);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[16 * c + i] = tc::fma2(tc::pack2(v[2 * i], v[2 * i + 1]), ss, acc[16 * c + i]);
+                }
+            }
+            auto lo = [&](int i) { return __uint_as_float((uint32_t)acc[i]); };
+            auto hi = [&](int i) { return __uint_as_float((uint32_t)(acc[i] >> 32)); };
+            // the staging's last tile has been read
+            if (mapped && issues) tc::store_wait_read();
+            if (kGated) {
+                uint32_t m = 0;
+                const int f0 = tn * kTile + group * 64;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const bool in = f0 + 2 * i < a.rows;  // rows are whole 16 bytes
+                    const float p = in ? gated(lo(i), lo(32 + i)) : 0.f, q = in ? gated(hi(i), hi(32 + i)) : 0.f;
+                    acc[i] = tc::pack2(__float_as_uint(p), __float_as_uint(q));
+                    m = max(m, max(magnitude(p), magnitude(q)));
+                }
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(top + group * 512), "r"(m) : "memory");
+                asm volatile("bar.sync 3, 256;" ::: "memory");  // both groups (and the issuing threads' waits)
+                m = max(m, ld_shared<uint32_t>(top + (group ^ 1) * 512));
+                const float s = scale_of(m);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint4 q;
+                    q.x = e4m3x4(lo(8 * j), hi(8 * j), lo(8 * j + 1), hi(8 * j + 1), s);
+                    q.y = e4m3x4(lo(8 * j + 2), hi(8 * j + 2), lo(8 * j + 3), hi(8 * j + 3), s);
+                    q.z = e4m3x4(lo(8 * j + 4), hi(8 * j + 4), lo(8 * j + 5), hi(8 * j + 5), s);
+                    q.w = e4m3x4(lo(8 * j + 6), hi(8 * j + 6), lo(8 * j + 7), hi(8 * j + 7), s);
+                    st_shared(swizzled(out_at, row, group * 4 + j), q);
+                }
+                if (live && group == 0) a.out_scale[token * a.os_token + tn * a.os_block] = s;
+                tc::fence_async();
+                asm volatile("bar.sync 3, 256;" ::: "memory");
+                if (issues && group == 0) {
+                    if (token0 < a.tokens) tc::tma_store_2d(&out_map, out_at, tn * kTile, (int)token0);
+                    tc::store_commit();
+                }
+            } else if (a.dtype == ZKV_DT_F32) {
+                // 32 features a tile, two tiles at a time
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (half && mapped && issues) tc::store_wait_read();
+                    group_sync(group);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int i = half * 32 + c * 16 + 2 * j;
+                            st_shared(swizzled(staging + c * kTileBytes, row, j),
+                                      make_uint4((uint32_t)acc[i], (uint32_t)(acc[i] >> 32), (uint32_t)acc[i + 1],
+                                                 (uint32_t)(acc[i + 1] >> 32)));
+                        }
+                    if (mapped) tc::fence_async();
+                    group_sync(group);
+                    const int f = tn * C::kFeatures + group * 128 + half * 64;
+                    for (int c = 0; c < 2; ++c) {
+                        const int fc = f + 32 * c;
+                        if (!mapped) copy_out<uint32_t>(a, staging + c * kTileBytes, token0, fc, 32);
+                        else if (issues && fc < a.rows && token0 < a.tokens)
+                            tc::tma_store_2d(&out_map, staging + c * kTileBytes, fc, (int)token0);
+                    }
+                    if (mapped && issues) tc::store_commit();
+                }
+            } else {
+                group_sync(group);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = c * 32 + 4 * j + i;
+                            if (a.dtype == ZKV_DT_BF16) {
+                                w[i] = pack_bf162(lo(at), hi(at));
+                            } else {
+                                const __half2 h = __floats2half2_rn(lo(at), hi(at));
+                                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                        }
+                        st_shared(swizzled(staging + c * kTileBytes, row, j), make_uint4(w[0], w[1], w[2], w[3]));
+                    }
+                if (mapped) tc::fence_async();
+                group_sync(group);
+                const int f = tn * C::kFeatures + group * 128;
+                for (int c = 0; c < 2; ++c) {
+                    const int fc = f + 64 * c;
+                    if (!mapped) copy_out<uint16_t>(a, staging + c * kTileBytes, token0, fc, 64);
+                    else if (issues && fc < a.rows && token0 < a.tokens)
+                        tc::tma_store_2d(&out_map, staging + c * kTileBytes, fc, (int)token0);
+                }
+                if (mapped && issues) tc::store_commit();
+            }
+        }
+        if (mapped && issues) tc::store_wait();  // the staging is read until then
+        tc::fence_before();
+    }
+    __syncthreads();
+    tc::cluster_sync();  // neither CTA's memory is given up while the other may use it
+    tc::fence_after();
+    if (warp == 1) tc::tmem_free_pair(tmem, 512);
+}
+
 // ------------------------------------------------------------ host
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -387,6 +730,51 @@ static int launch_few(const zkv_fp8_weight* w, const void* x, int64_t x_ld, cons
     return launch_status();
 }
 
+// The output for stores of tiles, 128 bytes of 128 rows.
+static bool encode_out(CUtensorMap* map, const Product& a, int element, int64_t columns) {
+    EncodeTiled fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)a.tokens}, strides[1] = {(cuuint64_t)(a.out_ld * element)};
+    const cuuint32_t size[2] = {(cuuint32_t)(128 / element), 128}, es[2] = {1, 1};
+    const CUtensorMapDataType type = element == 4   ? CU_TENSOR_MAP_DATA_TYPE_UINT32
+                                     : element == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    return fn(map, type, 2, a.out, dims, strides, size, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool kGated>
+static int launch_many(const zkv_fp8_weight* w, const void* x, int64_t x_ld, const Product& a, cudaStream_t stream) {
+    using C = Many<kGated>;
+    CUtensorMap maps[3];
+    memcpy(&maps[0], w->map, sizeof maps[0]);
+    if (!encode_rows(&maps[1], x, w->k, a.tokens, x_ld, 0, 128)) return ZKV_ERR_ARG;
+    const int element = kGated ? 1 : a.dtype == ZKV_DT_F32 ? 4 : 2;
+    const bool mapped = aligned16(a.out) && a.out_ld * element % 16 == 0 && a.out_ld * element < (int64_t)1 << 40;
+    if (!mapped) maps[2] = maps[1];
+    else if (!encode_out(&maps[2], a, element, a.rows)) return ZKV_ERR_ARG;
+    const int64_t m = (a.tokens + C::kTokens - 1) / C::kTokens, n = kGated ? a.row_blocks : (a.row_blocks + 1) / 2;
+    if (m * n > INT32_MAX / 2) return ZKV_ERR_CAPACITY;
+    const int sms = sm_count();
+    if (!sms) return launch_refused();
+    auto kernel = many_kernel<kGated>;
+    if (!raise_smem_limit((const void*)kernel, C::kSmem)) return launch_refused();
+    const ManyTiles tiles = {(int)m, (int)n, (int)(m * n)};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>(2 * m * n, sms / 2 * 2), 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], a, tiles, mapped) != cudaSuccess) return launch_refused();
+    return launch_status();
+}
+
 static int check_weight(const zkv_fp8_weight* w) {
     if (!w || !w->w || !w->scale || w->rows < 1 || w->k < 1 || w->ld < w->k) return ZKV_ERR_ARG;
     if (w->parts != 1 && w->parts != 2) return ZKV_ERR_ARG;
@@ -417,7 +805,8 @@ static int launch(const zkv_fp8_weight* w, const void* x, int64_t x_ld, const Pr
     if (a.tokens <= 16) return launch_few<16, kParts>(w, x, x_ld, a, stream);
     if (a.tokens <= 32) return launch_few<32, kParts>(w, x, x_ld, a, stream);
     if (a.tokens <= 64) return launch_few<64, kParts>(w, x, x_ld, a, stream);
-    return launch_few<128, kParts>(w, x, x_ld, a, stream);
+    if (a.tokens <= 256) return launch_few<128, kParts>(w, x, x_ld, a, stream);
+    return launch_many<kParts == 2>(w, x, x_ld, a, stream);
 }
 
 }  // namespace fp8
