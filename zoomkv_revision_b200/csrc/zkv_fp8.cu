@@ -62,11 +62,12 @@ __device__ __forceinline__ void store_block(const float (&y)[16], const RowArgs&
     for (int off = 4; off >= 1; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
     if (!in) return;
     const float s = scale_of(m);
+    const Quotient by(s);
     uint4 q;
-    q.x = e4m3x4(y[0], y[1], y[2], y[3], s);
-    q.y = e4m3x4(y[4], y[5], y[6], y[7], s);
-    q.z = e4m3x4(y[8], y[9], y[10], y[11], s);
-    q.w = e4m3x4(y[12], y[13], y[14], y[15], s);
+    q.x = by.e4m3(y[0], y[1], y[2], y[3]);
+    q.y = by.e4m3(y[4], y[5], y[6], y[7]);
+    q.z = by.e4m3(y[8], y[9], y[10], y[11]);
+    q.w = by.e4m3(y[12], y[13], y[14], y[15]);
     *reinterpret_cast<uint4*>(a.out + row * a.out_ld + at) = q;
     if (at % kBlock == 0) a.scale[row * a.scale_token + (at / kBlock) * a.scale_block] = s;
 }

@@ -104,7 +104,8 @@ __device__ __forceinline__ void store4(const Product& a, int64_t token, int f, f
     }
 }
 
-__device__ __forceinline__ float gated(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+// silu(g) u; a quotient by an infinite sum is 0, as silu is there.
+__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
 template <int kTok, int kParts>
 __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
@@ -294,7 +295,8 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
                     0xffffffffu, max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w))));
                 const float s = scale_of(m);
                 if (f < a.rows)
-                    *reinterpret_cast<uint32_t*>((uint8_t*)a.out + token * a.out_ld + f) = e4m3x4(v.x, v.y, v.z, v.w, s);
+                    *reinterpret_cast<uint32_t*>((uint8_t*)a.out + token * a.out_ld + f) =
+                        Quotient(s).e4m3(v.x, v.y, v.z, v.w);
                 if (lane == 0) a.out_scale[token * a.os_token + tile * a.os_block] = s;
             }
         }
@@ -564,13 +566,14 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
                 asm volatile("bar.sync 3, 256;" ::: "memory");  // both groups (and the issuing threads' waits)
                 m = max(m, ld_shared<uint32_t>(top + (group ^ 1) * 512));
                 const float s = scale_of(m);
+                const Quotient by(s);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     uint4 q;
-                    q.x = e4m3x4(lo(8 * j), hi(8 * j), lo(8 * j + 1), hi(8 * j + 1), s);
-                    q.y = e4m3x4(lo(8 * j + 2), hi(8 * j + 2), lo(8 * j + 3), hi(8 * j + 3), s);
-                    q.z = e4m3x4(lo(8 * j + 4), hi(8 * j + 4), lo(8 * j + 5), hi(8 * j + 5), s);
-                    q.w = e4m3x4(lo(8 * j + 6), hi(8 * j + 6), lo(8 * j + 7), hi(8 * j + 7), s);
+                    q.x = by.e4m3(lo(8 * j), hi(8 * j), lo(8 * j + 1), hi(8 * j + 1));
+                    q.y = by.e4m3(lo(8 * j + 2), hi(8 * j + 2), lo(8 * j + 3), hi(8 * j + 3));
+                    q.z = by.e4m3(lo(8 * j + 4), hi(8 * j + 4), lo(8 * j + 5), hi(8 * j + 5));
+                    q.w = by.e4m3(lo(8 * j + 6), hi(8 * j + 6), lo(8 * j + 7), hi(8 * j + 7));
                     st_shared(swizzled(out_at, row, group * 4 + j), q);
                 }
                 if (live && group == 0) a.out_scale[token * a.os_token + tn * a.os_block] = s;
