@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
                    sum_empty = sum_full + 8 * C::kBufs, tmem_at = sum_empty + 8 * C::kBufs;
     uint8_t* const generic = smem_raw + (base - smem_u32(smem_raw));
     float* const scales = reinterpret_cast<float*>(generic + C::kStages * C::kStage);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_rank(), parts = tc::cluster_size();
     const int tile = blockIdx.x / parts;
     const int64_t t0 = (int64_t)blockIdx.y * kTok;
@@ -150,33 +150,33 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
     for (int c = 0; c < C::kMine; ++c) acc[c] = 0.f;
 
     if (warp == 0) {
-        if (lane == 0) {
-            int got = 0;
-            for (; got < n; ++got) {
-                const int s = got % C::kStages, turn = got / C::kStages;
-                if (turn > 0 && !tc::wait_for(empty + 8 * s, (turn - 1) & 1, a.status)) break;
-                const uint32_t at = base + s * C::kStage, bar = full + 8 * s;
+        int got = 0;
+        for (; got < n; ++got) {
+            const int s = got % C::kStages, turn = got / C::kStages;
+            if (turn > 0 && !tc::wait_all(empty + 8 * s, (turn - 1) & 1, a.status)) break;
+            const uint32_t at = base + s * C::kStage, bar = full + 8 * s;
+            if (tc::elected()) {
                 tc::arrive_expect_tx(bar, C::kStage);
                 for (int p = 0; p < kParts; ++p)
                     tc::tma_3d(at + p * kTileBytes, &w_map, (b0 + got) * kBlock, tile * kTile, p, bar);
                 tc::tma_2d(at + kParts * kTileBytes, &x_map, (b0 + got) * kBlock, (int)t0, bar);
             }
-            // every copy has landed before the CTA ends, whatever became of the others
-            for (int i = got > C::kStages ? got - C::kStages : 0; i < got; ++i)
-                if (!tc::wait_for(full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.status)) break;
+            __syncwarp();
         }
-        __syncwarp();
+        // every copy has landed before the CTA ends, whatever became of the others
+        for (int i = got > C::kStages ? got - C::kStages : 0; i < got; ++i)
+            if (!tc::wait_all(full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.status)) break;
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t desc = tc::e4m3_desc(kTile, kTok);
-            int done = 0;
-            for (; done < n; ++done) {
-                const int s = done % C::kStages, b = done % C::kBufs, turn = done / C::kBufs;
-                if (!tc::wait_for(full + 8 * s, (done / C::kStages) & 1, a.status)) break;
-                if (turn > 0 && !tc::wait_for(sum_empty + 8 * b, (turn - 1) & 1, a.status)) break;
-                tc::fence_after();
-                const uint32_t at = base + s * C::kStage;
-                const uint64_t x = tc::tile_desc(at + kParts * kTileBytes);
+        constexpr uint32_t desc = tc::e4m3_desc(kTile, kTok);
+        int done = 0;
+        for (; done < n; ++done) {
+            const int s = done % C::kStages, b = done % C::kBufs, turn = done / C::kBufs;
+            if (!tc::wait_all(full + 8 * s, (done / C::kStages) & 1, a.status)) break;
+            if (turn > 0 && !tc::wait_all(sum_empty + 8 * b, (turn - 1) & 1, a.status)) break;
+            tc::fence_after();
+            const uint32_t at = base + s * C::kStage;
+            const uint64_t x = tc::tile_desc(at + kParts * kTileBytes);
+            if (tc::elected()) {
 #pragma unroll
                 for (int p = 0; p < kParts; ++p) {
                     const uint64_t w = tc::tile_desc(at + p * kTileBytes);
@@ -187,10 +187,10 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
                 tc::commit(empty + 8 * s);
                 tc::commit(sum_full + 8 * b);
             }
-            // the last products have ended before tensor memory is given back
-            if (done > 0) tc::wait_for(sum_full + 8 * ((done - 1) % C::kBufs), ((done - 1) / C::kBufs) & 1, a.status);
+            __syncwarp();
         }
-        __syncwarp();
+        // the last products have ended before tensor memory is given back
+        if (done > 0) tc::wait_all(sum_full + 8 * ((done - 1) % C::kBufs), ((done - 1) / C::kBufs) & 1, a.status);
     } else {
         const int e = threadIdx.x - 64, group = (warp - 2) >> 2;
         const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21) + group * C::kMine;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
                    bars = slots + C::kSlots * C::kSlot;
     const uint32_t full = bars, empty = full + 8 * C::kStages, sum_full = empty + 8 * C::kStages, sum_empty = sum_full + 16,
                    slot_full = sum_empty + 16, slot_empty = slot_full + 8 * C::kSlots, tmem_at = slot_empty + 8 * C::kSlots;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_rank();
     const int n = a.k_blocks, pairs = gridDim.x >> 1;
 
@@ -424,55 +424,53 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
       if (warp == 0) {
-        if (lane == 0) {
-            const uint32_t leader = tc::in_cta(full, 0);
-            int got = 0;
-            bool ok = true;
-            for (int t = blockIdx.x >> 1; t < tiles.total && ok; t += pairs) {
-                int tm, tn;
-                tiles.at(t, tm, tn);
-                const int token = tm * C::kTokens + rank * 128;
-                for (int kb = 0; kb < n; ++kb, ++got) {
-                    const int s = got % C::kStages, turn = got / C::kStages;
-                    if (turn > 0 && !(ok = tc::wait_for(empty + 8 * s, (turn - 1) & 1, a.status))) break;
-                    const uint32_t at = base + s * C::kStage;
+        const uint32_t leader = tc::in_cta(full, 0);
+        int got = 0;
+        bool ok = true;
+        for (int t = blockIdx.x >> 1; t < tiles.total && ok; t += pairs) {
+            int tm, tn;
+            tiles.at(t, tm, tn);
+            const int token = tm * C::kTokens + rank * 128;
+            const int feature = kGated ? tn * kTile : (2 * tn + (int)rank) * kTile, part = kGated ? (int)rank : 0;
+            for (int kb = 0; kb < n; ++kb, ++got) {
+                const int s = got % C::kStages, turn = got / C::kStages;
+                if (turn > 0 && !(ok = tc::wait_all(empty + 8 * s, (turn - 1) & 1, a.status))) break;
+                const uint32_t at = base + s * C::kStage;
+                if (tc::elected()) {
                     if (rank == 0) tc::arrive_expect_tx(full + 8 * s, 2 * C::kStage);
                     tc::tma_2d_pair(at, &x_map, kb * kBlock, token, leader + 8 * s);
-                    if (kGated)
-                        tc::tma_3d_pair(at + kTileBytes, &w_map, kb * kBlock, tn * kTile, (int)rank, leader + 8 * s);
-                    else
-                        tc::tma_3d_pair(at + kTileBytes, &w_map, kb * kBlock, (2 * tn + (int)rank) * kTile, 0, leader + 8 * s);
+                    tc::tma_3d_pair(at + kTileBytes, &w_map, kb * kBlock, feature, part, leader + 8 * s);
                 }
+                __syncwarp();
             }
-            // both CTAs' copies have landed before either ends, whatever became of the others
-            if (rank == 0)
-                for (int i = got > C::kStages ? got - C::kStages : 0; i < got; ++i)
-                    if (!tc::wait_for(full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.status)) break;
         }
-        __syncwarp();
-      } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            constexpr uint32_t desc = tc::e4m3_desc(256, C::kFeatures);
-            int done = 0;
-            bool ok = true;
-            for (int t = blockIdx.x >> 1; t < tiles.total && ok; t += pairs) {
-                for (int kb = 0; kb < n; ++kb, ++done) {
-                    const int s = done % C::kStages, b = done & 1, turn = done >> 1;
-                    if (!(ok = tc::wait_for(full + 8 * s, (done / C::kStages) & 1, a.status))) break;
-                    if (turn > 0 && !(ok = tc::wait_for(sum_empty + 8 * b, (turn - 1) & 1, a.status))) break;
-                    tc::fence_after();
-                    const uint64_t x = tc::tile_desc(base + s * C::kStage), w = tc::tile_desc(base + s * C::kStage + kTileBytes);
+        // both CTAs' copies have landed before either ends, whatever became of the others
+        if (rank == 0)
+            for (int i = got > C::kStages ? got - C::kStages : 0; i < got; ++i)
+                if (!tc::wait_all(full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.status)) break;
+      } else if (warp == 1 && rank == 0) {
+        constexpr uint32_t desc = tc::e4m3_desc(256, C::kFeatures);
+        int done = 0;
+        bool ok = true;
+        for (int t = blockIdx.x >> 1; t < tiles.total && ok; t += pairs) {
+            for (int kb = 0; kb < n; ++kb, ++done) {
+                const int s = done % C::kStages, b = done & 1, turn = done >> 1;
+                if (turn > 0 && !(ok = tc::wait_all(sum_empty + 8 * b, (turn - 1) & 1, a.status))) break;
+                if (!(ok = tc::wait_all(full + 8 * s, (done / C::kStages) & 1, a.status))) break;
+                tc::fence_after();
+                const uint64_t x = tc::tile_desc(base + s * C::kStage), w = tc::tile_desc(base + s * C::kStage + kTileBytes);
+                if (tc::elected()) {
 #pragma unroll
                     for (int k = 0; k < kBlock / 32; ++k)
                         tc::mma_e4m3_pair(tmem + b * C::kFeatures, x + 2 * k, w + 2 * k, desc, k > 0);
-                    tc::commit_pair(empty + 8 * s);
                     tc::commit_pair(sum_full + 8 * b);
+                    tc::commit_pair(empty + 8 * s);
                 }
+                __syncwarp();
             }
-            // the last products have ended before tensor memory is given back
-            if (done > 0) tc::wait_for(sum_full + 8 * ((done - 1) & 1), ((done - 1) >> 1) & 1, a.status);
         }
-        __syncwarp();
+        // the last products have ended before tensor memory is given back
+        if (done > 0) tc::wait_all(sum_full + 8 * ((done - 1) & 1), ((done - 1) >> 1) & 1, a.status);
       } else if (warp == 2) {
         const int64_t up = (int64_t)a.row_blocks * a.k_blocks;
         int got = 0;

@@ -9,6 +9,18 @@ namespace tc {
 
 constexpr uint64_t kWaitNs = 2000000000ull;  // longest wait of a kernel on its own copies and products
 
+// One lane of a whole warp, always the same.  Copies and products are issued under it in code that the whole warp runs:
+// their operands live in uniform registers, and under a test of the lane number the compiler moves them there for each.
+__device__ __forceinline__ bool elected() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -32,6 +44,11 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int32_t*
         }
     }
     return true;
+}
+
+// The same for a whole warp, which goes on together.
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, int32_t* status) {
+    return __all_sync(0xffffffffu, wait_for(bar, parity, status));
 }
 
 __device__ __forceinline__ void arrive(uint32_t bar) {
