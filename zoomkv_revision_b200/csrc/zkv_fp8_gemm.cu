@@ -27,6 +27,7 @@ namespace fp8 {
 
 constexpr int kTile = 128;       // features of a tile
 constexpr int kTileBytes = kTile * kBlock;
+constexpr int kBox = 64;         // features of a copy
 constexpr int kSmemSM = 228 * 1024, kSmemReserved = 1024;
 
 struct Product {
@@ -157,8 +158,8 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
             const uint32_t at = base + s * C::kStage, bar = full + 8 * s;
             if (tc::elected()) {
                 tc::arrive_expect_tx(bar, C::kStage);
-                for (int p = 0; p < kParts; ++p)
-                    tc::tma_3d(at + p * kTileBytes, &w_map, (b0 + got) * kBlock, tile * kTile, p, bar);
+                for (int p = 0; p < 2 * kParts; ++p)
+                    tc::tma_3d(at + p * kBox * kBlock, &w_map, (b0 + got) * kBlock, tile * kTile + (p & 1) * kBox, p >> 1, bar);
                 tc::tma_2d(at + kParts * kTileBytes, &x_map, (b0 + got) * kBlock, (int)t0, bar);
             }
             __syncwarp();
@@ -232,9 +233,9 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
             if (ok) {
 #pragma unroll
                 for (int c = 0; c < C::kMine; c += 16) {
-                    float v[16];
+                    uint32_t v[16];
                     tc::ld16(mine + b * C::kCols + c, v);
-                    tc::wait_ld();
+                    tc::wait_ld(v);
                     if (c + 16 == C::kMine) {
                         tc::fence_before();
                         if (lane == 0) tc::arrive(sum_empty + 8 * b);
@@ -242,10 +243,10 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float4 s = by[c / 4 + i];
-                        acc[c + 4 * i] = fmaf(v[4 * i], s.x, acc[c + 4 * i]);
-                        acc[c + 4 * i + 1] = fmaf(v[4 * i + 1], s.y, acc[c + 4 * i + 1]);
-                        acc[c + 4 * i + 2] = fmaf(v[4 * i + 2], s.z, acc[c + 4 * i + 2]);
-                        acc[c + 4 * i + 3] = fmaf(v[4 * i + 3], s.w, acc[c + 4 * i + 3]);
+                        acc[c + 4 * i] = fmaf(__uint_as_float(v[4 * i]), s.x, acc[c + 4 * i]);
+                        acc[c + 4 * i + 1] = fmaf(__uint_as_float(v[4 * i + 1]), s.y, acc[c + 4 * i + 1]);
+                        acc[c + 4 * i + 2] = fmaf(__uint_as_float(v[4 * i + 2]), s.z, acc[c + 4 * i + 2]);
+                        acc[c + 4 * i + 3] = fmaf(__uint_as_float(v[4 * i + 3]), s.w, acc[c + 4 * i + 3]);
                     }
                 }
             }
@@ -310,24 +311,28 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
 // of each part), by a pair of CTAs whose tensor cores share the features'
 // operand, so that a CTA loads 32 KB for a block of the inner dimension
 // instead of 48 (96 bytes a clock at the full rate, more than L2 gives an SM).
-// A thread of the eight that read tensor memory has one token and 128
-// features in registers: both scales are its own, one packed product-and-sum
-// for two elements.  The two halves of tensor memory take the blocks in turn,
-// so that a tile's output is written while the next tile's first two blocks
-// are multiplied.
+// Each block's sums go to tensor memory, and from there, scaled, into fp32
+// registers: a thread has one token and 64 features, both scales are its own,
+// and one packed product-and-sum takes two elements.  The tensor core would
+// have to wait while a block's sums are read and the barriers pass between
+// the two CTAs (some 1100 clocks for the 512 of a block), so the tile is
+// multiplied in two halves of 128 features with two buffers of tensor memory
+// each, every half by an issuing warp and two warpgroups of readers of its
+// own.
 template <bool kGated>
 struct Many {
     static constexpr int kTokens = 256, kFeatures = 256;
-    // A warpgroup for the copies and products, two that read tensor memory, which take the registers that the first gives
-    // up: 128 x 64 + 256 x 208 of the 384 x 168 of the launch.
-    static constexpr int kThreads = 384;
-    static constexpr int kStages = kGated ? 6 : 5;
+    // A warpgroup for the copies and products, four of readers, which take the registers that the first gives up:
+    // 128 x 40 + 512 x 104 of the 640 x 96 of the launch.
+    static constexpr int kReaders = 512, kThreads = 128 + kReaders;
+    static constexpr int kStages = 4;
     static constexpr int kStage = 2 * kTileBytes;  // 128 rows of tokens, 128 of features
-    static constexpr int kOut = (kGated ? 1 : 4) * kTileBytes;  // output staging; 16- and 32-bit: half for each warpgroup
-    static constexpr int kTop = kGated ? 1024 : 0;
-    // Scales come to shared memory a few blocks ahead, by a warp of their own: loaded one block ahead by the threads that
-    // use them, they took 1.1 us a block (4096 x 6144 x 4096: 220 us).
-    static constexpr int kSlots = kGated ? 4 : 3, kSlot = 528;  // 128 tokens, two of the weights
+    // Output staging: a tile for each warpgroup; gated: one in all, and the sums that warpgroups exchange.
+    static constexpr int kOut = (kGated ? 5 : 4) * kTileBytes;
+    static constexpr int kTop = kGated ? 2048 : 0;
+    // Scales come to shared memory by a warp of their own, four blocks of the inner dimension at a time: loaded one block
+    // ahead by the threads that use them, they took 1.1 us a block (4096 x 6144 x 4096: 220 us).
+    static constexpr int kBatch = 4, kSlots = 2, kSlot = kBatch * 4 * (128 + 2);  // 128 tokens, two of the weights
     static constexpr int kSmem = 1024 + kStages * kStage + kOut + kTop + kSlots * kSlot + 256;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -347,12 +352,17 @@ __device__ __forceinline__ void group_sync(int group) {
     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
 }
 
+__device__ __forceinline__ void readers_sync() { asm volatile("bar.sync 5, 512;" ::: "memory"); }
+
 // 16 bytes of row r of a swizzled tile of 128-byte rows.
 __device__ __forceinline__ uint32_t swizzled(uint32_t tile, int r, int chunk) {
     return tile + r * 128 + ((chunk ^ (r & 7)) << 4);
 }
 __device__ __forceinline__ void st_shared(uint32_t at, uint4 v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void st_shared1(uint32_t at, uint32_t v) {
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 template <typename T>
 __device__ __forceinline__ T ld_shared(uint32_t at) {
@@ -364,6 +374,12 @@ __device__ __forceinline__ T ld_shared(uint32_t at) {
     uint32_t v;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
     return (T)v;
+}
+
+__device__ __forceinline__ float4 ld_shared4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
 }
 
 // One swizzled tile of 128 rows to an output whose rows do not start on 16 bytes: by a warpgroup, element by element.
@@ -390,8 +406,8 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
     uint8_t* const generic = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t out_at = base + C::kStages * C::kStage, top_at = out_at + C::kOut, slots = top_at + C::kTop,
                    bars = slots + C::kSlots * C::kSlot;
-    const uint32_t full = bars, empty = full + 8 * C::kStages, sum_full = empty + 8 * C::kStages, sum_empty = sum_full + 16,
-                   slot_full = sum_empty + 16, slot_empty = slot_full + 8 * C::kSlots, tmem_at = slot_empty + 8 * C::kSlots;
+    const uint32_t full = bars, empty = full + 8 * C::kStages, sum_full = empty + 8 * C::kStages, sum_empty = sum_full + 32,
+                   slot_full = sum_empty + 32, slot_empty = slot_full + 8 * C::kSlots, tmem_at = slot_empty + 8 * C::kSlots;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_rank();
     const int n = a.k_blocks, pairs = gridDim.x >> 1;
@@ -400,15 +416,15 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
         auto bar = [&](uint32_t at) { return reinterpret_cast<uint64_t*>(generic + (at - base)); };
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(bar(full + 8 * i), 1);
-            mbar_init(bar(empty + 8 * i), 1);
+            mbar_init(bar(empty + 8 * i), 2);  // both halves
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             mbar_init(bar(sum_full + 8 * i), 1);
-            mbar_init(bar(sum_empty + 8 * i), 16);  // 8 warps of both CTAs
+            mbar_init(bar(sum_empty + 8 * i), 16);  // a half's 8 warps of readers, of both CTAs
         }
         for (int i = 0; i < C::kSlots; ++i) {
             mbar_init(bar(slot_full + 8 * i), 32);
-            mbar_init(bar(slot_empty + 8 * i), 8);
+            mbar_init(bar(slot_empty + 8 * i), C::kReaders / 32);
         }
         mbar_fence_init();
         tc::prefetch_map(&w_map);
@@ -422,7 +438,7 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(generic + (tmem_at - base));
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
       if (warp == 0) {
         const uint32_t leader = tc::in_cta(full, 0);
         int got = 0;
@@ -431,7 +447,8 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
             int tm, tn;
             tiles.at(t, tm, tn);
             const int token = tm * C::kTokens + rank * 128;
-            const int feature = kGated ? tn * kTile : (2 * tn + (int)rank) * kTile, part = kGated ? (int)rank : 0;
+            // 64 of each half's 128 features
+            const int first = (kGated ? tn : 2 * tn) * kTile + (int)rank * kBox, second = kGated ? first : first + kTile;
             for (int kb = 0; kb < n; ++kb, ++got) {
                 const int s = got % C::kStages, turn = got / C::kStages;
                 if (turn > 0 && !(ok = tc::wait_all(empty + 8 * s, (turn - 1) & 1, a.status))) break;
@@ -439,7 +456,9 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
                 if (tc::elected()) {
                     if (rank == 0) tc::arrive_expect_tx(full + 8 * s, 2 * C::kStage);
                     tc::tma_2d_pair(at, &x_map, kb * kBlock, token, leader + 8 * s);
-                    tc::tma_3d_pair(at + kTileBytes, &w_map, kb * kBlock, feature, part, leader + 8 * s);
+                    tc::tma_3d_pair(at + kTileBytes, &w_map, kb * kBlock, first, 0, leader + 8 * s);
+                    tc::tma_3d_pair(at + kTileBytes + kBox * kBlock, &w_map, kb * kBlock, second, kGated ? 1 : 0,
+                                    leader + 8 * s);
                 }
                 __syncwarp();
             }
@@ -448,21 +467,23 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
         if (rank == 0)
             for (int i = got > C::kStages ? got - C::kStages : 0; i < got; ++i)
                 if (!tc::wait_all(full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.status)) break;
-      } else if (warp == 1 && rank == 0) {
-        constexpr uint32_t desc = tc::e4m3_desc(256, C::kFeatures);
+      } else if (warp != 2 && rank == 0) {
+        const int half = warp >> 1;
+        constexpr uint32_t desc = tc::e4m3_desc(256, kTile);
         int done = 0;
         bool ok = true;
         for (int t = blockIdx.x >> 1; t < tiles.total && ok; t += pairs) {
             for (int kb = 0; kb < n; ++kb, ++done) {
-                const int s = done % C::kStages, b = done & 1, turn = done >> 1;
+                const int s = done % C::kStages, b = half + 2 * (done & 1), turn = done >> 1;
                 if (turn > 0 && !(ok = tc::wait_all(sum_empty + 8 * b, (turn - 1) & 1, a.status))) break;
                 if (!(ok = tc::wait_all(full + 8 * s, (done / C::kStages) & 1, a.status))) break;
                 tc::fence_after();
-                const uint64_t x = tc::tile_desc(base + s * C::kStage), w = tc::tile_desc(base + s * C::kStage + kTileBytes);
+                const uint64_t x = tc::tile_desc(base + s * C::kStage),
+                               w = tc::tile_desc(base + s * C::kStage + kTileBytes + half * kBox * kBlock);
                 if (tc::elected()) {
 #pragma unroll
                     for (int k = 0; k < kBlock / 32; ++k)
-                        tc::mma_e4m3_pair(tmem + b * C::kFeatures, x + 2 * k, w + 2 * k, desc, k > 0);
+                        tc::mma_e4m3_pair(tmem + b * kTile, x + 2 * k, w + 2 * k, desc, k > 0);
                     tc::commit_pair(sum_full + 8 * b);
                     tc::commit_pair(empty + 8 * s);
                 }
@@ -470,7 +491,8 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
             }
         }
         // the last products have ended before tensor memory is given back
-        if (done > 0) tc::wait_all(sum_full + 8 * ((done - 1) & 1), ((done - 1) >> 1) & 1, a.status);
+        if (done > 0)
+            tc::wait_all(sum_full + 8 * (half + 2 * ((done - 1) & 1)), ((done - 1) >> 1) & 1, a.status);
       } else if (warp == 2) {
         const int64_t up = (int64_t)a.row_blocks * a.k_blocks;
         int got = 0;
@@ -480,162 +502,174 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
             tiles.at(t, tm, tn);
             const int64_t token = (int64_t)tm * C::kTokens + rank * 128 + lane;
             const float* xs = a.x_scale + token * a.xs_token;
-            // lanes 0 and 1: the weights' scales of the two groups' features, or of the two parts
+            // lanes 0 and 1: the weights' scales of the two halves
             const int wb = kGated ? tn : min(2 * tn + lane, a.row_blocks - 1);
             const float* ws = a.w_scale + (int64_t)wb * a.k_blocks + (kGated ? lane * up : 0);
-            for (int kb = 0; kb < n; ++kb, ++got) {
+            for (int kb = 0; kb < n; kb += C::kBatch, ++got) {
                 const int s = got % C::kSlots, turn = got / C::kSlots;
                 const uint32_t at = slots + s * C::kSlot;
-                ok = __all_sync(0xffffffffu, turn == 0 || tc::wait_for(slot_empty + 8 * s, (turn - 1) & 1, a.status));
-                if (!ok) break;
+                if (turn > 0 && !(ok = tc::wait_all(slot_empty + 8 * s, (turn - 1) & 1, a.status))) break;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool in = token + 32 * i < a.tokens;
-                    tc::copy4(at + (lane + 32 * i) * 4, in ? xs + 32 * i * a.xs_token : a.x_scale, in);
+                for (int j = 0; j < C::kBatch; ++j) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool in = kb + j < n && token + 32 * i < a.tokens;
+                        tc::copy4(at + (lane + 32 * i) * 16 + 4 * j,
+                                  in ? xs + 32 * i * a.xs_token + (kb + j) * a.xs_block : a.x_scale, in);
+                    }
+                    if (lane < 2) tc::copy4(at + 2048 + lane * 16 + 4 * j, kb + j < n ? ws + kb + j : a.w_scale, kb + j < n);
                 }
-                if (lane < 2) tc::copy4(at + 512 + lane * 4, ws + kb, true);
                 tc::copy4_arrive(slot_full + 8 * s);
-                xs += a.xs_block;
             }
         }
         tc::copy4_wait();
       }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int group = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
-        // this thread's columns of tensor memory: 128 of the group's, or 64 of each part
-        const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21) + (kGated ? 64 : 128) * group;
-        const uint32_t empty_at[2] = {tc::in_cta(sum_empty, 0), tc::in_cta(sum_empty + 8, 0)};
-        const uint32_t staging = out_at + group * 2 * kTileBytes;
-        const uint32_t top = top_at + row * 4;  // [2][128]: a group's largest magnitude of a token
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const int group = (warp - 4) >> 2, half = group >> 1, row = (warp & 3) * 32 + lane;
+        // this thread's columns of tensor memory: 64 of a half
+        const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21) + 64 * group;
+        const uint32_t empty_at = tc::in_cta(sum_empty + 8 * half, 0);
+        const uint32_t staging = out_at + group * kTileBytes;
+        const uint32_t top = top_at + row * 4;  // [4][128]: a group's largest magnitude of a token
         const bool issues = threadIdx.x == 128 + 128 * group;
         bool ok = true;
-        int done = 0;
+        int done = 0, batch = 0;
         for (int t = blockIdx.x >> 1; t < tiles.total; t += pairs) {
             int tm, tn;
             tiles.at(t, tm, tn);
             const int64_t token0 = (int64_t)tm * C::kTokens + rank * 128, token = token0 + row;
             const bool live = token < a.tokens;
-            uint64_t acc[64];
+            float acc[64];
 #pragma unroll
-            for (int c = 0; c < 64; ++c) acc[c] = 0;
-            for (int kb = 0; kb < n; ++kb, ++done) {
-                const int b = done & 1, slot = done % C::kSlots;
+            for (int c = 0; c < 64; ++c) acc[c] = 0.f;
+            for (int kb = 0; kb < n; kb += C::kBatch, ++batch) {
+                const int slot = batch % C::kSlots;
+                ok = ok && tc::wait_all(slot_full + 8 * slot, (batch / C::kSlots) & 1, a.status);
                 const uint32_t scales = slots + slot * C::kSlot;
-                ok = __all_sync(0xffffffffu, ok && tc::wait_for(slot_full + 8 * slot, (done / C::kSlots) & 1, a.status) &&
-                                                 tc::wait_for(sum_full + 8 * b, (done >> 1) & 1, a.status));
-                tc::fence_after();
-                if (!ok) continue;
-                const float x = __uint_as_float(ld_shared<uint32_t>(scales + row * 4));
-                const float s0 = x * __uint_as_float(ld_shared<uint32_t>(scales + 512 + (kGated ? 0 : group * 4)));
-                const float s1 = kGated ? x * __uint_as_float(ld_shared<uint32_t>(scales + 516)) : s0;
+                const float4 x4 = ld_shared4(scales + row * 16), w4 = ld_shared4(scales + 2048 + half * 16);
+                const float by[4] = {x4.x * w4.x, x4.y * w4.y, x4.z * w4.z, x4.w * w4.w};
                 __syncwarp();
                 if (lane == 0) tc::arrive(slot_empty + 8 * slot);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32];
-                    tc::ld32(mine + b * C::kFeatures + (kGated ? (c & 1) * 32 + (c >> 1) * 128 : c * 32), v);
-                    tc::wait_ld();
-                    if (c == 3) {
-                        tc::fence_before();
-                        if (lane == 0) tc::arrive_cluster(empty_at[b]);
-                    }
-                    const uint32_t s = __float_as_uint(c < 2 ? s0 : s1);
-                    const uint64_t ss = tc::pack2(s, s);
+                for (int j = 0; j < C::kBatch; ++j) {
+                    if (kb + j >= n) break;
+                    ok = ok && tc::wait_all(sum_full + 8 * (half + 2 * (done & 1)), (done >> 1) & 1, a.status);
+                    tc::fence_after();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[16 * c + i] = tc::fma2(tc::pack2(v[2 * i], v[2 * i + 1]), ss, acc[16 * c + i]);
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t v[32];
+                        tc::ld32(mine + (done & 1) * 2 * kTile + 32 * c, v);
+                        tc::wait_ld(v);
+                        if (c == 1) {
+                            tc::fence_before();
+                            if (lane == 0) tc::arrive_cluster(empty_at + 16 * (done & 1));
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            acc[32 * c + i] = fmaf(__uint_as_float(v[i]), by[j], acc[32 * c + i]);
+                    }
+                    ++done;
                 }
             }
-            auto lo = [&](int i) { return __uint_as_float((uint32_t)acc[i]); };
-            auto hi = [&](int i) { return __uint_as_float((uint32_t)(acc[i] >> 32)); };
+            auto lo = [&](int i) { return acc[2 * i]; };
+            auto hi = [&](int i) { return acc[2 * i + 1]; };
             // the staging's last tile has been read
             if (mapped && issues) tc::store_wait_read();
             if (kGated) {
-                uint32_t m = 0;
-                const int f0 = tn * kTile + group * 64;
+                // Groups 0 and 1 hold the gate's features 0..63 and 64..127, 2 and 3 the up part's: each gives its partner
+                // half of what it has and finishes the features of the other half.
+                const uint32_t give = out_at + kTileBytes + group * kTileBytes + row * 4;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
+                for (int i = 0; i < 16; ++i) {
+                    st_shared1(give + (2 * i) * 512, __float_as_uint(group < 2 ? lo(16 + i) : lo(i)));
+                    st_shared1(give + (2 * i + 1) * 512, __float_as_uint(group < 2 ? hi(16 + i) : hi(i)));
+                }
+                readers_sync();
+                const uint32_t from = out_at + kTileBytes + (group ^ 2) * kTileBytes + row * 4;
+                uint32_t m = 0;
+                const int at = (group & 1) * 64 + half * 32, f0 = tn * kTile + at;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float o0 = group < 2 ? lo(i) : lo(16 + i), o1 = group < 2 ? hi(i) : hi(16 + i);
+                    const float t0 = __uint_as_float(ld_shared<uint32_t>(from + (2 * i) * 512));
+                    const float t1 = __uint_as_float(ld_shared<uint32_t>(from + (2 * i + 1) * 512));
                     const bool in = f0 + 2 * i < a.rows;  // rows are whole 16 bytes
-                    const float p = in ? gated(lo(i), lo(32 + i)) : 0.f, q = in ? gated(hi(i), hi(32 + i)) : 0.f;
-                    acc[i] = tc::pack2(__float_as_uint(p), __float_as_uint(q));
+                    const float p = in ? gated(group < 2 ? o0 : t0, group < 2 ? t0 : o0) : 0.f;
+                    const float q = in ? gated(group < 2 ? o1 : t1, group < 2 ? t1 : o1) : 0.f;
+                    acc[2 * i] = p, acc[2 * i + 1] = q;
                     m = max(m, max(magnitude(p), magnitude(q)));
                 }
                 asm volatile("st.shared.u32 [%0], %1;" ::"r"(top + group * 512), "r"(m) : "memory");
-                asm volatile("bar.sync 3, 256;" ::: "memory");  // both groups (and the issuing threads' waits)
-                m = max(m, ld_shared<uint32_t>(top + (group ^ 1) * 512));
+                readers_sync();  // every group's
+#pragma unroll
+                for (int g = 0; g < 4; ++g) m = max(m, ld_shared<uint32_t>(top + g * 512));
                 const float s = scale_of(m);
                 const Quotient by(s);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 2; ++j) {
                     uint4 q;
                     q.x = by.e4m3(lo(8 * j), hi(8 * j), lo(8 * j + 1), hi(8 * j + 1));
                     q.y = by.e4m3(lo(8 * j + 2), hi(8 * j + 2), lo(8 * j + 3), hi(8 * j + 3));
                     q.z = by.e4m3(lo(8 * j + 4), hi(8 * j + 4), lo(8 * j + 5), hi(8 * j + 5));
                     q.w = by.e4m3(lo(8 * j + 6), hi(8 * j + 6), lo(8 * j + 7), hi(8 * j + 7));
-                    st_shared(swizzled(out_at, row, group * 4 + j), q);
+                    st_shared(swizzled(out_at, row, at / 16 + j), q);
                 }
                 if (live && group == 0) a.out_scale[token * a.os_token + tn * a.os_block] = s;
                 tc::fence_async();
-                asm volatile("bar.sync 3, 256;" ::: "memory");
+                readers_sync();
                 if (issues && group == 0) {
                     if (token0 < a.tokens) tc::tma_store_2d(&out_map, out_at, tn * kTile, (int)token0);
                     tc::store_commit();
                 }
             } else if (a.dtype == ZKV_DT_F32) {
-                // 32 features a tile, two tiles at a time
+                // 32 features a tile, one half after the other
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (half && mapped && issues) tc::store_wait_read();
+                for (int side = 0; side < 2; ++side) {
+                    if (side && mapped && issues) tc::store_wait_read();
                     group_sync(group);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const int i = half * 32 + c * 16 + 2 * j;
-                            st_shared(swizzled(staging + c * kTileBytes, row, j),
-                                      make_uint4((uint32_t)acc[i], (uint32_t)(acc[i] >> 32), (uint32_t)acc[i + 1],
-                                                 (uint32_t)(acc[i + 1] >> 32)));
-                        }
+                    for (int j = 0; j < 8; ++j) {
+                        const float* v = acc + side * 32 + 4 * j;
+                        st_shared(swizzled(staging, row, j), make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
+                                                                        __float_as_uint(v[2]), __float_as_uint(v[3])));
+                    }
                     if (mapped) tc::fence_async();
                     group_sync(group);
-                    const int f = tn * C::kFeatures + group * 128 + half * 64;
-                    for (int c = 0; c < 2; ++c) {
-                        const int fc = f + 32 * c;
-                        if (!mapped) copy_out<uint32_t>(a, staging + c * kTileBytes, token0, fc, 32);
-                        else if (issues && fc < a.rows && token0 < a.tokens)
-                            tc::tma_store_2d(&out_map, staging + c * kTileBytes, fc, (int)token0);
+                    const int f = tn * C::kFeatures + group * 64 + side * 32;
+                    if (!mapped) {
+                        copy_out<uint32_t>(a, staging, token0, f, 32);
+                    } else if (issues) {
+                        if (f < a.rows && token0 < a.tokens) tc::tma_store_2d(&out_map, staging, f, (int)token0);
+                        tc::store_commit();
                     }
-                    if (mapped && issues) tc::store_commit();
                 }
             } else {
                 group_sync(group);
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t w[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int at = c * 32 + 4 * j + i;
-                            if (a.dtype == ZKV_DT_BF16) {
-                                w[i] = pack_bf162(lo(at), hi(at));
-                            } else {
-                                const __half2 h = __floats2half2_rn(lo(at), hi(at));
-                                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-                            }
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = 4 * j + i;
+                        if (a.dtype == ZKV_DT_BF16) {
+                            w[i] = pack_bf162(lo(at), hi(at));
+                        } else {
+                            const __half2 h = __floats2half2_rn(lo(at), hi(at));
+                            w[i] = *reinterpret_cast<const uint32_t*>(&h);
                         }
-                        st_shared(swizzled(staging + c * kTileBytes, row, j), make_uint4(w[0], w[1], w[2], w[3]));
                     }
+                    st_shared(swizzled(staging, row, j), make_uint4(w[0], w[1], w[2], w[3]));
+                }
                 if (mapped) tc::fence_async();
                 group_sync(group);
-                const int f = tn * C::kFeatures + group * 128;
-                for (int c = 0; c < 2; ++c) {
-                    const int fc = f + 64 * c;
-                    if (!mapped) copy_out<uint16_t>(a, staging + c * kTileBytes, token0, fc, 64);
-                    else if (issues && fc < a.rows && token0 < a.tokens)
-                        tc::tma_store_2d(&out_map, staging + c * kTileBytes, fc, (int)token0);
+                const int f = tn * C::kFeatures + group * 64;
+                if (!mapped) {
+                    copy_out<uint16_t>(a, staging, token0, f, 64);
+                } else if (issues) {
+                    if (f < a.rows && token0 < a.tokens) tc::tma_store_2d(&out_map, staging, f, (int)token0);
+                    tc::store_commit();
                 }
-                if (mapped && issues) tc::store_commit();
             }
         }
         if (mapped && issues) tc::store_wait();  // the staging is read until then
@@ -819,7 +853,7 @@ extern "C" int zkv_fp8_weight_init(zkv_fp8_weight* w) {
     if (const int rc = fp8::check_weight(w)) return rc;
     static_assert(sizeof(CUtensorMap) == sizeof w->map, "map");
     CUtensorMap map;
-    if (!fp8::encode_rows(&map, w->w, w->k, w->rows, w->ld, w->parts, fp8::kTile)) return ZKV_ERR_ARG;
+    if (!fp8::encode_rows(&map, w->w, w->k, w->rows, w->ld, w->parts, fp8::kBox)) return ZKV_ERR_ARG;
     memcpy(w->map, &map, sizeof map);
     return ZKV_OK;
 }

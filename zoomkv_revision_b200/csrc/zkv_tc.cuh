@@ -159,7 +159,19 @@ __device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Until this thread's loads have landed.  The registers are named, so that no use of them is moved before it.
+template <int N>
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[N]) {
+    static_assert(N == 16 || N == 32, "the loads below");
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+    if (N == 32)
+        asm volatile(""
+                     : "+r"(r[N - 16]), "+r"(r[N - 15]), "+r"(r[N - 14]), "+r"(r[N - 13]), "+r"(r[N - 12]), "+r"(r[N - 11]),
+                       "+r"(r[N - 10]), "+r"(r[N - 9]), "+r"(r[N - 8]), "+r"(r[N - 7]), "+r"(r[N - 6]), "+r"(r[N - 5]),
+                       "+r"(r[N - 4]), "+r"(r[N - 3]), "+r"(r[N - 2]), "+r"(r[N - 1])::"memory");
+}
 
 // Arrives on `bar` when the products issued by this thread so far are done.
 __device__ __forceinline__ void commit(uint32_t bar) {
@@ -167,8 +179,7 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 }
 
 // 16 columns of the warp's 32 lanes: thread = lane, register = column.
-__device__ __forceinline__ void ld16(uint32_t at, float* v) {
-    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+__device__ __forceinline__ void ld16(uint32_t at, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
