@@ -80,6 +80,8 @@ __global__ void __launch_bounds__(kQuantThreads) quant_kernel(RowArgs a, int blo
     const int64_t row = item / blocks;
     const int at = (int)(item - row * blocks) * kBlock + (threadIdx.x & 7) * 16;
     const bool in = row < a.tokens && at < a.dim;
+    grid_dep_launch_next();
+    grid_dep_wait();
     float y[16] = {};
     if (in) load16<kBf16>(a.x + row * a.x_ld + at, y);
     store_block(y, a, row, at, in);
@@ -98,6 +100,8 @@ __global__ void __launch_bounds__(kRow < 128 ? 128 : kRow) norm_kernel(RowArgs a
     const bool live = row < a.tokens;
     float x[kTurns][16] = {};
     float ss = 0.f;
+    grid_dep_launch_next();
+    grid_dep_wait();
 #pragma unroll
     for (int j = 0; j < kTurns; ++j) {
         const int at = (j * kRow + t) * 16;
@@ -148,8 +152,8 @@ __global__ void __launch_bounds__(kRow < 128 ? 128 : kRow) norm_kernel(RowArgs a
 template <bool kBf16, int kRow, int kTurns>
 static int launch_norm(const RowArgs& a, cudaStream_t stream) {
     constexpr int kThreads = kRow < 128 ? 128 : kRow, kRows = kThreads / kRow;
-    norm_kernel<kBf16, kRow, kTurns><<<(unsigned)((a.tokens + kRows - 1) / kRows), kThreads, 0, stream>>>(a);
-    return launch_status();
+    return launch_pdl_kernel(norm_kernel<kBf16, kRow, kTurns>, dim3((unsigned)((a.tokens + kRows - 1) / kRows)),
+                             dim3(kThreads), 0, stream, a);
 }
 
 template <bool kBf16>
@@ -188,11 +192,8 @@ extern "C" int zkv_quant_fp8(const void* x, int64_t x_ld, int dtype, int64_t tok
     const int64_t ctas = (tokens * blocks * 8 + fp8::kQuantThreads - 1) / fp8::kQuantThreads;
     if (ctas > INT32_MAX) return ZKV_ERR_CAPACITY;
     if (tokens == 0) return ZKV_OK;
-    if (dtype == ZKV_DT_BF16)
-        fp8::quant_kernel<true><<<(unsigned)ctas, fp8::kQuantThreads, 0, (cudaStream_t)stream>>>(a, blocks);
-    else
-        fp8::quant_kernel<false><<<(unsigned)ctas, fp8::kQuantThreads, 0, (cudaStream_t)stream>>>(a, blocks);
-    return launch_status();
+    return launch_pdl_kernel(dtype == ZKV_DT_BF16 ? fp8::quant_kernel<true> : fp8::quant_kernel<false>, dim3((unsigned)ctas),
+                             dim3(fp8::kQuantThreads), 0, (cudaStream_t)stream, a, blocks);
 }
 
 extern "C" int zkv_rmsnorm_fp8(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, void* residual_out,

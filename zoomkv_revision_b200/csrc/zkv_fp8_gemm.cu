@@ -28,7 +28,6 @@ namespace fp8 {
 constexpr int kTile = 128;       // features of a tile
 constexpr int kTileBytes = kTile * kBlock;
 constexpr int kBox = 64;         // features of a copy
-constexpr int kSmemSM = 228 * 1024, kSmemReserved = 1024;
 
 struct Product {
     const float* x_scale;
@@ -49,26 +48,25 @@ struct Product {
 template <int kTok, int kParts>
 struct Few {
     static constexpr int kCols = kTok * kParts;
-    static constexpr int kGroups = kCols > 64 ? 2 : 1;  // warpgroups that take the sums out of tensor memory
-    static constexpr int kThreads = 64 + 128 * kGroups;
+    static constexpr int kGroups = kCols >= 128 ? 4 : kCols >= 64 ? 2 : 1;  // warpgroups that take the sums out of tensor memory
+    static constexpr int kReaders = 128 * kGroups, kThreads = 64 + kReaders;
     static constexpr int kMine = kCols / kGroups;  // columns of a thread
-    static constexpr int kBufs = kCols <= 64 ? 4 : 2;
+    static constexpr int kLoad = kMine == 32 ? 32 : 16;  // columns of a load (64 columns: what registers leave room for)
+    // One CTA an SM: its ring takes the shared memory, and no second CTA of these kernels fits beside it, so that no
+    // cluster's CTA waits for tensor memory which another cluster, waiting for a CTA of its own, holds.
+    static constexpr int kBufs = 512 / kCols < 8 ? 512 / kCols : 8;
     static constexpr int kTmem = kCols * kBufs;
-    // Two CTAs an SM, but for the widest.  CTAs of a cluster wait for one
-    // another, so a set of them must never hold tensor memory that another
-    // set's CTA waits for on the same SM: at most 256 of 512 columns for a
-    // CTA that is not alone, and shared memory of which no third fits.
-    static constexpr int kPerSM = kTmem <= 256 ? 2 : 1;
     static constexpr int kStage = kParts * kTileBytes + kTok * kBlock;
     static constexpr int kAhead = 4;  // blocks of scales staged at a time
     static constexpr int kScales = 2 * kAhead * kCols * 4;
-    static constexpr int kRoom = kSmemSM / kPerSM - kSmemReserved - 1024 - kScales - 512;
-    static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
+    static constexpr int kRoom = 227 * 1024 - 1024 - kScales - 512;
+    static constexpr int kStages = kRoom / kStage < 12 ? kRoom / kStage : 12;
     static constexpr int kSmem = 1024 + kStages * kStage + kScales + 512;
     static constexpr int kJoin = kParts == 2 && kTok > 64 ? 64 : kTok;  // tokens joined at a time
     static_assert(kTmem >= 32 && kTmem <= 512 && (kTmem & (kTmem - 1)) == 0, "tensor memory comes in powers of two");
-    static_assert(kStages >= 2, "a ring");
-    static_assert(kSmem > kSmemSM / 3, "no third CTA on an SM");
+    static_assert(kMine % kLoad == 0, "whole loads");
+    static_assert(16 * (kStages + kBufs) + 4 <= 512, "barriers");
+    static_assert(kSmem > 114 * 1024 && kSmem <= 227 * 1024, "one CTA an SM");
     static_assert(kJoin * kParts * kTile * 4 <= kStages * kStage, "the parts are joined in the ring's place");
 };
 
@@ -140,11 +138,17 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
         tc::prefetch_map(&w_map);
         tc::prefetch_map(&x_map);
     }
-    if (warp == 1) tc::tmem_alloc(tmem_at, C::kTmem);
+    if (warp == 1) tc::tmem_alloc<C::kTmem>(tmem_at);
+    // while the kernel before this one may still run: the first weights on their way into L2
+    if (warp == 0 && t0 == 0)
+        for (int i = lane; i < 2 * kParts * min(n, C::kStages); i += 32)
+            tc::prefetch_3d(&w_map, (b0 + i / (2 * kParts)) * kBlock, tile * kTile + (i & 1) * kBox, i / 2 % kParts);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(generic + (tmem_at - base));
+    grid_dep_launch_next();
+    grid_dep_wait();
 
     float acc[C::kMine];
 #pragma unroll
@@ -197,13 +201,13 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
         const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21) + group * C::kMine;
         const float* ws = a.w_scale + (int64_t)tile * a.k_blocks + b0;
         const int64_t up = (int64_t)a.row_blocks * a.k_blocks;
-        constexpr int kEach = (C::kAhead * kTok + C::kThreads - 65) / (C::kThreads - 64);
+        constexpr int kEach = (C::kAhead * kTok + C::kReaders - 1) / C::kReaders;
         // token scales of a few blocks times the weights' scale, one turn ahead in registers, then in shared memory
         float next[kEach][kParts];
         auto fetch = [&](int first) {
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
-                const int i = e + j * (C::kThreads - 64), b = first + i / kTok;
+                const int i = e + j * C::kReaders, b = first + i / kTok;
                 const int64_t t = t0 + i % kTok;
                 const bool in = i < C::kAhead * kTok && b < n && t < a.tokens;
                 const float x = in ? a.x_scale[t * a.xs_token + (b0 + b) * a.xs_block] : 0.f;
@@ -218,12 +222,12 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
             if (kb % C::kAhead == 0) {
 #pragma unroll
                 for (int j = 0; j < kEach; ++j) {
-                    const int i = e + j * (C::kThreads - 64);
+                    const int i = e + j * C::kReaders;
                     if (i < C::kAhead * kTok)
 #pragma unroll
                         for (int p = 0; p < kParts; ++p) sc[(i / kTok) * C::kCols + p * kTok + i % kTok] = next[j][p];
                 }
-                asm volatile("bar.sync 1, %0;" ::"n"(C::kThreads - 64) : "memory");
+                asm volatile("bar.sync 1, %0;" ::"n"(C::kReaders) : "memory");
                 fetch(kb + C::kAhead);
             }
             const float4* by = reinterpret_cast<const float4*>(sc + (kb % C::kAhead) * C::kCols + group * C::kMine);
@@ -232,16 +236,16 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
             tc::fence_after();
             if (ok) {
 #pragma unroll
-                for (int c = 0; c < C::kMine; c += 16) {
-                    uint32_t v[16];
-                    tc::ld16(mine + b * C::kCols + c, v);
+                for (int c = 0; c < C::kMine; c += C::kLoad) {
+                    uint32_t v[C::kLoad];
+                    tc::ld(mine + b * C::kCols + c, v);
                     tc::wait_ld(v);
-                    if (c + 16 == C::kMine) {
+                    if (c + C::kLoad == C::kMine) {
                         tc::fence_before();
                         if (lane == 0) tc::arrive(sum_empty + 8 * b);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < C::kLoad / 4; ++i) {
                         const float4 s = by[c / 4 + i];
                         acc[c + 4 * i] = fmaf(__uint_as_float(v[4 * i]), s.x, acc[c + 4 * i]);
                         acc[c + 4 * i + 1] = fmaf(__uint_as_float(v[4 * i + 1]), s.y, acc[c + 4 * i + 1]);
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
     }
     __syncthreads();
     tc::fence_after();
-    if (warp == 1) tc::tmem_free(tmem, C::kTmem);
+    if (warp == 1) tc::tmem_free<C::kTmem>(tmem);
 
     // The CTAs' parts, token by token [part][token][feature] in the ring's place; the cluster's CTAs take the tokens in turn.
     float* const join = reinterpret_cast<float*>(generic);
@@ -436,6 +440,8 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
     tc::cluster_sync();  // both CTAs' barriers
     tc::fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(generic + (tmem_at - base));
+    grid_dep_launch_next();
+    grid_dep_wait();
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -559,7 +565,7 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         uint32_t v[32];
-                        tc::ld32(mine + (done & 1) * 2 * kTile + 32 * c, v);
+                        tc::ld(mine + (done & 1) * 2 * kTile + 32 * c, v);
                         tc::wait_ld(v);
                         if (c == 1) {
                             tc::fence_before();
@@ -724,13 +730,54 @@ static int sm_count() {
     return count[dev];
 }
 
-// CTAs of a cluster that share a tile's inner dimension: the number for which the waves of CTAs take the fewest blocks
+static cudaLaunchConfig_t configure(cudaLaunchAttribute (&attr)[2], unsigned x, unsigned y, int threads, int smem,
+                                    unsigned cluster, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(x, y, 1);
+    cfg.blockDim = dim3((unsigned)threads, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cfg;
+}
+
+// Clusters of s CTAs (s = 1..8) that the current device holds at once: a cluster lies within one of its groups of SMs, so
+// that of three, five or seven CTAs many SMs stay empty.  The same for all of these kernels, which have an SM to
+// themselves.
+struct Places {
+    int clusters[9];
+};
+template <typename Kernel>
+static const Places* places(Kernel kernel, int threads, int smem) {
+    static std::mutex mutex;
+    static Places known[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    const std::lock_guard<std::mutex> lock(mutex);
+    Places& p = known[dev];
+    if (!p.clusters[1])
+        for (int s = 8; s >= 1; --s) {
+            cudaLaunchAttribute attr[2];
+            cudaLaunchConfig_t cfg = configure(attr, 64 * s, 1, threads, smem, s, nullptr);
+            if (cudaOccupancyMaxActiveClusters(&p.clusters[s], kernel, &cfg) != cudaSuccess) return nullptr;
+        }
+    return &p;
+}
+
+// CTAs of a cluster that share a tile's inner dimension: the number for which the waves of clusters take the fewest blocks
 // after one another, each wave with a fixed cost of about four blocks (filling the ring, joining the parts).
-static int parts_of(int64_t tiles, int k_blocks, int places) {
+static int parts_of(int64_t tiles, int k_blocks, const Places& p) {
     int best = 1;
     int64_t least = INT64_MAX;
     for (int s = 1; s <= 8 && s <= k_blocks; ++s) {
-        const int64_t waves = (tiles * s + places - 1) / places, cost = waves * ((k_blocks + s - 1) / s + 4);
+        if (p.clusters[s] < 1) continue;
+        const int64_t waves = (tiles + p.clusters[s] - 1) / p.clusters[s], cost = waves * ((k_blocks + s - 1) / s + 4);
         if (cost < least) least = cost, best = s;
     }
     return best;
@@ -741,24 +788,16 @@ static int launch_few(const zkv_fp8_weight* w, const void* x, int64_t x_ld, cons
     using C = Few<kTok, kParts>;
     CUtensorMap x_map;
     if (!encode_rows(&x_map, x, w->k, a.tokens, x_ld, 0, kTok)) return ZKV_ERR_ARG;
-    const int sms = sm_count();
-    if (!sms) return launch_refused();
     const int64_t wide = (a.tokens + kTok - 1) / kTok;
     if (wide > 65535) return ZKV_ERR_CAPACITY;
-    const int parts = parts_of(a.row_blocks * wide, a.k_blocks, sms * C::kPerSM);
     auto kernel = few_kernel<kTok, kParts>;
     if (!raise_smem_limit((const void*)kernel, C::kSmem)) return launch_refused();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.row_blocks * parts), (unsigned)wide, 1);
-    cfg.blockDim = dim3(C::kThreads, 1, 1);
-    cfg.dynamicSmemBytes = C::kSmem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)parts;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    const Places* p = places(kernel, C::kThreads, C::kSmem);
+    if (!p) return launch_refused();
+    const int parts = parts_of(a.row_blocks * wide, a.k_blocks, *p);
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t cfg =
+        configure(attr, (unsigned)(a.row_blocks * parts), (unsigned)wide, C::kThreads, C::kSmem, (unsigned)parts, stream);
     CUtensorMap w_map;
     memcpy(&w_map, w->map, sizeof w_map);
     if (cudaLaunchKernelEx(&cfg, kernel, w_map, x_map, a) != cudaSuccess) return launch_refused();
@@ -795,17 +834,9 @@ static int launch_many(const zkv_fp8_weight* w, const void* x, int64_t x_ld, con
     auto kernel = many_kernel<kGated>;
     if (!raise_smem_limit((const void*)kernel, C::kSmem)) return launch_refused();
     const ManyTiles tiles = {(int)m, (int)n, (int)(m * n)};
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)std::min<int64_t>(2 * m * n, sms / 2 * 2), 1, 1);
-    cfg.blockDim = dim3(C::kThreads, 1, 1);
-    cfg.dynamicSmemBytes = C::kSmem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t cfg =
+        configure(attr, (unsigned)std::min<int64_t>(2 * m * n, sms / 2 * 2), 1, C::kThreads, C::kSmem, 2, stream);
     if (cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], a, tiles, mapped) != cudaSuccess) return launch_refused();
     return launch_status();
 }

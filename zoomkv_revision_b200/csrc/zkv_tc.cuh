@@ -73,6 +73,11 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const void* map, int x, int
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
+// The tile into L2 only: it may be asked for before an earlier kernel has ended, as L2 is where its writes go too.
+__device__ __forceinline__ void prefetch_3d(const void* map, int x, int y, int z) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const void* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -150,12 +155,14 @@ __device__ __forceinline__ void copy4_wait() { asm volatile("cp.async.wait_all;"
 
 // ------------------------------------------------------------ tensor memory
 // 128 lanes x 512 columns of 32 bits an SM.  alloc and free by one whole warp.
-__device__ __forceinline__ void tmem_alloc(uint32_t to, uint32_t columns) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "r"(columns) : "memory");
+template <int kColumns>
+__device__ __forceinline__ void tmem_alloc(uint32_t to) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "n"(kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
+template <int kColumns>
+__device__ __forceinline__ void tmem_free(uint32_t at) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "n"(kColumns) : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -179,7 +186,7 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 }
 
 // 16 columns of the warp's 32 lanes: thread = lane, register = column.
-__device__ __forceinline__ void ld16(uint32_t at, uint32_t (&r)[16]) {
+__device__ __forceinline__ void ld(uint32_t at, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
@@ -188,7 +195,7 @@ __device__ __forceinline__ void ld16(uint32_t at, uint32_t (&r)[16]) {
 }
 
 // 32 columns of the warp's 32 lanes.
-__device__ __forceinline__ void ld32(uint32_t at, uint32_t (&r)[32]) {
+__device__ __forceinline__ void ld(uint32_t at, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
         "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
