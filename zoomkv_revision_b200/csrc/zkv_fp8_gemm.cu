@@ -52,22 +52,32 @@ struct Few {
     static constexpr int kReaders = 128 * kGroups, kThreads = 64 + kReaders;
     static constexpr int kMine = kCols / kGroups;  // columns of a thread
     static constexpr int kLoad = kMine == 32 ? 32 : 16;  // columns of a load (64 columns: what registers leave room for)
-    // One CTA an SM: its ring takes the shared memory, and no second CTA of these kernels fits beside it, so that no
-    // cluster's CTA waits for tensor memory which another cluster, waiting for a CTA of its own, holds.
-    static constexpr int kBufs = 512 / kCols < 8 ? 512 / kCols : 8;
+    static constexpr int kBufs = kCols >= 128 ? 2 : kCols == 64 ? 4 : 8;
     static constexpr int kTmem = kCols * kBufs;
     static constexpr int kStage = kParts * kTileBytes + kTok * kBlock;
     static constexpr int kAhead = 4;  // blocks of scales staged at a time
     static constexpr int kScales = 2 * kAhead * kCols * 4;
-    static constexpr int kRoom = 227 * 1024 - 1024 - kScales - 512;
-    static constexpr int kStages = kRoom / kStage < 12 ? kRoom / kStage : 12;
-    static constexpr int kSmem = 1024 + kStages * kStage + kScales + 512;
     static constexpr int kJoin = kParts == 2 && kTok > 64 ? 64 : kTok;  // tokens joined at a time
+    static constexpr int kMost = 12;  // stages of the ring: barriers
+    static constexpr int smem(int stages) { return 1024 + stages * kStage + kScales + 512; }
+    static constexpr int stages_in(int bytes) {
+        return (bytes - smem(0)) / kStage < kMost ? (bytes - smem(0)) / kStage : kMost;
+    }
+    // The ring takes an SM's shared memory, or half of it, for two CTAs an SM.  The CTAs of a cluster wait for one
+    // another, so none may have to wait for tensor memory that a CTA of another cluster holds on its SM: at most two of
+    // these kernels' CTAs fit on one (each takes more than a third of the shared memory), with at most half of the tensor
+    // memory each; or one alone.
+    // Two an SM for one part and up to 32 tokens (151936 x 4096: 8 tokens 97 us, 106 with one; 32 tokens 101 and 119):
+    // more take the registers of one, and two parts' stages are too few in half the memory (8 tokens of 12288 x 4096: 23.3
+    // us, 21.7 with one).
+    static constexpr bool kHalves = kParts == 1 && kTok <= 32;
+    static constexpr int kStages = stages_in((kHalves ? 113 : 227) * 1024);
     static_assert(kTmem >= 32 && kTmem <= 512 && (kTmem & (kTmem - 1)) == 0, "tensor memory comes in powers of two");
+    static_assert(kTmem <= 256 || smem(kStages) > (227 - 76) * 1024, "alone on its SM");
+    static_assert(smem(kStages) > 76 * 1024, "no third CTA on an SM");
     static_assert(kMine % kLoad == 0, "whole loads");
-    static_assert(16 * (kStages + kBufs) + 4 <= 512, "barriers");
-    static_assert(kSmem > 114 * 1024 && kSmem <= 227 * 1024, "one CTA an SM");
-    static_assert(kJoin * kParts * kTile * 4 <= kStages * kStage, "the parts are joined in the ring's place");
+    static_assert(16 * (kMost + kBufs) + 4 <= 512, "barriers");
+    static_assert(kStages >= 2 && kJoin * kParts * kTile * 4 <= kStages * kStage, "the parts are joined in the ring's place");
 };
 
 __device__ __forceinline__ void store4(const Product& a, int64_t token, int f, float4 y) {
@@ -107,7 +117,7 @@ __device__ __forceinline__ void store4(const Product& a, int64_t token, int f, f
 __device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
 template <int kTok, int kParts>
-__global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
+__global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
     few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, Product a) {
     using C = Few<kTok, kParts>;
     extern __shared__ uint8_t smem_raw[];
@@ -155,10 +165,9 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
     for (int c = 0; c < C::kMine; ++c) acc[c] = 0.f;
 
     if (warp == 0) {
-        int got = 0;
+        int got = 0, s = 0, phase = 1;  // of `empty`: a fresh barrier's last phase counts as over
         for (; got < n; ++got) {
-            const int s = got % C::kStages, turn = got / C::kStages;
-            if (turn > 0 && !tc::wait_all(empty + 8 * s, (turn - 1) & 1, a.status)) break;
+            if (!tc::wait_all(empty + 8 * s, phase, a.status)) break;
             const uint32_t at = base + s * C::kStage, bar = full + 8 * s;
             if (tc::elected()) {
                 tc::arrive_expect_tx(bar, C::kStage);
@@ -167,17 +176,18 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
                 tc::tma_2d(at + kParts * kTileBytes, &x_map, (b0 + got) * kBlock, (int)t0, bar);
             }
             __syncwarp();
+            if (++s == C::kStages) s = 0, phase ^= 1;
         }
         // every copy has landed before the CTA ends, whatever became of the others
         for (int i = got > C::kStages ? got - C::kStages : 0; i < got; ++i)
             if (!tc::wait_all(full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.status)) break;
     } else if (warp == 1) {
         constexpr uint32_t desc = tc::e4m3_desc(kTile, kTok);
-        int done = 0;
+        int done = 0, s = 0, phase = 0;
         for (; done < n; ++done) {
-            const int s = done % C::kStages, b = done % C::kBufs, turn = done / C::kBufs;
-            if (!tc::wait_all(full + 8 * s, (done / C::kStages) & 1, a.status)) break;
+            const int b = done % C::kBufs, turn = done / C::kBufs;
             if (turn > 0 && !tc::wait_all(sum_empty + 8 * b, (turn - 1) & 1, a.status)) break;
+            if (!tc::wait_all(full + 8 * s, phase, a.status)) break;
             tc::fence_after();
             const uint32_t at = base + s * C::kStage;
             const uint64_t x = tc::tile_desc(at + kParts * kTileBytes);
@@ -189,10 +199,11 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads)
                     for (int k = 0; k < kBlock / 32; ++k)  // 32 bytes further: 2 of the descriptor's 16
                         tc::mma_e4m3(tmem + b * C::kCols + p * kTok, w + 2 * k, x + 2 * k, desc, k > 0);
                 }
-                tc::commit(empty + 8 * s);
                 tc::commit(sum_full + 8 * b);
+                tc::commit(empty + 8 * s);
             }
             __syncwarp();
+            if (++s == C::kStages) s = 0, phase ^= 1;
         }
         // the last products have ended before tensor memory is given back
         if (done > 0) tc::wait_all(sum_full + 8 * ((done - 1) % C::kBufs), ((done - 1) / C::kBufs) & 1, a.status);
@@ -770,14 +781,17 @@ static const Places* places(Kernel kernel, int threads, int smem) {
     return &p;
 }
 
-// CTAs of a cluster that share a tile's inner dimension: the number for which the waves of clusters take the fewest blocks
-// after one another, each wave with a fixed cost of about four blocks (filling the ring, joining the parts).
-static int parts_of(int64_t tiles, int k_blocks, const Places& p) {
+// How the inner dimension is cut over a cluster's CTAs: the number for which the waves of clusters take the fewest blocks
+// after one another, each wave with a fixed cost of some blocks (filling the ring, joining the parts).  `halves`: two CTAs
+// an SM.  8 tokens, us by CTAs of a cluster: 4096 x 4096 1: 10.3, 2: 7.6, 4: 6.2, 8: 6.9; 6144 x 4096 11.0, 7.8, 6.9, 11.0;
+// 4096 x 12288 26.7, 16.7, 13.1, 12.4; 151936 x 4096 97, 102, 124, 194.
+static int parts_of(int64_t tiles, int k_blocks, bool halves, const Places& p) {
     int best = 1;
     int64_t least = INT64_MAX;
     for (int s = 1; s <= 8 && s <= k_blocks; ++s) {
-        if (p.clusters[s] < 1) continue;
-        const int64_t waves = (tiles + p.clusters[s] - 1) / p.clusters[s], cost = waves * ((k_blocks + s - 1) / s + 4);
+        const int64_t at_once = (halves ? 2 : 1) * p.clusters[s];
+        if (at_once < 1) continue;
+        const int64_t waves = (tiles + at_once - 1) / at_once, cost = waves * ((k_blocks + s - 1) / s + 4 + s);
         if (cost < least) least = cost, best = s;
     }
     return best;
@@ -791,13 +805,13 @@ static int launch_few(const zkv_fp8_weight* w, const void* x, int64_t x_ld, cons
     const int64_t wide = (a.tokens + kTok - 1) / kTok;
     if (wide > 65535) return ZKV_ERR_CAPACITY;
     auto kernel = few_kernel<kTok, kParts>;
-    if (!raise_smem_limit((const void*)kernel, C::kSmem)) return launch_refused();
-    const Places* p = places(kernel, C::kThreads, C::kSmem);
+    if (!raise_smem_limit((const void*)kernel, C::smem(C::kStages))) return launch_refused();
+    const Places* p = places(kernel, C::kThreads, C::smem(C::kStages));
     if (!p) return launch_refused();
-    const int parts = parts_of(a.row_blocks * wide, a.k_blocks, *p);
+    const int parts = parts_of(a.row_blocks * wide, a.k_blocks, C::kHalves, *p);
     cudaLaunchAttribute attr[2];
-    const cudaLaunchConfig_t cfg =
-        configure(attr, (unsigned)(a.row_blocks * parts), (unsigned)wide, C::kThreads, C::kSmem, (unsigned)parts, stream);
+    const cudaLaunchConfig_t cfg = configure(attr, (unsigned)(a.row_blocks * parts), (unsigned)wide, C::kThreads,
+                                             C::smem(C::kStages), (unsigned)parts, stream);
     CUtensorMap w_map;
     memcpy(&w_map, w->map, sizeof w_map);
     if (cudaLaunchKernelEx(&cfg, kernel, w_map, x_map, a) != cudaSuccess) return launch_refused();
