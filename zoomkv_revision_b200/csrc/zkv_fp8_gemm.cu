@@ -47,9 +47,12 @@ struct Product {
 // kTok tokens and kParts tiles of 128 features a CTA.
 template <int kTok, int kParts>
 struct Few {
-    static constexpr int kCols = kTok * kParts;
+    // 128 tokens are the rows of the tensor core's tile themselves: a reader then has a token of its own and one scale for
+    // all its columns, where with features as rows it loads a scale for each (as many bytes of shared memory as of sums).
+    static constexpr bool kTokenRows = kTok == kTile;
+    static constexpr int kCols = kTok * kParts;  // columns of tensor memory for a block
     static constexpr int kGroups = kCols >= 128 ? 4 : kCols >= 64 ? 2 : 1;  // warpgroups that take the sums out of tensor memory
-    static constexpr int kReaders = 128 * kGroups, kThreads = 64 + kReaders;
+    static constexpr int kReaders = 128 * kGroups, kThreads = 96 + kReaders;
     static constexpr int kMine = kCols / kGroups;  // columns of a thread
     static constexpr int kLoad = kMine == 32 ? 32 : 16;  // columns of a load (64 columns: what registers leave room for)
     static constexpr int kBufs = kCols >= 128 ? 2 : kCols == 64 ? 4 : 8;
@@ -58,6 +61,7 @@ struct Few {
     static constexpr int kAhead = 4;  // blocks of scales staged at a time
     static constexpr int kScales = 2 * kAhead * kCols * 4;
     static constexpr int kJoin = kParts == 2 && kTok > 64 ? 64 : kTok;  // tokens joined at a time
+    static constexpr int kPitch = kTokenRows ? kTile + 4 : kTile;  // floats from token to token where they are joined
     static constexpr int kMost = 12;  // stages of the ring: barriers
     static constexpr int smem(int stages) { return 1024 + stages * kStage + kScales + 512; }
     static constexpr int stages_in(int bytes) {
@@ -71,13 +75,17 @@ struct Few {
     // more take the registers of one, and two parts' stages are too few in half the memory (8 tokens of 12288 x 4096: 23.3
     // us, 21.7 with one).
     static constexpr bool kHalves = kParts == 1 && kTok <= 32;
-    static constexpr int kStages = stages_in((kHalves ? 113 : 227) * 1024);
+    // Even, as the buffers are: a stage is always the same issuing warp's.  A wait for a phase by its parity lets a warp
+    // through at once while the phase before, another warp's, has not ended.
+    static constexpr int kStages = stages_in((kHalves ? 113 : 227) * 1024) / 2 * 2;
+    static_assert(kStages % 2 == 0 && kBufs % 2 == 0, "a stage and a buffer have one issuing warp");
     static_assert(kTmem >= 32 && kTmem <= 512 && (kTmem & (kTmem - 1)) == 0, "tensor memory comes in powers of two");
     static_assert(kTmem <= 256 || smem(kStages) > (227 - 76) * 1024, "alone on its SM");
     static_assert(smem(kStages) > 76 * 1024, "no third CTA on an SM");
     static_assert(kMine % kLoad == 0, "whole loads");
     static_assert(16 * (kMost + kBufs) + 4 <= 512, "barriers");
-    static_assert(kStages >= 2 && kJoin * kParts * kTile * 4 <= kStages * kStage, "the parts are joined in the ring's place");
+    static_assert(kTokenRows || kJoin == kTok, "token chunks");
+    static_assert(kStages >= 2 && kJoin * kParts * kPitch * 4 <= kStages * kStage, "the parts are joined in the ring's place");
 };
 
 __device__ __forceinline__ void store4(const Product& a, int64_t token, int f, float4 y) {
@@ -181,34 +189,42 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
         // every copy has landed before the CTA ends, whatever became of the others
         for (int i = got > C::kStages ? got - C::kStages : 0; i < got; ++i)
             if (!tc::wait_all(full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.status)) break;
-    } else if (warp == 1) {
-        constexpr uint32_t desc = tc::e4m3_desc(kTile, kTok);
-        int done = 0, s = 0, phase = 0;
-        for (; done < n; ++done) {
-            const int b = done % C::kBufs, turn = done / C::kBufs;
+    } else if (warp <= 2) {
+        // Two warps issue every other block's products: a pass of two barriers takes one some 400 clocks.
+        int done = warp - 1;
+        for (; done < n; done += 2) {
+            const int s = done % C::kStages, b = done % C::kBufs, turn = done / C::kBufs;
             if (turn > 0 && !tc::wait_all(sum_empty + 8 * b, (turn - 1) & 1, a.status)) break;
-            if (!tc::wait_all(full + 8 * s, phase, a.status)) break;
+            if (!tc::wait_all(full + 8 * s, (done / C::kStages) & 1, a.status)) break;
             tc::fence_after();
-            const uint32_t at = base + s * C::kStage;
+            const uint32_t at = base + s * C::kStage, d = tmem + b * C::kCols;
             const uint64_t x = tc::tile_desc(at + kParts * kTileBytes);
             if (tc::elected()) {
-#pragma unroll
-                for (int p = 0; p < kParts; ++p) {
-                    const uint64_t w = tc::tile_desc(at + p * kTileBytes);
+                if (C::kTokenRows) {
+                    constexpr uint32_t desc = tc::e4m3_desc(kTile, kParts * kTile);
+                    const uint64_t w = tc::tile_desc(at);
 #pragma unroll
                     for (int k = 0; k < kBlock / 32; ++k)  // 32 bytes further: 2 of the descriptor's 16
-                        tc::mma_e4m3(tmem + b * C::kCols + p * kTok, w + 2 * k, x + 2 * k, desc, k > 0);
+                        tc::mma_e4m3(d, x + 2 * k, w + 2 * k, desc, k > 0);
+                } else {
+                    constexpr uint32_t desc = tc::e4m3_desc(kTile, kTok);
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p) {
+                        const uint64_t w = tc::tile_desc(at + p * kTileBytes);
+#pragma unroll
+                        for (int k = 0; k < kBlock / 32; ++k) tc::mma_e4m3(d + p * kTok, w + 2 * k, x + 2 * k, desc, k > 0);
+                    }
                 }
                 tc::commit(sum_full + 8 * b);
                 tc::commit(empty + 8 * s);
             }
             __syncwarp();
-            if (++s == C::kStages) s = 0, phase ^= 1;
         }
-        // the last products have ended before tensor memory is given back
-        if (done > 0) tc::wait_all(sum_full + 8 * ((done - 1) % C::kBufs), ((done - 1) / C::kBufs) & 1, a.status);
+        // its last products have ended before tensor memory is given back
+        done -= 2;
+        if (done >= 0) tc::wait_all(sum_full + 8 * (done % C::kBufs), (done / C::kBufs) & 1, a.status);
     } else {
-        const int e = threadIdx.x - 64, group = (warp - 2) >> 2;
+        const int e = threadIdx.x - 96, group = (warp - 3) >> 2;
         const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21) + group * C::kMine;
         const float* ws = a.w_scale + (int64_t)tile * a.k_blocks + b0;
         const int64_t up = (int64_t)a.row_blocks * a.k_blocks;
@@ -241,7 +257,9 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
                 asm volatile("bar.sync 1, %0;" ::"n"(C::kReaders) : "memory");
                 fetch(kb + C::kAhead);
             }
-            const float4* by = reinterpret_cast<const float4*>(sc + (kb % C::kAhead) * C::kCols + group * C::kMine);
+            const float* by = sc + (kb % C::kAhead) * C::kCols +
+                              (C::kTokenRows ? group * C::kMine / kTile * kTile + (warp & 3) * 32 + lane : group * C::kMine);
+            const float own = *by;  // token rows: this thread's
             const int b = kb % C::kBufs;
             ok = __all_sync(0xffffffffu, ok && tc::wait_for(sum_full + 8 * b, (kb / C::kBufs) & 1, a.status));
             tc::fence_after();
@@ -256,12 +274,13 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
                         if (lane == 0) tc::arrive(sum_empty + 8 * b);
                     }
 #pragma unroll
-                    for (int i = 0; i < C::kLoad / 4; ++i) {
-                        const float4 s = by[c / 4 + i];
-                        acc[c + 4 * i] = fmaf(__uint_as_float(v[4 * i]), s.x, acc[c + 4 * i]);
-                        acc[c + 4 * i + 1] = fmaf(__uint_as_float(v[4 * i + 1]), s.y, acc[c + 4 * i + 1]);
-                        acc[c + 4 * i + 2] = fmaf(__uint_as_float(v[4 * i + 2]), s.z, acc[c + 4 * i + 2]);
-                        acc[c + 4 * i + 3] = fmaf(__uint_as_float(v[4 * i + 3]), s.w, acc[c + 4 * i + 3]);
+                    for (int i = 0; i < C::kLoad; i += 4) {
+                        const float4 s = C::kTokenRows ? make_float4(own, own, own, own)
+                                                       : *reinterpret_cast<const float4*>(by + c + i);
+                        acc[c + i] = fmaf(__uint_as_float(v[i]), s.x, acc[c + i]);
+                        acc[c + i + 1] = fmaf(__uint_as_float(v[i + 1]), s.y, acc[c + i + 1]);
+                        acc[c + i + 2] = fmaf(__uint_as_float(v[i + 2]), s.z, acc[c + i + 2]);
+                        acc[c + i + 3] = fmaf(__uint_as_float(v[i + 3]), s.w, acc[c + i + 3]);
                     }
                 }
             }
@@ -272,48 +291,74 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
     tc::fence_after();
     if (warp == 1) tc::tmem_free<C::kTmem>(tmem);
 
-    // The CTAs' parts, token by token [part][token][feature] in the ring's place; the cluster's CTAs take the tokens in turn.
+    // The CTAs' parts, token by token [part][token][feature] in the ring's place; the cluster's CTAs take the tokens in
+    // turn, a warp a token, two at a time.
     float* const join = reinterpret_cast<float*>(generic);
 #pragma unroll
     for (int c0 = 0; c0 < kTok; c0 += C::kJoin) {
-        if (warp >= 2) {
-            const int f = (warp & 3) * 32 + lane, first = (warp - 2) / 4 * C::kMine;
+        if (warp >= 3) {
+            const int row = (warp & 3) * 32 + lane, first = (warp - 3) / 4 * C::kMine;
+            if (C::kTokenRows) {
+                if (row >= c0 && row < c0 + C::kJoin) {
+                    float* to = join + (first / kTile * C::kJoin + row - c0) * C::kPitch + first % kTile;
 #pragma unroll
-            for (int c = 0; c < C::kMine; ++c) {
-                const int col = first + c, t = col % kTok - c0;
-                if (t >= 0 && t < C::kJoin) join[(col / kTok * C::kJoin + t) * kTile + f] = acc[c];
+                    for (int c = 0; c < C::kMine; c += 4)
+                        *reinterpret_cast<float4*>(to + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < C::kMine; ++c) {
+                    const int col = first + c;
+                    join[(col / kTok * C::kJoin + col % kTok) * C::kPitch + row] = acc[c];
+                }
             }
         }
         if (parts > 1) tc::cluster_sync();
         else __syncthreads();
-        for (int t = warp * parts + rank; t < C::kJoin; t += C::kThreads / 32 * parts) {
+        const int turn = C::kThreads / 32 * parts, f = tile * kTile + lane * 4;
+        for (int t = warp * parts + rank; t < C::kJoin; t += 2 * turn) {
             const int64_t token = t0 + c0 + t;
             if (token >= a.tokens) break;
-            float4 y[kParts];
+            const bool both = t + turn < C::kJoin && token + turn < a.tokens;
+            float4 y[2][kParts];
 #pragma unroll
-            for (int p = 0; p < kParts; ++p) {
-                const uint32_t at = base + ((p * C::kJoin + t) * kTile + lane * 4) * 4;
-                y[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (uint32_t r = 0; r < parts; ++r) {
-                    const float4 v = tc::ld_cluster(tc::in_cta(at, r));
-                    y[p].x += v.x, y[p].y += v.y, y[p].z += v.z, y[p].w += v.w;
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    const int at = (p * C::kJoin + (u && both ? t + turn : t)) * C::kPitch + lane * 4;
+                    if (parts == 1) {
+                        y[u][p] = *reinterpret_cast<const float4*>(join + at);
+                    } else {
+                        y[u][p] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (uint32_t r = 0; r < parts; ++r) {
+                            const float4 v = tc::ld_cluster(tc::in_cta(base + at * 4, r));
+                            y[u][p].x += v.x, y[u][p].y += v.y, y[u][p].z += v.z, y[u][p].w += v.w;
+                        }
+                    }
                 }
-            }
-            const int f = tile * kTile + lane * 4;
             if (kParts == 1) {
-                store4(a, token, f, y[0]);
+                store4(a, token, f, y[0][0]);
+                if (both) store4(a, token + turn, f, y[1][0]);
             } else {
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (f < a.rows)  // rows are whole 16 bytes
-                    v = make_float4(gated(y[0].x, y[kParts - 1].x), gated(y[0].y, y[kParts - 1].y),
-                                    gated(y[0].z, y[kParts - 1].z), gated(y[0].w, y[kParts - 1].w));
-                const uint32_t m = __reduce_max_sync(
-                    0xffffffffu, max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w))));
-                const float s = scale_of(m);
-                if (f < a.rows)
-                    *reinterpret_cast<uint32_t*>((uint8_t*)a.out + token * a.out_ld + f) =
-                        Quotient(s).e4m3(v.x, v.y, v.z, v.w);
-                if (lane == 0) a.out_scale[token * a.os_token + tile * a.os_block] = s;
+                uint32_t q[2];
+                float s[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float4 g = y[u][0], h = y[u][kParts - 1];
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (f < a.rows)  // rows are whole 16 bytes
+                        v = make_float4(gated(g.x, h.x), gated(g.y, h.y), gated(g.z, h.z), gated(g.w, h.w));
+                    s[u] = scale_of(__reduce_max_sync(
+                        0xffffffffu, max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w)))));
+                    q[u] = Quotient(s[u]).e4m3(v.x, v.y, v.z, v.w);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (u && !both) break;
+                    const int64_t to = token + (u ? turn : 0);
+                    if (f < a.rows) *reinterpret_cast<uint32_t*>((uint8_t*)a.out + to * a.out_ld + f) = q[u];
+                    if (lane == 0) a.out_scale[to * a.os_token + tile * a.os_block] = s[u];
+                }
             }
         }
         if (parts > 1) tc::cluster_sync();
