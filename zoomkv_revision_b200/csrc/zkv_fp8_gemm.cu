@@ -830,14 +830,17 @@ static const Places* places(Kernel kernel, int threads, int smem) {
 // after one another, each wave with a fixed cost of some blocks (filling the ring, joining the parts).  `halves`: two CTAs
 // an SM.  8 tokens, us by CTAs of a cluster: 4096 x 4096 1: 10.3, 2: 7.6, 4: 6.2, 8: 6.9; 6144 x 4096 11.0, 7.8, 6.9, 11.0;
 // 4096 x 12288 26.7, 16.7, 13.1, 12.4; 151936 x 4096 97, 102, 124, 194.
-static int parts_of(int64_t tiles, int k_blocks, bool halves, const Places& p) {
-    int best = 1;
-    int64_t least = INT64_MAX;
+struct Cut {
+    int parts;
+    int64_t cost;  // in blocks of the inner dimension
+};
+static Cut cut_of(int64_t tiles, int k_blocks, bool halves, const Places& p) {
+    Cut best = {1, INT64_MAX};
     for (int s = 1; s <= 8 && s <= k_blocks; ++s) {
         const int64_t at_once = (halves ? 2 : 1) * p.clusters[s];
         if (at_once < 1) continue;
         const int64_t waves = (tiles + at_once - 1) / at_once, cost = waves * ((k_blocks + s - 1) / s + 4 + s);
-        if (cost < least) least = cost, best = s;
+        if (cost < best.cost) best = {s, cost};
     }
     return best;
 }
@@ -853,7 +856,7 @@ static int launch_few(const zkv_fp8_weight* w, const void* x, int64_t x_ld, cons
     if (!raise_smem_limit((const void*)kernel, C::smem(C::kStages))) return launch_refused();
     const Places* p = places(kernel, C::kThreads, C::smem(C::kStages));
     if (!p) return launch_refused();
-    const int parts = parts_of(a.row_blocks * wide, a.k_blocks, C::kHalves, *p);
+    const int parts = cut_of(a.row_blocks * wide, a.k_blocks, C::kHalves, *p).parts;
     cudaLaunchAttribute attr[2];
     const cudaLaunchConfig_t cfg = configure(attr, (unsigned)(a.row_blocks * parts), (unsigned)wide, C::kThreads,
                                              C::smem(C::kStages), (unsigned)parts, stream);
@@ -925,12 +928,26 @@ static int check_call(const void* x, int64_t x_ld, const float* x_scale, int64_t
     return ZKV_OK;
 }
 
+// Up to 64 tokens features are the rows of a tile.  Above, CTAs of 128 tokens and one part's 128 features each (a cluster
+// may share a tile), or pairs of CTAs of 256 tokens and 256 features: by the blocks that the waves of either take after one
+// another.  A block takes the pair a little longer, and CTAs of two parts twice as long.  us of the first and of the second
+// kind: 333 x 4096 x 4096 16.3 and 19.3, 768 x 4096 x 4096 34.5 and 20.5, 512 x 4096 x 12288 41.1 and 46.5, 129 x 2 x 12288
+// x 4096 60.9 and 43.0, 1024 x 1024 x 4096 11.7 and 18.6.
 template <int kParts>
 static int launch(const zkv_fp8_weight* w, const void* x, int64_t x_ld, const Product& a, cudaStream_t stream) {
     if (a.tokens <= 16) return launch_few<16, kParts>(w, x, x_ld, a, stream);
     if (a.tokens <= 32) return launch_few<32, kParts>(w, x, x_ld, a, stream);
     if (a.tokens <= 64) return launch_few<64, kParts>(w, x, x_ld, a, stream);
-    if (a.tokens <= 256) return launch_few<128, kParts>(w, x, x_ld, a, stream);
+    using C = Few<128, kParts>;
+    auto kernel = few_kernel<128, kParts>;
+    const Places* p = raise_smem_limit((const void*)kernel, C::smem(C::kStages)) ? places(kernel, C::kThreads, C::smem(C::kStages))
+                                                                                 : nullptr;
+    if (!p) return launch_refused();
+    const int64_t few = kParts * cut_of(a.row_blocks * ((a.tokens + 127) / 128), a.k_blocks, false, *p).cost;
+    const int64_t pairs = std::max(p->clusters[2], 1);
+    const int64_t tiles = (a.tokens + 255) / 256 * (kParts == 2 ? a.row_blocks : (a.row_blocks + 1) / 2);
+    const int64_t many = (tiles + pairs - 1) / pairs * a.k_blocks * 11 / 10 + 9;
+    if (few <= many) return launch_few<128, kParts>(w, x, x_ld, a, stream);
     return launch_many<kParts == 2>(w, x, x_ld, a, stream);
 }
 
