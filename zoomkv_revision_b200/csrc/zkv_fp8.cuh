@@ -28,27 +28,30 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     return lo | (hi << 16);
 }
 
-// e4m3 of the fp32 quotient by a block's scale, two roundings as defined, and
-// nearly always without a division: x times the reciprocal shrunk and grown
-// by 2^-21 encloses the quotient and its rounding (the products are off by
-// 3 * 2^-24 at most), rounding is monotone, so where both ends give one code
-// the quotient has it; else (that close to the middle of two codes) the
-// elements are divided.  A scale of 0 stores zeros.
+// e4m3 of the fp32 quotient by a block's scale, two roundings as defined,
+// without a division an element: from the correctly rounded reciprocal r, the
+// product q = x r and the remainder x - q s, which is exact in one fused
+// operation, q + r (x - q s) is the rounded quotient (P. Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000
+// processor", IBM J. Res. Dev. 34, 1990).  The division took 16383 x 4096
+// elements 53 us, and 50 to 69 where it decided only what two enclosing
+// products left open: an element in 16 of every seventh block of bf16 numbers
+// is the exact middle of two codes.  A scale of 0 stores zeros.
 struct Quotient {
-    float scale, low, high;
-    bool divide;  // the reciprocal is not an ordinary number
+    float scale, r;
+    bool divide;  // no ordinary numbers: the remainder could leave fp32's range
 
     __device__ __forceinline__ explicit Quotient(float s) {
-        const float r = __fdiv_rn(1.f, s);
         scale = s;
-        low = r * (1.f - 4.76837158203125e-7f);
-        high = r * (1.f + 4.76837158203125e-7f);
-        divide = !(s > 1e-30f && s < 1e30f);
+        r = __fdiv_rn(1.f, s);
+        divide = !(s > 1e-20f && s < 1e20f);
+    }
+    __device__ __forceinline__ float of(float x) const {
+        const float q = x * r;
+        return copysignf(fmaf(fmaf(-q, scale, x), r, q), x);  // (the remainder of -0 is +0)
     }
     __device__ __forceinline__ uint32_t e4m3(float a, float b, float c, float d) const {
-        const uint32_t x = e4m3x4(a * low, b * low, c * low, d * low);
-        const uint32_t y = e4m3x4(a * high, b * high, c * high, d * high);
-        if (x == y && !divide) return x;
+        if (!divide) return e4m3x4(of(a), of(b), of(c), of(d));
         if (scale == 0.f) return 0u;
         return e4m3x4(__fdiv_rn(a, scale), __fdiv_rn(b, scale), __fdiv_rn(c, scale), __fdiv_rn(d, scale));
     }
