@@ -38,22 +38,20 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 // products left open: an element in 16 of every seventh block of bf16 numbers
 // is the exact middle of two codes.  A scale of 0 stores zeros.
 struct Quotient {
-    float scale, r;
-    bool divide;  // no ordinary numbers: the remainder could leave fp32's range
+    float lift, scale, r;  // lift: a power of two that keeps a remainder within fp32's range
 
     __device__ __forceinline__ explicit Quotient(float s) {
-        scale = s;
-        r = __fdiv_rn(1.f, s);
-        divide = !(s > 1e-20f && s < 1e20f);
+        lift = s < 1e-20f ? 18446744073709551616.f : s > 1e20f ? 5.421010862427522e-20f : 1.f;
+        scale = s * lift;
+        r = scale == 0.f ? 0.f : __fdiv_rn(1.f, scale);
     }
     __device__ __forceinline__ float of(float x) const {
+        x *= lift;
         const float q = x * r;
         return copysignf(fmaf(fmaf(-q, scale, x), r, q), x);  // (the remainder of -0 is +0)
     }
     __device__ __forceinline__ uint32_t e4m3(float a, float b, float c, float d) const {
-        if (!divide) return e4m3x4(of(a), of(b), of(c), of(d));
-        if (scale == 0.f) return 0u;
-        return e4m3x4(__fdiv_rn(a, scale), __fdiv_rn(b, scale), __fdiv_rn(c, scale), __fdiv_rn(d, scale));
+        return e4m3x4(of(a), of(b), of(c), of(d));
     }
 };
 
