@@ -16,11 +16,15 @@ drop-in cache:
     layer's norm, QKV and RoPE) are replayed as one CUDA graph per layer, the
     RoPE position read from a device counter, so a step issues 36 graph
     launches plus the attention calls, whose arguments change every step;
+  * with Fp8Weights the dense half runs in 8 bits (e4m3, scales for blocks of
+    128), which halves the weights that a step reads; the reference has no
+    such mode (python -m zoomkv_revision_b200.decode_loop --fp8 times it);
   * sampling: temperature, top-k, top-p (nucleus), as sample_next_token,
     with a seeded generator.
 """
 from __future__ import annotations
 
+import argparse
 from dataclasses import dataclass
 from typing import Optional
 
@@ -128,11 +132,40 @@ class Weights:
             ))
 
 
+class Fp8Weights:
+    """The same weights in 8 bits: every product's matrix e4m3 with a scale for each block of 128 x 128 (ops.Fp8Weight), the
+    embedding and the norms as they are.  `of`: any Weights, whose matrices are let go layer by layer where `consume` is
+    true."""
+
+    def __init__(self, of: Weights, consume: bool = False):
+        self.embed, self.norm = of.embed, of.norm
+        self.lm_head = ops.Fp8Weight.quantize(of.lm_head)
+        self.layers = []
+        for L in of.layers:
+            self.layers.append(dict(
+                in_norm=L["in_norm"], post_norm=L["post_norm"], q_norm=L["q_norm"], k_norm=L["k_norm"],
+                wqkv=ops.Fp8Weight.quantize(L["wqkv"]), wo=ops.Fp8Weight.quantize(L["wo"]),
+                gate_up=ops.Fp8Weight.quantize(L["gate_up"], 2), down=ops.Fp8Weight.quantize(L["down"])))
+            if consume:
+                L.clear()
+
+    def check(self) -> None:
+        """Raises if a wait inside a product ran out (waits for the GPU)."""
+        for L in self.layers:
+            for name in ("wqkv", "wo", "gate_up", "down"):
+                L[name].check()
+        self.lm_head.check()
+
+
 class DecodeLoop:
     """A Qwen3-shape decoder over `cache` (the polar_cache drop-in, built
     with the same layer count, batch and heads).  prefill(prompt) then
     step() per generated token; `use_graphs` replays the dense segments as
-    CUDA graphs."""
+    CUDA graphs.  With Fp8Weights the dense segments run in 8 bits: the norms
+    (with the residual's addition) and the attention's output are quantised in
+    blocks of 128 and multiplied with e4m3 weights, and the gate and up
+    products, SiLU and their product are one kernel; the residual stream, q, k,
+    v and the attention stay 16-bit, the logits fp32."""
 
     def __init__(self, shape: Shape, weights: Weights, cache, batch: int, max_pos: int, device,
                  use_graphs: bool = True, temperature: float = 0.6, top_p: float = 0.95, top_k: int = 20,
@@ -158,6 +191,12 @@ class DecodeLoop:
         self.gu = torch.zeros(batch, 2 * shape.ffn, dtype=bf, device=self.dev)
         self.act = torch.zeros(batch, shape.ffn, dtype=bf, device=self.dev)
         self.lg = torch.zeros(batch, shape.vocab, dtype=bf, device=self.dev)
+        self.fp8 = isinstance(weights, Fp8Weights)
+        if self.fp8:
+            def rows8(n):   # e4m3 rows and their scales
+                return (torch.zeros(batch, n, dtype=torch.float8_e4m3fn, device=self.dev),
+                        torch.zeros(-(-n // 128), batch, device=self.dev).t())
+            self.attn8, self.h8, self.act8 = rows8(shape.heads * D), rows8(H), rows8(shape.ffn)
         self.graphs: list = []
         self.position = 0
 
@@ -166,8 +205,10 @@ class DecodeLoop:
         """x [B, T, H] -> q [B, T, heads, D], k / v [B, T, kv, D] (qwen.py:439-453, :550-612)."""
         s = self.s
         B, T, _ = x.shape
-        h = rmsnorm(x, L["in_norm"], s.rms_eps)
-        qkv = F.linear(h, L["wqkv"])
+        if self.fp8:
+            qkv = ops.fp8_linear(*ops.rmsnorm_fp8(x, L["in_norm"], s.rms_eps), L["wqkv"])
+        else:
+            qkv = F.linear(rmsnorm(x, L["in_norm"], s.rms_eps), L["wqkv"])
         q, k, v = qkv.split([s.heads * s.head_dim, s.kv_heads * s.head_dim, s.kv_heads * s.head_dim], dim=-1)
         q = rmsnorm(q.reshape(B, T, s.heads, s.head_dim), L["q_norm"], s.rms_eps)
         k = rmsnorm(k.reshape(B, T, s.kv_heads, s.head_dim), L["k_norm"], s.rms_eps)
@@ -178,6 +219,12 @@ class DecodeLoop:
         """o_proj + residual, RMSNorm, SwiGLU MLP + residual (LLM.py:240-249)."""
         s = self.s
         B, T = attn.shape[:2]
+        if self.fp8:
+            x = x.clone()
+            proj = ops.fp8_linear(*ops.quant_fp8(attn.reshape(B, T, s.heads * s.head_dim)), L["wo"])
+            h = ops.rmsnorm_fp8(proj, L["post_norm"], s.rms_eps, residual=x)
+            act, scale = ops.fp8_swiglu(*h, L["gate_up"])
+            return x + ops.fp8_linear(act, scale, L["down"])
         x = x + F.linear(attn.reshape(B, T, s.heads * s.head_dim), L["wo"])
         h = rmsnorm(x, L["post_norm"], s.rms_eps)
         gu = F.linear(h, L["gate_up"])
@@ -185,6 +232,8 @@ class DecodeLoop:
         return x + F.linear(F.silu(g) * u, L["down"])
 
     def _lm(self, x: torch.Tensor) -> torch.Tensor:
+        if self.fp8:
+            return ops.fp8_linear(*ops.rmsnorm_fp8(x, self.w.norm, self.s.rms_eps), self.w.lm_head, dtype=torch.float32)
         return F.linear(rmsnorm(x, self.w.norm, self.s.rms_eps), self.w.lm_head).float()
 
     # ------------------------------------------------------------------ prefill
@@ -218,6 +267,8 @@ class DecodeLoop:
         kernels; every tensor is a preallocated buffer."""
         s = self.s
         x = self.hidden.view(self.B, s.hidden)
+        if self.fp8:
+            return self._segment8(l, x)
         if l > 0:
             L = self.w.layers[l - 1]
             x.addmm_(self.attn.view(self.B, s.heads * s.head_dim), L["wo"].t())
@@ -235,6 +286,27 @@ class DecodeLoop:
             ops.rmsnorm(x, self.w.norm, s.rms_eps, out=self.h)
             torch.matmul(self.h, self.w.lm_head.t(), out=self.lg)
             self.logits.copy_(self.lg)
+
+    def _segment8(self, l: int, x: torch.Tensor) -> None:
+        """The same in 8 bits.  A product's output is added to the residual stream by the norm that follows it."""
+        s, proj = self.s, None
+        if l > 0:
+            L = self.w.layers[l - 1]
+            ops.quant_fp8(self.attn.view(self.B, s.heads * s.head_dim), out=self.attn8[0], scale=self.attn8[1])
+            ops.fp8_linear(*self.attn8, L["wo"], out=self.h)
+            ops.rmsnorm_fp8(self.h, L["post_norm"], s.rms_eps, residual=x, out=self.h8[0], scale=self.h8[1])
+            ops.fp8_swiglu(*self.h8, L["gate_up"], out=self.act8[0], scale=self.act8[1])
+            proj = ops.fp8_linear(*self.act8, L["down"], out=self.h)
+        w = self.w.layers[l]["in_norm"] if l < s.layers else self.w.norm
+        ops.rmsnorm_fp8(x if proj is None else proj, w, s.rms_eps, residual=None if proj is None else x, out=self.h8[0],
+                        scale=self.h8[1])
+        if l < s.layers:
+            L = self.w.layers[l]
+            ops.fp8_linear(*self.h8, L["wqkv"], out=self.qkv)
+            ops.qk_norm_rope(self.qkv, L["q_norm"], L["k_norm"], self.cos, self.sin, self.pos, s.heads, s.kv_heads,
+                             s.rms_eps, self.q, self.k, self.v)
+        else:
+            ops.fp8_linear(*self.h8, self.w.lm_head, out=self.logits)
 
     def _build_graphs(self) -> None:
         side = torch.cuda.Stream(device=self.dev)
@@ -279,3 +351,47 @@ def config4_cache_kwargs(shape: Shape, batch: int, prompt: int, max_new: int, de
                 dtype=torch.bfloat16, layer_mapping={str(l): str(device) for l in range(shape.layers)},
                 max_new_length=max_new, sink_size=64, local_size=256, final_topk=100,
                 dynamic_update_interval=512, full_attention_threshold=2048, enable_offload=True)
+
+
+def generate(shape: Shape, batch: int, prompt: int, steps: int, fp8: bool, device="cuda", seed: int = 0) -> dict:
+    """`steps` decode steps after a random prompt, dense attention over the pooled cache: ms of the prompt and of a step."""
+    from .pool_cache import PoolCache
+    w = Weights(shape, device, seed)
+    if fp8:
+        w = Fp8Weights(w, consume=True)
+    cache = PoolCache(shape.layers, batch, shape.kv_heads, shape.head_dim, prompt + steps + 1, device=device)
+    loop = DecodeLoop(shape, w, cache, batch, prompt + steps + 1, device, seed=seed)
+    ids = torch.randint(0, shape.vocab, (batch, prompt), generator=torch.Generator().manual_seed(seed)).to(device)
+    ev = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
+    ev[0].record()
+    tok = loop.prefill(ids)
+    ev[1].record()
+    for i in range(steps):
+        if i == 1:           # the first step captures the graphs
+            ev[2].record()
+        tok = loop.step(tok)
+    ev[3].record()
+    torch.cuda.synchronize()
+    cache.check()
+    if fp8:
+        w.check()
+    return dict(prefill_ms=ev[0].elapsed_time(ev[1]), step_ms=ev[2].elapsed_time(ev[3]) / (steps - 1), tokens=tok.tolist())
+
+
+def main(argv=None) -> None:
+    ap = argparse.ArgumentParser(description="decode steps of a random-init Qwen3-8B over the pooled cache")
+    ap.add_argument("--layers", type=int, default=QWEN3_8B.layers)
+    ap.add_argument("--batch", type=int, default=32)
+    ap.add_argument("--prompt", type=int, default=512)
+    ap.add_argument("--steps", type=int, default=64)
+    ap.add_argument("--fp8", action="store_true", help="8-bit weights and products")
+    a = ap.parse_args(argv)
+    if a.steps < 2:
+        ap.error("--steps: two at least, the first one captures the graphs")
+    got = generate(Shape(layers=a.layers), a.batch, a.prompt, a.steps, a.fp8)
+    print(f"{a.layers} layers, {'e4m3' if a.fp8 else 'bf16'} weights, batch {a.batch}: prompt of {a.prompt} in "
+          f"{got['prefill_ms']:.1f} ms, {got['step_ms']:.3f} ms per decode step = {a.batch / got['step_ms'] * 1e3:.0f} tokens/s")
+
+
+if __name__ == "__main__":
+    main()

@@ -1511,45 +1511,46 @@ _QUANT_BLOCK = 128
 
 
 def _fp8_in(name, t, el):
-    """(t, rows, last dim, row stride) of rows [..., dim] that start on 16 bytes (a copy where they do not)."""
+    """(t, address, rows, last dim, row stride) of rows [..., dim] of `el`-byte elements that start on 16 bytes (a copy where
+    they do not)."""
     shape = t.shape
     if not shape:
         raise ValueError(f"{name} must have rows")
-    dim = shape[-1]
-    if t.is_contiguous():
-        rows, ld = t.numel() // dim if dim else 0, dim
-    elif len(shape) == 2 and t.stride(1) == 1 and t.stride(0) >= dim:
-        rows, ld = shape[0], t.stride(0)
-    else:
-        t = t.contiguous()
-        rows, ld = t.numel() // dim if dim else 0, dim
-    if (t.data_ptr() | ld * el) & 15:
+    dim = ld = shape[-1]
+    if not t.is_contiguous():
+        if len(shape) == 2 and t.stride(1) == 1 and t.stride(0) >= dim:
+            ld = t.stride(0)
+        else:
+            t = t.contiguous()
+    at = t.data_ptr()
+    if (at | ld * el) & 15:
         if dim * el & 15:
             raise ValueError(f"{name}: the last dim must be a multiple of 16; got {dim}")
         t, ld = t.clone(memory_format=torch.contiguous_format), dim
-    return t, rows, dim, ld
+        at = t.data_ptr()
+    return t, at, shape[0] if len(shape) == 2 else t.numel() // dim if dim else 0, dim, ld
 
 
-def _fp8_out(name, t, shape, dtype, dev, whole=True):
-    """The row stride of an output like `shape` (whole: its rows start on 16 bytes)."""
+def _fp8_out(name, t, shape, dtype, dev, el):
+    """(address, row stride) of an output of `shape`, whose rows start on 16 bytes where `el` is not 0."""
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}; got {t.dtype}")
     if t.shape != shape or t.get_device() != dev:
         raise ValueError(f"{name} must be {tuple(shape)} on the device of x; got {tuple(t.shape)}")
-    dim = shape[-1]
-    if t.is_contiguous():
-        ld = dim
-    elif len(shape) == 2 and t.stride(1) == 1 and t.stride(0) >= dim:
-        ld = t.stride(0)
-    else:
-        raise ValueError(f"{name} must have contiguous rows that do not overlap")
-    if whole and (t.data_ptr() | ld * t.element_size()) & 15:
+    ld = shape[-1]
+    if not t.is_contiguous():
+        if len(shape) == 2 and t.stride(1) == 1 and t.stride(0) >= ld:
+            ld = t.stride(0)
+        else:
+            raise ValueError(f"{name} must have contiguous rows that do not overlap")
+    at = t.data_ptr()
+    if el and (at | ld * el) & 15:
         raise ValueError(f"{name} must have rows that start on 16 bytes")
-    return ld
+    return at, ld
 
 
 def _row_scales(name, t, rows, blocks, dev, out):
-    """(token stride, block stride) of fp32 [rows, blocks] scales."""
+    """(address, token stride, block stride) of fp32 [rows, blocks] scales."""
     if t.dtype is not _F32:
         raise TypeError(f"{name} must be torch.float32; got {t.dtype}")
     if t.shape != (rows, blocks) or t.get_device() != dev:
@@ -1560,9 +1561,9 @@ def _row_scales(name, t, rows, blocks, dev, out):
             token = blocks * block
         if blocks <= 1:
             block = rows * token
-        if not ((block >= 1 and token >= blocks * block) or (token >= 1 and block >= rows * token)):
+        if not ((token >= 1 and block >= rows * token) or (block >= 1 and token >= blocks * block)):
             raise ValueError(f"{name} must not overlap itself")
-    return token, block
+    return t.data_ptr(), token, block
 
 
 def _new_scales(like, rows, blocks):
@@ -1583,20 +1584,19 @@ def quant_fp8(x, *, out=None, scale=None):
     dev = x.get_device()
     if dev < 0:
         raise ValueError("x must be a CUDA tensor")
-    x, rows, dim, ld = _fp8_in("x", x, 2)
+    x, at, rows, dim, ld = _fp8_in("x", x, 2)
     blocks = -(-dim // _QUANT_BLOCK)
     if out is None:
         out = torch.empty(x.shape, dtype=_F8, device=x.device)
-    out_ld = _fp8_out("out", out, x.shape, _F8, dev)
+    to, out_ld = _fp8_out("out", out, x.shape, _F8, dev, 1)
     if scale is None:
         scale = _new_scales(x, rows, blocks)
-    st, sb = _row_scales("scale", scale, rows, blocks, dev, True)
+    sp, st, sb = _row_scales("scale", scale, rows, blocks, dev, True)
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return quant_fp8(x, out=out, scale=scale)
     if rows:
-        rc = lib().zkv_quant_fp8(x.data_ptr(), ld, code, rows, dim, out.data_ptr(), out_ld, scale.data_ptr(), st, sb,
-                                 _raw_stream(dev))
+        rc = lib().zkv_quant_fp8(at, ld, code, rows, dim, to, out_ld, sp, st, sb, _raw_stream(dev))
         if rc:
             check(rc, "zkv_quant_fp8")
     return out, scale
@@ -1615,43 +1615,44 @@ def rmsnorm_fp8(x, w, eps: float, *, residual=None, residual_out=None, out=None,
     dev = x.get_device()
     if dev < 0:
         raise ValueError("x must be a CUDA tensor")
-    x, rows, dim, ld = _fp8_in("x", x, 2)
+    x, at, rows, dim, ld = _fp8_in("x", x, 2)
     if w.dtype is not dt:
         raise TypeError(f"w must be {dt}; got {w.dtype}")
     if w.shape != (dim,) or w.get_device() != dev or not w.is_contiguous():
         raise ValueError(f"w must be contiguous [{dim}] on the device of x")
-    if w.data_ptr() & 15:
+    wp = w.data_ptr()
+    if wp & 15:
         w = w.clone()
-    res, res_ld, to, to_ld = None, 0, None, 0
+        wp = w.data_ptr()
+    shape = x.shape
+    res, res_ld, kept, kept_ld = None, 0, None, 0
     if residual is not None:
         if residual_out is None:
             residual_out = residual
-        to_ld = _fp8_out("residual_out", residual_out, x.shape, dt, dev)
-        to = residual_out.data_ptr()
+        kept, kept_ld = _fp8_out("residual_out", residual_out, shape, dt, dev, 2)
         if residual is residual_out:
-            res, res_ld = to, to_ld
+            res, res_ld = kept, kept_ld
         else:
             if residual.dtype is not dt:
                 raise TypeError(f"residual must be {dt}; got {residual.dtype}")
-            if residual.shape != x.shape or residual.get_device() != dev:
-                raise ValueError(f"residual must be {tuple(x.shape)} on the device of x; got {tuple(residual.shape)}")
-            residual, _, _, res_ld = _fp8_in("residual", residual, 2)
-            res = residual.data_ptr()
+            if residual.shape != shape or residual.get_device() != dev:
+                raise ValueError(f"residual must be {tuple(shape)} on the device of x; got {tuple(residual.shape)}")
+            residual, res, _, _, res_ld = _fp8_in("residual", residual, 2)
     elif residual_out is not None:
         raise ValueError("residual_out belongs to a residual")
     blocks = -(-dim // _QUANT_BLOCK)
     if out is None:
-        out = torch.empty(x.shape, dtype=_F8, device=x.device)
-    out_ld = _fp8_out("out", out, x.shape, _F8, dev)
+        out = torch.empty(shape, dtype=_F8, device=x.device)
+    to, out_ld = _fp8_out("out", out, shape, _F8, dev, 1)
     if scale is None:
         scale = _new_scales(x, rows, blocks)
-    st, sb = _row_scales("scale", scale, rows, blocks, dev, True)
+    sp, st, sb = _row_scales("scale", scale, rows, blocks, dev, True)
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return rmsnorm_fp8(x, w, eps, residual=residual, residual_out=residual_out, out=out, scale=scale)
     if rows:
-        rc = lib().zkv_rmsnorm_fp8(x.data_ptr(), ld, res, res_ld, to, to_ld, w.data_ptr(), code, rows, dim, eps,
-                                   out.data_ptr(), out_ld, scale.data_ptr(), st, sb, _raw_stream(dev))
+        rc = lib().zkv_rmsnorm_fp8(at, ld, res, res_ld, kept, kept_ld, wp, code, rows, dim, eps, to, out_ld, sp, st, sb,
+                                   _raw_stream(dev))
         if rc:
             check(rc, "zkv_rmsnorm_fp8")
     return out, scale
@@ -1732,16 +1733,15 @@ class Fp8Weight:
 
 
 def _fp8_product(x, x_scale, weight, parts):
-    """(x, rows, row stride, token stride, block stride of the scales) of a product's input."""
+    """(x, address, rows, row stride, address, token stride and block stride of the scales) of a product's input."""
     if x.dtype is not _F8:
         raise TypeError(f"x must be float8_e4m3fn; got {x.dtype}")
     if weight.parts != parts:
         raise ValueError(f"the weight must have {parts} part(s); it has {weight.parts}")
     if not x.shape or x.shape[-1] != weight.k or x.get_device() != weight.index:
         raise ValueError(f"x must be [..., {weight.k}] on the weight's device; got {tuple(x.shape)}")
-    x, rows, dim, ld = _fp8_in("x", x, 1)
-    st, sb = _row_scales("x_scale", x_scale, rows, -(-dim // _QUANT_BLOCK), weight.index, False)
-    return x, rows, ld, st, sb
+    x, at, rows, dim, ld = _fp8_in("x", x, 1)
+    return (x, at, rows, ld, *_row_scales("x_scale", x_scale, rows, -(-dim // _QUANT_BLOCK), weight.index, False))
 
 
 def fp8_linear(x, x_scale, weight: Fp8Weight, *, out=None, dtype=torch.bfloat16):
@@ -1749,20 +1749,21 @@ def fp8_linear(x, x_scale, weight: Fp8Weight, *, out=None, dtype=torch.bfloat16)
     rmsnorm_fp8, or any fp32 scales for blocks of 128, any strides) times
     weight^T: out [..., n] bf16, fp16 or fp32 (`dtype`, or that of the given
     out).  Sums in fp32, one rounding at the end."""
-    x, rows, ld, st, sb = _fp8_product(x, x_scale, weight, 1)
+    x, at, rows, ld, sp, st, sb = _fp8_product(x, x_scale, weight, 1)
     dev = weight.index
+    shape = (*x.shape[:-1], weight.rows)
     if out is None:
-        out = torch.empty(*x.shape[:-1], weight.rows, dtype=dtype, device=weight.device)
-    code = _OUT_DTYPES.get(out.dtype)
+        out = torch.empty(shape, dtype=dtype, device=weight.device)
+    dtype = out.dtype
+    code = _OUT_DTYPES.get(dtype)
     if code is None:
-        raise TypeError(f"out must be bfloat16, float16 or float32; got {out.dtype}")
-    out_ld = _fp8_out("out", out, x.shape[:-1] + (weight.rows,), out.dtype, dev, False)
+        raise TypeError(f"out must be bfloat16, float16 or float32; got {dtype}")
+    to, out_ld = _fp8_out("out", out, shape, dtype, dev, 0)
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return fp8_linear(x, x_scale, weight, out=out)
     if rows:
-        rc = lib().zkv_fp8_linear(x.data_ptr(), ld, x_scale.data_ptr(), st, sb, rows, weight.ref, out.data_ptr(), out_ld,
-                                  code, weight.status_at, _raw_stream(dev))
+        rc = lib().zkv_fp8_linear(at, ld, sp, st, sb, rows, weight.ref, to, out_ld, code, weight.status_at, _raw_stream(dev))
         if rc:
             check(rc, "zkv_fp8_linear")
     return out
@@ -1773,21 +1774,22 @@ def fp8_swiglu(x, x_scale, weight: Fp8Weight, *, out=None, scale=None):
     times the two parts of `weight`, in fp32, and what is stored is quant_fp8
     of their product without a rounding in between.  Returns (out [..., f],
     scale [rows, ceil(f / 128)])."""
-    x, rows, ld, st, sb = _fp8_product(x, x_scale, weight, 2)
+    x, at, rows, ld, sp, st, sb = _fp8_product(x, x_scale, weight, 2)
     dev = weight.index
+    shape = (*x.shape[:-1], weight.rows)
     if out is None:
-        out = torch.empty(*x.shape[:-1], weight.rows, dtype=_F8, device=weight.device)
-    out_ld = _fp8_out("out", out, x.shape[:-1] + (weight.rows,), _F8, dev)
+        out = torch.empty(shape, dtype=_F8, device=weight.device)
+    to, out_ld = _fp8_out("out", out, shape, _F8, dev, 1)
     blocks = -(-weight.rows // _QUANT_BLOCK)
     if scale is None:
         scale = _new_scales(x, rows, blocks)
-    ot, ob = _row_scales("scale", scale, rows, blocks, dev, True)
+    op, ot, ob = _row_scales("scale", scale, rows, blocks, dev, True)
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return fp8_swiglu(x, x_scale, weight, out=out, scale=scale)
     if rows:
-        rc = lib().zkv_fp8_swiglu(x.data_ptr(), ld, x_scale.data_ptr(), st, sb, rows, weight.ref, out.data_ptr(), out_ld,
-                                  scale.data_ptr(), ot, ob, weight.status_at, _raw_stream(dev))
+        rc = lib().zkv_fp8_swiglu(at, ld, sp, st, sb, rows, weight.ref, to, out_ld, op, ot, ob, weight.status_at,
+                                  _raw_stream(dev))
         if rc:
             check(rc, "zkv_fp8_swiglu")
     return out, scale
