@@ -382,14 +382,14 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
 template <bool kGated>
 struct Many {
     static constexpr int kTokens = 256, kFeatures = 256;
-    // A warpgroup for the copies and products, four of readers, which take the registers that the first gives up:
-    // 128 x 40 + 512 x 104 of the 640 x 96 of the launch.
-    static constexpr int kReaders = 512, kThreads = 128 + kReaders;
+    // A warpgroup for the copies and products, two of readers, which take the registers that the first gives up:
+    // 128 x 72 + 256 x 216 of the 384 x 168 of the launch.
+    static constexpr int kReaders = 256, kThreads = 128 + kReaders;
     static constexpr int kStages = 4;
     static constexpr int kStage = 2 * kTileBytes;  // 128 rows of tokens, 128 of features
-    // Output staging: a tile for each warpgroup; gated: one in all, and the sums that warpgroups exchange.
+    // Output staging: two tiles for each warpgroup; gated: one in all, and the sums that warpgroups exchange.
     static constexpr int kOut = (kGated ? 5 : 4) * kTileBytes;
-    static constexpr int kTop = kGated ? 2048 : 0;
+    static constexpr int kTop = kGated ? 1024 : 0;
     // Scales come to shared memory by a warp of their own, four blocks of the inner dimension at a time: loaded one block
     // ahead by the threads that use them, they took 1.1 us a block (4096 x 6144 x 4096: 220 us).
     static constexpr int kBatch = 4, kSlots = 2, kSlot = kBatch * 4 * (128 + 2);  // 128 tokens, two of the weights
@@ -412,7 +412,7 @@ __device__ __forceinline__ void group_sync(int group) {
     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
 }
 
-__device__ __forceinline__ void readers_sync() { asm volatile("bar.sync 5, 512;" ::: "memory"); }
+__device__ __forceinline__ void readers_sync() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
 
 // 16 bytes of row r of a swizzled tile of 128-byte rows.
 __device__ __forceinline__ uint32_t swizzled(uint32_t tile, int r, int chunk) {
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(bar(sum_full + 8 * i), 1);
-            mbar_init(bar(sum_empty + 8 * i), 16);  // a half's 8 warps of readers, of both CTAs
+            mbar_init(bar(sum_empty + 8 * i), 8);  // a half's 4 warps of readers, of both CTAs
         }
         for (int i = 0; i < C::kSlots; ++i) {
             mbar_init(bar(slot_full + 8 * i), 32);
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
     grid_dep_wait();
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
       if (warp == 0) {
         const uint32_t leader = tc::in_cta(full, 0);
         int got = 0;
@@ -587,14 +587,13 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
         tc::copy4_wait();
       }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-        const int group = (warp - 4) >> 2, half = group >> 1, row = (warp & 3) * 32 + lane;
-        // this thread's columns of tensor memory: 64 of a half
-        const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21) + 64 * group;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int half = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;  // a warpgroup reads one half
+        const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21) + half * kTile;
         const uint32_t empty_at = tc::in_cta(sum_empty + 8 * half, 0);
-        const uint32_t staging = out_at + group * kTileBytes;
-        const uint32_t top = top_at + row * 4;  // [4][128]: a group's largest magnitude of a token
-        const bool issues = threadIdx.x == 128 + 128 * group;
+        const uint32_t staging = out_at + half * 2 * kTileBytes;
+        const uint32_t top = top_at + row * 4;  // [2][128]: a group's largest magnitude of a token
+        const bool issues = threadIdx.x == 128 + 128 * half;
         bool ok = true;
         int done = 0, batch = 0;
         for (int t = blockIdx.x >> 1; t < tiles.total; t += pairs) {
@@ -602,9 +601,14 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
             tiles.at(t, tm, tn);
             const int64_t token0 = (int64_t)tm * C::kTokens + rank * 128, token = token0 + row;
             const bool live = token < a.tokens;
-            float acc[64];
+            float acc[128];
 #pragma unroll
-            for (int c = 0; c < 64; ++c) acc[c] = 0.f;
+            for (int c = 0; c < 128; ++c) acc[c] = 0.f;
+            uint32_t even[32], odd[32];
+            auto add = [&](int c, const uint32_t(&v)[32], float by) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(v[i]), by, acc[32 * c + i]);
+            };
             for (int kb = 0; kb < n; kb += C::kBatch, ++batch) {
                 const int slot = batch % C::kSlots;
                 ok = ok && tc::wait_all(slot_full + 8 * slot, (batch / C::kSlots) & 1, a.status);
@@ -618,120 +622,118 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
                     if (kb + j >= n) break;
                     ok = ok && tc::wait_all(sum_full + 8 * (half + 2 * (done & 1)), (done >> 1) & 1, a.status);
                     tc::fence_after();
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t v[32];
-                        tc::ld(mine + (done & 1) * 2 * kTile + 32 * c, v);
-                        tc::wait_ld(v);
-                        if (c == 1) {
-                            tc::fence_before();
-                            if (lane == 0) tc::arrive_cluster(empty_at + 16 * (done & 1));
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            acc[32 * c + i] = fmaf(__uint_as_float(v[i]), by[j], acc[32 * c + i]);
-                    }
+                    const uint32_t at = mine + (done & 1) * 2 * kTile;
+                    tc::ld(at, even);
+                    tc::wait_ld(even);
+                    tc::ld(at + 32, odd);
+                    add(0, even, by[j]);
+                    tc::wait_ld(odd);
+                    tc::ld(at + 64, even);
+                    add(1, odd, by[j]);
+                    tc::wait_ld(even);
+                    tc::ld(at + 96, odd);
+                    add(2, even, by[j]);
+                    tc::wait_ld(odd);
+                    tc::fence_before();
+                    if (lane == 0) tc::arrive_cluster(empty_at + 16 * (done & 1));
+                    add(3, odd, by[j]);
                     ++done;
                 }
             }
-            auto lo = [&](int i) { return acc[2 * i]; };
-            auto hi = [&](int i) { return acc[2 * i + 1]; };
             // the staging's last tile has been read
             if (mapped && issues) tc::store_wait_read();
             if (kGated) {
-                // Groups 0 and 1 hold the gate's features 0..63 and 64..127, 2 and 3 the up part's: each gives its partner
-                // half of what it has and finishes the features of the other half.
-                const uint32_t give = out_at + kTileBytes + group * kTileBytes + row * 4;
+                // One warpgroup holds the gate's 128 features of a token, the other the up part's: each gives the other half of
+                // them and finishes the other half.
+                const uint32_t give = out_at + kTileBytes + half * 2 * kTileBytes + row * 4;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    st_shared1(give + (2 * i) * 512, __float_as_uint(group < 2 ? lo(16 + i) : lo(i)));
-                    st_shared1(give + (2 * i + 1) * 512, __float_as_uint(group < 2 ? hi(16 + i) : hi(i)));
-                }
+                for (int i = 0; i < 64; ++i) st_shared1(give + i * 512, __float_as_uint(half ? acc[i] : acc[64 + i]));
                 readers_sync();
-                const uint32_t from = out_at + kTileBytes + (group ^ 2) * kTileBytes + row * 4;
+                const uint32_t from = out_at + kTileBytes + (half ^ 1) * 2 * kTileBytes + row * 4;
                 uint32_t m = 0;
-                const int at = (group & 1) * 64 + half * 32, f0 = tn * kTile + at;
+                const int f0 = tn * kTile + half * 64;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float o0 = group < 2 ? lo(i) : lo(16 + i), o1 = group < 2 ? hi(i) : hi(16 + i);
-                    const float t0 = __uint_as_float(ld_shared<uint32_t>(from + (2 * i) * 512));
-                    const float t1 = __uint_as_float(ld_shared<uint32_t>(from + (2 * i + 1) * 512));
-                    const bool in = f0 + 2 * i < a.rows;  // rows are whole 16 bytes
-                    const float p = in ? gated(group < 2 ? o0 : t0, group < 2 ? t0 : o0) : 0.f;
-                    const float q = in ? gated(group < 2 ? o1 : t1, group < 2 ? t1 : o1) : 0.f;
-                    acc[2 * i] = p, acc[2 * i + 1] = q;
-                    m = max(m, max(magnitude(p), magnitude(q)));
+                for (int i = 0; i < 64; ++i) {
+                    const float own = half ? acc[64 + i] : acc[i], other = __uint_as_float(ld_shared<uint32_t>(from + i * 512));
+                    const bool in = f0 + i < a.rows;
+                    acc[i] = in ? gated(half ? other : own, half ? own : other) : 0.f;
+                    m = max(m, magnitude(acc[i]));
                 }
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(top + group * 512), "r"(m) : "memory");
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(top + half * 512), "r"(m) : "memory");
                 readers_sync();  // every group's
-#pragma unroll
-                for (int g = 0; g < 4; ++g) m = max(m, ld_shared<uint32_t>(top + g * 512));
+                m = max(m, ld_shared<uint32_t>(top + (half ^ 1) * 512));
                 const float s = scale_of(m);
                 const Quotient by(s);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < 4; ++j) {
+                    const float* v = acc + 16 * j;
                     uint4 q;
-                    q.x = by.e4m3(lo(8 * j), hi(8 * j), lo(8 * j + 1), hi(8 * j + 1));
-                    q.y = by.e4m3(lo(8 * j + 2), hi(8 * j + 2), lo(8 * j + 3), hi(8 * j + 3));
-                    q.z = by.e4m3(lo(8 * j + 4), hi(8 * j + 4), lo(8 * j + 5), hi(8 * j + 5));
-                    q.w = by.e4m3(lo(8 * j + 6), hi(8 * j + 6), lo(8 * j + 7), hi(8 * j + 7));
-                    st_shared(swizzled(out_at, row, at / 16 + j), q);
+                    q.x = by.e4m3(v[0], v[1], v[2], v[3]);
+                    q.y = by.e4m3(v[4], v[5], v[6], v[7]);
+                    q.z = by.e4m3(v[8], v[9], v[10], v[11]);
+                    q.w = by.e4m3(v[12], v[13], v[14], v[15]);
+                    st_shared(swizzled(out_at, row, half * 4 + j), q);
                 }
-                if (live && group == 0) a.out_scale[token * a.os_token + tn * a.os_block] = s;
+                if (live && half == 0) a.out_scale[token * a.os_token + tn * a.os_block] = s;
                 tc::fence_async();
                 readers_sync();
-                if (issues && group == 0) {
+                if (issues && half == 0) {
                     if (token0 < a.tokens) tc::tma_store_2d(&out_map, out_at, tn * kTile, (int)token0);
                     tc::store_commit();
                 }
             } else if (a.dtype == ZKV_DT_F32) {
-                // 32 features a tile, one half after the other
+                // 32 features a tile, two tiles at a time
 #pragma unroll
                 for (int side = 0; side < 2; ++side) {
                     if (side && mapped && issues) tc::store_wait_read();
-                    group_sync(group);
+                    group_sync(half);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float* v = acc + side * 32 + 4 * j;
-                        st_shared(swizzled(staging, row, j), make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
-                                                                        __float_as_uint(v[2]), __float_as_uint(v[3])));
-                    }
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float* v = acc + side * 64 + c * 32 + 4 * j;
+                            st_shared(swizzled(staging + c * kTileBytes, row, j),
+                                      make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                                 __float_as_uint(v[3])));
+                        }
                     if (mapped) tc::fence_async();
-                    group_sync(group);
-                    const int f = tn * C::kFeatures + group * 64 + side * 32;
-                    if (!mapped) {
-                        copy_out<uint32_t>(a, staging, token0, f, 32);
-                    } else if (issues) {
-                        if (f < a.rows && token0 < a.tokens) tc::tma_store_2d(&out_map, staging, f, (int)token0);
-                        tc::store_commit();
+                    group_sync(half);
+                    for (int c = 0; c < 2; ++c) {
+                        const int f = tn * C::kFeatures + half * kTile + side * 64 + c * 32;
+                        if (!mapped) copy_out<uint32_t>(a, staging + c * kTileBytes, token0, f, 32);
+                        else if (issues && f < a.rows && token0 < a.tokens)
+                            tc::tma_store_2d(&out_map, staging + c * kTileBytes, f, (int)token0);
                     }
+                    if (mapped && issues) tc::store_commit();
                 }
             } else {
-                group_sync(group);
+                group_sync(half);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint32_t w[4];
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int at = 4 * j + i;
-                        if (a.dtype == ZKV_DT_BF16) {
-                            w[i] = pack_bf162(lo(at), hi(at));
-                        } else {
-                            const __half2 h = __floats2half2_rn(lo(at), hi(at));
-                            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float* v = acc + c * 64 + 8 * j + 2 * i;
+                            if (a.dtype == ZKV_DT_BF16) {
+                                w[i] = pack_bf162(v[0], v[1]);
+                            } else {
+                                const __half2 h = __floats2half2_rn(v[0], v[1]);
+                                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
                         }
+                        st_shared(swizzled(staging + c * kTileBytes, row, j), make_uint4(w[0], w[1], w[2], w[3]));
                     }
-                    st_shared(swizzled(staging, row, j), make_uint4(w[0], w[1], w[2], w[3]));
-                }
                 if (mapped) tc::fence_async();
-                group_sync(group);
-                const int f = tn * C::kFeatures + group * 64;
-                if (!mapped) {
-                    copy_out<uint16_t>(a, staging, token0, f, 64);
-                } else if (issues) {
-                    if (f < a.rows && token0 < a.tokens) tc::tma_store_2d(&out_map, staging, f, (int)token0);
-                    tc::store_commit();
+                group_sync(half);
+                for (int c = 0; c < 2; ++c) {
+                    const int f = tn * C::kFeatures + half * kTile + c * 64;
+                    if (!mapped) copy_out<uint16_t>(a, staging + c * kTileBytes, token0, f, 64);
+                    else if (issues && f < a.rows && token0 < a.tokens)
+                        tc::tma_store_2d(&out_map, staging + c * kTileBytes, f, (int)token0);
                 }
+                if (mapped && issues) tc::store_commit();
             }
         }
         if (mapped && issues) tc::store_wait();  // the staging is read until then
