@@ -55,12 +55,11 @@ struct Few {
     static constexpr int kReaders = 128 * kGroups, kThreads = 96 + kReaders;
     static constexpr int kMine = kCols / kGroups;  // columns of a thread
     static constexpr int kLoad = kMine == 32 ? 32 : 16;  // columns of a load (64 columns: what registers leave room for)
-    static constexpr int kBufs = kCols >= 128 ? 2 : kCols == 64 ? 4 : 8;
+    static constexpr int kBufs = kCols == 256 ? 2 : kCols >= 64 ? 4 : 8;
     static constexpr int kTmem = kCols * kBufs;
     static constexpr int kStage = kParts * kTileBytes + kTok * kBlock;
     static constexpr int kAhead = 4;  // blocks of scales staged at a time
     static constexpr int kScales = 2 * kAhead * kCols * 4;
-    static constexpr int kJoin = kParts == 2 && kTok > 64 ? 64 : kTok;  // tokens joined at a time
     static constexpr int kPitch = kTokenRows ? kTile + 4 : kTile;  // floats from token to token where they are joined
     static constexpr int kMost = 12;  // stages of the ring: barriers
     static constexpr int smem(int stages) { return 1024 + stages * kStage + kScales + 512; }
@@ -84,8 +83,7 @@ struct Few {
     static_assert(smem(kStages) > 76 * 1024, "no third CTA on an SM");
     static_assert(kMine % kLoad == 0, "whole loads");
     static_assert(16 * (kMost + kBufs) + 4 <= 512, "barriers");
-    static_assert(kTokenRows || kJoin == kTok, "token chunks");
-    static_assert(kStages >= 2 && kJoin * kParts * kPitch * 4 <= kStages * kStage, "the parts are joined in the ring's place");
+    static_assert(kStages >= 2 && kTok * kParts * kPitch * 4 <= kStages * kStage, "the parts are joined in the ring's place");
 };
 
 __device__ __forceinline__ void store4(const Product& a, int64_t token, int f, float4 y) {
@@ -292,78 +290,76 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
     if (warp == 1) tc::tmem_free<C::kTmem>(tmem);
 
     // The CTAs' parts, token by token [part][token][feature] in the ring's place; the cluster's CTAs take the tokens in
-    // turn, a warp a token, two at a time.
+    // turn, a warp some at a time.
     float* const join = reinterpret_cast<float*>(generic);
+    if (warp >= 3) {
+        const int row = (warp & 3) * 32 + lane, first = (warp - 3) / 4 * C::kMine;
+        if (C::kTokenRows) {
+            float* to = join + (first / kTile * kTok + row) * C::kPitch + first % kTile;
 #pragma unroll
-    for (int c0 = 0; c0 < kTok; c0 += C::kJoin) {
-        if (warp >= 3) {
-            const int row = (warp & 3) * 32 + lane, first = (warp - 3) / 4 * C::kMine;
-            if (C::kTokenRows) {
-                if (row >= c0 && row < c0 + C::kJoin) {
-                    float* to = join + (first / kTile * C::kJoin + row - c0) * C::kPitch + first % kTile;
+            for (int c = 0; c < C::kMine; c += 4)
+                *reinterpret_cast<float4*>(to + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+        } else {
 #pragma unroll
-                    for (int c = 0; c < C::kMine; c += 4)
-                        *reinterpret_cast<float4*>(to + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < C::kMine; ++c) {
-                    const int col = first + c;
-                    join[(col / kTok * C::kJoin + col % kTok) * C::kPitch + row] = acc[c];
-                }
+            for (int c = 0; c < C::kMine; ++c) {
+                const int col = first + c;
+                join[(col / kTok * kTok + col % kTok) * C::kPitch + row] = acc[c];
             }
         }
-        if (parts > 1) tc::cluster_sync();
-        else __syncthreads();
-        const int turn = C::kThreads / 32 * parts, f = tile * kTile + lane * 4;
-        for (int t = warp * parts + rank; t < C::kJoin; t += 2 * turn) {
-            const int64_t token = t0 + c0 + t;
-            if (token >= a.tokens) break;
-            const bool both = t + turn < C::kJoin && token + turn < a.tokens;
-            float4 y[2][kParts];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int p = 0; p < kParts; ++p) {
-                    const int at = (p * C::kJoin + (u && both ? t + turn : t)) * C::kPitch + lane * 4;
-                    if (parts == 1) {
-                        y[u][p] = *reinterpret_cast<const float4*>(join + at);
-                    } else {
-                        y[u][p] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        for (uint32_t r = 0; r < parts; ++r) {
-                            const float4 v = tc::ld_cluster(tc::in_cta(base + at * 4, r));
-                            y[u][p].x += v.x, y[u][p].y += v.y, y[u][p].z += v.z, y[u][p].w += v.w;
-                        }
-                    }
-                }
-            if (kParts == 1) {
-                store4(a, token, f, y[0][0]);
-                if (both) store4(a, token + turn, f, y[1][0]);
-            } else {
-                uint32_t q[2];
-                float s[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float4 g = y[u][0], h = y[u][kParts - 1];
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (f < a.rows)  // rows are whole 16 bytes
-                        v = make_float4(gated(g.x, h.x), gated(g.y, h.y), gated(g.z, h.z), gated(g.w, h.w));
-                    s[u] = scale_of(__reduce_max_sync(
-                        0xffffffffu, max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w)))));
-                    q[u] = Quotient(s[u]).e4m3(v.x, v.y, v.z, v.w);
-                }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    if (u && !both) break;
-                    const int64_t to = token + (u ? turn : 0);
-                    if (f < a.rows) *reinterpret_cast<uint32_t*>((uint8_t*)a.out + to * a.out_ld + f) = q[u];
-                    if (lane == 0) a.out_scale[to * a.os_token + tile * a.os_block] = s[u];
-                }
-            }
-        }
-        if (parts > 1) tc::cluster_sync();
-        else if (c0 + C::kJoin < kTok) __syncthreads();
     }
+    if (parts > 1) tc::cluster_sync();
+    else __syncthreads();
+    constexpr int kAtOnce = kTok >= 128 && kParts == 2 ? 4 : 2;
+    const int turn = C::kThreads / 32 * parts, f = tile * kTile + lane * 4;
+    const int most = (int)min((int64_t)kTok, a.tokens - t0);  // tokens of this tile
+    for (int t = warp * parts + rank; t < most; t += kAtOnce * turn) {
+        float4 y[kAtOnce][kParts];
+        auto at = [&](int u, int p) { return (p * kTok + min(t + u * turn, most - 1)) * C::kPitch + lane * 4; };
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+            for (int p = 0; p < kParts; ++p)
+                y[u][p] = parts == 1 ? *reinterpret_cast<const float4*>(join + at(u, p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t r = 0; parts > 1 && r < parts; ++r) {
+            const uint32_t from = tc::in_cta(base, r);
+            float4 v[kAtOnce][kParts];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) v[u][p] = tc::ld_cluster(from + at(u, p) * 4);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                for (int p = 0; p < kParts; ++p)
+                    y[u][p].x += v[u][p].x, y[u][p].y += v[u][p].y, y[u][p].z += v[u][p].z, y[u][p].w += v[u][p].w;
+        }
+        if (kParts == 1) {
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (t + u * turn < most) store4(a, t0 + t + u * turn, f, y[u][0]);
+        } else {
+            uint32_t q[kAtOnce];
+            float s[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const float4 g = y[u][0], h = y[u][kParts - 1];
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (f < a.rows)  // rows are whole 16 bytes
+                    v = make_float4(gated(g.x, h.x), gated(g.y, h.y), gated(g.z, h.z), gated(g.w, h.w));
+                s[u] = scale_of(__reduce_max_sync(
+                    0xffffffffu, max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w)))));
+                q[u] = Quotient(s[u]).e4m3(v.x, v.y, v.z, v.w);
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int64_t to = t0 + t + u * turn;
+                if (t + u * turn >= most) break;
+                if (f < a.rows) *reinterpret_cast<uint32_t*>((uint8_t*)a.out + to * a.out_ld + f) = q[u];
+                if (lane == 0) a.out_scale[to * a.os_token + tile * a.os_block] = s[u];
+            }
+        }
+    }
+    if (parts > 1) tc::cluster_sync();
 }
 
 // ------------------------------------------------------------ many tokens
