@@ -826,7 +826,7 @@ static const Places* places(Kernel kernel, int threads, int smem) {
 
 // How the inner dimension is cut over a cluster's CTAs: the number for which the waves of clusters take the fewest blocks
 // after one another, each wave with a fixed cost of some blocks (filling the ring, joining the parts).  `halves`: two CTAs
-// an SM.  8 tokens, us by CTAs of a cluster: 4096 x 4096 1: 10.3, 2: 7.6, 4: 6.2, 8: 6.9; 6144 x 4096 11.0, 7.8, 6.9, 11.0;
+// an SM, so that an even cluster lies on half as many SMs.  8 tokens, us by CTAs of a cluster: 4096 x 4096 1: 10.3, 2: 7.6, 4: 6.2, 8: 6.9; 6144 x 4096 11.0, 7.8, 6.9, 11.0;
 // 4096 x 12288 26.7, 16.7, 13.1, 12.4; 151936 x 4096 97, 102, 124, 194.
 struct Cut {
     int parts;
@@ -835,7 +835,7 @@ struct Cut {
 static Cut cut_of(int64_t tiles, int k_blocks, bool halves, const Places& p) {
     Cut best = {1, INT64_MAX};
     for (int s = 1; s <= 8 && s <= k_blocks; ++s) {
-        const int64_t at_once = (halves ? 2 : 1) * p.clusters[s];
+        const int64_t at_once = !halves ? p.clusters[s] : s % 2 ? 2 * p.clusters[s] : p.clusters[s / 2];
         if (at_once < 1) continue;
         const int64_t waves = (tiles + at_once - 1) / at_once, cost = waves * ((k_blocks + s - 1) / s + 4 + s);
         if (cost < best.cost) best = {s, cost};
