@@ -435,3 +435,77 @@ def test_chain_against_64_bits():
     q2, s2 = ops.fp8_swiglu(q, s, p["gate_up"])
     check_swiglu(q2, s2, q, s, p["gate_up"])
     check_linear(ops.fp8_linear(q2, s2, p["down"]), q2, s2, p["down"])
+
+
+def test_products_of_all_kinds_at_once():
+    """Clusters, single CTAs and pairs on three streams, over and over: every result as when it runs alone."""
+    p = layer_parts()
+    sizes = (5, 40, 100, 700)
+    ins = [ops.quant_fp8(rows(T, T, 512, BF)) for T in sizes]
+    wide = make_weight(5, 2000, 512)
+    want = [(ops.fp8_linear(q, s, wide), *ops.fp8_swiglu(q, s, p["gate_up"])) for q, s in ins]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sizes]
+    got = [None] * len(sizes)
+    for _ in range(30):
+        for i, (q, s) in enumerate(ins):
+            with torch.cuda.stream(streams[i]):
+                got[i] = (ops.fp8_linear(q, s, wide), *ops.fp8_swiglu(q, s, p["gate_up"]))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1].view(torch.uint8), b[1].view(torch.uint8)) and torch.equal(a[2], b[2])
+    wide.check()
+    p["gate_up"].check()
+
+
+def test_weights_written_just_before_they_are_read():
+    """The products ask for their first weights early; what a call before them wrote is what they multiply."""
+    q, s = ops.quant_fp8(rows(1, 8, 2048, BF))
+    a, b = make_weight(1, 3000, 2048), make_weight(2, 3000, 2048)
+    w = ops.Fp8Weight(a.w.clone(), a.scale.clone())
+    want = [ops.fp8_linear(q, s, x) for x in (a, b)]
+    for i in range(40):
+        src = (a, b)[i % 2]
+        w.w.view(torch.uint8).copy_(src.w.view(torch.uint8))
+        w.scale.copy_(src.scale)
+        ops.quant_fp8(rows(1, 8, 2048, BF))   # a launch between them that lets the next begin early
+        assert torch.equal(ops.fp8_linear(q, s, w), want[i % 2]), i
+
+
+def test_offsets_past_32_bits():
+    """Rows whose first element is past 2^31 elements, of inputs and outputs."""
+    T, n = 540000, 4096
+    x = torch.zeros(T, n, dtype=BF, device=DEV)
+    tail = rows(1, 300, n, BF)
+    x[-300:] = tail
+    q, s = ops.quant_fp8(x)
+    pq, ps = plain_quant(tail)
+    assert torch.equal(q[-300:].cpu().view(torch.uint8), pq.view(torch.uint8)) and torch.equal(s[-300:].cpu(), ps)
+    assert bool((s[:-300] == 0).all())
+    w = torch.ones(n, dtype=BF, device=DEV)
+    q2, s2 = ops.rmsnorm_fp8(x, w, 1e-6, residual=x)
+    r64 = (tail.float() * 2).to(BF).double()
+    y = r64 * torch.rsqrt((r64 * r64).mean(-1, keepdim=True) + 1e-6)
+    check_stored(q2[-300:], s2[-300:], y, NORM_E * y.abs(), NORM_E)
+    assert torch.equal(x[-300:].double(), r64)
+    del x, q2, s2
+    wt = make_weight(1, 4200, n)
+    out = ops.fp8_linear(q, s, wt)
+    check_linear(out[-300:], q[-300:], s[-300:], wt)
+    assert bool((out[:1000] == 0).all())
+    wt.check()
+
+
+def test_first_call_of_a_kernel_may_be_captured():
+    """In a process of its own: nothing has been launched before the capture."""
+    import subprocess
+    import sys
+    code = ("import torch\nfrom zoomkv_revision_b200 import ops\n"
+            "q = torch.zeros(90, 256, device='cuda').to(torch.float8_e4m3fn); s = torch.ones(90, 2, device='cuda')\n"
+            "w = ops.Fp8Weight(torch.ones(300, 256, device='cuda').to(torch.float8_e4m3fn), torch.ones(3, 2, device='cuda'))\n"
+            "q.view(torch.uint8).fill_(0x38)\ng = torch.cuda.CUDAGraph()\ntorch.cuda.synchronize()\n"
+            "with torch.cuda.graph(g):\n    a = ops.fp8_linear(q, s, w); b = ops.fp8_linear(q[:7], s[:7], w)\n"
+            "g.replay(); torch.cuda.synchronize()\n"
+            "assert bool((a == 256).all()) and bool((b == 256).all())\nprint('captured')\n")
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert got.returncode == 0 and "captured" in got.stdout, got.stderr[-2000:]

@@ -80,8 +80,8 @@ __global__ void __launch_bounds__(kQuantThreads) quant_kernel(RowArgs a, int blo
     const int64_t row = item / blocks;
     const int at = (int)(item - row * blocks) * kBlock + (threadIdx.x & 7) * 16;
     const bool in = row < a.tokens && at < a.dim;
-    grid_dep_launch_next();
     grid_dep_wait();
+    grid_dep_launch_next();
     float y[16] = {};
     if (in) load16<kBf16>(a.x + row * a.x_ld + at, y);
     store_block(y, a, row, at, in);
@@ -100,8 +100,8 @@ __global__ void __launch_bounds__(kRow < 128 ? 128 : kRow) norm_kernel(RowArgs a
     const bool live = row < a.tokens;
     float x[kTurns][16] = {};
     float ss = 0.f;
-    grid_dep_launch_next();
     grid_dep_wait();
+    grid_dep_launch_next();
 #pragma unroll
     for (int j = 0; j < kTurns; ++j) {
         const int at = (j * kRow + t) * 16;

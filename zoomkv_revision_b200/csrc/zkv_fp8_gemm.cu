@@ -7,12 +7,16 @@
 // sum of 128 products (tcgen05, fp32 in tensor memory) is read back, scaled
 // and added in fp32 registers.
 //
-// Features are the matrix rows of the tensor core's tile (128 lanes), tokens
-// its columns: a step of few tokens fills the tile all the same, and the
-// weights go from memory to the tensor core without passing a register.  What
-// bounds such a call is reading the weights once; tiles that are fewer than
-// the SMs are cut along the inner dimension over a cluster, whose CTAs add
-// their parts through distributed shared memory in the order of their ranks.
+// Up to 64 tokens features are the rows of the tensor core's tile (128 lanes)
+// and tokens its columns: a step of few tokens fills the tile all the same,
+// and the weights go from memory to the tensor core without passing a
+// register.  What bounds such a call is reading the weights once (32 tokens x
+// 151936 x 4096: 103 us, 6.2 TB/s), and below some 50 MB of weights the chain
+// launch - first copies - products - join (8 tokens x 4096 x 4096: 6.2 us for
+// 2.6 of bytes).  Tiles that are fewer than the SMs are cut along the inner
+// dimension over a cluster, whose CTAs add their parts through distributed
+// shared memory in the order of their ranks.  From 65 tokens on the tokens are
+// the rows; long prompts take pairs of CTAs (below).
 #include <cuda.h>
 
 #include <algorithm>
@@ -66,13 +70,12 @@ struct Few {
     static constexpr int stages_in(int bytes) {
         return (bytes - smem(0)) / kStage < kMost ? (bytes - smem(0)) / kStage : kMost;
     }
-    // The ring takes an SM's shared memory, or half of it, for two CTAs an SM.  The CTAs of a cluster wait for one
-    // another, so none may have to wait for tensor memory that a CTA of another cluster holds on its SM: at most two of
-    // these kernels' CTAs fit on one (each takes more than a third of the shared memory), with at most half of the tensor
-    // memory each; or one alone.
-    // Two an SM for one part and up to 32 tokens (151936 x 4096: 8 tokens 97 us, 106 with one; 32 tokens 101 and 119):
-    // more take the registers of one, and two parts' stages are too few in half the memory (8 tokens of 12288 x 4096: 23.3
-    // us, 21.7 with one).
+    // The ring takes an SM's shared memory, or half of it, for two CTAs an SM: for one part and up to 32 tokens (151936 x
+    // 4096: 8 tokens 97 us, 106 with one; 32 tokens 101 and 119).  More tokens take the registers of one, and two parts'
+    // stages are too few in half the memory (8 tokens of 12288 x 4096: 23.3 us, 21.7 with one).
+    // The CTAs of a cluster wait for one another, so none may have to wait for tensor memory that a CTA of another cluster
+    // holds on its SM: at most two CTAs of this file's kernels fit on an SM (each takes more than a third of its shared
+    // memory), with at most half of the tensor memory each; one that takes more of it fits beside none.
     static constexpr bool kHalves = kParts == 1 && kTok <= 32;
     // Even, as the buffers are: a stage is always the same issuing warp's.  A wait for a phase by its parity lets a warp
     // through at once while the phase before, another warp's, has not ended.
@@ -163,8 +166,8 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(generic + (tmem_at - base));
-    grid_dep_launch_next();
     grid_dep_wait();
+    grid_dep_launch_next();
 
     float acc[C::kMine];
 #pragma unroll
@@ -188,7 +191,7 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
         for (int i = got > C::kStages ? got - C::kStages : 0; i < got; ++i)
             if (!tc::wait_all(full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.status)) break;
     } else if (warp <= 2) {
-        // Two warps issue every other block's products: a pass of two barriers takes one some 400 clocks.
+        // Two warps issue every other block's products: to pass two barriers takes a warp some 400 clocks, to issue 400 more.
         int done = warp - 1;
         for (; done < n; done += 2) {
             const int s = done % C::kStages, b = done % C::kBufs, turn = done / C::kBufs;
@@ -368,13 +371,17 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
 // operand, so that a CTA loads 32 KB for a block of the inner dimension
 // instead of 48 (96 bytes a clock at the full rate, more than L2 gives an SM).
 // Each block's sums go to tensor memory, and from there, scaled, into fp32
-// registers: a thread has one token and 64 features, both scales are its own,
-// and one packed product-and-sum takes two elements.  The tensor core would
-// have to wait while a block's sums are read and the barriers pass between
-// the two CTAs (some 1100 clocks for the 512 of a block), so the tile is
-// multiplied in two halves of 128 features with two buffers of tensor memory
-// each, every half by an issuing warp and two warpgroups of readers of its
-// own.
+// registers: a thread has one token and 128 features, and both scales are its
+// own.  The tensor core would have to wait while a block's sums are read and
+// the barriers pass between the two CTAs (some 1100 clocks for the 512 of a
+// block), so the tile is multiplied in two halves of 128 features with two
+// buffers of tensor memory each, every half by an issuing warp and a
+// warpgroup of readers of its own.
+// 4096 x 6144 x 4096: 93 us (2.2 PFLOP/s; 78 us with the readers' loop taken
+// out of a copy, six waves of tiles for 5.2); in a loop at the power limit 107
+// us at 1.49 GHz (92 without the readers).  Sixteen warps of readers with 64
+// features each took 105 and 121: more instructions for the same sums.  Packed
+// products and sums of two elements changed nothing.
 template <bool kGated>
 struct Many {
     static constexpr int kTokens = 256, kFeatures = 256;
@@ -492,8 +499,8 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
     tc::cluster_sync();  // both CTAs' barriers
     tc::fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(generic + (tmem_at - base));
-    grid_dep_launch_next();
     grid_dep_wait();
+    grid_dep_launch_next();
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");

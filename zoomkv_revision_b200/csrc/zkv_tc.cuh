@@ -87,7 +87,7 @@ __device__ __forceinline__ void prefetch_map(const void* map) {
 // Copies and arrivals on barriers of the other CTA.
 // The arrival publishes nothing but that tensor memory has been read, which the tcgen05 fences order: a release at cluster
 // scope waits for the thread's outstanding accesses of every kind and made a block of the inner dimension take 2400
-// clocks instead of 600.
+// clocks instead of 1000 (4096 x 6144 x 4096: 217 us, 104 without).
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {  // an address of in_cta()
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -204,13 +204,6 @@ __device__ __forceinline__ void ld(uint32_t at, uint32_t (&r)[32]) {
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(at));
-}
-// Two fp32 products and sums in one instruction.
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
 }
 
 // ------------------------------------------------------------ products
