@@ -53,16 +53,14 @@ __device__ __forceinline__ void load16(const uint16_t* p, float (&v)[16]) {
     for (int i = 0; i < 8; ++i) to_floats<kBf16>(w[i], v[2 * i], v[2 * i + 1]);
 }
 
-// 16 elements of a thread; the 8 threads of a block of 128 find its scale.
-__device__ __forceinline__ void store_block(const float (&y)[16], const RowArgs& a, int64_t row, int at, bool in) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m = max(m, magnitude(y[i]));
+// 16 elements of a thread, m the largest magnitude of them; the 8 threads of a block of 128 find its scale.
+__device__ __forceinline__ void store_block(float (&y)[16], uint32_t m, const RowArgs& a, int64_t row, int at, bool in) {
 #pragma unroll
     for (int off = 4; off >= 1; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
     if (!in) return;
     const float s = scale_of(m);
     const Quotient by(s);
+    by.prepare(y);
     uint4 q;
     q.x = by.e4m3(y[0], y[1], y[2], y[3]);
     q.y = by.e4m3(y[4], y[5], y[6], y[7]);
@@ -83,8 +81,22 @@ __global__ void __launch_bounds__(kQuantThreads) quant_kernel(RowArgs a, int blo
     grid_dep_wait();
     grid_dep_launch_next();
     float y[16] = {};
-    if (in) load16<kBf16>(a.x + row * a.x_ld + at, y);
-    store_block(y, a, row, at, in);
+    uint32_t m = 0;
+    if (in) {
+        const uint4* x = reinterpret_cast<const uint4*>(a.x + row * a.x_ld + at);
+        const uint4 p = x[0], q = x[1];
+        const uint32_t w[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+        // 16-bit magnitudes are ordered as the numbers are, infinities and NaN above: two in one comparison
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+            to_floats<kBf16>(w[i], y[2 * i], y[2 * i + 1]);
+        }
+        float lo, hi;
+        to_floats<kBf16>(m, lo, hi);
+        m = max(magnitude(lo), magnitude(hi));
+    }
+    store_block(y, m, a, row, at, in);
 }
 
 // kRow threads a row (a power of two, whole warps), kTurns x 16 elements of
@@ -145,7 +157,10 @@ __global__ void __launch_bounds__(kRow < 128 ? 128 : kRow) norm_kernel(RowArgs a
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[j][i] = x[j][i] * inv * w[i];
         }
-        store_block(x[j], a, row, at, in);
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = max(m, magnitude(x[j][i]));
+        store_block(x[j], m, a, row, at, in);
     }
 }
 

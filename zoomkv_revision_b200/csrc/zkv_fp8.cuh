@@ -36,7 +36,7 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 // processor", IBM J. Res. Dev. 34, 1990).  The division took 16383 x 4096
 // elements 53 us, and 50 to 69 where it decided only what two enclosing
 // products left open: an element in 16 of every seventh block of bf16 numbers
-// is the exact middle of two codes.  A scale of 0 stores zeros.
+// is the exact middle of two codes; 40.5 so.  A scale of 0 stores zeros.
 struct Quotient {
     float lift, scale, r;  // lift: a power of two that keeps a remainder within fp32's range
 
@@ -45,13 +45,35 @@ struct Quotient {
         scale = s * lift;
         r = scale == 0.f ? 0.f : __fdiv_rn(1.f, scale);
     }
-    __device__ __forceinline__ float of(float x) const {
-        x *= lift;
-        const float q = x * r;
-        return copysignf(fmaf(fmaf(-q, scale, x), r, q), x);  // (the remainder of -0 is +0)
+    // To be called once on what e4m3 is given.
+    template <int N>
+    __device__ __forceinline__ void prepare(float (&x)[N]) const {
+        if (lift != 1.f)
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] *= lift;
+    }
+    // Two quotients at once: packed products and sums (16383 x 4096 elements 43.8 -> 40.5 us).  The remainder of -0 is +0, so
+    // the sign is the element's own.
+    __device__ __forceinline__ void of(float& a, float& b) const {
+        asm("{\n\t"
+            ".reg .b64 x, y, s, q, t;\n\t"
+            ".reg .b32 u, v;\n\t"
+            "mov.b64 x, {%0, %1};\n\t"
+            "mov.b64 y, {%2, %2};\n\t"
+            "mov.b64 s, {%3, %3};\n\t"
+            "mul.rn.f32x2 q, x, y;\n\t"
+            "fma.rn.f32x2 t, q, s, x;\n\t"
+            "fma.rn.f32x2 t, t, y, q;\n\t"
+            "mov.b64 {u, v}, t;\n\t"
+            "copysign.f32 %0, %0, u;\n\t"
+            "copysign.f32 %1, %1, v;\n\t}"
+            : "+f"(a), "+f"(b)
+            : "f"(r), "f"(-scale));
     }
     __device__ __forceinline__ uint32_t e4m3(float a, float b, float c, float d) const {
-        return e4m3x4(of(a), of(b), of(c), of(d));
+        of(a, b);
+        of(c, d);
+        return e4m3x4(a, b, c, d);
     }
 };
 

@@ -351,7 +351,10 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
                     v = make_float4(gated(g.x, h.x), gated(g.y, h.y), gated(g.z, h.z), gated(g.w, h.w));
                 s[u] = scale_of(__reduce_max_sync(
                     0xffffffffu, max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w)))));
-                q[u] = Quotient(s[u]).e4m3(v.x, v.y, v.z, v.w);
+                const Quotient by(s[u]);
+                float e[4] = {v.x, v.y, v.z, v.w};
+                by.prepare(e);
+                q[u] = by.e4m3(e[0], e[1], e[2], e[3]);
             }
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
@@ -667,6 +670,9 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
                 m = max(m, ld_shared<uint32_t>(top + (half ^ 1) * 512));
                 const float s = scale_of(m);
                 const Quotient by(s);
+                if (by.lift != 1.f)
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) acc[i] *= by.lift;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float* v = acc + 16 * j;
