@@ -509,3 +509,71 @@ def test_first_call_of_a_kernel_may_be_captured():
             "assert bool((a == 256).all()) and bool((b == 256).all())\nprint('captured')\n")
     got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert got.returncode == 0 and "captured" in got.stdout, got.stderr[-2000:]
+
+
+# ------------------------------------------------------------------ long prompts (pairs of CTAs)
+@pytest.mark.parametrize("T", [1500, 2049])
+@pytest.mark.parametrize("dtype", [BF, HF, FL])
+def test_linear_long(T, dtype):
+    """A last tile of tokens and of features that is not full, a last block of the inner dimension of 16; rows of the output
+    that start on 16 bytes and rows that do not; scales in any order."""
+    n, k = 4001, 1040
+    q, s = ops.quant_fp8(rows(T, T, k, BF))
+    w = make_weight(n, n, k, ld=1088)
+    check_linear(ops.fp8_linear(q, s, w, dtype=dtype), q, s, w)
+    buf = torch.full((T, 4016), 5.0, dtype=dtype, device=DEV)
+    ops.fp8_linear(q, s.contiguous(), w, out=buf[:, :n])
+    check_linear(buf[:, :n], q, s, w)
+    assert bool((buf[:, n:] == 5).all())
+    one = s[:1].expand(T, blocks(k))
+    check_linear(ops.fp8_linear(q, one, w, out=buf[:, :n]), q, one, w)
+    w.check()
+
+
+@pytest.mark.parametrize("T,f,k", [(1500, 4000, 1040), (2049, 4112, 256), (700, 12288, 512)])
+def test_swiglu_long(T, f, k):
+    q, s = ops.quant_fp8(rows(T, T, k, BF) * 0.05)
+    w = make_weight(f, f, k, 2)
+    out, scale = torch.full((T, f + 32), 9, dtype=torch.uint8, device=DEV), torch.full((T, blocks(f) + 1), -1.0, device=DEV)
+    ops.fp8_swiglu(q, s, w, out=out.view(F8)[:, 16: 16 + f], scale=scale[:, :-1])
+    check_swiglu(out.view(F8)[:, 16: 16 + f], scale[:, :-1], q, s, w)
+    assert bool((out[:, :16] == 9).all()) and bool((out[:, 16 + f:] == 9).all()) and bool((scale[:, -1] == -1).all())
+    w.check()
+
+
+def test_long_rows_do_not_touch_one_another():
+    T = 1500
+    q, s = ops.quant_fp8(rows(T, T, 512, BF) * 0.1)
+    w, w2 = make_weight(1, 4001, 512), make_weight(2, 4000, 512, 2)
+    out, gated = ops.fp8_linear(q, s, w), ops.fp8_swiglu(q, s, w2)
+    q2, s2 = q.clone(), s.clone()
+    q2.view(torch.uint8)[200] = 0x7f
+    s2[1301] = float("inf")
+    got, g2 = ops.fp8_linear(q2, s2, w), ops.fp8_swiglu(q2, s2, w2)
+    keep = torch.ones(T, dtype=torch.bool, device=DEV)
+    keep[200] = keep[1301] = False
+    assert torch.equal(got[keep], out[keep]) and torch.equal(g2[0].view(torch.uint8)[keep], gated[0].view(torch.uint8)[keep])
+    assert torch.equal(g2[1][keep], gated[1][keep])
+    assert bool(torch.isnan(got[200]).all()) and not bool(torch.isfinite(got[1301]).any())
+    assert bool(torch.isnan(value(*g2)[~keep]).all())
+
+
+def test_long_chain_in_a_graph():
+    """Prompts of 1500 tokens through a layer, captured and replayed, on another stream too."""
+    T, p = 1500, layer_parts()
+    x, attn = rows(1, T, 512, BF) * 0.3, rows(2, T, 256, BF) * 0.1
+    start = x.clone()
+    want = layer(x, attn, p)
+    kept = x.clone()
+    x.copy_(start)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer(x, attn, p)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(5):
+            x.copy_(start)
+            graph.replay()
+    side.synchronize()
+    assert torch.equal(y, want) and torch.equal(x, kept)

@@ -462,6 +462,11 @@ __device__ __forceinline__ void copy_out(const Product& a, uint32_t tile, int64_
     }
 }
 
+// Whether a row's last features end inside 16 bytes of this tile: a tensor map's store writes those 16 bytes whole.
+__device__ __forceinline__ bool cut_short(int rows, int f, int columns, int element) {
+    return f + columns > rows && rows * (int64_t)element % 16;
+}
+
 template <bool kGated>
 __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
     many_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
@@ -709,7 +714,7 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
                     group_sync(half);
                     for (int c = 0; c < 2; ++c) {
                         const int f = tn * C::kFeatures + half * kTile + side * 64 + c * 32;
-                        if (!mapped) copy_out<uint32_t>(a, staging + c * kTileBytes, token0, f, 32);
+                        if (!mapped || cut_short(a.rows, f, 32, 4)) copy_out<uint32_t>(a, staging + c * kTileBytes, token0, f, 32);
                         else if (issues && f < a.rows && token0 < a.tokens)
                             tc::tma_store_2d(&out_map, staging + c * kTileBytes, f, (int)token0);
                     }
@@ -738,7 +743,7 @@ __global__ void __launch_bounds__(Many<kGated>::kThreads, 1)
                 group_sync(half);
                 for (int c = 0; c < 2; ++c) {
                     const int f = tn * C::kFeatures + half * kTile + c * 64;
-                    if (!mapped) copy_out<uint16_t>(a, staging + c * kTileBytes, token0, f, 64);
+                    if (!mapped || cut_short(a.rows, f, 64, 2)) copy_out<uint16_t>(a, staging + c * kTileBytes, token0, f, 64);
                     else if (issues && f < a.rows && token0 < a.tokens)
                         tc::tma_store_2d(&out_map, staging + c * kTileBytes, f, (int)token0);
                 }
