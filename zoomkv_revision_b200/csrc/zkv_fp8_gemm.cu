@@ -317,19 +317,22 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
     const int most = (int)min((int64_t)kTok, a.tokens - t0);  // tokens of this tile
     for (int t = warp * parts + rank; t < most; t += kAtOnce * turn) {
         float4 y[kAtOnce][kParts];
-        auto at = [&](int u, int p) { return (p * kTok + min(t + u * turn, most - 1)) * C::kPitch + lane * 4; };
+        auto at = [&](int u, int p) { return (p * kTok + t + u * turn) * C::kPitch + lane * 4; };
+        auto have = [&](int u) { return t + u * turn < most; };
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
             for (int p = 0; p < kParts; ++p)
-                y[u][p] = parts == 1 ? *reinterpret_cast<const float4*>(join + at(u, p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                y[u][p] = parts == 1 && have(u) ? *reinterpret_cast<const float4*>(join + at(u, p))
+                                                : make_float4(0.f, 0.f, 0.f, 0.f);
         for (uint32_t r = 0; parts > 1 && r < parts; ++r) {
             const uint32_t from = tc::in_cta(base, r);
             float4 v[kAtOnce][kParts];
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
-                for (int p = 0; p < kParts; ++p) v[u][p] = tc::ld_cluster(from + at(u, p) * 4);
+                for (int p = 0; p < kParts; ++p)
+                    v[u][p] = have(u) ? tc::ld_cluster(from + at(u, p) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
         if (kParts == 1) {
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u)
-                if (t + u * turn < most) store4(a, t0 + t + u * turn, f, y[u][0]);
+                if (have(u)) store4(a, t0 + t + u * turn, f, y[u][0]);
         } else {
             uint32_t q[kAtOnce];
             float s[kAtOnce];
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
                 const int64_t to = t0 + t + u * turn;
-                if (t + u * turn >= most) break;
+                if (!have(u)) break;
                 if (f < a.rows) *reinterpret_cast<uint32_t*>((uint8_t*)a.out + to * a.out_ld + f) = q[u];
                 if (lane == 0) a.out_scale[to * a.os_token + tile * a.os_block] = s[u];
             }
@@ -947,8 +950,8 @@ static int check_call(const void* x, int64_t x_ld, const float* x_scale, int64_t
 // Up to 64 tokens features are the rows of a tile.  Above, CTAs of 128 tokens and one part's 128 features each (a cluster
 // may share a tile), or pairs of CTAs of 256 tokens and 256 features: by the blocks that the waves of either take after one
 // another.  A block takes the pair a little longer, and CTAs of two parts twice as long.  us of the first and of the second
-// kind: 333 x 4096 x 4096 16.3 and 19.3, 768 x 4096 x 4096 34.5 and 20.5, 512 x 4096 x 12288 41.1 and 46.5, 129 x 2 x 12288
-// x 4096 60.9 and 43.0, 1024 x 1024 x 4096 11.7 and 18.6.
+// kind: 333 x 4096 x 4096 13.9 and 17.8, 768 x 4096 x 4096 32.9 and 18.9, 512 x 4096 x 12288 38.4 and 42.4, 129 x 2 x 12288
+// x 4096 49.4 and 44.9, 1024 x 1024 x 4096 11.7 and 17.7.
 template <int kParts>
 static int launch(const zkv_fp8_weight* w, const void* x, int64_t x_ld, const Product& a, cudaStream_t stream) {
     if (a.tokens <= 16) return launch_few<16, kParts>(w, x, x_ld, a, stream);
