@@ -822,27 +822,48 @@ static cudaLaunchConfig_t configure(cudaLaunchAttribute (&attr)[2], unsigned x, 
     return cfg;
 }
 
-// Clusters of s CTAs (s = 1..8) that the current device holds at once: a cluster lies within one of its groups of SMs, so
-// that of three, five or seven CTAs many SMs stay empty.  The same for all of these kernels, which have an SM to
-// themselves.
+// Clusters of s CTAs (s = 1..8) that the current device holds at once with one CTA an SM: a cluster lies within one of its
+// groups of SMs, so that of three, five or seven CTAs many SMs stay empty.  Asked for one kernel that has an SM to itself
+// and used for all products, so that how a product is cut depends neither on which ran first nor on whether the driver's
+// count looks at what a kernel takes (580.159 counts one CTA an SM for those that share one, too).
 struct Places {
     int clusters[9];
 };
-template <typename Kernel>
-static const Places* places(Kernel kernel, int threads, int smem) {
+static const Places* places() {
+    using C = Few<128, 1>;
+    static_assert(2 * (C::smem(C::kStages) + 1024) > 228 * 1024, "an SM to itself");
     static std::mutex mutex;
     static Places known[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    auto kernel = few_kernel<128, 1>;
     const std::lock_guard<std::mutex> lock(mutex);
     Places& p = known[dev];
-    if (!p.clusters[1])
-        for (int s = 8; s >= 1; --s) {
-            cudaLaunchAttribute attr[2];
-            cudaLaunchConfig_t cfg = configure(attr, 64 * s, 1, threads, smem, s, nullptr);
-            if (cudaOccupancyMaxActiveClusters(&p.clusters[s], kernel, &cfg) != cudaSuccess) return nullptr;
-        }
+    if (p.clusters[1]) return &p;
+    if (!raise_smem_limit((const void*)kernel, C::smem(C::kStages))) return nullptr;
+    for (int s = 8; s >= 1; --s) {
+        cudaLaunchAttribute attr[2];
+        cudaLaunchConfig_t cfg = configure(attr, 64 * s, 1, C::kThreads, C::smem(C::kStages), s, nullptr);
+        if (cudaOccupancyMaxActiveClusters(&p.clusters[s], kernel, &cfg) != cudaSuccess) return nullptr;
+    }
     return &p;
+}
+
+// Whether two CTAs of a kernel run on an SM of the current device: 1 or 0, -1 where it cannot be asked.  The kernel's
+// shared-memory limit has been raised.
+template <int kTok, int kParts>
+static int shares_sm() {
+    using C = Few<kTok, kParts>;
+    if (!C::kHalves) return 0;
+    static std::mutex mutex;
+    static int known[64] = {};  // CTAs an SM
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+    const std::lock_guard<std::mutex> lock(mutex);
+    if (!known[dev] && cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known[dev], few_kernel<kTok, kParts>, C::kThreads,
+                                                                     C::smem(C::kStages)) != cudaSuccess)
+        return -1;
+    return known[dev] >= 2;
 }
 
 // How the inner dimension is cut over a cluster's CTAs: the number for which the waves of clusters take the fewest blocks
@@ -873,9 +894,10 @@ static int launch_few(const zkv_fp8_weight* w, const void* x, int64_t x_ld, cons
     if (wide > 65535) return ZKV_ERR_CAPACITY;
     auto kernel = few_kernel<kTok, kParts>;
     if (!raise_smem_limit((const void*)kernel, C::smem(C::kStages))) return launch_refused();
-    const Places* p = places(kernel, C::kThreads, C::smem(C::kStages));
-    if (!p) return launch_refused();
-    const int parts = cut_of(a.row_blocks * wide, a.k_blocks, C::kHalves, *p).parts;
+    const Places* p = places();
+    const int shares = shares_sm<kTok, kParts>();
+    if (!p || shares < 0) return launch_refused();
+    const int parts = cut_of(a.row_blocks * wide, a.k_blocks, shares, *p).parts;
     cudaLaunchAttribute attr[2];
     const cudaLaunchConfig_t cfg = configure(attr, (unsigned)(a.row_blocks * parts), (unsigned)wide, C::kThreads,
                                              C::smem(C::kStages), (unsigned)parts, stream);
@@ -957,10 +979,7 @@ static int launch(const zkv_fp8_weight* w, const void* x, int64_t x_ld, const Pr
     if (a.tokens <= 16) return launch_few<16, kParts>(w, x, x_ld, a, stream);
     if (a.tokens <= 32) return launch_few<32, kParts>(w, x, x_ld, a, stream);
     if (a.tokens <= 64) return launch_few<64, kParts>(w, x, x_ld, a, stream);
-    using C = Few<128, kParts>;
-    auto kernel = few_kernel<128, kParts>;
-    const Places* p = raise_smem_limit((const void*)kernel, C::smem(C::kStages)) ? places(kernel, C::kThreads, C::smem(C::kStages))
-                                                                                 : nullptr;
+    const Places* p = places();
     if (!p) return launch_refused();
     const int64_t few = kParts * cut_of(a.row_blocks * ((a.tokens + 127) / 128), a.k_blocks, false, *p).cost;
     const int64_t pairs = std::max(p->clusters[2], 1);
