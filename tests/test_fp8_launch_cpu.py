@@ -88,5 +88,14 @@ def test_a_shared_sm_is_asked_for(launches):
     assert launches([(8, 4096, 12288, 1)], "single") == [(0, [("few 16 1", 128, 1, 4)])]
 
 
+def test_millions_of_tokens(launches):
+    """A grid has room for 65535 tiles of tokens; the pairs take more."""
+    most = 65535 * 128
+    got = launches([(most, 128, 8192, 1), (most + 1, 128, 8192, 1), (2 * most, 16, 6528, 1), (most + 1, 128, 8192, 2)])
+    assert [rc for rc, _ in got] == [0] * 4
+    assert [lines[0][0] for _, lines in got] == ["few 128 1", "many 1", "many 1", "many 2"]
+    assert got[0][1][0][2] == 65535
+
+
 if __name__ == "__main__":
     print(json.dumps(child(json.loads(sys.argv[1]))))

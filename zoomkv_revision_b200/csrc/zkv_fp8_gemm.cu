@@ -885,13 +885,14 @@ static Cut cut_of(int64_t tiles, int k_blocks, bool halves, const Places& p) {
     return best;
 }
 
+constexpr int kMostWide = 65535;  // tiles of tokens that a grid's second dimension holds
+
 template <int kTok, int kParts>
 static int launch_few(const zkv_fp8_weight* w, const void* x, int64_t x_ld, const Product& a, cudaStream_t stream) {
     using C = Few<kTok, kParts>;
     CUtensorMap x_map;
     if (!encode_rows(&x_map, x, w->k, a.tokens, x_ld, 0, kTok)) return ZKV_ERR_ARG;
-    const int64_t wide = (a.tokens + kTok - 1) / kTok;
-    if (wide > 65535) return ZKV_ERR_CAPACITY;
+    const int64_t wide = (a.tokens + kTok - 1) / kTok;  // at most kMostWide, as launch() chooses
     auto kernel = few_kernel<kTok, kParts>;
     if (!raise_smem_limit((const void*)kernel, C::smem(C::kStages))) return launch_refused();
     const Places* p = places();
@@ -973,12 +974,13 @@ static int check_call(const void* x, int64_t x_ld, const float* x_scale, int64_t
 // may share a tile), or pairs of CTAs of 256 tokens and 256 features: by the blocks that the waves of either take after one
 // another.  A block takes the pair a little longer, and CTAs of two parts twice as long.  us of the first and of the second
 // kind: 333 x 4096 x 4096 13.9 and 17.8, 768 x 4096 x 4096 32.9 and 18.9, 512 x 4096 x 12288 38.4 and 42.4, 129 x 2 x 12288
-// x 4096 49.4 and 44.9, 1024 x 1024 x 4096 11.7 and 17.7.
+// x 4096 49.4 and 44.9, 1024 x 1024 x 4096 11.7 and 17.7.  More tokens than a grid of the first kind holds go to the pairs.
 template <int kParts>
 static int launch(const zkv_fp8_weight* w, const void* x, int64_t x_ld, const Product& a, cudaStream_t stream) {
     if (a.tokens <= 16) return launch_few<16, kParts>(w, x, x_ld, a, stream);
     if (a.tokens <= 32) return launch_few<32, kParts>(w, x, x_ld, a, stream);
     if (a.tokens <= 64) return launch_few<64, kParts>(w, x, x_ld, a, stream);
+    if (a.tokens > (int64_t)kMostWide * 128) return launch_many<kParts == 2>(w, x, x_ld, a, stream);
     const Places* p = places();
     if (!p) return launch_refused();
     const int64_t few = kParts * cut_of(a.row_blocks * ((a.tokens + 127) / 128), a.k_blocks, false, *p).cost;
