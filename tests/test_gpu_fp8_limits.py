@@ -24,3 +24,25 @@ def test_more_tiles_of_tokens_than_a_grid_holds():
     assert bool((out[200: -500] == 0).all()) and bool((scale[200: -500] == 0).all())
     one.check()
     two.check()
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_check_waits_for_every_stream(own):
+    """What a product on another stream reports is seen, by a check on the default stream or on one of its own, and the word
+    is zero for every stream once check has raised.  (The report is a copy to the status word behind a wait of some 50 ms:
+    no product's wait runs out here.)"""
+    w = make_weight(1, 128, 128)
+    q, s = ops.quant_fp8(rows(1, 4, 128, BF))
+    work, mine = torch.cuda.Stream(), torch.cuda.Stream() if own else torch.cuda.current_stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(work):
+        torch.cuda._sleep(100_000_000)
+        ops.fp8_linear(q, s, w)
+        w.status.fill_(6)
+    with torch.cuda.stream(mine):
+        with pytest.raises(RuntimeError, match="status 6"):
+            w.check()
+    with torch.cuda.stream(work):
+        seen = w.status.clone()
+    w.check()
+    assert int(seen.cpu()) == 0

@@ -1725,10 +1725,13 @@ class Fp8Weight:
         return self.w.float() * self.scale[at].repeat_interleave(S, 1)[:, : self.k]
 
     def check(self) -> None:
-        """Raises if a wait inside a product with this weight ran out since the last check (waits for the GPU)."""
+        """Raises if a wait inside a product with this weight ran out since the last check (waits for the weight's device, all
+        streams of it)."""
+        torch.cuda.synchronize(self.device)
         code = int(self.status.item())
         if code:
             self.status.zero_()
+            torch.cuda.synchronize(self.device)   # what a product on any stream reports from here on is kept
             check(code, "8-bit product")
 
 
