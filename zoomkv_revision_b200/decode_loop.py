@@ -150,7 +150,7 @@ class Fp8Weights:
                 L.clear()
 
     def check(self) -> None:
-        """Raises if a wait inside a product ran out (waits for the GPU)."""
+        """Raises if a wait inside a product ran out (waits for the GPU, all streams)."""
         for L in self.layers:
             for name in ("wqkv", "wo", "gate_up", "down"):
                 L[name].check()

@@ -1189,6 +1189,18 @@ def rq_popcount_topk(cand, lay: RqLayout, planes, qparams, K: int, *, C: int | N
 _POOL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 _INT32 = torch.int32
 
+
+def take_status(status) -> int:
+    """What calls on any stream have reported to a status word, which is zero from then on for every stream (waits for the
+    word's device)."""
+    torch.cuda.synchronize(status.device)
+    code = int(status.item())
+    if code:
+        status.zero_()
+        torch.cuda.synchronize(status.device)
+    return code
+
+
 class KVPool:
     """One layer's pooled KV cache: k, v [n_blocks, block_size, kv_heads, head_dim]
     bf16, fp16 or float8_e4m3fn CUDA tensors, any strides with whole 16-byte
@@ -1243,10 +1255,9 @@ class KVPool:
 
     def check(self) -> None:
         """Raises if a pool_write or pool_decode that was given no status word met a slot, block id or length outside the
-        pool or its table, or a wait that ran out, since the last check (waits for the GPU)."""
-        code = int(self.status.item())
+        pool or its table, or a wait that ran out, since the last check (waits for the pool's device, all streams of it)."""
+        code = take_status(self.status)
         if code:
-            self.status.zero_()
             check(code, "pooled KV cache")
 
 
@@ -1727,11 +1738,8 @@ class Fp8Weight:
     def check(self) -> None:
         """Raises if a wait inside a product with this weight ran out since the last check (waits for the weight's device, all
         streams of it)."""
-        torch.cuda.synchronize(self.device)
-        code = int(self.status.item())
+        code = take_status(self.status)
         if code:
-            self.status.zero_()
-            torch.cuda.synchronize(self.device)   # what a product on any stream reports from here on is kept
             check(code, "8-bit product")
 
 

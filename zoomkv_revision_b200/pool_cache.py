@@ -94,10 +94,9 @@ class PoolCache:
             self.bound = int(bound)
 
     def check(self) -> None:
-        """Raises if a step found no room for a request or met an index outside the pool (waits for the GPU)."""
-        code = int(self.status.item())
+        """Raises if a step found no room for a request or met an index outside the pool (waits for the GPU, all streams)."""
+        code = ops.take_status(self.status)
         if code:
-            self.status.zero_()
             raise RuntimeError(f"pool cache: {ops.lib().zkv_status_string(code).decode()}")
 
     # ------------------------------------------------------------------ hooks of the decode loop
