@@ -1684,13 +1684,7 @@ class Fp8Weight:
         _cuda(("w", w), ("scale", scale))
         _dtype("w", w, _F8)
         _dtype("scale", scale, _F32)
-        if parts not in (1, 2):
-            raise ValueError(f"parts must be 1 or 2; got {parts}")
-        if w.dim() != 2 or w.shape[0] % parts or not w.numel():
-            raise ValueError(f"w must be [n, k], n a multiple of parts; got {tuple(w.shape)}")
-        n, k = w.shape[0] // parts, w.shape[1]
-        if k % 16 or (parts == 2 and n % 16):
-            raise ValueError(f"k (and f of two parts) must be multiples of 16; got {tuple(w.shape)}")
+        n, k = self._part(w, parts)
         want = (parts * -(-n // _QUANT_BLOCK), -(-k // _QUANT_BLOCK))
         if tuple(scale.shape) != want or not scale.is_contiguous() or scale.device != w.device:
             raise ValueError(f"scale must be contiguous {want} on the device of w; got {tuple(scale.shape)}")
@@ -1704,13 +1698,24 @@ class Fp8Weight:
         self.status = torch.zeros(1, dtype=_INT32, device=w.device)
         self.status_at = self.status.data_ptr()
 
+    @staticmethod
+    def _part(w, parts):
+        """(rows, k) of a part of w."""
+        if parts not in (1, 2):
+            raise ValueError(f"parts must be 1 or 2; got {parts}")
+        if w.dim() != 2 or w.shape[0] % parts or not w.numel():
+            raise ValueError(f"w must be [n, k], n a multiple of parts; got {tuple(w.shape)}")
+        n, k = w.shape[0] // parts, w.shape[1]
+        if k % 16 or (parts == 2 and n % 16):
+            raise ValueError(f"k (and f of two parts) must be multiples of 16; got {tuple(w.shape)}")
+        return n, k
+
     @classmethod
     def quantize(cls, w, parts: int = 1):
         """The handle of 16- or 32-bit weights [n, k]: scale = amax / 448 of a block, stored = e4m3(w / scale).  For
         loading: elementary operations, 16384 rows at a time."""
-        if w.dim() != 2 or w.shape[0] % parts:
-            raise ValueError(f"w must be [n, k], n a multiple of parts; got {tuple(w.shape)}")
-        n, k = w.shape[0] // parts, w.shape[1]
+        n, k = cls._part(w, parts)
+        _cuda(("w", w))
         nb, kb, S = -(-n // _QUANT_BLOCK), -(-k // _QUANT_BLOCK), _QUANT_BLOCK
         q = torch.empty(w.shape, dtype=_F8, device=w.device)
         scale = torch.empty(parts * nb, kb, dtype=_F32, device=w.device)
