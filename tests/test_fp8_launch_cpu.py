@@ -97,5 +97,12 @@ def test_millions_of_tokens(launches):
     assert got[0][1][0][2] == 65535
 
 
+def test_the_pairs_sizes(launches):
+    """Sizes that the GPU tests mean for the pairs are theirs, whatever the output's type; and one tile of tokens more."""
+    sizes = [(2048, 4096, 1024), (1500, 4001, 1040), (1600, 4096, 1040), (2049, 4001, 1040)]
+    for rc, lines in launches([(*x, 1, kind) for x in sizes for kind in (0, 1, 3)]):
+        assert rc == 0 and [name for name, *_ in lines] == ["many 1"]
+
+
 if __name__ == "__main__":
     print(json.dumps(child(json.loads(sys.argv[1]))))

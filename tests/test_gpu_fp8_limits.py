@@ -3,7 +3,7 @@ test_gpu_fp8.py leaves out.  Tolerances are that file's."""
 import pytest
 import torch
 
-from test_gpu_fp8 import BF, DEV, F8, blocks, check_linear, check_stored, check_swiglu, gen, make_weight, rows, spread, value
+from test_gpu_fp8 import BF, DEV, F8, FL, HF, blocks, check_linear, check_stored, check_swiglu, gen, make_weight, rows, spread, value
 from zoomkv_revision_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +81,93 @@ def test_swiglu_of_gates_far_below_zero(T):
     q, s, w, g, u = one_product(torch.cat([xs / 100, -xs / 100]), f, 1.0, 1.0, T)
     a = g * torch.sigmoid(g) * u
     check_stored(*ops.fp8_swiglu(q, s, w), a, (2.5 * g.abs() + 10) * 2.0 ** -23 * a.abs(), (2.5 * 2 + 10) * 2.0 ** -23)
+
+
+@pytest.mark.parametrize("T", [8, 12, 30, 50, 700])
+@pytest.mark.parametrize("power", [-126, -90, 90, 110])
+def test_swiglu_of_scales_far_from_one(T, power):
+    """Blocks of the output whose scale is below 1e-20, subnormal ones among them, or above 1e20 (their quotients are lifted by
+    a power of two).  The bound is that of test_swiglu_of_gates_far_below_zero; a subnormal scale has a step of 2^-149, at
+    most 2^-22 of the scales here."""
+    f = 1040
+    xs = torch.linspace(1, 2, T, device=DEV)
+    q, s, w, g, u = one_product(torch.cat([xs, -xs]), f, 1.0, 2.0 ** power, T)
+    a = g * torch.sigmoid(g) * u
+    out, scale = ops.fp8_swiglu(q, s, w)
+    full = scale[:, :-1]
+    assert bool(((full < 1e-20) | (full > 1e20)).all()) and bool((full > 2.0 ** -128).all())
+    check_stored(out, scale, a, (2.5 * g.abs() + 10) * 2.0 ** -23 * a.abs(), 15 * 2.0 ** -23)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n", [256, 528, 4112, 16400])
+def test_norm_of_rows_that_are_not_finite(dtype, n):
+    """An infinity: the sum of squares is one, so the row's other elements are zeros and the infinity's block reads back as NaN;
+    a NaN makes the row NaN.  So too where the sum with the residual overflows.  Other rows are as without them."""
+    big = torch.finfo(dtype).max
+    x, res, w = rows(n, 9, n, dtype), rows(n + 1, 9, n, dtype), torch.ones(n, dtype=dtype, device=DEV)
+    clean = ops.rmsnorm_fp8(x, w, 1e-6, residual=res.clone())
+    x[1, n - 20], x[3, 5], res[4, 130], res[6, n // 2] = float("inf"), float("nan"), float("-inf"), float("nan")
+    x[7, 200] = res[7, 200] = big
+    q, s = ops.rmsnorm_fp8(x, w, 1e-6, residual=res)
+    r = res.double()     # the kept sum
+    assert bool(torch.isinf(r[7, 200])) and bool(torch.isnan(r[3, 5])) and bool(torch.isinf(r[1, n - 20]))
+    y = r * torch.rsqrt((r * r).mean(-1, keepdim=True) + 1e-6)
+    bad, got = torch.isnan(y), value(q, s)
+    for i in (1, 3, 4, 6, 7):
+        for b in range(blocks(n)):
+            part = slice(128 * b, min(n, 128 * b + 128))
+            if bool(bad[i, part].any()):
+                assert bool(torch.isnan(got[i, part]).all()), (i, b)
+            else:
+                assert bool((got[i, part] == 0).all()), (i, b)
+    for i in (0, 2, 5, 8):
+        assert torch.equal(q[i].view(torch.uint8), clean[0][i].view(torch.uint8)) and torch.equal(s[i], clean[1][i])
+
+
+PAIRS = [(2048, 4096, 1024, BF), (1500, 4001, 1040, FL), (1600, 4096, 1040, HF), (1500, 4001, 1040, BF)]
+
+
+def test_pairs_of_several_products_at_once_and_in_a_graph():
+    """Products that pairs of CTAs take (test_fp8_launch_cpu.py: test_the_pairs_sizes), with outputs of each type whose rows start
+    on 16 bytes and ones whose rows do not: on streams at the same time, with small products between, and captured and replayed
+    with other inputs.  Every result is, bit for bit, that of a call alone."""
+    ins = [[ops.quant_fp8(rows(T + i, T, k, BF)) for T, _, k, _ in PAIRS] for i in range(2)]
+    ws = [make_weight(n, n, k) for _, n, k, _ in PAIRS]
+    few, wf = ops.quant_fp8(rows(1, 30, 1040, BF)), make_weight(1, 500, 1040)
+
+    def buffers():
+        return [torch.zeros(T, n + 3 * (i == 3), dtype=dtype, device=DEV)[:, 2 * (i == 3):][:, :n]
+                for i, (T, n, _, dtype) in enumerate(PAIRS)]
+
+    want = []
+    for one in ins:
+        outs = buffers()
+        for (q, s), w, out in zip(one, ws, outs):
+            ops.fp8_linear(q, s, w, out=out)
+            check_linear(out, q, s, w)
+        want.append(outs)
+    small = ops.fp8_linear(*few, wf)
+    torch.cuda.synchronize()
+    streams, got, smalls = [torch.cuda.Stream() for _ in PAIRS], buffers(), []
+    for _ in range(10):
+        for i, (q, s) in enumerate(ins[0]):
+            with torch.cuda.stream(streams[i]):
+                ops.fp8_linear(q, s, ws[i], out=got[i])
+                smalls.append(ops.fp8_linear(*few, wf))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0])) and all(torch.equal(x, small) for x in smalls)
+    held = [(q.clone(), s.clone()) for q, s in ins[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for (q, s), w, out in zip(held, ws, got):
+            ops.fp8_linear(q, s, w, out=out)
+            between = ops.fp8_linear(*few, wf)
+    for i in (1, 0):
+        for (q, s), (nq, ns) in zip(held, ins[i]):
+            q.view(torch.uint8).copy_(nq.view(torch.uint8))
+            s.copy_(ns)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i])) and torch.equal(between, small)
+    for w in ws:
+        w.check()
