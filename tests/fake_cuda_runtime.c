@@ -1,8 +1,8 @@
 /* A CUDA runtime with a device of 148 SMs and no GPU behind it, preloaded
  * before the library under test: launches are written down instead of made.
- * FAKE_CTAS_AN_SM=footprint: clusters are counted with as many CTAs an SM as
- * its shared memory holds; otherwise with one, whatever they take.
- * FAKE_CTAS_AN_SM=single: an SM has room for one CTA of every kernel. */
+ * FAKE_CTAS_AN_SM=footprint: the occupancy calls count as many CTAs an SM as
+ * its shared memory holds; otherwise one, whatever they take, as driver
+ * 580.159 does for these kernels. */
 #include <cuda_runtime_api.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -46,24 +46,25 @@ cudaError_t cudaFuncSetAttribute(const void* fn, enum cudaFuncAttribute a, int v
     return cudaSuccess;
 }
 
-static int footprint(size_t smem) { return (int)(228 * 1024 / (smem + 1024)); }
+static int ctas_an_sm(size_t smem) {
+    const char* how = getenv("FAKE_CTAS_AN_SM");
+    return how && !strcmp(how, "footprint") ? (int)(228 * 1024 / (smem + 1024)) : 1;
+}
 
 cudaError_t cudaOccupancyMaxActiveBlocksPerMultiprocessorWithFlags(int* n, const void* fn, int threads, size_t smem, unsigned flags) {
     (void)threads, (void)flags;
     const int i = find(fn);
-    const char* how = getenv("FAKE_CTAS_AN_SM");
     if (i < 0 || smem > (size_t)kernels[i].smem) return cudaErrorInvalidValue;
-    *n = how && !strcmp(how, "single") ? 1 : footprint(smem);
+    *n = ctas_an_sm(smem);
     return cudaSuccess;
 }
 
 cudaError_t cudaOccupancyMaxActiveClusters(int* n, const void* fn, const cudaLaunchConfig_t* c) {
     static const int clusters[] = {0, 148, 74, 45, 33, 26, 22, 15, 15}; /* as a B200 has them */
-    const char* how = getenv("FAKE_CTAS_AN_SM");
-    const int i = find(fn), each = how && !strcmp(how, "footprint") ? footprint(c->dynamicSmemBytes) : 1;
+    const int i = find(fn);
     if (i < 0 || c->dynamicSmemBytes > (size_t)kernels[i].smem) return cudaErrorInvalidValue;
     if (c->attrs[0].val.clusterDim.x > 8) return cudaErrorInvalidValue;
-    *n = each * clusters[c->attrs[0].val.clusterDim.x];
+    *n = ctas_an_sm(c->dynamicSmemBytes) * clusters[c->attrs[0].val.clusterDim.x];
     return cudaSuccess;
 }
 

@@ -82,10 +82,13 @@ def test_a_call_is_cut_the_same_whichever_came_before(launches):
             assert launches([first] + SHAPES, how)[1:] == want, (how, first)
 
 
-def test_a_shared_sm_is_asked_for(launches):
-    """32 tiles of 96 blocks in clusters of eight fit the device at once only where two CTAs share an SM."""
-    assert launches([(8, 4096, 12288, 1)]) == [(0, [("few 16 1", 256, 1, 8)])]
-    assert launches([(8, 4096, 12288, 1)], "single") == [(0, [("few 16 1", 128, 1, 4)])]
+def test_two_ctas_share_an_sm(launches):
+    """Up to 32 tokens: 32 tiles of 96 blocks fit the device at once in clusters of eight, 48 of 32 blocks in clusters of four,
+    where two CTAs share an SM, whatever the occupancy calls count.  64 tokens have an SM a CTA."""
+    for how in ("one", "footprint"):
+        got = launches([(8, 4096, 12288, 1), (32, 4096, 12288, 1), (1, 6144, 4096, 1), (64, 4096, 12288, 1)], how)
+        assert got == [(0, [("few 16 1", 256, 1, 8)]), (0, [("few 32 1", 256, 1, 8)]), (0, [("few 16 1", 192, 1, 4)]),
+                       (0, [("few 64 1", 128, 1, 4)])]
 
 
 def test_millions_of_tokens(launches):

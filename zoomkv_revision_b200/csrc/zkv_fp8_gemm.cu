@@ -84,6 +84,8 @@ struct Few {
     static_assert(kTmem >= 32 && kTmem <= 512 && (kTmem & (kTmem - 1)) == 0, "tensor memory comes in powers of two");
     static_assert(kTmem <= 256 || smem(kStages) > (227 - 76) * 1024, "alone on its SM");
     static_assert(smem(kStages) > 76 * 1024, "no third CTA on an SM");
+    // and the registers are the launch bounds'
+    static_assert(!kHalves || (2 * (smem(kStages) + 1024) <= 228 * 1024 && 2 * kTmem <= 512), "two CTAs an SM");
     static_assert(kMine % kLoad == 0, "whole loads");
     static_assert(16 * (kMost + kBufs) + 4 <= 512, "barriers");
     static_assert(kStages >= 2 && kTok * kParts * kPitch * 4 <= kStages * kStage, "the parts are joined in the ring's place");
@@ -136,7 +138,7 @@ __device__ __forceinline__ float gated(float g, float u) {
 }
 
 template <int kTok, int kParts>
-__global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, 1)
+__global__ void __launch_bounds__(Few<kTok, kParts>::kThreads, Few<kTok, kParts>::kHalves ? 2 : 1)
     few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, Product a) {
     using C = Few<kTok, kParts>;
     extern __shared__ uint8_t smem_raw[];
@@ -835,7 +837,7 @@ static cudaLaunchConfig_t configure(cudaLaunchAttribute (&attr)[2], unsigned x, 
 // Clusters of s CTAs (s = 1..8) that the current device holds at once with one CTA an SM: a cluster lies within one of its
 // groups of SMs, so that of three, five or seven CTAs many SMs stay empty.  Asked for one kernel that has an SM to itself
 // and used for all products, so that how a product is cut depends neither on which ran first nor on whether the driver's
-// count looks at what a kernel takes (580.159 counts one CTA an SM for those that share one, too).
+// count looks at what a kernel takes (580.159 counts one CTA an SM for those that share one, too; that two fit, Few asserts).
 struct Places {
     int clusters[9];
 };
@@ -857,23 +859,6 @@ static const Places* places() {
         if (cudaOccupancyMaxActiveClusters(&p.clusters[s], kernel, &cfg) != cudaSuccess) return nullptr;
     }
     return &p;
-}
-
-// Whether two CTAs of a kernel run on an SM of the current device: 1 or 0, -1 where it cannot be asked.  The kernel's
-// shared-memory limit has been raised.
-template <int kTok, int kParts>
-static int shares_sm() {
-    using C = Few<kTok, kParts>;
-    if (!C::kHalves) return 0;
-    static std::mutex mutex;
-    static int known[64] = {};  // CTAs an SM
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
-    const std::lock_guard<std::mutex> lock(mutex);
-    if (!known[dev] && cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known[dev], few_kernel<kTok, kParts>, C::kThreads,
-                                                                     C::smem(C::kStages)) != cudaSuccess)
-        return -1;
-    return known[dev] >= 2;
 }
 
 // How the inner dimension is cut over a cluster's CTAs: the number for which the waves of clusters take the fewest blocks
@@ -906,9 +891,8 @@ static int launch_few(const zkv_fp8_weight* w, const void* x, int64_t x_ld, cons
     auto kernel = few_kernel<kTok, kParts>;
     if (!raise_smem_limit((const void*)kernel, C::smem(C::kStages))) return launch_refused();
     const Places* p = places();
-    const int shares = shares_sm<kTok, kParts>();
-    if (!p || shares < 0) return launch_refused();
-    const int parts = cut_of(a.row_blocks * wide, a.k_blocks, shares, *p).parts;
+    if (!p) return launch_refused();
+    const int parts = cut_of(a.row_blocks * wide, a.k_blocks, C::kHalves, *p).parts;
     cudaLaunchAttribute attr[2];
     const cudaLaunchConfig_t cfg = configure(attr, (unsigned)(a.row_blocks * parts), (unsigned)wide, C::kThreads,
                                              C::smem(C::kStages), (unsigned)parts, stream);
