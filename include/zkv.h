@@ -823,10 +823,11 @@ typedef struct zkv_fp8_weight {
  * called once per weight, and again when a field above `map` changes.      */
 int zkv_fp8_weight_init(zkv_fp8_weight* w);
 
-/* out[i][n] = sum over blocks b of x_scale[i][b] * w.scale[n / 128][b] * (sum
- * of the block's products), for w of one part.  Products and sums in fp32,
- * one rounding to `dtype` (bf16, fp16 or fp32) at the end; the inner
- * dimension may be summed in parts, joined in a fixed order.
+/* out[i][n] = sum over blocks b of (x_scale[i][b] * w.scale[n / 128][b]) * (sum
+ * of the block's products), for w of one part.  Products and sums in fp32 (that
+ * of the two scales first: it too has fp32's range), one rounding to `dtype`
+ * (bf16, fp16 or fp32) at the end; the inner dimension may be summed in parts,
+ * joined in a fixed order.
  *   x [tokens][k] e4m3, row i at i * x_ld bytes (16-byte rows)
  *   out [tokens][rows], row i at i * out_ld elements
  * `status` (may be NULL) gets ZKV_ERR_TIMEOUT for a wait that ran out.     */

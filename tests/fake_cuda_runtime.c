@@ -91,6 +91,7 @@ static int encode(void* map, int type, unsigned rank, void* at, const unsigned l
     for (unsigned i = 0; i + 1 < rank; ++i)
         if (strides[i] % 16 || strides[i] >= 1ull << 40) return 1;
     memset(map, 0, 128);
+    memcpy(map, &at, sizeof at); /* not all zeros, as no map is */
     return 0;
 }
 

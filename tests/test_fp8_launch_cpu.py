@@ -22,19 +22,20 @@ pytestmark = pytest.mark.skipif(shutil.which("gcc") is None or not os.path.exist
 
 
 def child(calls):
-    """In a process with the fake preloaded: [status, launches] of each call (tokens, rows, k, parts, output's bytes an element)."""
+    """In a process with the fake preloaded: [status, launches] of each call (tokens, rows, k, parts, the output's type of a
+    product of one part, whether the handle was initialised)."""
     spec = importlib.util.spec_from_file_location("zkv_lib", os.path.join(ROOT, "zoomkv_revision_b200", "_lib.py"))
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
     lib, fake = mod.lib(), ctypes.CDLL(None)
     fake.fake_launches.restype = ctypes.c_char_p
     got = []
-    for tokens, rows, k, parts, kind in calls:
+    for tokens, rows, k, parts, kind, init in calls:
         w = mod.ZkvFp8Weight(w=1 << 32, scale=1 << 33, ld=k, rows=rows, k=k, parts=parts)
-        assert lib.zkv_fp8_weight_init(ctypes.addressof(w)) == 0
+        assert not init or lib.zkv_fp8_weight_init(ctypes.addressof(w)) == 0
         fake.fake_forget()
-        x = (1 << 34, k, 1 << 35, 1, tokens, tokens, ctypes.addressof(w), 1 << 36, rows)
-        rc = lib.zkv_fp8_linear(*x, kind, None, None) if parts == 1 else lib.zkv_fp8_swiglu(*x, 1 << 37, 1, tokens, None, None)
+        x = (1 << 34, k, 1 << 35, 1, max(tokens, 1), tokens, ctypes.addressof(w), 1 << 36, rows)
+        rc = lib.zkv_fp8_linear(*x, kind, None, None) if parts == 1 else lib.zkv_fp8_swiglu(*x, 1 << 37, 1, max(tokens, 1), None, None)
         got.append([rc, fake.fake_launches().decode()])
     return got
 
@@ -46,7 +47,7 @@ def launches(tmp_path_factory):
                     os.path.join(HERE, "fake_cuda_runtime.c")], check=True)
 
     def run(calls, how="one"):
-        calls = [(*c, 0)[:5] for c in calls]
+        calls = [(*c, *(0, True)[len(c) - 4:]) for c in calls]
         env = dict(os.environ, LD_PRELOAD=str(so), FAKE_CTAS_AN_SM=how)
         out = subprocess.run([sys.executable, os.path.abspath(__file__), json.dumps(calls)], env=env, capture_output=True,
                              text=True, timeout=60)
@@ -105,6 +106,13 @@ def test_the_pairs_sizes(launches):
     sizes = [(2048, 4096, 1024), (1500, 4001, 1040), (1600, 4096, 1040), (2049, 4001, 1040)]
     for rc, lines in launches([(*x, 1, kind) for x in sizes for kind in (0, 1, 3)]):
         assert rc == 0 and [name for name, *_ in lines] == ["many 1"]
+
+
+def test_a_handle_that_was_not_initialised_is_refused(launches):
+    """Its tensor map would be read by the copies as it is; a call of no tokens reads none."""
+    for tokens, parts in [(1, 1), (100, 1), (4096, 1), (8, 2), (4096, 2)]:
+        assert launches([(tokens, 4096, 1024, parts, 0, False)]) == [(1, [])]
+    assert launches([(0, 4096, 1024, parts, 0, False) for parts in (1, 2)]) == [(0, [])] * 2
 
 
 if __name__ == "__main__":

@@ -971,6 +971,9 @@ static int check_call(const void* x, int64_t x_ld, const float* x_scale, int64_t
 // x 4096 49.4 and 44.9, 1024 x 1024 x 4096 11.7 and 17.7.  More tokens than a grid of the first kind holds go to the pairs.
 template <int kParts>
 static int launch(const zkv_fp8_weight* w, const void* x, int64_t x_ld, const Product& a, cudaStream_t stream) {
+    uint64_t any = 0;
+    for (uint64_t word : w->map) any |= word;
+    if (!any) return ZKV_ERR_ARG;  // zkv_fp8_weight_init was not called
     if (a.tokens <= 16) return launch_few<16, kParts>(w, x, x_ld, a, stream);
     if (a.tokens <= 32) return launch_few<32, kParts>(w, x, x_ld, a, stream);
     if (a.tokens <= 64) return launch_few<64, kParts>(w, x, x_ld, a, stream);
