@@ -967,8 +967,8 @@ static int check_call(const void* x, int64_t x_ld, const float* x_scale, int64_t
 // Up to 64 tokens features are the rows of a tile.  Above, CTAs of 128 tokens and one part's 128 features each (a cluster
 // may share a tile), or pairs of CTAs of 256 tokens and 256 features: by the blocks that the waves of either take after one
 // another.  A block takes the pair a little longer, and CTAs of two parts twice as long.  us of the first and of the second
-// kind: 333 x 4096 x 4096 13.9 and 17.8, 768 x 4096 x 4096 32.9 and 18.9, 512 x 4096 x 12288 38.4 and 42.4, 129 x 2 x 12288
-// x 4096 49.4 and 44.9, 1024 x 1024 x 4096 11.7 and 17.7.  More tokens than a grid of the first kind holds go to the pairs.
+// kind: 333 x 4096 x 4096 13.7 and 16.4, 768 x 4096 x 4096 31.2 and 18.1, 512 x 4096 x 12288 37.0 and 41.1, 129 x 2 x 12288
+// x 4096 48.0 and 41.8, 1024 x 1024 x 4096 11.2 and 16.1.  More tokens than a grid of the first kind holds go to the pairs.
 template <int kParts>
 static int launch(const zkv_fp8_weight* w, const void* x, int64_t x_ld, const Product& a, cudaStream_t stream) {
     uint64_t any = 0;
