@@ -836,7 +836,7 @@ int zkv_fp8_linear(const void* x, int64_t x_ld, const float* x_scale, int64_t xs
 
 /* silu(g) * u, quantised in blocks of 128 features: g and u as
  * zkv_fp8_linear gives them for the two parts of w, in fp32, and their
- * product to a relative (|g| + 8) 2^-23 (zeros for g < -174).
+ * product to a relative (|g| + 8) 2^-23 (zeros for g < -175).
  *   out [tokens][rows] e4m3, row i at i * out_ld bytes (16-byte rows)      */
 int zkv_fp8_swiglu(const void* x, int64_t x_ld, const float* x_scale, int64_t xs_token, int64_t xs_block, int64_t tokens,
                    const zkv_fp8_weight* w, void* out, int64_t out_ld, float* out_scale, int64_t os_token,
